@@ -111,7 +111,9 @@ __device__ __forceinline__ void load_half_rows(const float *__restrict__ row, in
   load_row8(row + 64, lane, hi);
 }
 
-template <bool kSeqStride>
+// kAt: tokens are rotated at positions[tok] instead of the position of the slot
+// they are written to (drafted tokens: depth in their tree against place in it).
+template <bool kSeqStride, bool kAt>
 __global__ __launch_bounds__(256) void qknorm_rope_append_kernel(
     const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
     uint16_t *__restrict__ q_out, int64_t qo_ss, int64_t qo_st, int64_t qo_sh,
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(256) void qknorm_rope_append_kernel(
     const int32_t *__restrict__ q_start, const int32_t *__restrict__ cache_lens,
     const int32_t *__restrict__ page_table, int64_t pt_stride, int num_seqs,
     int total_tokens, int num_q_heads, int num_kv_heads, int page_size,
-    int max_positions) {
+    int max_positions, const int32_t *__restrict__ positions) {
   const int lane = threadIdx.x & 7;          // position in the row's 8-lane group
   const int slot = (threadIdx.x >> 3) & 7;   // row group within the wave
   const int tok = __builtin_amdgcn_readfirstlane(blockIdx.x * kTokensPerBlock + (threadIdx.x >> 6));
@@ -182,7 +184,8 @@ __global__ __launch_bounds__(256) void qknorm_rope_append_kernel(
   if (rot) {
     // Positions must be below max_positions (the caller's contract); the
     // clamp only keeps a call that breaks it inside the tables.
-    const int64_t off = static_cast<int64_t>(min(pos, max_positions - 1)) * kHeadDim;
+    const int rot_pos = kAt ? max(positions[tok], 0) : pos;
+    const int64_t off = static_cast<int64_t>(min(rot_pos, max_positions - 1)) * kHeadDim;
     load_half_rows(cos_t + off, lane, cl, ch);
     load_half_rows(sin_t + off, lane, sl, sh);
   }
@@ -345,6 +348,60 @@ extern "C" int hy_kv_append(void *k_pool, void *v_pool,
   return hy::launch_status("hy_kv_append");
 }
 
+static int qknorm_rope_append_impl(
+    const char *name,
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
+    int64_t q_stride_head, void *q_out, int64_t qo_stride_seq,
+    int64_t qo_stride_tok, int64_t qo_stride_head, const void *k,
+    int64_t k_stride_seq, int64_t k_stride_tok, int64_t k_stride_head,
+    const void *v, int64_t v_stride_seq, int64_t v_stride_tok,
+    int64_t v_stride_head, const void *q_norm_weight,
+    const void *k_norm_weight, float q_eps, float k_eps, const float *cos_table,
+    const float *sin_table, int32_t max_positions, void *k_pool, void *v_pool,
+    int64_t pool_head_stride, const int32_t *q_start,
+    const int32_t *cache_lens, const int32_t *page_table,
+    int64_t page_table_stride, int32_t num_seqs, int32_t total_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, const int32_t *positions, void *stream) {
+  if (int rc = check_common(num_seqs, total_tokens, num_kv_heads, head_dim, page_size))
+    return rc;
+  HY_REQUIRE(num_q_heads >= 1, "num_q_heads must be positive");
+  HY_REQUIRE(q && q_out && k && v && k_pool && v_pool && q_start &&
+                 cache_lens && page_table,
+             "%s: null pointer argument", name);
+  HY_REQUIRE((cos_table == nullptr) == (sin_table == nullptr),
+             "cos_table and sin_table must both be given or both be NULL");
+  HY_REQUIRE(cos_table == nullptr || max_positions > 0,
+             "max_positions must be positive when tables are given");
+  if (total_tokens == 0) return HY_OK;
+  HY_REQUIRE(num_q_heads + 2 * num_kv_heads <= 65535, "too many heads (%d q, %d kv)",
+             num_q_heads, num_kv_heads);
+  const int gq = (num_q_heads + hy::kQChunk - 1) / hy::kQChunk;
+  const int gkv = (num_kv_heads + hy::kKvChunk - 1) / hy::kKvChunk;
+  // Row addresses that need no sequence index let the kernel load rows
+  // before it searches for the token's sequence.
+  const bool seq_stride = q_stride_seq || qo_stride_seq || k_stride_seq || v_stride_seq;
+  auto kernel = positions ? seq_stride ? hy::qknorm_rope_append_kernel<true, true>
+                                       : hy::qknorm_rope_append_kernel<false, true>
+                : seq_stride ? hy::qknorm_rope_append_kernel<true, false>
+                             : hy::qknorm_rope_append_kernel<false, false>;
+  hipLaunchKernelGGL(
+      kernel, dim3((total_tokens + hy::kTokensPerBlock - 1) / hy::kTokensPerBlock, gq + gkv),
+      dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const uint16_t *>(q),
+      q_stride_seq, q_stride_tok, q_stride_head, static_cast<uint16_t *>(q_out),
+      qo_stride_seq, qo_stride_tok, qo_stride_head,
+      static_cast<const uint16_t *>(k), k_stride_seq, k_stride_tok,
+      k_stride_head, static_cast<const uint16_t *>(v), v_stride_seq,
+      v_stride_tok, v_stride_head,
+      static_cast<const uint16_t *>(q_norm_weight),
+      static_cast<const uint16_t *>(k_norm_weight), q_eps, k_eps, cos_table, sin_table,
+      static_cast<uint16_t *>(k_pool), static_cast<uint16_t *>(v_pool),
+      pool_head_stride, q_start, cache_lens, page_table, page_table_stride,
+      num_seqs, total_tokens, num_q_heads, num_kv_heads, page_size, max_positions,
+      positions);
+  return hy::launch_status(name);
+}
+
 extern "C" int hy_qknorm_rope_append(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
     int64_t q_stride_head, void *q_out, int64_t qo_stride_seq,
@@ -360,40 +417,40 @@ extern "C" int hy_qknorm_rope_append(
     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
     int32_t page_size, void *stream) {
   hy::clear_error();
-  if (int rc = check_common(num_seqs, total_tokens, num_kv_heads, head_dim, page_size))
-    return rc;
-  HY_REQUIRE(num_q_heads >= 1, "num_q_heads must be positive");
-  HY_REQUIRE(q && q_out && k && v && k_pool && v_pool && q_start &&
-                 cache_lens && page_table,
-             "hy_qknorm_rope_append: null pointer argument");
-  HY_REQUIRE((cos_table == nullptr) == (sin_table == nullptr),
-             "cos_table and sin_table must both be given or both be NULL");
-  HY_REQUIRE(cos_table == nullptr || max_positions > 0,
-             "max_positions must be positive when tables are given");
-  if (total_tokens == 0) return HY_OK;
-  HY_REQUIRE(num_q_heads + 2 * num_kv_heads <= 65535, "too many heads (%d q, %d kv)",
-             num_q_heads, num_kv_heads);
-  const int gq = (num_q_heads + hy::kQChunk - 1) / hy::kQChunk;
-  const int gkv = (num_kv_heads + hy::kKvChunk - 1) / hy::kKvChunk;
-  // Row addresses that need no sequence index let the kernel load rows
-  // before it searches for the token's sequence.
-  const bool seq_stride = q_stride_seq || qo_stride_seq || k_stride_seq || v_stride_seq;
-  auto kernel = seq_stride ? hy::qknorm_rope_append_kernel<true>
-                           : hy::qknorm_rope_append_kernel<false>;
-  hipLaunchKernelGGL(
-      kernel, dim3((total_tokens + hy::kTokensPerBlock - 1) / hy::kTokensPerBlock, gq + gkv),
-      dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const uint16_t *>(q),
-      q_stride_seq, q_stride_tok, q_stride_head, static_cast<uint16_t *>(q_out),
-      qo_stride_seq, qo_stride_tok, qo_stride_head,
-      static_cast<const uint16_t *>(k), k_stride_seq, k_stride_tok,
-      k_stride_head, static_cast<const uint16_t *>(v), v_stride_seq,
-      v_stride_tok, v_stride_head,
-      static_cast<const uint16_t *>(q_norm_weight),
-      static_cast<const uint16_t *>(k_norm_weight), q_eps, k_eps, cos_table, sin_table,
-      static_cast<uint16_t *>(k_pool), static_cast<uint16_t *>(v_pool),
-      pool_head_stride, q_start, cache_lens, page_table, page_table_stride,
-      num_seqs, total_tokens, num_q_heads, num_kv_heads, page_size, max_positions);
-  return hy::launch_status("hy_qknorm_rope_append");
+  return qknorm_rope_append_impl(
+      "hy_qknorm_rope_append", q, q_stride_seq, q_stride_tok, q_stride_head, q_out,
+      qo_stride_seq, qo_stride_tok, qo_stride_head, k, k_stride_seq, k_stride_tok, k_stride_head,
+      v, v_stride_seq, v_stride_tok, v_stride_head, q_norm_weight, k_norm_weight, q_eps, k_eps,
+      cos_table, sin_table, max_positions, k_pool, v_pool, pool_head_stride, q_start, cache_lens,
+      page_table, page_table_stride, num_seqs, total_tokens, num_q_heads, num_kv_heads, head_dim,
+      page_size, nullptr, stream);
+}
+
+extern "C" int hy_qknorm_rope_append_at(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
+    int64_t q_stride_head, void *q_out, int64_t qo_stride_seq,
+    int64_t qo_stride_tok, int64_t qo_stride_head, const void *k,
+    int64_t k_stride_seq, int64_t k_stride_tok, int64_t k_stride_head,
+    const void *v, int64_t v_stride_seq, int64_t v_stride_tok,
+    int64_t v_stride_head, const void *q_norm_weight,
+    const void *k_norm_weight, float q_eps, float k_eps, const float *cos_table,
+    const float *sin_table, int32_t max_positions,
+    const int32_t *positions, void *k_pool, void *v_pool,
+    int64_t pool_head_stride, const int32_t *q_start,
+    const int32_t *cache_lens, const int32_t *page_table,
+    int64_t page_table_stride, int32_t num_seqs, int32_t total_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(positions != nullptr || total_tokens == 0,
+             "hy_qknorm_rope_append_at: null pointer argument");
+  return qknorm_rope_append_impl(
+      "hy_qknorm_rope_append_at", q, q_stride_seq, q_stride_tok, q_stride_head, q_out,
+      qo_stride_seq, qo_stride_tok, qo_stride_head, k, k_stride_seq, k_stride_tok, k_stride_head,
+      v, v_stride_seq, v_stride_tok, v_stride_head, q_norm_weight, k_norm_weight, q_eps, k_eps,
+      cos_table, sin_table, max_positions, k_pool, v_pool, pool_head_stride, q_start, cache_lens,
+      page_table, page_table_stride, num_seqs, total_tokens, num_q_heads, num_kv_heads, head_dim,
+      page_size, positions, stream);
 }
 
 extern "C" int hy_page_gather(const void *pool, int64_t pool_layer_stride,

@@ -20,12 +20,14 @@
 
 #include <algorithm>
 #include <functional>
+#include <new>
 #include <queue>
 #include <vector>
 
 #include "../../include/hayate_attn.h"
 #include "decode_shape.h"
 #include "prefill_shape.h"
+#include "tree_shape.h"
 
 namespace hy {
 void set_error(const char *fmt, ...);
@@ -456,4 +458,208 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
   counts_out[5] = n_pslots;
   counts_out[6] = n_pieces;
   return HY_OK;
+}
+
+namespace {
+
+// Cost of a piece of drafted-tree attention after a chunk's first, in key steps.
+constexpr int64_t kTreePieceCost = 1;
+
+struct TreePieceRec {
+  int32_t tile, step0, step1;  // query tile, and its key steps
+};
+
+// Cuts the key steps of the query tiles, in order, into at most n_chunks
+// chunks of equal cost: chunk i holds pieces [ends[i - 1], ends[i]). Returns
+// the costliest chunk's cost. `total` is what the whole stream is taken to cost.
+int64_t cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total,
+                 std::vector<TreePieceRec> &pieces, std::vector<int32_t> &ends) {
+  pieces.clear();
+  ends.clear();
+  int64_t spent = 0, in_chunk = 0, worst = 0;
+  int32_t first = 0;
+  auto close = [&]() {
+    worst = std::max(worst, in_chunk);
+    spent += in_chunk;
+    in_chunk = 0;
+    first = static_cast<int32_t>(pieces.size());
+    ends.push_back(first);
+  };
+  for (size_t t = 0; t < steps.size(); ++t) {
+    int32_t at = 0;
+    while (at < steps[t]) {
+      const int64_t left = n_chunks - static_cast<int64_t>(ends.size());  // this one included
+      const int64_t share = left > 1 ? (std::max<int64_t>(total - spent, 1) + left - 1) / left : INT64_MAX;
+      const int64_t extra = static_cast<int32_t>(pieces.size()) > first ? kTreePieceCost : 0;
+      const int64_t room = share - in_chunk - extra;
+      if (room <= 0 && static_cast<int32_t>(pieces.size()) > first) {
+        close();
+        continue;
+      }
+      const int32_t n = static_cast<int32_t>(
+          std::min<int64_t>(steps[t] - at, std::max<int64_t>(room, 1)));
+      pieces.push_back({static_cast<int32_t>(t), at, at + n});
+      in_chunk += n + extra;
+      at += n;
+    }
+  }
+  if (static_cast<int32_t>(pieces.size()) > first) close();
+  return worst;
+}
+
+int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t G,
+              int32_t num_kv_heads, int32_t num_cus, int32_t *items, int32_t item_capacity,
+              int32_t *merge_items, int32_t merge_capacity, int32_t *counts_out) {
+  struct Tile {
+    int32_t seq, q0, q1, kv_end;
+  };
+  std::vector<Tile> tiles;
+  std::vector<int32_t> q_begin(static_cast<size_t>(num_seqs) + 1, 0), steps;
+  int64_t all = 0;
+  int32_t max_rows = 0;
+  for (int b = 0; b < num_seqs; ++b) {
+    q_begin[b + 1] = q_begin[b] + q_lens[b];
+    // nodes beyond one workgroup's rows: tiles of equal size
+    const int32_t per = hy::kTreeRows / G;
+    const int32_t n = (q_lens[b] + per - 1) / per;
+    for (int32_t i = 0; i < n; ++i) {
+      const int32_t q0 = static_cast<int32_t>(static_cast<int64_t>(q_lens[b]) * i / n);
+      const int32_t q1 = static_cast<int32_t>(static_cast<int64_t>(q_lens[b]) * (i + 1) / n);
+      const int32_t end = kv_lens[b] - q_lens[b] + q1;
+      tiles.push_back({b, q0, q1, end});
+      steps.push_back((end + hy::kTreeTileKeys - 1) / hy::kTreeTileKeys);
+      all += steps.back();
+      max_rows = std::max(max_rows, (q1 - q0) * G);
+    }
+  }
+  const int64_t cus = num_cus > 0 ? num_cus : 256;
+  const int64_t n_chunks =
+      std::max<int64_t>(1, std::min<int64_t>((cus + num_kv_heads - 1) / num_kv_heads, all));
+  std::vector<TreePieceRec> pieces, trial;
+  std::vector<int32_t> ends, trial_ends;
+  int64_t worst = cut_tree(steps, n_chunks, all, pieces, ends);
+  for (int pass = 0; pass < 3 && !pieces.empty(); ++pass) {
+    const int64_t total = all + kTreePieceCost * static_cast<int64_t>(
+        (pass ? trial : pieces).size() - (pass ? trial_ends : ends).size());
+    const int64_t w = cut_tree(steps, n_chunks, total, trial, trial_ends);
+    if (w < worst) {
+      worst = w;
+      pieces = trial;
+      ends = trial_ends;
+    }
+  }
+  const int64_t need = 2 * static_cast<int64_t>(ends.size()) + static_cast<int64_t>(pieces.size());
+  if (need > item_capacity) {
+    hy::set_error("hy_plan_tree: item capacity %d too small (need %lld)", item_capacity,
+                  static_cast<long long>(need));
+    return HY_ENOSPACE;
+  }
+  int32_t n_merge = 0;
+  int64_t n_slots = 0;
+  int32_t *rec = items + hy::kTreeChunkInts * static_cast<int64_t>(ends.size());
+  for (size_t i = 0; i < pieces.size(); ++i) {
+    const Tile &t = tiles[pieces[i].tile];
+    const int32_t blocks = ((t.q1 - t.q0) * G + 31) / 32;
+    const bool whole = pieces[i].step0 == 0 && pieces[i].step1 == steps[pieces[i].tile];
+    if (!whole) {
+      if (pieces[i].step0 == 0) {
+        if (n_merge >= merge_capacity) {
+          hy::set_error("hy_plan_tree: merge capacity %d too small", merge_capacity);
+          return HY_ENOSPACE;
+        }
+        int32_t *m = merge_items + 8 * n_merge++;
+        m[0] = t.seq;
+        m[1] = t.q0;
+        m[2] = t.q1;
+        m[3] = static_cast<int32_t>(n_slots);
+        m[4] = 0;
+        m[5] = q_begin[t.seq];
+        m[6] = blocks;
+        m[7] = 0;
+      }
+      ++merge_items[8 * (n_merge - 1) + 4];  // a tile's pieces are consecutive
+    }
+    int32_t *r = rec + 8 * i;
+    r[0] = t.seq;
+    r[1] = t.q0;
+    r[2] = t.q1;
+    r[3] = pieces[i].step0 * hy::kTreeTileKeys;
+    r[4] = std::min(t.kv_end, pieces[i].step1 * hy::kTreeTileKeys);
+    r[5] = whole ? -1 : static_cast<int32_t>(n_slots);
+    r[6] = q_begin[t.seq];
+    r[7] = kv_lens[t.seq] - q_lens[t.seq];
+    if (!whole) n_slots += blocks;
+    if (n_slots > INT32_MAX) {
+      hy::set_error("hy_plan_tree: too many partials");
+      return HY_EINVAL;
+    }
+  }
+  for (size_t i = 0; i < ends.size(); ++i) {
+    const int32_t first = i ? ends[i - 1] : 0;
+    int32_t *ch = items + hy::kTreeChunkInts * i;
+    int32_t n = 0;
+    for (int32_t p = first; p < ends[i]; ++p) n += pieces[p].step1 - pieces[p].step0;
+    ch[0] = first;
+    ch[1] = ends[i];
+    ch[2] = n;
+    for (int j = 3; j < 8; ++j) ch[j] = 0;
+    for (int j = 0; j < 8; ++j) ch[8 + j] = rec[8 * first + j];
+  }
+  counts_out[0] = static_cast<int32_t>(ends.size());
+  counts_out[1] = static_cast<int32_t>(pieces.size());
+  counts_out[2] = n_merge;
+  counts_out[3] = static_cast<int32_t>(n_slots);
+  counts_out[4] = max_rows;
+  return HY_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t hy_tree_max_nodes(void) { return hy::kTreeMaxNodes; }
+
+extern "C" int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs,
+                            int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
+                            int32_t *items, int32_t item_capacity, int32_t *merge_items,
+                            int32_t merge_capacity, int32_t *counts_out) {
+  hy::clear_error();
+  if (num_seqs < 0 || (num_seqs > 0 && (q_lens == nullptr || kv_lens == nullptr)) ||
+      counts_out == nullptr || (item_capacity > 0 && items == nullptr) ||
+      (merge_capacity > 0 && merge_items == nullptr)) {
+    hy::set_error("hy_plan_tree: invalid arrays");
+    return HY_EINVAL;
+  }
+  if (num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads % num_kv_heads) {
+    hy::set_error("hy_plan_tree: num_q_heads (%d) must be a multiple of num_kv_heads (%d)",
+                  num_q_heads, num_kv_heads);
+    return HY_EINVAL;
+  }
+  const int32_t G = num_q_heads / num_kv_heads;
+  if (G > 16 || (G & (G - 1))) {
+    hy::set_error("hy_plan_tree: GQA group size %d unsupported (1, 2, 4, 8, 16)", G);
+    return HY_EUNSUPPORTED;
+  }
+  int64_t rows = 0;
+  for (int b = 0; b < num_seqs; ++b) {
+    if (q_lens[b] < 1 || kv_lens[b] < q_lens[b]) {
+      hy::set_error("hy_plan_tree: sequence %d has q_len %d, kv_len %d", b, q_lens[b], kv_lens[b]);
+      return HY_EINVAL;
+    }
+    if (q_lens[b] > hy::kTreeMaxNodes) {
+      hy::set_error("hy_plan_tree: sequence %d has %d nodes, at most %d are supported", b,
+                    q_lens[b], hy::kTreeMaxNodes);
+      return HY_EUNSUPPORTED;
+    }
+    rows += q_lens[b];
+  }
+  if (rows > INT32_MAX) {
+    hy::set_error("hy_plan_tree: too many rows");
+    return HY_EINVAL;
+  }
+  try {
+    return plan_tree(q_lens, kv_lens, num_seqs, G, num_kv_heads, num_cus, items, item_capacity,
+                     merge_items, merge_capacity, counts_out);
+  } catch (const std::bad_alloc &) {
+    hy::set_error("hy_plan_tree: out of host memory");
+    return HY_ENOSPACE;
+  }
 }

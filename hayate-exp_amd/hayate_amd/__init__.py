@@ -5,7 +5,13 @@ for gfx950, C ABI in include/hayate_attn.h).
 """
 
 from .cache import Cache
-from .paged_cache import PagedCacheHandle, PagedKVBatch, PagedKVCacheManager, PagedPrefix
+from .paged_cache import (
+    PagedCacheHandle,
+    PagedKVBatch,
+    PagedKVCacheManager,
+    PagedPrefix,
+    PagedTreeBatch,
+)
 from .prefix_cache import PrefixCache, PrefixCacheMatch
 from .rope import compute_rope_params
 
@@ -15,6 +21,7 @@ __all__ = [
     "PagedKVBatch",
     "PagedKVCacheManager",
     "PagedPrefix",
+    "PagedTreeBatch",
     "PrefixCache",
     "PrefixCacheMatch",
     "compute_rope_params",

@@ -114,6 +114,31 @@ _SIGNATURES = {
         [_P, _I64, _I32, _I32, _P, _I64, _I32, _P, _I64, _P, _I64, _P],
         ctypes.c_int,
     ),
+    "hy_qknorm_rope_append_at": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P,
+         _I64, _I64, _I64, _P, _P, _F32, _F32, _P, _P, _I32, _P, _P, _P, _I64, _P, _P,
+         _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_tree_max_nodes": ([], ctypes.c_int32),
+    "hy_plan_tree": (
+        [_P, _P, _I32, _I32, _I32, _I32, _P, _I32, _P, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_tree_workspace_bytes": ([_I32, _I32, _I32], ctypes.c_int64),
+    "hy_paged_tree": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _I32,
+         _P, _I32, _I32, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _F32, _P],
+        ctypes.c_int,
+    ),
+    "hy_kv_move": (
+        [_P, _P, _I64, _I64, _I64, _P, _P, _I32, _I32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_page_copy": (
+        [_P, _P, _I64, _I64, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -243,3 +268,47 @@ def decode_workspace_bytes(n_slots: int, num_q_heads: int, head_dim: int) -> int
 
 def prefill_workspace_bytes(n_slots: int, num_kv_heads: int, head_dim: int) -> int:
     return int(lib().hy_prefill_workspace_bytes(n_slots, num_kv_heads, head_dim))
+
+
+class TreePlan:
+    """Host copy of one tree tick's work lists (hy_plan_tree)."""
+
+    __slots__ = ("items", "n_chunks", "merge", "n_slots", "max_rows")
+
+    def __init__(self, items, n_chunks, merge, n_slots, max_rows):
+        # int32 (2 n_chunks + n_pieces, 8): chunk records of two rows {piece_begin,
+        # piece_end, n_steps, 0..} and the first piece, then piece records {seq, q_begin,
+        # q_end, kv_begin, kv_end, slot, q_row, cache_len}
+        self.items = items
+        self.n_chunks = n_chunks
+        self.merge = merge  # int32 (n, 8) {seq, q_begin, q_end, first_slot, splits, q_row, blocks, 0}
+        self.n_slots = n_slots
+        self.max_rows = max_rows
+
+
+def plan_tree(
+    q_lens: np.ndarray, kv_lens: np.ndarray, num_q_heads: int, num_kv_heads: int, num_cus: int
+) -> TreePlan:
+    """Run the native planner of drafted-tree attention."""
+    q_lens = np.ascontiguousarray(q_lens, dtype=np.int32)
+    kv_lens = np.ascontiguousarray(kv_lens, dtype=np.int32)
+    n = int(q_lens.shape[0])
+    # at most 16 heads a group, so a tree has at most 16 tiles of 256 rows, and every
+    # cut between chunks adds one piece
+    tiles = n * 16
+    chunks = -(-(num_cus if num_cus > 0 else 256) // max(1, num_kv_heads)) + 1
+    items = np.zeros((3 * chunks + tiles, 8), dtype=np.int32)
+    merge = np.zeros((tiles + 1, 8), dtype=np.int32)
+    counts = np.zeros(5, dtype=np.int32)
+    rc = lib().hy_plan_tree(
+        q_lens.ctypes.data, kv_lens.ctypes.data, n, num_q_heads, num_kv_heads, num_cus,
+        items.ctypes.data, len(items), merge.ctypes.data, len(merge), counts.ctypes.data,
+    )
+    check(rc, "hy_plan_tree")
+    n_chunks, n_pieces, n_merge, n_slots, max_rows = (int(x) for x in counts)
+    return TreePlan(items[: 2 * n_chunks + n_pieces].copy(), n_chunks, merge[:n_merge].copy(),
+                    n_slots, max_rows)
+
+
+def tree_workspace_bytes(n_slots: int, num_kv_heads: int, head_dim: int) -> int:
+    return int(lib().hy_tree_workspace_bytes(n_slots, num_kv_heads, head_dim))

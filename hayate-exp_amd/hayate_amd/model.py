@@ -202,7 +202,8 @@ class Qwen3Model(nn.Module):
         """token_ids (B, T) on a uniform batch (begin_batch) or (1, N) packed
         tokens on a varlen tick (begin_tick). Returns (logits, None, None):
         logits (B, 1, vocab) of each sequence's last token, as qwen.py:162-165
-        returns for the uniform case."""
+        returns for the uniform case, or (N, 1, vocab) of every node of a
+        drafted-tree tick (begin_tree)."""
         if paged_cache is None:
             raise NotImplementedError("only the paged path is provided (pass paged_cache)")
         if self.cos is None:
@@ -211,9 +212,8 @@ class Qwen3Model(nn.Module):
         for layer_idx, block in enumerate(self.layers):
             x, _, _ = block(x, self.cos, self.sin, None, None, None, None, paged_cache, layer_idx)
         if paged_cache.varlen:
-            # each sequence's last packed token
-            last = paged_cache.q_start[1:].to(torch.long) - 1
-            x = x[0].index_select(0, last).unsqueeze(1)
+            rows = paged_cache.logit_rows()
+            x = (x[0] if rows is None else x[0].index_select(0, rows)).unsqueeze(1)
         else:
             x = x[:, -1:, :]
         if (linear.few_rows(x) and linear.plain(x, norms=(self.norm,), linears=(self.out_head,))

@@ -25,7 +25,9 @@ Data operations need the pool on a HIP device; on any other device they raise
 
 from __future__ import annotations
 
+import contextlib
 import math
+import operator
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -106,6 +108,35 @@ def _stream_handle(device: torch.device) -> int:
                              else device.index)
 
 
+def _index(x, what: str) -> int:
+    """A whole number given as an int (or a type that stands for one)."""
+    try:
+        if isinstance(x, bool):
+            raise TypeError
+        return operator.index(x)
+    except TypeError:
+        raise TypeError(f"{what} must be a whole number, not {x!r}") from None
+
+
+def _int_array(values, what: str) -> np.ndarray:
+    """A 1-D array of whole numbers, from a sequence, an array or a tensor."""
+    if isinstance(values, torch.Tensor):
+        values = values.cpu().numpy()
+    a = np.asarray(values)
+    if a.size == 0 and a.ndim <= 1:
+        return np.zeros(0, dtype=np.int64)
+    if a.ndim != 1 or a.dtype.kind not in "iu":
+        raise TypeError(f"{what} must be a list of whole numbers")
+    return a.astype(np.int64, copy=False)
+
+
+def _current_device(device: torch.device):
+    """Makes `device` current for a launch, which goes to its current stream."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def _require_hip(t: torch.Tensor, what: str) -> None:
     if t.device.type != "cuda":
         raise RuntimeError(
@@ -139,7 +170,9 @@ def _row_strides(t: torch.Tensor, layout: str, q_len: int):
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     st = t.stride()
-    if st[-1] != 1 or t.data_ptr() & 15:
+    if t.data_ptr() & 15:  # contiguous() would return contiguous rows as they are
+        return t.clone(memory_format=torch.contiguous_format)
+    if st[-1] != 1:
         return t.contiguous()
     acc = 0
     for x in st[:-1]:
@@ -226,6 +259,7 @@ class PagedKVBatch:
         varlen: bool,
         num_q_heads: Optional[int],
         tokens_per_split: int = 0,
+        extra: Optional[np.ndarray] = None,
     ):
         self.k_cache = manager.k_cache
         self.v_cache = manager.v_cache
@@ -263,6 +297,8 @@ class PagedKVBatch:
                 np.asarray(cache_lens_host, dtype=np.int32),
                 np.asarray(self.kv_lens_host, dtype=np.int32),
                 q_start,
+                # a subclass's own metadata travels in the same copy
+                *(() if extra is None else (extra,)),
             ]
         )
         meta = torch.from_numpy(self._meta_np).to(self.device)
@@ -271,6 +307,7 @@ class PagedKVBatch:
         self.cache_lens_i32 = meta[n : n + b]
         self.kv_lens = meta[n + b : n + 2 * b]
         self.q_start = meta[n + 2 * b : n + 3 * b + 1]
+        self._extra = meta[n + 3 * b + 1 :]
         self.cache_lens = self.cache_lens_i32.to(torch.long)
         self._meta = meta
         self._pt_ptr = self.page_table.data_ptr()
@@ -374,15 +411,24 @@ class PagedKVBatch:
         a = self._append_inputs("norm_rope_write_layer", q, k, v, q_norm_weight,
                                 k_norm_weight, cos, sin)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
-        rc = _native.lib().hy_qknorm_rope_append(
-            *a.head, float(eps), float(eps if k_eps is None else k_eps), *a.tables,
+        name, at = self._append_call
+        rc = getattr(_native.lib(), name)(
+            *a.head, float(eps), float(eps if k_eps is None else k_eps), *a.tables, *at,
             k_ptr, v_ptr, hs,
             self._q_start_ptr, self._cache_lens_ptr, self._pt_ptr, self._pt_stride,
             self.num_seqs, self.total_tokens, a.num_q_heads, self.num_kv_heads,
             self.head_dim, self.page_size, _stream_handle(self.device),
         )
-        _native.check(rc, "hy_qknorm_rope_append")
+        _native.check(rc, name)
         return a.q_out
+
+    # the append entry point, and what it takes behind the rope tables
+    _append_call: tuple = ("hy_qknorm_rope_append", ())
+
+    def logit_rows(self) -> Optional[torch.Tensor]:
+        """Packed rows whose logits a varlen tick is run for: each sequence's
+        last token."""
+        return self.q_start[1:].to(torch.long) - 1
 
     def _append_inputs(self, what, q, k, v, q_norm_weight, k_norm_weight, cos, sin):
         """Checked, 16-byte-aligned inputs of the fused norm + rope + append
@@ -603,6 +649,142 @@ class PagedKVBatch:
                 num_q_heads, self.num_kv_heads, self.head_dim, stream,
             )
         return result
+
+
+class PagedTreeBatch(PagedKVBatch):
+    """A tick that checks drafted tokens: each request's tokens form a tree.
+
+    Node i of a request with c cached tokens holds slot c + i of its cache, is
+    rotated at position c + depth(i) and sees the c cached tokens, its ancestors and
+    itself, so one forward pass gives every node the states it would have at the end
+    of its own branch. ``parents[b][i]`` is node i's parent, an earlier node of the
+    request, or -1 for a child of the cached context (several nodes may be). A node
+    alone is a decode token. Tensors are packed (tokens, heads, dim) in handle order,
+    as in a ``begin_tick`` batch; ``write_layer``, ``norm_rope_write_layer`` and
+    ``attend_layer`` are called as there. ``positions`` holds each packed node's rope
+    position (int32). No reference counterpart: the reference decodes one token at a
+    time (engine.py:278-289).
+
+    A slot is written before a node that sees it attends; K and V that a node does not
+    see never reach it, whatever their bits. The partials of requests that are cut
+    for the GPU live in the batch's workspace, so calls of one batch, captured ones
+    included, are not run at the same time on two streams.
+    """
+
+    def __init__(self, manager: "PagedKVCacheManager", parents: list[list[int]],
+                 cache_lens_host: list[int], page_lists: list[list[int]],
+                 num_q_heads: Optional[int]):
+        q_lens = [len(p) for p in parents]
+        self.parents = parents
+        self.line_words = -(-max(q_lens) // 32)
+        depths, lines = [], np.zeros((sum(q_lens), self.line_words), dtype=np.uint32)
+        row = 0
+        for tree in parents:
+            first = row
+            for i, p in enumerate(tree):
+                if p >= 0:
+                    lines[row] = lines[first + p]
+                lines[row, i >> 5] |= np.uint32(1 << (i & 31))
+                depths.append(depths[first + p] + 1 if p >= 0 else 0)
+                row += 1
+        positions = np.repeat(np.asarray(cache_lens_host, dtype=np.int32), q_lens)
+        positions += np.asarray(depths, dtype=np.int32)
+        self._tree_plans: dict[int, _DeviceTreePlan] = {}
+        super().__init__(manager, q_lens, cache_lens_host, page_lists, varlen=True,
+                         num_q_heads=None,
+                         extra=np.concatenate([positions, lines.reshape(-1).view(np.int32)]))
+        # every tree goes through the tree kernel, requests with one node included
+        self.decode_only = False
+        self.positions = self._extra[: self.total_tokens]
+        self._lines_ptr = self._extra[self.total_tokens :].data_ptr()
+        self._append_call = ("hy_qknorm_rope_append_at", (self.positions.data_ptr(),))
+        if num_q_heads is not None and self.device.type == "cuda":
+            self.plan(num_q_heads)
+
+    def plan(self, num_q_heads: int) -> "_DeviceTreePlan":
+        """Work lists of this tick (built once per query-head count)."""
+        cached = self._tree_plans.get(num_q_heads)
+        if cached is None:
+            host = _native.plan_tree(
+                np.asarray(self.q_lens, dtype=np.int32),
+                np.asarray(self.kv_lens_host, dtype=np.int32), num_q_heads, self.num_kv_heads,
+                self._num_cus)
+            cached = _DeviceTreePlan(host, self.num_kv_heads, self.head_dim, self.device)
+            self._tree_plans[num_q_heads] = cached
+        return cached
+
+    def logit_rows(self) -> None:
+        """Every node's logits are wanted."""
+        return None
+
+    def attend_layer(
+        self, q: torch.Tensor, layer_idx: int, scale: Optional[float] = None
+    ) -> torch.Tensor:
+        """Attention of every node over its request's cached tokens, its ancestors and
+        itself in this layer's pages: q packed (tokens, Hq, D), returns the same."""
+        _require_hip(q, "attend_layer")
+        q = _aligned_rows(q)
+        if q.dtype != self.k_cache.dtype:
+            raise TypeError("q dtype must match the pool dtype")
+        qs = self._layout(q, "thd")
+        num_q_heads = q.shape[1]
+        if q.shape[2] != self.head_dim:
+            raise ValueError("q head_dim does not match the pool")
+        if q.device != self.device:
+            raise ValueError(f"q is on {q.device}, the pool on {self.device}")
+        if num_q_heads == 0 or num_q_heads % self.num_kv_heads:
+            raise ValueError("query heads must be a multiple of kv heads")
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        plan = self.plan(num_q_heads)
+        out = torch.empty((self.total_tokens, num_q_heads, self.head_dim), dtype=q.dtype,
+                          device=q.device)
+        k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
+        self._launch("hy_paged_tree", _native.lib().hy_paged_tree,
+            q.data_ptr(), *qs, out.data_ptr(), 0, out.stride(0), out.stride(1), k_ptr, v_ptr, hs,
+            self._pt_ptr, self._pt_stride, self._lines_ptr, self.line_words, plan.items_ptr,
+            plan.n_chunks, plan.max_rows, plan.merge_ptr, plan.n_merge, plan.n_slots,
+            plan.workspace_ptr, plan.workspace_bytes, num_q_heads, self.num_kv_heads,
+            self.head_dim, self.page_size, float(scale), _stream_handle(self.device),
+        )
+        return out
+
+    def check_path(self, seq: int, path: Sequence[int]) -> list[int]:
+        """`path` as ints, if it is one: nodes of request `seq` from a child of the
+        cached context down, each the parent of the next (empty: nothing accepted)."""
+        tree, last, nodes = self.parents[seq], -1, []
+        for i in path:
+            i = _index(i, "a node")
+            if not 0 <= i < len(tree) or tree[i] != last:
+                raise ValueError(
+                    f"request {seq}: node {i} does not follow "
+                    + (f"node {last}" if nodes else "the cached context"))
+            nodes.append(i)
+            last = i
+        return nodes
+
+
+class _DeviceTreePlan:
+    """One tree tick's work lists on the device plus its split workspace."""
+
+    def __init__(self, host: "_native.TreePlan", num_kv_heads: int, head_dim: int,
+                 device: torch.device):
+        self.host = host
+        self.n_chunks = host.n_chunks
+        self.n_merge = len(host.merge)
+        self.n_slots = host.n_slots
+        self.max_rows = host.max_rows
+        packed = np.concatenate([host.items.reshape(-1), host.merge.reshape(-1)])
+        self.lists = torch.from_numpy(packed).to(device)
+        self.items_ptr = self.lists.data_ptr()
+        self.merge_ptr = self.items_ptr + 4 * host.items.size if self.n_merge else None
+        self.workspace_bytes = _native.tree_workspace_bytes(self.n_slots, num_kv_heads, head_dim)
+        self.workspace = (
+            torch.empty(self.workspace_bytes // 4, dtype=torch.float32, device=device)
+            if self.workspace_bytes
+            else None
+        )
+        self.workspace_ptr = None if self.workspace is None else self.workspace.data_ptr()
 
 
 class PagedKVCacheManager:
@@ -837,44 +1019,239 @@ class PagedKVCacheManager:
         handle.pages.extend(wanted)
 
     # -------------------------------------------------------------- sharing
-    def fork(self, handle: PagedCacheHandle, length: int | None = None) -> PagedCacheHandle:
+    def fork(self, handle: PagedCacheHandle, length: int | None = None,
+             copy: bool = False) -> PagedCacheHandle:
         """New handle whose first `length` tokens (default: all of them)
         reference the same physical pages, a partly filled last page
         included. Shared pages are read-only; the first append into one (by
-        either handle) copies it."""
+        either handle) copies it. copy=True gives the new handle pages of its own
+        instead, copied in one launch."""
         if handle.released:
             raise RuntimeError("cannot fork a released cache handle")
         if length is None:
             length = handle.length
         if length < 0 or length > handle.length:
             raise ValueError("fork length must be within the current cache length")
-        child = self.allocate()
         shared = handle.pages[: -(-length // self.page_size)]
-        self._ref_pages(shared)
-        child.pages = list(shared)
+        if not copy:
+            child = self.allocate()
+            self._ref_pages(shared)
+            child.pages = list(shared)
+            child.length = length
+            return child
+        if shared:
+            _require_hip(self.k_cache, "fork with copies")
+        child = self.allocate()
+        try:
+            self.reserve(child, length)
+            tokens = [min(self.page_size, length - i * self.page_size) for i in range(len(shared))]
+            self._copy_pages(shared, child.pages, tokens)
+        except Exception:
+            self.release(child)
+            raise
         child.length = length
         return child
 
     def _make_private(self, handle: PagedCacheHandle, start: int, end: int) -> None:
         """Copy-on-write every shared page that positions [start, end) touch."""
-        if end <= start:
-            return
-        first = start // self.page_size
-        last = (end - 1) // self.page_size
-        for idx in range(first, min(last + 1, len(handle.pages))):
-            page = handle.pages[idx]
-            if self._refs[page] <= 1:
+        self._make_all_private([(handle, start, end, handle.length)])
+
+    def _make_all_private(
+        self, spans: Sequence[tuple[PagedCacheHandle, int, int, int]]
+    ) -> None:
+        """Copy-on-write, in one launch, every shared page that the spans (handle,
+        first, end, filled) touch: a copy holds the page's tokens below `filled`.
+        Raises before it changes anything if the pool has no room."""
+        refs: dict[int, int] = {}
+        found = []
+        for handle, start, end, filled in spans:
+            if end <= start:
                 continue
-            _require_hip(self.k_cache, "copy-on-write of a shared page")
-            if not self._free_pages:
-                raise MemoryError("paged KV cache is full: no page for copy-on-write")
-            (new_page,) = self._take_pages(1)
-            lo, hi = page * self.page_size, (page + 1) * self.page_size
-            nlo, nhi = new_page * self.page_size, (new_page + 1) * self.page_size
-            self.k_cache[:, :, :, nlo:nhi].copy_(self.k_cache[:, :, :, lo:hi])
-            self.v_cache[:, :, :, nlo:nhi].copy_(self.v_cache[:, :, :, lo:hi])
+            last = (end - 1) // self.page_size
+            for idx in range(start // self.page_size, min(last + 1, len(handle.pages))):
+                page = handle.pages[idx]
+                shared = refs.get(page, self._refs[page])
+                if shared <= 1:
+                    continue
+                refs[page] = shared - 1  # the last sharer of the batch keeps the page
+                tokens = min(self.page_size, max(0, filled - idx * self.page_size))
+                found.append((handle, idx, page, tokens))
+        if not found:
+            return
+        _require_hip(self.k_cache, "copy-on-write of a shared page")
+        if len(found) > len(self._free_pages):
+            raise MemoryError("paged KV cache is full: no page for copy-on-write")
+        new = self._take_pages(len(found))
+        try:
+            self._copy_pages([page for _, _, page, _ in found], new, [n for *_, n in found])
+        except Exception:
+            self._drop_pages(reversed(new))
+            raise
+        for (handle, idx, page, _), copy in zip(found, new):
             self._refs[page] -= 1
-            handle.pages[idx] = new_page
+            handle.pages[idx] = copy
+
+    # ----------------------------------------------------------- moved data
+    def _copy_pages(self, src: Sequence[int], dst: Sequence[int], tokens: Sequence[int]) -> None:
+        if self.device.type != "cuda":
+            # a pool in host memory, for its bookkeeping: callers that compute refuse it
+            for a, b, n in zip(src, dst, tokens):
+                a, b = a * self.page_size, b * self.page_size
+                for pool in (self.k_cache, self.v_cache):
+                    pool[:, :, :, b : b + n].copy_(pool[:, :, :, a : a + n])
+            return
+        src, dst, tokens = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst, tokens))
+        with _current_device(self.device):
+            rc = _native.lib().hy_page_copy(
+                self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_cache.stride(0),
+                self.k_cache.stride(2), self.num_pages, src.ctypes.data, dst.ctypes.data,
+                tokens.ctypes.data, len(src), self.num_layers, self.num_kv_heads, self.head_dim,
+                self.page_size, _stream_handle(self.device),
+            )
+        _native.check(rc, "hy_page_copy")
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int],
+                   tokens: Optional[Sequence[int]] = None) -> None:
+        """Copy the first tokens[i] tokens (default: all) of page src[i] to page dst[i],
+        K and V of every layer, in one launch. The source pages are in use, the
+        targets owned by one holder each, and no page is both or written twice."""
+        _require_hip(self.k_cache, "copy_pages")
+        a, b = _int_array(src, "src"), _int_array(dst, "dst")
+        if len(a) != len(b):
+            raise ValueError("one target page per source page is required")
+        if tokens is None:
+            n = np.full(len(a), self.page_size)
+        else:
+            n = _int_array(tokens, "tokens")
+            if len(n) != len(a):
+                raise ValueError("one token count per page is required")
+            if len(n) and (n.min() < 0 or n.max() > self.page_size):
+                raise ValueError(f"a page holds 0 to {self.page_size} tokens")
+        for pages in (a, b):
+            if len(pages) and (pages.min() < 0 or pages.max() >= self.num_pages):
+                raise ValueError(f"page ids lie in 0 .. {self.num_pages - 1}")
+        if any(self._refs[p] < 1 for p in a.tolist()):
+            raise ValueError("a source page is not in use")
+        if any(self._refs[p] != 1 for p in b.tolist()):
+            raise ValueError("a target page must have exactly one owner")
+        self._copy_pages(a, b, n)
+
+    def move_tokens(self, handles: Sequence[PagedCacheHandle], sources: Sequence[Sequence[int]],
+                    starts: Sequence[int]) -> None:
+        """Fill positions starts[b], starts[b] + 1, ... of every handle's cache with its
+        tokens at positions sources[b] (ascending, none before the position it fills),
+        K and V of every layer, as if all were read before any is written. Positions
+        may lie past the handle's length, in space reserved for it; lengths do not
+        change. Shared pages that would be written are copied first."""
+        handles = list(handles)
+        _require_hip(self.k_cache, "move_tokens")
+        if len(sources) != len(handles) or len(starts) != len(handles):
+            raise ValueError("one source list and one start per handle is required")
+        if any(h.released for h in handles):
+            raise RuntimeError("cannot move tokens of a released cache handle")
+        if len({id(h) for h in handles}) != len(handles):
+            raise ValueError("the same cache handle is given twice")
+        moves, spans = [], []
+        for h, source, start in zip(handles, sources, starts):
+            src, start = _int_array(source, "sources"), _index(start, "a start")
+            if start < 0:
+                raise ValueError("starts must be non-negative")
+            if not len(src):
+                continue
+            dst = np.arange(start, start + len(src))
+            if (np.diff(src) <= 0).any() or src[0] < start:
+                raise ValueError("sources must ascend, none before the position it fills")
+            if src[-1] >= len(h.pages) * self.page_size:
+                raise ValueError(f"position {src[-1]} is past the cache's reserved space")
+            # ascending on both sides, so the tokens that stay are the first ones
+            stay = int(np.count_nonzero(src == dst))
+            if stay < len(src):
+                moves.append((h, src[stay:], dst[stay:]))
+                spans.append((h, start + stay, start + len(src),
+                              max(h.length, int(src[-1]) + 1)))
+        if not moves:
+            return
+        self._make_all_private(spans)
+        rows = []
+        for h, *ends in moves:
+            pages = np.asarray(h.pages, dtype=np.int64)
+            rows.append([pages[x // self.page_size] * self.page_size + x % self.page_size
+                         for x in ends])
+        src, dst = (np.ascontiguousarray(np.concatenate(x), dtype=np.int32) for x in zip(*rows))
+        with _current_device(self.device):
+            rc = _native.lib().hy_kv_move(
+                self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_cache.stride(0),
+                self.k_cache.stride(2), self.capacity_tokens, src.ctypes.data, dst.ctypes.data,
+                len(src), self.num_layers, self.num_kv_heads, self.head_dim,
+                _stream_handle(self.device),
+            )
+        _native.check(rc, "hy_kv_move")
+
+    def _set_length(self, handle: PagedCacheHandle, length: int) -> None:
+        keep = -(-length // self.page_size)
+        self._drop_pages(handle.pages[keep:])
+        handle.pages = handle.pages[:keep]
+        handle.length = length
+
+    def compact(self, handle: PagedCacheHandle, keep: Sequence[int]) -> None:
+        """Keep only the tokens at positions `keep` (ascending), closed up in every
+        layer, and return the pages that this empties. Keys stay rotated at the positions they
+        were written for."""
+        if handle.released:
+            raise RuntimeError("cannot compact a released cache handle")
+        kept = _int_array(keep, "keep")
+        if len(kept) and (kept[0] < 0 or kept[-1] >= handle.length or (np.diff(kept) <= 0).any()):
+            raise ValueError("keep must be ascending positions within the cache's length")
+        if len(kept) and kept[-1] != len(kept) - 1:
+            self.move_tokens([handle], [kept], [0])
+        self._set_length(handle, len(kept))
+
+    # ---------------------------------------------------------- drafted trees
+    def begin_tree(self, handles: Sequence[PagedCacheHandle],
+                   parents: Sequence[Sequence[int]]) -> PagedTreeBatch:
+        """A tick that checks drafted tokens: one tree per handle, parents[b][i] the
+        parent of node i among the nodes before it, or -1 for a child of the cached
+        context. Reserves a slot per node; commit with ``commit_tree``."""
+        handles = list(handles)
+        self._validate_handles(handles)
+        if len(parents) != len(handles):
+            raise ValueError("one tree per handle is required")
+        most = int(_native.lib().hy_tree_max_nodes())
+        trees = []
+        for tree in parents:
+            tree = _int_array(tree, "a tree's parents").tolist()
+            if not 1 <= len(tree) <= most:
+                raise ValueError(f"a tree has 1 to {most} nodes, not {len(tree)}")
+            if any(not -1 <= p < i for i, p in enumerate(tree)):
+                raise ValueError("a node's parent is an earlier node, or -1")
+            trees.append(tree)
+        self.reserve_tick(handles, [len(t) for t in trees])
+        return PagedTreeBatch(self, trees, [h.length for h in handles],
+                              [list(h.pages) for h in handles], self.num_q_heads)
+
+    def commit_tree(self, handles: Sequence[PagedCacheHandle], batch: PagedTreeBatch,
+                    accepted: Sequence[Sequence[int]]) -> None:
+        """Keep of each handle's tree the nodes accepted[b] (a path from a child of the
+        cached context down, possibly empty): their K and V move to the positions behind the
+        cached tokens in every layer, the length grows by as many and the other nodes'
+        pages are returned."""
+        handles = list(handles)
+        if len(handles) != batch.num_seqs or len(accepted) != batch.num_seqs:
+            raise ValueError("one handle and one path per tree is required")
+        if batch.k_cache is not self.k_cache:
+            raise ValueError("the batch belongs to another pool")
+        if any(h.released for h in handles):
+            raise RuntimeError("cannot commit a released cache handle")
+        if [h.length for h in handles] != batch.cache_lens_host:
+            raise ValueError("a handle is not at the length the batch began with")
+        for h, q in zip(handles, batch.q_lens):
+            if h.length + q > len(h.pages) * self.page_size:
+                raise RuntimeError("paged cache append space was not reserved")
+        paths = [batch.check_path(b, path) for b, path in enumerate(accepted)]
+        self.move_tokens(handles, [[h.length + i for i in path] for h, path in zip(handles, paths)],
+                         [h.length for h in handles])
+        for h, path in zip(handles, paths):
+            self._set_length(h, h.length + len(path))
 
     # ---------------------------------------------------------- tick setup
     def _validate_handles(self, handles: Sequence[PagedCacheHandle]) -> None:
@@ -929,8 +1306,8 @@ class PagedKVCacheManager:
             )
         for h, kv in zip(handles, kv_lengths):
             self.reserve(h, kv)
-        for h, q in zip(handles, q_lens):
-            self._make_private(h, h.length, h.length + q)
+        self._make_all_private([(h, h.length, h.length + q, h.length)
+                                for h, q in zip(handles, q_lens)])
 
     def begin_batch(
         self, handles: Sequence[PagedCacheHandle], query_len: int

@@ -420,6 +420,122 @@ int hy_sample(const void *logits, int64_t row_stride, int32_t dtype,
               int64_t workspace_bytes, void *stream);
 int64_t hy_sample_workspace_bytes(int32_t n_rows, int32_t vocab);
 
+/*
+ * Trees of drafted tokens. A sequence of cache_lens[b] cached tokens and q_len_b
+ * drafted ones (nodes) holds node i in slot cache_lens[b] + i; nodes come in an
+ * order in which every parent precedes its children.
+ *
+ * hy_qknorm_rope_append_at is hy_qknorm_rope_append with the rotation of token tok
+ * (packed index q_start[b] + i) taken at positions[tok] (>= 0, device memory)
+ * instead of the position of its slot: the node's depth in the sequence. A token whose
+ * position is its slot's gets the same bits from both. positions[tok] <
+ * max_positions is the caller's guarantee, as there.
+ * With hayate/model/attention.py:62-75 as the reference for one linear sequence.
+ */
+int hy_qknorm_rope_append_at(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
+    int64_t q_stride_head, void *q_out, int64_t qo_stride_seq,
+    int64_t qo_stride_tok, int64_t qo_stride_head, const void *k,
+    int64_t k_stride_seq, int64_t k_stride_tok, int64_t k_stride_head,
+    const void *v, int64_t v_stride_seq, int64_t v_stride_tok,
+    int64_t v_stride_head, const void *q_norm_weight,
+    const void *k_norm_weight, float q_eps, float k_eps,
+    const float *cos_table,
+    const float *sin_table, int32_t max_positions, const int32_t *positions,
+    void *k_pool, void *v_pool,
+    int64_t pool_head_stride, const int32_t *q_start,
+    const int32_t *cache_lens, const int32_t *page_table,
+    int64_t page_table_stride, int32_t num_seqs, int32_t total_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, void *stream);
+
+/* Nodes of one tree at most (256). */
+int32_t hy_tree_max_nodes(void);
+
+/*
+ * Planner of hy_paged_tree (host only): q_lens[b] >= 1 nodes on kv_lens[b] -
+ * q_lens[b] cached tokens. The (node, query head) rows of a sequence form query
+ * tiles of at most 256 rows per kv head; the 64-key steps of all tiles, in order,
+ * are cut into chunks of equal cost, one per CU and kv head. items:
+ *   n_chunks chunk records int32[16] = {piece_begin, piece_end, n_steps, 0, 0, 0, 0, 0,
+ *   the first piece's record}, then the piece records int32[8] = {seq, q_begin, q_end,
+ *   kv_begin, kv_end, slot, q_row, cache_len}: kv_begin a multiple of 64, slot the
+ *   piece's first 32-row block of partials, -1 for a tile in one piece, which is
+ *   written to out directly; q_row = q_start[seq];
+ * merge_items int32[8] = {seq, q_begin, q_end, first_slot, splits, q_row, blocks a
+ * split, 0}, one per tile in several pieces. A chunk record with n_steps 0 and a merge
+ * record with splits 0 are empty, so both lists can be padded to a fixed launch size
+ * (the piece records then start after all chunk records). item_capacity is in units of
+ * int32[8] (two for a chunk record), at least 3 per chunk and per tile.
+ * counts_out (int32[5]) = {n_chunks, n_pieces, n_merge, n_slots, max_rows}.
+ */
+int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs,
+                 int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
+                 int32_t *items, int32_t item_capacity, int32_t *merge_items,
+                 int32_t merge_capacity, int32_t *counts_out);
+
+/* Bytes of n_slots 32-row blocks of fp32 partials for every kv head. */
+int64_t hy_tree_workspace_bytes(int32_t n_slots, int32_t num_kv_heads,
+                                int32_t head_dim);
+
+/*
+ * Attention of the nodes over their caches: node i of sequence b sees its cached
+ * tokens, its ancestors and itself,
+ *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j,
+ * K and V read through the page table. lines is device memory, line_words 32-bit words
+ * (1 .. 8) for each packed node: bit j of them is set when the node sees drafted slot j.
+ * Slots that no row of a tile sees, and the rest of a page, may hold any bits.
+ * Plan and workspace (hy_tree_workspace_bytes(n_slots), NULL when 0) are those of
+ * hy_plan_tree; max_rows as counted there. One call launches the attention and, when
+ * n_merge > 0, the merge of split tiles. fp32 scores, sums and accumulators; the
+ * probabilities are rounded to bf16 before they meet V, the result once. Rows,
+ * pools and out are 16-byte aligned with strides that are multiples of 8.
+ * No reference counterpart: the reference decodes one token at a time
+ * (hayate/engine/engine.py:278-289).
+ */
+int hy_paged_tree(const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
+                  int64_t q_stride_head, void *out, int64_t o_stride_seq,
+                  int64_t o_stride_tok, int64_t o_stride_head,
+                  const void *k_pool, const void *v_pool,
+                  int64_t pool_head_stride, const int32_t *page_table,
+                  int64_t page_table_stride, const uint32_t *lines,
+                  int32_t line_words, const int32_t *items, int32_t n_chunks,
+                  int32_t max_rows, const int32_t *merge_items, int32_t n_merge,
+                  int32_t n_slots, void *workspace, int64_t workspace_bytes,
+                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                  int32_t page_size, float scale, void *stream);
+
+/*
+ * Token moves: for i in order, pool[l, h, dst[i]] = pool[l, h, src[i]] for every layer
+ * l and kv head h of the K and the V pool. src and dst are host arrays of n physical
+ * tokens (page * page_size + offset), read before the call returns and checked:
+ * indexes below pool_tokens, no token written twice, none read after an earlier
+ * move wrote it (a token may be written after it was read, so a sequence can be moved
+ * forward over itself); otherwise HY_EINVAL and nothing is enqueued. Consecutive moves
+ * of consecutive tokens are taken together.
+ * No reference counterpart (its caches only grow or are cut, paged_cache.py:168-178).
+ */
+int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
+               int64_t pool_head_stride, int64_t pool_tokens,
+               const int32_t *src, const int32_t *dst, int32_t n,
+               int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
+               void *stream);
+
+/*
+ * Page copies: the first tokens[i] tokens (NULL: all) of page src_pages[i] to page
+ * dst_pages[i], in every layer and kv head of the K and the V pool. Host arrays, read
+ * before the call returns and checked: pages below num_pages, no page written twice,
+ * none both read and written; otherwise HY_EINVAL and nothing is enqueued.
+ * Serves the copy-on-write of shared pages, for which the reference copies a whole
+ * cache (paged_cache.py:153-166, prefix_cache.py:72).
+ */
+int hy_page_copy(void *k_pool, void *v_pool, int64_t pool_layer_stride,
+                 int64_t pool_head_stride, int32_t num_pages,
+                 const int32_t *src_pages, const int32_t *dst_pages,
+                 const int32_t *tokens, int32_t n, int32_t num_layers,
+                 int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

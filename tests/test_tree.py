@@ -1,0 +1,334 @@
+"""Drafted trees, token moves and page copies without a GPU: the planner, the
+metadata, the bookkeeping, and what is refused before any device work."""
+
+import ctypes
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from hayate_amd import PagedKVCacheManager, PagedTreeBatch, _native
+from tree_util import chain, depth, line, wide_tree
+
+
+def pool(pages=12, page=128, layers=1, slots=6):
+    return PagedKVCacheManager(layers, 8, 128, pages * page, page, slots, torch.bfloat16, "cpu",
+                               num_q_heads=32)
+
+
+def handle(m, length):
+    h = m.allocate()
+    m.reserve(h, length)
+    h.length = length
+    return h
+
+
+# ----------------------------------------------------------------- planner
+def check_plan(q_lens, kv_lens, hq=32, hkv=8, cus=256):
+    """Every (tile, key step) of every request is in one piece of one chunk, pieces keep to the
+    page table's range, and partials do not overlap."""
+    q, kv = np.asarray(q_lens), np.asarray(kv_lens)
+    p = _native.plan_tree(q, kv, hq, hkv, cus)
+    group = hq // hkv
+    chunks = p.items[: 2 * p.n_chunks].reshape(-1, 16)
+    pieces = p.items[2 * p.n_chunks :]
+    assert 1 <= p.n_chunks <= -(-cus // hkv)
+    assert chunks[0, 0] == 0 and chunks[-1, 1] == len(pieces)
+    assert (chunks[1:, 0] == chunks[:-1, 1]).all() and (chunks[:, 1] > chunks[:, 0]).all()
+    steps = -(-(pieces[:, 4] - pieces[:, 3]) // 64)
+    assert (steps > 0).all()
+    for ch in chunks:
+        assert ch[2] == steps[ch[0] : ch[1]].sum()
+        assert (ch[8:] == pieces[ch[0]]).all()
+    starts = np.concatenate([[0], np.cumsum(q)])
+    at, used, merged, rows = 0, [], {}, 0
+    for m in p.merge:
+        merged[int(m[0]), int(m[1])] = m
+    for b in range(len(q)):
+        node = 0
+        while node < q[b]:
+            seq, q0, q1 = pieces[at, :3]
+            assert seq == b and q0 == node and node < q1 <= q[b]
+            assert (q1 - q0) * group <= 256
+            rows = max(rows, (q1 - q0) * group)
+            blocks = -(-int(q1 - q0) * group // 32)
+            end, key, first = kv[b] - q[b] + q1, 0, at
+            while key < end:
+                r = pieces[at]
+                assert tuple(r[:3]) == (seq, q0, q1) and r[3] == key and key < r[4] <= end
+                assert r[3] % 64 == 0 and (r[4] % 64 == 0 or r[4] == end)
+                assert r[6] == starts[b] and r[7] == kv[b] - q[b]
+                key = r[4]
+                at += 1
+            if at == first + 1:
+                assert pieces[first, 5] == -1 and (seq, q0) not in merged
+            else:
+                m = merged.pop((int(seq), int(q0)))
+                assert m[2] == q1 and m[4] == at - first and m[5] == starts[b] and m[6] == blocks
+                for i in range(first, at):
+                    assert pieces[i, 5] == m[3] + (i - first) * blocks
+                    used += range(pieces[i, 5], pieces[i, 5] + blocks)
+            node = q1
+    assert at == len(pieces) and not merged
+    assert sorted(used) == list(range(p.n_slots)) and p.max_rows == rows
+    cost = chunks[:, 2] + (chunks[:, 1] - chunks[:, 0] - 1)
+    return p, cost
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_plan_covers_everything_once(seed):
+    rng = np.random.default_rng(seed)
+    n = int(rng.integers(1, 60))
+    q = rng.integers(1, int(rng.choice([2, 30, 257])), size=n)
+    kv = q + rng.integers(0, int(rng.choice([2, 500, 20000])), size=n)
+    for hq, hkv in ((32, 8), (8, 8), (16, 1), (64, 4)):
+        check_plan(q, kv, hq, hkv)
+
+
+def test_plan_shares_the_steps_evenly():
+    rng = np.random.default_rng(3)
+    q = rng.integers(4, 20, size=20)
+    _, cost = check_plan(q, q + rng.integers(200, 4000, size=20))
+    assert len(cost) == 32 and cost.max() <= cost.mean() + 2
+    _, cost = check_plan([64] * 8, [32064] * 8)
+    assert len(cost) == 32 and cost.max() - cost.min() <= 1
+
+
+def test_plan_of_small_work_and_few_units():
+    p, _ = check_plan([1], [1])
+    assert p.n_chunks == 1 and not len(p.merge) and p.n_slots == 0
+    check_plan([256] * 3, [256] * 3, 128, 8)
+    check_plan([5] * 300, [6] * 300)
+    check_plan([5, 9], [500, 700], cus=1)
+    check_plan([5, 9], [500, 700], 64, 64, cus=8)
+
+
+def test_plan_refusals():
+    def call(q, kv, hq=32, hkv=8, items=1000, merges=1000):
+        q, kv = np.asarray(q, dtype=np.int32), np.asarray(kv, dtype=np.int32)
+        a, b = np.zeros((items, 8), np.int32), np.zeros((merges, 8), np.int32)
+        c = np.zeros(5, np.int32)
+        return _native.lib().hy_plan_tree(q.ctypes.data, kv.ctypes.data, len(q), hq, hkv, 256,
+                                          a.ctypes.data, items, b.ctypes.data, merges, c.ctypes.data)
+
+    assert call([3], [10]) == _native.HY_OK
+    assert call([0], [10]) == _native.HY_EINVAL
+    assert call([11], [10]) == _native.HY_EINVAL
+    assert call([257], [300]) == _native.HY_EUNSUPPORTED
+    assert call([3], [10], hq=24) == _native.HY_EUNSUPPORTED
+    assert call([3], [10], hq=30) == _native.HY_EINVAL
+    assert call([3], [10000], items=4) == _native.HY_ENOSPACE
+    assert call([3], [10000], merges=0) == _native.HY_ENOSPACE
+
+
+# ---------------------------------------------------------------- metadata
+@pytest.mark.parametrize("sizes", [[1], [3, 40], [256, 1, 33]])
+def test_batch_metadata(sizes):
+    rng = random.Random(sum(sizes))
+    trees = [wide_tree(rng, n) for n in sizes]
+    m = pool(pages=20)
+    handles = [handle(m, rng.randint(1, 300)) for _ in sizes]
+    batch = m.begin_tree(handles, trees)
+    assert isinstance(batch, PagedTreeBatch) and batch.varlen and not batch.decode_only
+    assert batch.logit_rows() is None
+    words = batch.line_words
+    assert words == -(-max(sizes) // 32)
+    lines = batch._extra[batch.total_tokens :].numpy().view(np.uint32).reshape(-1, words)
+    row = 0
+    for h, tree in zip(handles, trees):
+        assert len(h.pages) == -(-(h.length + len(tree)) // 128)
+        for i in range(len(tree)):
+            assert batch.positions[row] == h.length + depth(tree, i)
+            got = [j for j in range(32 * words) if lines[row, j >> 5] >> (j & 31) & 1]
+            assert got == line(tree, i)
+            row += 1
+
+
+def test_begin_tree_refusals_change_nothing():
+    m = pool()
+    a, b = handle(m, 100), handle(m, 20)
+    free = m.free_page_count
+    for trees in ([[-1]], [[-1], []], [[-1], [0]], [[-1], [-1, 1]], [[-1], [-1, -2]],
+                  [[-1], chain(257)]):
+        with pytest.raises(ValueError):
+            m.begin_tree([a, b], trees)
+    for trees in ([[-1], [-1.0]], [[-1], [None]], [[-1], [[-1]]], [[-1], "ab"], [[-1], [True]]):
+        with pytest.raises(TypeError):
+            m.begin_tree([a, b], trees)
+    with pytest.raises(ValueError):
+        m.begin_tree([a, a], [[-1], [-1]])
+    with pytest.raises(ValueError):
+        m.begin_tree([], [])
+    m.release(b)
+    with pytest.raises(RuntimeError):
+        m.begin_tree([a, b], [[-1], [-1]])
+    big = handle(m, m.free_page_count * 128)
+    with pytest.raises(MemoryError):
+        m.begin_tree([a, big], [chain(10), chain(10)])
+    m.release(big)
+    assert m.free_page_count == free + 1 and len(a.pages) == 1
+
+
+def test_paths():
+    m = pool()
+    tree = [-1, 0, 0, 1, -1, 4]
+    batch = m.begin_tree([handle(m, 5)], [tree])
+    assert batch.check_path(0, []) == []
+    assert batch.check_path(0, np.array([0, 1, 3])) == [0, 1, 3]
+    assert batch.check_path(0, [4, 5]) == [4, 5]
+    for bad in ([1], [0, 3], [0, 1, 2], [6], [-1], [0, 0]):
+        with pytest.raises(ValueError):
+            batch.check_path(0, bad)
+    with pytest.raises(TypeError):
+        batch.check_path(0, [0.0])
+
+
+def test_commit_tree_without_moves_is_bookkeeping(monkeypatch):
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    m = pool()
+    a, b = handle(m, 100), handle(m, 250)
+    batch = m.begin_tree([a, b], [chain(40), chain(10)])
+    assert [len(h.pages) for h in (a, b)] == [2, 3]
+    free = m.free_page_count
+    with pytest.raises(ValueError):
+        m.commit_tree([a], batch, [[0]])
+    with pytest.raises(ValueError):
+        m.commit_tree([a, b], batch, [[0], [1]])
+    with pytest.raises(ValueError):
+        m.commit_tree([b, a], batch, [[0], [0]])
+    with pytest.raises(ValueError):
+        pool().commit_tree([a, b], batch, [[0], [0]])
+    assert (a.length, b.length) == (100, 250)
+    m.commit_tree([a, b], batch, [[0, 1, 2], range(8)])
+    assert (a.length, b.length) == (103, 258)
+    assert [len(h.pages) for h in (a, b)] == [1, 3] and m.free_page_count == free + 1
+    with pytest.raises(ValueError):  # committed already
+        m.commit_tree([a, b], batch, [[0], [0]])
+
+
+# ------------------------------------------------------------ moves, copies
+def test_data_operations_need_a_gpu():
+    m = pool()
+    h = handle(m, 300)
+    with pytest.raises(RuntimeError):
+        m.move_tokens([h], [[5]], [1])
+    with pytest.raises(RuntimeError):
+        m.copy_pages([h.pages[0]], [h.pages[1]])
+    with pytest.raises(RuntimeError):
+        m.fork(h, copy=True)
+    with pytest.raises(RuntimeError):
+        m.compact(h, [3])
+    assert h.length == 300 and len(h.pages) == 3 and m.free_page_count == 9
+
+
+def test_move_and_copy_refusals(monkeypatch):
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    m = pool()
+    h, g = handle(m, 300), handle(m, 128)
+    for src, start in (([5, 5], 0), ([5, 4], 0), ([5], 6), ([384], 0), ([-1], 0), ([3], -1),
+                       ([2, 3], 3)):
+        with pytest.raises(ValueError):
+            m.move_tokens([h], [src], [start])
+    for src, start in (([5.0], 0), ([[5]], 0), (["a"], 0), ([5], 0.5), ([5], True)):
+        with pytest.raises(TypeError):
+            m.move_tokens([h], [src], [start])
+    with pytest.raises(ValueError):
+        m.move_tokens([h, h], [[5], [6]], [0, 0])
+    with pytest.raises(ValueError):
+        m.move_tokens([h], [[5], [6]], [0])
+    m.move_tokens([], [], [])
+    m.move_tokens([h], [[]], [0])
+    m.move_tokens([h], [[7, 8]], [7])
+    for src, dst, n in (([0], [0, 1], None), ([99], [g.pages[0]], None), ([-1], [g.pages[0]], None),
+                        ([h.pages[0]], [12], None), (h.pages[:1], g.pages, [129]),
+                        (h.pages[:1], g.pages, [-1]), (h.pages[:1], g.pages, [1, 2]),
+                        (h.pages[:1], [m._free_pages[-1]], None), ([m._free_pages[-1]], g.pages, None)):
+        with pytest.raises(ValueError):
+            m.copy_pages(src, dst, n)
+    child = m.fork(h)
+    with pytest.raises(ValueError):  # a shared page is not written
+        m.copy_pages(g.pages, h.pages[:1])
+    for keep in ([300], [-1], [4, 4], [5, 4]):
+        with pytest.raises(ValueError):
+            m.compact(h, keep)
+    m.release(child)
+    m.compact(h, range(130))
+    assert h.length == 130 and len(h.pages) == 2
+    m.release(g)
+    for call in (lambda: m.move_tokens([g], [[1]], [0]), lambda: m.compact(g, []),
+                 lambda: m.fork(g, copy=True)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def c_arrays(*lists):
+    return [(ctypes.c_int32 * max(1, len(x)))(*x) for x in lists]
+
+
+@pytest.mark.parametrize("src,dst", [([0, 1], [5, 5]), ([0, 5], [5, 6]), ([-1], [3]), ([3], [-1]),
+                                     ([1000], [3]), ([3], [1000]), ([2, 1], [1, 0])])
+def test_c_moves_are_checked_before_any_launch(src, dst):
+    lib = _native.lib()
+    a, b = c_arrays(src, dst)
+    call = lambda **kw: lib.hy_kv_move(4096, 4096, 8 * 1000 * 128, 1000 * 128, 1000, a, b,  # noqa: E731
+                                       len(src), kw.get("layers", 2), 8, kw.get("dim", 128), None)
+    assert call() == _native.HY_EINVAL and _native.last_error()
+    assert call(layers=0) == _native.HY_EINVAL
+    assert call(dim=64) == _native.HY_EUNSUPPORTED
+
+
+def test_c_pools_are_checked():
+    lib = _native.lib()
+    a, b = c_arrays([1], [0])
+    good = [4096, 4096, 8 * 1000 * 128, 1000 * 128, 1000, a, b, 1, 2, 8, 128, None]
+    for at, bad in ((0, None), (1, None), (0, 4098), (2, 1000 * 128), (3, 128), (3, 1000 * 128 + 4),
+                    (4, 0), (4, 1 << 31), (5, None), (6, None), (7, -1), (9, 0)):
+        args = list(good)
+        args[at] = bad
+        assert lib.hy_kv_move(*args) == _native.HY_EINVAL, (at, bad)
+    assert lib.hy_kv_move(*good[:7], 0, *good[8:]) == _native.HY_OK  # nothing to move
+    # a token that stays is no write: reading it afterwards is allowed, so only the range is at fault
+    a, b = c_arrays([1, 1, 2000], [1, 0, 3])
+    assert lib.hy_kv_move(*good[:5], a, b, 3, *good[8:]) == _native.HY_EINVAL
+    assert "move 2" in _native.last_error()
+
+
+@pytest.mark.parametrize("src,dst,tokens", [([0, 1], [2, 2], None), ([0, 1], [1, 2], None),
+                                            ([3], [3], None), ([-1], [0], None), ([0], [8], None),
+                                            ([0], [1], [129]), ([0], [1], [-1])])
+def test_c_copies_are_checked_before_any_launch(src, dst, tokens):
+    lib = _native.lib()
+    a, b, t = c_arrays(src, dst, tokens or [])
+    assert lib.hy_page_copy(4096, 4096, 8 * 1024 * 128, 1024 * 128, 8, a, b, t if tokens else None,
+                            len(src), 2, 8, 128, 128, None) == _native.HY_EINVAL
+    assert _native.last_error()
+
+
+def test_c_tree_attention_is_checked():
+    lib = _native.lib()
+    good = dict(q=4096, qs=0, qt=4096, qh=128, out=4096, os=0, ot=4096, oh=128, k=4096, v=4096,
+                hs=128 * 1000, pt=4096, pts=4, lines=4096, words=1, items=4096, chunks=1, rows=32,
+                merge=None, merges=0, slots=0, ws=None, wsb=0, hq=32, hkv=8, dim=128, page=128,
+                scale=0.1, stream=None)
+
+    def call(**kw):
+        args = {**good, **kw}
+        return lib.hy_paged_tree(*args.values())
+
+    for kw in (dict(scale=0.0), dict(scale=float("nan")), dict(hq=30), dict(chunks=-1),
+               dict(chunks=65536), dict(rows=0), dict(rows=257), dict(words=0), dict(words=9),
+               dict(q=None), dict(out=None), dict(k=None), dict(v=None), dict(pt=None),
+               dict(lines=None), dict(items=None), dict(merges=1, slots=2, ws=4096, wsb=1 << 30),
+               dict(q=4098), dict(qh=100), dict(ot=4), dict(hs=1001)):
+        assert call(**kw) == _native.HY_EINVAL, kw
+    for kw in (dict(dim=64), dict(page=96), dict(page=16), dict(hq=24), dict(hq=256)):
+        assert call(**kw) == _native.HY_EUNSUPPORTED, kw
+    assert call(slots=2) == _native.HY_ENOSPACE
+    assert call(chunks=0) == _native.HY_OK
+    assert lib.hy_tree_workspace_bytes(0, 8, 128) == 0
+    assert lib.hy_tree_workspace_bytes(3, 8, 128) == 3 * 8 * 32 * (128 + 2) * 4
