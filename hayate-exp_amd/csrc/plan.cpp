@@ -602,7 +602,12 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
     ch[0] = first;
     ch[1] = ends[i];
     ch[2] = n;
-    for (int j = 3; j < 8; ++j) ch[j] = 0;
+    ch[3] = 1;
+    for (int32_t p = first; p < ends[i]; ++p) {
+      const Tile &t = tiles[pieces[p].tile];
+      if (t.q1 - t.q0 < q_lens[t.seq]) ch[3] = 0;
+    }
+    for (int j = 4; j < 8; ++j) ch[j] = 0;
     for (int j = 0; j < 8; ++j) ch[8 + j] = rec[8 * first + j];
   }
   counts_out[0] = static_cast<int32_t>(ends.size());

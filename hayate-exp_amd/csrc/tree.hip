@@ -24,7 +24,9 @@
 // to bf16 for the second product, the matrix core's input type.
 //
 // Only the blocks that hold drafted slots are masked: a node's line is a bit mask
-// over the slots, kept in LDS per row.
+// over the slots, loaded to LDS with the rows of Q.
+
+#include <type_traits>
 
 #include "hy_common.h"
 #include "tree_shape.h"
@@ -39,27 +41,66 @@ constexpr int kTile = kTreeTileKeys;
 constexpr int kStage = 2 * kTile * kHeadDim;  // halfs per stage: K tile, then V tile
 constexpr int kStages = 4;
 constexpr int kMaskWords = kTreeMaxNodes / 32;
-constexpr int kMaskStride = kMaskWords + 1;  // a zero word behind, and rows on other banks
+
+// Instruction classes for __builtin_amdgcn_sched_group_barrier.
+constexpr int kSchedMfma = 0x008;
+constexpr int kSchedValu = 0x002 | 0x400;  // VALU incl. transcendentals
+constexpr int kSchedDsRead = 0x100;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ s16x4 tr_read(const uint16_t *p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(const_cast<uint16_t *>(p)));
 }
 
-// 16 bytes from base + off (bytes) straight into LDS: lane l's land at lds + 16 l
+// 16 bytes from each lane's own address straight into LDS: lane l's land at lds + 16 l
 // (lds wave-uniform, through M0, with the wait state the ISA asks for between
 // its write and the load). The caller waits (wait_loads) before it reads them.
-__device__ __forceinline__ void load_to_lds(const uint16_t *base, uint32_t off,
-                                            const uint16_t *lds) {
+// Four of them with the instruction's offset, which counts on both sides: 4 KiB (16 rows)
+// from rows + off[i] + 1024 i to lds + 1024 i + 16 l, for one M0. kStream:
+// nontemporal, for lines that no other workgroup reads.
+template <bool kStream>
+__device__ __forceinline__ void load_rows_to_lds(const uint16_t *rows, const uint32_t (&off)[4],
+                                                 const uint16_t *lds) {
+  // wave-uniform, and held in scalar registers
+  const uint64_t at = reinterpret_cast<uintptr_t>(rows);
+  const uint64_t base =
+      static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32))) << 32 |
+      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)));
   const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (const __attribute__((address_space(3))) uint16_t *)lds));
-  __asm__ volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+  if constexpr (kStream)
+    __asm__ volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %4 nt\n\t"
+        "global_load_lds_dwordx4 %1, %4 offset:1024 nt\n\t"
+        "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:3072 nt"
+        :
+        : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base),
+          "s"(__builtin_amdgcn_readfirstlane(m0))
+        : "memory");
+  else
+    __asm__ volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %4\n\t"
+        "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+        "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:3072"
+        :
+        : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base),
+          "s"(__builtin_amdgcn_readfirstlane(m0))
+        : "memory");
+}
+
+__device__ __forceinline__ void load_to_lds(const uint16_t *g, const uint16_t *lds) {
+  const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (const __attribute__((address_space(3))) uint16_t *)lds));
+  __asm__ volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                    :
-                   : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0))
+                   : "v"(g), "s"(__builtin_amdgcn_readfirstlane(m0))
                    : "memory");
 }
 
@@ -83,6 +124,21 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Every wave's LDS accesses before it are done (LDS only: loads in flight stay so).
+__device__ __forceinline__ void barrier() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __asm__ volatile("" ::: "memory");
+}
+
+// x, opaquely: what is computed from it in a rare branch is not kept in registers across
+// the loop around it.
+__device__ __forceinline__ int here(int x) {
+  __asm__ volatile("" : "+v"(x));
+  return x;
+}
+
 struct Piece {
   int seq, q0, q1, kv0, kv1, slot, q_row, cache;
   __device__ __forceinline__ int tiles() const { return (kv1 - kv0 + kTile - 1) / kTile; }
@@ -92,8 +148,12 @@ __device__ __forceinline__ Piece load_piece(const int32_t *r) {
   return Piece{r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};
 }
 
-template <int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W > 4 ? 2 : 1, W > 4 ? 2 : 1)))
+// RW waves side by side hold 32 rows each; KS of them hold the same rows and share the
+// 32-key blocks of a tile (KS == 2: one block each). LW more waves do nothing but load; with
+// LW == 0 the others load as well.
+template <int RW, int KS, int LW>
+__global__ __launch_bounds__(64 * (RW * KS + LW))
+    __attribute__((amdgpu_waves_per_eu(RW * KS + LW > 4 ? 2 : 1, RW * KS + LW > 4 ? 2 : 1)))
 void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
                  uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
                  const uint16_t *__restrict__ k_pool, const uint16_t *__restrict__ v_pool,
@@ -102,17 +162,26 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
                  const uint32_t *__restrict__ lines, int line_words, float *__restrict__ ws_acc,
                  float *__restrict__ ws_ml, int n_slots, int group_shift, int page_shift,
                  float scale_log2) {
-  constexpr int kLoads = 32 / W;  // load instructions of a wave per tile
+  constexpr int W = RW * KS + LW;
+  constexpr int kLoaders = LW > 0 ? LW : W;
+  constexpr int kLoads = 32 / kLoaders;       // load instructions of a loading wave per stage
+  constexpr int kQStages = (RW + 3) / 4;      // 128 rows a stage
+  constexpr int kLineWords = kLoaders * 256;  // one load instruction of every loading wave
+  static_assert(kLineWords >= RW * 32 * kMaskWords, "a line for every row");
   __shared__ __attribute__((aligned(1024))) uint16_t ring[kStages * kStage];
-  __shared__ uint32_t line[W * 32 * kMaskStride];
+  // A piece has two stages at least, so the one issued three stages ahead belongs at most to
+  // the piece after the next.
+  __shared__ __attribute__((aligned(1024))) uint32_t line[3][kLineWords];
+  __shared__ float2 other_ml[RW * 32];
+  __shared__ uint32_t sick[kMaskWords];  // drafted slots with an infinity or NaN in V
 
   const int32_t *ch = items + kTreeChunkInts * blockIdx.y;
   const int32_t *pieces = items + kTreeChunkInts * n_chunks;
   const int kvh = blockIdx.x;
   const int p_end = ch[1];
-  const int n_tiles = ch[2];
   // an empty chunk record pads a list to a fixed launch size
-  if (n_tiles <= 0) return;
+  if (ch[2] <= 0) return;
+  const int n_stages = ch[2] + kQStages * (p_end - ch[0]);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -124,63 +193,134 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   const uint16_t *kh = k_pool + kvh * pool_hs;
   const uint16_t *vh = v_pool + kvh * pool_hs;
 
-  // ---- tile loads -------------------------------------------------------
-  // Issue cursor: the piece holding the next tile to load. A tile's two
-  // 32-key halves each lie in one page (pages hold at least 32 keys, pieces
-  // start at multiples of 64). Keys past the piece are read from its last page:
-  // in bounds, and masked.
+  // ---- stage loads ------------------------------------------------------
+  // Issue cursor: the piece of the next stage to load, and the stage's step in it:
+  // -kQStages .. -1 its rows of Q (and, with the first, their lines), then its tiles.
+  // A tile's two 32-key halves each lie in one page (pages hold at least 32 keys, pieces
+  // start at multiples of 64). Keys past the piece are read from its last page: in
+  // bounds, and masked.
   Piece ip = load_piece(ch + 8);
-  int ip_index = ch[0], ip_tile = 0;  // its record, and its first tile in the chunk
-  struct Tile {
-    uint32_t page[2];
-    int key;
-  };
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    while (t >= ip_tile + ip.tiles()) {
-      ip_tile += ip.tiles();
-      ip = load_piece(pieces + 8 * ++ip_index);
-    }
-    Tile x;
-    x.key = ip.kv0 + kTile * (t - ip_tile);
+  int ip_index = ch[0], ip_step = -kQStages;
+  uint32_t page0 = 0, page1 = 0;
+  auto fetch = [&]() __attribute__((always_inline)) {
+    if (ip_step < 0) return;
     const int32_t *pt = page_table + ip.seq * pt_stride;
+    const int key = ip.kv0 + kTile * ip_step;
     // held unsigned: page ids are non-negative, and widen without a sign
-    x.page[0] = static_cast<uint32_t>(pt[x.key >> page_shift]);
-    x.page[1] = static_cast<uint32_t>(pt[min(x.key + 32, ip.kv1 - 1) >> page_shift]);
-    return x;
+    page0 = static_cast<uint32_t>(pt[key >> page_shift]);
+    page1 = static_cast<uint32_t>(pt[min(key + 32, ip.kv1 - 1) >> page_shift]);
   };
-  // The layouts of the prefill kernel, conflict-free for the reads below; in
-  // units of 8 dims: K unit(row, chunk) = (row / 16) * 256 + (chunk / 4) * 64 +
-  // (row % 16) * 4 + (chunk % 4 ^ row / 4 % 4), V unit(row, chunk) = (row / 4) *
-  // 64 + (chunk / 4) * 16 + (row % 4) * 4 + chunk % 4. K instruction i loads 16
-  // rows (16 (i / 4) ..) of four chunks, V instruction i four whole rows.
-  const uint32_t k_off = 256 * (lane >> 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
-  const uint32_t v_off = 256 * ((lane >> 2) & 3) + 64 * (lane >> 4) + 16 * (lane & 3);
-  auto issue = [&](const Tile &x, int t) __attribute__((always_inline)) {
-    uint16_t *dst = ring + (t % kStages) * kStage;
-#pragma unroll
-    for (int j = 0; j < kLoads / 2; ++j) {
-      const int i = wave * (kLoads / 2) + j;
-      const int half = i >> 3;
-      const int64_t row = (static_cast<int64_t>(half ? x.page[1] : x.page[0]) << page_shift) +
-                          ((x.key + 32 * half) & page_mask);
-      load_to_lds(kh + row * kHeadDim + 2048 * ((i >> 2) & 1) + 32 * (i & 3), k_off, dst + 512 * i);
-      load_to_lds(vh + row * kHeadDim + 512 * (i & 7), v_off, dst + kTile * kHeadDim + 512 * i);
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (++ip_step == ip.tiles()) {
+      ip = load_piece(pieces + 8 * ++ip_index);
+      ip_step = -kQStages;
     }
+    fetch();
+  };
+  // Both tiles keep the rows' order, four to a KiB, so that one load instruction takes four whole
+  // rows and its offset serves both sides; within, in units of 8 dims, unit(row, chunk) =
+  // (row / 4) * 64 + (chunk / 4) * 16 + (row % 4) * 4 + x with x = chunk % 4 in a V tile and
+  // chunk % 4 ^ row / 4 % 4 in a K tile (and for Q): the operand reads below are then
+  // free of bank conflicts, and four neighbouring lanes load 64 bytes of a row.
+  const int loader = LW > 0 ? wave - RW * KS : wave;
+  // whether no other chunk reads this chunk's keys for other rows
+  const bool alone = ch[3] != 0;
+  auto issue_tile = [&](auto stream, uint16_t *dst, int lane_) __attribute__((always_inline)) {
+    constexpr bool kStream = decltype(stream)::value;
+    const int key = ip.kv0 + kTile * ip_step;
+    const uint32_t row_off = 256 * ((lane_ >> 2) & 3) + 64 * (lane_ >> 4);
+    const uint32_t v_off[4] = {row_off + 16 * (lane_ & 3), row_off + 16 * (lane_ & 3),
+                               row_off + 16 * (lane_ & 3), row_off + 16 * (lane_ & 3)};
+    const uint32_t k_off[4] = {v_off[0], row_off + 16 * ((lane_ & 3) ^ 1),
+                               row_off + 16 * ((lane_ & 3) ^ 2), row_off + 16 * ((lane_ & 3) ^ 3)};
+    // groups of 16 rows: four of K, then four of V
+#pragma unroll
+    for (int j = 0; j < 8 / kLoaders; ++j) {
+      const int g = loader + kLoaders * j;
+      // its rows' page; picked by bits, as a choice by address would put both in memory, and a
+      // read from there waits for every load in flight
+      const uint32_t page = page0 ^ ((page0 ^ page1) & (0u - ((g >> 1) & 1u)));
+      const int64_t row = (static_cast<int64_t>(page) << page_shift) +
+                          ((key + 16 * (g & 3)) & page_mask);
+      if (g < 4)
+        load_rows_to_lds<kStream>(kh + row * kHeadDim, k_off, dst + 2048 * g);
+      else
+        load_rows_to_lds<kStream>(vh + row * kHeadDim, v_off, dst + 2048 * g);
+    }
+  };
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    if (LW > 0 && loader < 0) return;
+    uint16_t *dst = ring + (stage % kStages) * kStage;
+    const int lane_ = here(lane);
+    if (ip_step < 0) {
+      // rows past the piece's are read from its first node, and zeroed on use
+      const int row0 = 128 * (ip_step + kQStages);
+      const uint16_t *base = q + ip.seq * q_ss + static_cast<int64_t>(ip.q_row) * q_st;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int i = loader * kLoads + j;
+        const int row = row0 + 4 * i + ((lane_ >> 2) & 3);
+        const int tok = ip.q0 + (row >> group_shift);
+        load_to_lds(base + (tok < ip.q1 ? tok : ip.q0) * q_st + (h0 + (row & group_mask)) * q_sh +
+                        32 * (lane_ >> 4) + 8 * ((lane_ & 3) ^ (i & 3)),
+                    dst + 512 * i);
+      }
+      if (ip_step == -kQStages) {
+        const int last = (ip.q1 - ip.q0) * line_words - 4;
+        load_to_lds(reinterpret_cast<const uint16_t *>(
+                        lines + static_cast<int64_t>(ip.q_row + ip.q0) * line_words +
+                        min(256 * loader + 4 * lane_, last)),
+                    reinterpret_cast<uint16_t *>(line[ip_index % 3] + 256 * loader));
+      }
+      return;
+    }
+    if (alone)
+      issue_tile(std::true_type{}, dst, lane_);
+    else
+      issue_tile(std::false_type{}, dst, lane_);
   };
 
   // ---- this wave's rows of the piece being computed ----------------------
   Piece cp = ip;
-  int cp_index = ip_index, cp_tile = 0;
-  const int r = 32 * wave + c;
+  const uint32_t *own_line = line[0];
+  const int rw = wave % RW;
+  const int ks = wave / RW;
+  const int r = 32 * rw + c;
   bool wave_live = false, live = false;
-  bf16x8 qop[8];  // row c of Q^T
+  bf16x8 qop[2][4];  // row c of Q^T
   f32x16 acc[4];  // O^T[32 db + 8 (i / 4) + 4 h + i % 4][row c]
-  float base, shift, l_run;
-  uint32_t *row_line = line + r * kMaskStride;
+  float base = -INFINITY, shift = 0.f, l_run = 0.f;
+
+  // LDS read bases (u16 units).
+  const int r16 = lane & 15;
+  const int q16 = lane >> 4;
+  int k_base[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    k_base[i] = (c >> 2) * 512 + (c & 3) * 32 + 8 * ((2 * i + h) ^ ((c >> 2) & 3));
+  const int v_base = kTile * kHeadDim + 512 * (q16 >> 1) + 32 * (r16 >> 2) + 16 * (q16 & 1) +
+                     4 * (r16 & 3);
+  // Dims 64 half .. 64 half + 63 of 32 rows of K or Q, as the first product's operands.
+  auto read_rows = [&](bf16x8(&x)[4], const uint16_t *rows, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      x[kk] = *reinterpret_cast<const bf16x8 *>(rows + k_base[kk & 1] + 128 * (2 * half + (kk >> 1)));
+  };
+  auto scores = [&](f32x16 &s, const bf16x8(&kop)[4], int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[kk], qop[half][kk], s, 0, 0, 0);
+  };
+  auto first_scores = [&](f32x16 &s, const uint16_t *rows) __attribute__((always_inline)) {
+    s = f32x16{};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      bf16x8 kop[4];
+      read_rows(kop, rows, half);
+      scores(s, kop, half);
+    }
+  };
   auto start = [&]() __attribute__((always_inline)) {
-    const int rows = (cp.q1 - cp.q0) << group_shift;
-    wave_live = 32 * wave < rows;
-    live = r < rows;
     base = -INFINITY;
     shift = 0.f;
     l_run = 0.f;
@@ -188,115 +328,42 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
     for (int db = 0; db < 4; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
-    if (!wave_live) return;
-    const int64_t tok = cp.q_row + cp.q0 + (live ? r >> group_shift : 0);
-    const uint16_t *src = q + cp.seq * q_ss + tok * q_st + (h0 + (r & group_mask)) * q_sh + 8 * h;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      u32x4 w = load16(src + 16 * kk);
-      if (!live) w = u32x4{0u, 0u, 0u, 0u};
-      qop[kk] = __builtin_bit_cast(bf16x8, w);
-    }
-    if (h == 0)
-#pragma unroll
-      for (int j = 0; j < kMaskStride; ++j)
-        row_line[j] = live && j < line_words ? lines[tok * line_words + j] : 0u;
+    const int rows = (cp.q1 - cp.q0) << group_shift;
+    wave_live = wave < RW * KS && 32 * rw < rows;
+    live = r < rows;
   };
-  // Closes the piece: its output rows, or this wave's partial: fp32, in the
-  // accumulator's own order (16 groups of 64 lanes x 16 bytes), live rows only.
-  auto finish = [&]() __attribute__((always_inline)) {
-    if (!wave_live) return;
-    const float l = halves_sum(l_run);
-    if (cp.slot < 0) {
-      const float inv = 1.0f / l;
-      const int64_t tok = cp.q_row + cp.q0 + (r >> group_shift);
-      uint16_t *dst = out + cp.seq * o_ss + tok * o_st + (h0 + (r & group_mask)) * o_sh + 4 * h;
-      if (live)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int db = j >> 2, i = 4 * (j & 3);
-          *reinterpret_cast<uint2 *>(dst + 8 * j) =
-              make_uint2(pack_bf16x2_rne(acc[db][i] * inv, acc[db][i + 1] * inv),
-                         pack_bf16x2_rne(acc[db][i + 2] * inv, acc[db][i + 3] * inv));
-        }
-      return;
-    }
-    const int64_t block = static_cast<int64_t>(kvh) * n_slots + cp.slot + wave;
-    float *dst = ws_acc + block * 32 * kHeadDim + 4 * lane;
-    if (live) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int db = j >> 2, i = 4 * (j & 3);
-        *reinterpret_cast<f32x4 *>(dst + 256 * j) =
-            f32x4{acc[db][i], acc[db][i + 1], acc[db][i + 2], acc[db][i + 3]};
-      }
-      if (h == 0) *reinterpret_cast<float2 *>(ws_ml + (block * 32 + c) * 2) = make_float2(base, l);
-    }
-  };
-
-  // LDS read bases (u16 units), as in the prefill kernel.
-  const int r16 = lane & 15;
-  const int q16 = lane >> 4;
-  int k_base[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    k_base[i] = (c >> 4) * 2048 + (c & 15) * 32 + 8 * ((2 * i + h) ^ ((c >> 2) & 3));
-  const int v_base = kTile * kHeadDim + 512 * (q16 >> 1) + 32 * (r16 >> 2) + 16 * (q16 & 1) +
-                     4 * (r16 & 3);
 
   // The line bits of the 32 slots from key kb0 on (bit j: slot kb0 + j is seen);
   // slots before the drafted ones are all seen.
   auto line_bits = [&](int kb0) __attribute__((always_inline)) -> uint32_t {
-    const int d = kb0 - cp.cache;  // > -32
-    if (d < 0) return row_line[0] << -d | ((1u << -d) - 1);
-    const uint32_t lo = row_line[d >> 5], hi = row_line[(d >> 5) + 1];
-    return static_cast<uint32_t>((static_cast<uint64_t>(hi) << 32 | lo) >> (d & 31));
+    if (!live) return 0u;
+    const int row = 32 * rw + (here(lane) & 31);
+    const uint32_t *words = own_line + (row >> group_shift) * line_words;
+    const int d = kb0 - cp.cache;  // > -32, and below the tree's size
+    if (d < 0) return words[0] << -d | ((1u << -d) - 1);
+    const int w = d >> 5;
+    const uint32_t hi = w + 1 < line_words ? words[w + 1] : 0u;
+    return static_cast<uint32_t>((static_cast<uint64_t>(hi) << 32 | words[w]) >> (d & 31));
   };
 
-  // One block of 32 keys from kb0 on, in half b of the stage.
-  auto block = [&](const uint16_t *stage, int b, int kb0) __attribute__((always_inline)) {
-    const uint16_t *kb = stage + 4096 * b;
-    f32x16 s;
+  // Online softmax on raw scores: p = exp2(s scale log2(e) - shift), shift the row's
+  // exponent base (0 while it has none).
+  auto probs = [&](const f32x16 &s, bf16x8(&pop)[2]) __attribute__((always_inline)) {
+    float a[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      const bf16x8 kop = *reinterpret_cast<const bf16x8 *>(kb + k_base[kk & 1] + 512 * (kk >> 1));
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop, qop[kk], s, 0, 0, 0);
+    for (int i = 0; i < 16; ++i) {
+      a[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale_log2, -shift));
+      pop[i >> 3][i & 7] = static_cast<__bf16>(a[i]);
     }
-    const bool masked = kb0 + 32 > cp.cache;
-    uint32_t bits = 0xffffffffu;
-    if (masked) {
-      bits = live ? line_bits(kb0) : 0u;
-      const uint32_t mine = bits >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? s[i] : -INFINITY;
-    }
-    s16x8 vop[8];
-    const uint16_t *vb = kb + v_base;
+    for (int n = 8; n > 0; n >>= 1)  // pairwise: four dependent sums
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int kh2 = 0; kh2 < 2; ++kh2) {
-        const s16x4 lo = tr_read(vb + 2048 * kh2 + 128 * db);
-        const s16x4 hi = tr_read(vb + 2048 * kh2 + 128 * db + 1024);
-        vop[2 * db + kh2] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-
-    // Online softmax on raw scores: p = exp2(s scale log2(e) - shift), shift the row's
-    // exponent base (0 while it has none). The base moves only when a score exceeds
-    // it by 2^8; below that no lane's probabilities sum to more.
-    float p[16], psum;
-    auto probs = [&]() __attribute__((always_inline)) {
-      psum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale_log2, -shift));
-        psum += p[i];
-      }
-    };
-    probs();
+      for (int i = 0; i < n; ++i) a[i] = a[2 * i] + a[2 * i + 1];
+    return a[0];
+  };
+  // The base moves only when a score exceeds it by 2^8 (or the row sees its first key);
+  // below that no lane's probabilities sum to more. Rare, and then they are redone.
+  auto rebase = [&](const f32x16 &s, bf16x8(&pop)[2], float psum) __attribute__((always_inline)) {
     // !(psum <= ...) also catches an overflowed sum and NaN
     if (__builtin_expect(__any(base == -INFINITY || !(psum <= kLazyP)), 0)) {
       float m = s[0];
@@ -313,107 +380,284 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
         l_run *= alpha;
 #pragma unroll
         for (int db = 0; db < 4; ++db) acc[db] *= alpha;
-        probs();
+        psum = probs(s, pop);
       }
     }
     l_run += psum;
+  };
+  // V^T operands of a block, dims 64 half .. 64 half + 63, and their product.
+  auto read_v = [&](s16x8(&vop)[4], const uint16_t *kb, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint16_t *vb = kb + v_base + 128 * (2 * half + (x >> 1)) + 2048 * (x & 1);
+      vop[x] = __builtin_shufflevector(tr_read(vb), tr_read(vb + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  auto pv = [&](const s16x8(&vop)[4], const bf16x8(&pop)[2], int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      f32x16 &a = acc[2 * half + (x >> 1)];
+      a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vop[x]), pop[x & 1],
+                                                  a, 0, 0, 0);
+    }
+  };
+
+  // Drafted slots among the 32 keys from kb0 on: the rows' lines mask their scores.
+  auto mask = [&](f32x16 &s, int kb0) __attribute__((always_inline)) {
+    if (kb0 + 32 <= cp.cache) return;
+    const uint32_t mine = line_bits(kb0) >> (4 * (here(lane) >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? s[i] : -INFINITY;
+  };
+  // One block of 32 keys from kb0 on at kb (K rows; V behind), by itself: with up to 128 rows the
+  // loads take longer than a wave's blocks one after the other.
+  auto block = [&](const uint16_t *kb, int kb0) __attribute__((always_inline)) {
     bf16x8 pop[2];
+    s16x8 v0[4], v1[4];
+    f32x16 s;
+    first_scores(s, kb);
+    read_v(v0, kb, 0);
+    read_v(v1, kb, 1);
+    mask(s, kb0);
+    rebase(s, pop, probs(s, pop));
+    pv(v0, pop, 0);
+    pv(v1, pop, 1);
+  };
+  // The same with the wave's next blocks behind it (two blocks a tile, products near the time of
+  // the loads): s holds the block's scores, kop the K operands of the next, whose scores
+  // s_next takes from the matrix core while the VALU turns s into probabilities; kop then
+  // takes those of the block after, at kb_after. Past the piece there are no such blocks, and
+  // what comes of them is dropped.
+  bf16x8 kop[2][4];
+  auto piped_block = [&](f32x16 &s, f32x16 &s_next, const uint16_t *kb, const uint16_t *kb_after,
+                         int kb0) __attribute__((always_inline)) {
+    bf16x8 pop[2];
+    s16x8 v0[4], v1[4];
+    mask(s, kb0);
+    read_v(v0, kb, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    // the two waves of a SIMD take turns: the one here goes before the other's
+    // second product and reads
+    __builtin_amdgcn_s_setprio(1);
+    s_next = f32x16{};
+    scores(s_next, kop[0], 0);
+    scores(s_next, kop[1], 1);
+    read_v(v1, kb, 1);
+    const float psum = probs(s, pop);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      pop[0][i] = static_cast<__bf16>(p[i]);
-      pop[1][i] = static_cast<__bf16>(p[8 + i]);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedValu, 7, 0);
     }
-    bool odd = false;  // a drafted slot of the block holds an infinity or NaN in V
-    if (masked) {
-      // values of slots past the piece are zeroed (they may be any bits)
-      if (kb0 + 32 > cp.kv1) {
-#pragma unroll
-        for (int kh2 = 0; kh2 < 2; ++kh2) {
-          s16x8 keep;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            keep[j] = kb0 + 16 * kh2 + 8 * (j >> 2) + 4 * h + (j & 3) < cp.kv1 ? -1 : 0;
-#pragma unroll
-          for (int db = 0; db < 4; ++db) vop[2 * db + kh2] &= keep;
-        }
-      }
-      u16x2 top = {0, 0};
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const u32x4 w = __builtin_bit_cast(u32x4, vop[x]) & 0x7fff7fffu;
+    // counts as used here, so that the probabilities stay in this region
+    __asm__ volatile("" ::"v"(psum), "v"(pop[0]), "v"(pop[1]));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    rebase(s, pop, psum);
+    pv(v0, pop, 0);
+    pv(v1, pop, 1);
+    read_rows(kop[0], kb_after, 0);
+    read_rows(kop[1], kb_after, 1);
+  };
+
+  // V rows of drafted slots in the stage `cur`, keys from `key` on, before they meet the
+  // probabilities (0 times an infinity or NaN is NaN): rows past the piece, which may hold
+  // any bits, become 0, and so do infinities and NaN, whose slots are marked; finish()
+  // gives them to the rows that see them. Every thread of the workgroup takes part, and
+  // a barrier follows.
+  auto clean = [&](uint16_t *cur, int key) __attribute__((always_inline)) {
+    for (int u = 64 * wave + here(lane); u < kTile * kHeadDim / 8; u += 64 * W) {
+      const int slot_key = key + 4 * (u >> 6) + ((u >> 2) & 3);
+      if (slot_key < cp.cache) continue;
+      uint16_t *at = cur + kTile * kHeadDim + 8 * u;
+      u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+      bool found = slot_key >= cp.kv1;
+      if (found) {
+        x = u32x4{0u, 0u, 0u, 0u};
+      } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t pair = w[j];  // a bit cast of the element itself would take the first
-          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, pair));
+          const bool lo = (x[j] & 0x7f80u) == 0x7f80u, hi = (x[j] & 0x7f800000u) == 0x7f800000u;
+          found = found || lo || hi;
+          x[j] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+        }
+        const int slot = slot_key - cp.cache;
+        if (found) atomicOr(&sick[slot >> 5], 1u << (slot & 31));
+      }
+      if (found) *reinterpret_cast<u32x4 *>(at) = x;
+    }
+    barrier();
+  };
+
+  // Closes the piece: its output rows, or a partial: fp32, in the accumulator's own
+  // order (16 groups of 64 lanes x 16 bytes), live rows only. With KS == 2 the second
+  // wave's rows are joined first, through the stage of the tile just used: it is
+  // free once every wave has left it, until the loads that follow the next barrier.
+  auto finish = [&](uint16_t *stage) __attribute__((always_inline)) {
+    float l = halves_sum(l_run);
+    const int lane_ = here(lane), r_ = 32 * rw + (lane_ & 31), h_ = lane_ >> 5;
+    if (ks == 0 && wave_live) {
+      // infinities and NaN of marked slots (none, as a rule), from the pool
+      for (int w = 0; w < line_words; ++w) {
+        uint32_t marks = __builtin_amdgcn_readfirstlane(sick[w]);
+        while (marks != 0) {
+          const int key = cp.cache + 32 * w + __builtin_ctz(marks);
+          marks &= marks - 1;
+          const bool sees = live && own_line[(r_ >> group_shift) * line_words + w] >>
+                                        ((key - cp.cache) & 31) & 1;
+          const int64_t row =
+              (static_cast<int64_t>(page_table[cp.seq * pt_stride + (key >> page_shift)]) << page_shift) +
+              (key & page_mask);
+          const uint16_t *v = vh + row * kHeadDim + 4 * h_;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(v + 8 * j);
+            const float value[4] = {bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sees && (__float_as_uint(value[e]) & 0x7f800000u) == 0x7f800000u)
+                acc[j >> 2][4 * (j & 3) + e] += value[e];
+          }
         }
       }
-      odd = __any(top[0] >= 0x7f80 || top[1] >= 0x7f80);
     }
-    if (__builtin_expect(odd, 0)) {
-      // rare: such values leave the product (0 times them is NaN) and reach only
-      // the rows that see their slot
+    if constexpr (KS == 2) {
+      constexpr int kParts = RW > 2 ? 2 : 1;  // 16 KiB a wave, 32 KiB a stage
+      constexpr int kDb = 4 / kParts;
+      float *box = reinterpret_cast<float *>(stage) + rw * (kDb * 1024) + 4 * lane_;
+      float2 *ml = other_ml + r_;
+      float mine = 1.f, theirs = 0.f;
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
+      for (int part = 0; part < kParts; ++part) {
+        barrier();
+        if (ks == 1 && wave_live) {
+          if (part == 0 && h == 0) *ml = make_float2(base, l);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((vop[x][j] & 0x7f80) == 0x7f80) vop[x][j] = 0;
-      for (int key = 0; key < 32 && kb0 + key < cp.kv1; ++key) {
-        const uint16_t *row = kb + kTile * kHeadDim + 512 * (key >> 2) + 32 * (key & 3);
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int dim = 8 * (i >> 2) + 4 * h + (i & 3);  // of the 32-dim slice db
-            const uint16_t v = row[128 * db + 8 * (dim >> 3) + (dim & 7)];
-            if ((v & 0x7f80) == 0x7f80 && (bits >> key & 1))
-              acc[db][i] += __uint_as_float(static_cast<uint32_t>(v) << 16);
+          for (int j = 0; j < 4 * kDb; ++j) {
+            const f32x16 &a = acc[kDb * part + (j >> 2)];
+            const int i = 4 * (j & 3);
+            *reinterpret_cast<f32x4 *>(box + 256 * j) = f32x4{a[i], a[i + 1], a[i + 2], a[i + 3]};
           }
+        }
+        barrier();
+        if (ks == 0 && wave_live) {
+          if (part == 0) {
+            const float2 o = *ml;
+            const float top = fmaxf(base, o.x);
+            // a wave that saw nothing adds nothing (its sums are 0)
+            mine = base == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - top);
+            theirs = o.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(o.x - top);
+            l = l * mine + o.y * theirs;
+            base = top;
+          }
+#pragma unroll
+          for (int j = 0; j < 4 * kDb; ++j) {
+            f32x16 &a = acc[kDb * part + (j >> 2)];
+            const int i = 4 * (j & 3);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(box + 256 * j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[i + e] = a[i + e] * mine + x[e] * theirs;
+          }
+        }
       }
+      if (ks != 0) return;
     }
+    if (!wave_live) return;
+    if (cp.slot < 0) {
+      const float inv = 1.0f / l;
+      const int64_t tok = cp.q_row + cp.q0 + (r_ >> group_shift);
+      uint16_t *dst = out + cp.seq * o_ss + tok * o_st + (h0 + (r_ & group_mask)) * o_sh + 4 * h_;
+      if (live)
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
+        for (int j = 0; j < 16; ++j) {
+          const int db = j >> 2, i = 4 * (j & 3);
+          *reinterpret_cast<uint2 *>(dst + 8 * j) =
+              make_uint2(pack_bf16x2_rne(acc[db][i] * inv, acc[db][i + 1] * inv),
+                         pack_bf16x2_rne(acc[db][i + 2] * inv, acc[db][i + 3] * inv));
+        }
+      return;
+    }
+    const int64_t block = static_cast<int64_t>(kvh) * n_slots + cp.slot + rw;
+    float *dst = ws_acc + block * 32 * kHeadDim + 4 * lane_;
+    if (live) {
 #pragma unroll
-      for (int kh2 = 0; kh2 < 2; ++kh2)
-        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8, vop[2 * db + kh2]), pop[kh2], acc[db], 0, 0, 0);
+      for (int j = 0; j < 16; ++j) {
+        const int db = j >> 2, i = 4 * (j & 3);
+        *reinterpret_cast<f32x4 *>(dst + 256 * j) =
+            f32x4{acc[db][i], acc[db][i + 1], acc[db][i + 2], acc[db][i + 3]};
+      }
+      if (h == 0) *reinterpret_cast<float2 *>(ws_ml + (block * 32 + (lane_ & 31)) * 2) = make_float2(base, l);
+    }
   };
 
   // ---- the chunk ---------------------------------------------------------
-  start();
-  Tile next = fetch(0);
-  issue(next, 0);
-  if (n_tiles > 1) issue(next = fetch(1), 1);
-  if (n_tiles > 2) issue(next = fetch(2), 2);
-  if (n_tiles > 3) next = fetch(3);
-  for (int t = 0; t < n_tiles; ++t) {
-    // tile t has arrived in every wave, and every wave is done with tile t - 1,
-    // whose stage tile t + 3 takes
-    if (t + 2 < n_tiles)
-      wait_loads<(2 * kLoads < 63 ? 2 * kLoads : 63)>();
-    else if (t + 1 < n_tiles)
+  issue(0);
+  for (int i = 1; i < 3 && i < n_stages; ++i) {
+    advance();
+    issue(i);
+  }
+  if (n_stages > 3) advance();
+  int t = 0;  // stages computed
+  uint16_t *cur;
+  const uint16_t *nxt;
+  auto next_stage = [&]() __attribute__((always_inline)) {
+    // The page ids of the next loads are read here and waited for with the stage: a scalar
+    // load outstanding would make every wait for an LDS read in a block wait for it too.
+    if ((LW == 0 || loader >= 0) && t > 0 && t + 3 < n_stages) advance();
+    // stage t (with KS == 1, whose blocks read ahead, t + 1 too) has arrived in every wave,
+    // and every wave is done with stage t - 1, which stage t + 3 takes
+    if (LW > 0 && loader < 0) {
+      // (nothing of its own in flight)
+    } else if (t + 2 < n_stages) {
+      wait_loads<KS * kLoads>();
+    } else if (KS == 2 && t + 1 < n_stages) {
       wait_loads<kLoads>();
-    else
+    } else {
       wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
-    __asm__ volatile("" ::: "memory");
-    if (t + 3 < n_tiles) {
-      issue(next, t + 3);
-      if (t + 4 < n_tiles) next = fetch(t + 4);
     }
-    const uint16_t *stage = ring + (t % kStages) * kStage;
-    const int key = cp.kv0 + kTile * (t - cp_tile);
-    if (wave_live) {
-      block(stage, 0, key);
-      if (key + 32 < cp.kv1) block(stage, 1, key + 32);
-    }
-    if (key + kTile >= cp.kv1) {
-      finish();
-      if (cp_index + 1 < p_end) {
-        cp_tile = t + 1;
-        cp = load_piece(pieces + 8 * ++cp_index);
-        start();
+    barrier();
+    if (t + 3 < n_stages) issue(t + 3);
+    cur = ring + (t % kStages) * kStage;
+    nxt = ring + ((t + 1) % kStages) * kStage;
+    ++t;
+  };
+  for (int cp_index = ch[0]; cp_index < p_end; ++cp_index) {
+    cp = load_piece(pieces + 8 * cp_index);
+    own_line = line[cp_index % 3];
+    start();
+    for (int part = 0; part < kQStages; ++part) {
+      next_stage();
+      if (part == 0 && wave == 0 && lane < kMaskWords) sick[lane] = 0;
+      if (part == rw >> 2) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          read_rows(qop[half], cur + 4096 * (rw & 3), half);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (!live) qop[half][kk] = bf16x8{};
+        }
       }
     }
+    f32x16 s_a, s_b;  // scores of the wave's current and next block
+    if (KS == 1 && wave_live) {
+      first_scores(s_a, nxt);
+      read_rows(kop[0], nxt + 4096, 0);
+      read_rows(kop[1], nxt + 4096, 1);
+    }
+    for (int key = cp.kv0; key < cp.kv1; key += kTile) {
+      next_stage();
+      if (key + kTile > cp.cache) clean(cur, key);
+      if (!wave_live) continue;
+      if constexpr (KS == 2) {
+        if (key + 32 * ks < cp.kv1) block(cur + 4096 * ks, key + 32 * ks);
+      } else {
+        piped_block(s_a, s_b, cur, nxt, key);
+        if (key + 32 < cp.kv1) piped_block(s_b, s_a, cur + 4096, nxt + 4096, key + 32);
+      }
+    }
+    finish(cur);
   }
 }
 
@@ -521,8 +765,7 @@ extern "C" int hy_paged_tree(
              "%d chunks and %d merge items: the grid takes 65535", n_chunks, n_merge);
   HY_REQUIRE(max_rows >= 1 && max_rows <= hy::kTreeRows, "max_rows %d is not within 1 .. %d",
              max_rows, hy::kTreeRows);
-  HY_REQUIRE(line_words >= 1 && line_words <= hy::kMaskWords, "line_words %d is not within 1 .. %d",
-             line_words, hy::kMaskWords);
+  HY_REQUIRE(line_words == 4 || line_words == 8, "line_words is %d, not 4 or 8", line_words);
   HY_REQUIRE(q && out && k_pool && v_pool && page_table && lines && items &&
                  (merge_items || n_merge == 0),
              "hy_paged_tree: null pointer argument");
@@ -530,7 +773,8 @@ extern "C" int hy_paged_tree(
                o_stride_head | pool_head_stride) &
               7) == 0 &&
                  ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
-                   reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) &
+                   reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool) |
+                   reinterpret_cast<uintptr_t>(lines)) &
                   15) == 0,
              "hy_paged_tree: rows must be 16-byte aligned");
   const int64_t need = hy_tree_workspace_bytes(n_slots, num_kv_heads, head_dim);
@@ -556,12 +800,14 @@ extern "C" int hy_paged_tree(
                        line_words, ws_acc, ws_ml, n_slots, group_shift,
                        __builtin_ctz(static_cast<unsigned>(page_size)), scale * hy::kLog2e);
   };
-  if (max_rows <= 64)
-    launch(hy::tree_kernel<2>, 2);
+  if (max_rows <= 32)
+    launch(hy::tree_kernel<1, 2, 4>, 6);
+  else if (max_rows <= 64)
+    launch(hy::tree_kernel<2, 2, 4>, 8);
   else if (max_rows <= 128)
-    launch(hy::tree_kernel<4>, 4);
+    launch(hy::tree_kernel<4, 2, 0>, 8);
   else
-    launch(hy::tree_kernel<8>, 8);
+    launch(hy::tree_kernel<8, 1, 0>, 8);
   if (int rc = hy::launch_status("hy_paged_tree")) return rc;
   if (n_merge == 0) return HY_OK;
   hipLaunchKernelGGL(hy::tree_merge_kernel, dim3(num_kv_heads, n_merge, (max_rows + 31) / 32),

@@ -297,17 +297,21 @@ class PagedKVBatch:
                 np.asarray(cache_lens_host, dtype=np.int32),
                 np.asarray(self.kv_lens_host, dtype=np.int32),
                 q_start,
-                # a subclass's own metadata travels in the same copy
-                *(() if extra is None else (extra,)),
             ]
         )
+        n_meta = self._meta_np.size
+        if extra is not None:
+            # a subclass's own metadata travels in the same copy, from 16 bytes on
+            n_meta += -n_meta % 4
+            self._meta_np = np.concatenate(
+                [self._meta_np, np.zeros(n_meta - self._meta_np.size, dtype=np.int32), extra])
         meta = torch.from_numpy(self._meta_np).to(self.device)
         n, b = table.size, self.num_seqs
         self.page_table = meta[:n].view(self.num_seqs, width)
         self.cache_lens_i32 = meta[n : n + b]
         self.kv_lens = meta[n + b : n + 2 * b]
         self.q_start = meta[n + 2 * b : n + 3 * b + 1]
-        self._extra = meta[n + 3 * b + 1 :]
+        self._extra = meta[n_meta:]
         self.cache_lens = self.cache_lens_i32.to(torch.long)
         self._meta = meta
         self._pt_ptr = self.page_table.data_ptr()
@@ -676,7 +680,8 @@ class PagedTreeBatch(PagedKVBatch):
                  num_q_heads: Optional[int]):
         q_lens = [len(p) for p in parents]
         self.parents = parents
-        self.line_words = -(-max(q_lens) // 32)
+        # a node's line: a bit for each drafted slot, in whole 16-byte units
+        self.line_words = 4 * -(-max(q_lens) // 128)
         depths, lines = [], np.zeros((sum(q_lens), self.line_words), dtype=np.uint32)
         row = 0
         for tree in parents:
@@ -692,11 +697,12 @@ class PagedTreeBatch(PagedKVBatch):
         self._tree_plans: dict[int, _DeviceTreePlan] = {}
         super().__init__(manager, q_lens, cache_lens_host, page_lists, varlen=True,
                          num_q_heads=None,
-                         extra=np.concatenate([positions, lines.reshape(-1).view(np.int32)]))
+                         extra=np.concatenate([lines.reshape(-1).view(np.int32), positions]))
         # every tree goes through the tree kernel, requests with one node included
         self.decode_only = False
-        self.positions = self._extra[: self.total_tokens]
-        self._lines_ptr = self._extra[self.total_tokens :].data_ptr()
+        self.lines = self._extra[: lines.size]
+        self.positions = self._extra[lines.size :]
+        self._lines_ptr = self.lines.data_ptr()
         self._append_call = ("hy_qknorm_rope_append_at", (self.positions.data_ptr(),))
         if num_q_heads is not None and self.device.type == "cuda":
             self.plan(num_q_heads)

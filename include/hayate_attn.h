@@ -457,8 +457,9 @@ int32_t hy_tree_max_nodes(void);
  * q_lens[b] cached tokens. The (node, query head) rows of a sequence form query
  * tiles of at most 256 rows per kv head; the 64-key steps of all tiles, in order,
  * are cut into chunks of equal cost, one per CU and kv head. items:
- *   n_chunks chunk records int32[16] = {piece_begin, piece_end, n_steps, 0, 0, 0, 0, 0,
- *   the first piece's record}, then the piece records int32[8] = {seq, q_begin, q_end,
+ *   n_chunks chunk records int32[16] = {piece_begin, piece_end, n_steps, alone, 0, 0, 0,
+ *   0, the first piece's record} (alone: 1 when its sequences have one tile each, so
+ *   that their keys are read once), then the piece records int32[8] = {seq, q_begin, q_end,
  *   kv_begin, kv_end, slot, q_row, cache_len}: kv_begin a multiple of 64, slot the
  *   piece's first 32-row block of partials, -1 for a tile in one piece, which is
  *   written to out directly; q_row = q_start[seq];
@@ -482,8 +483,9 @@ int64_t hy_tree_workspace_bytes(int32_t n_slots, int32_t num_kv_heads,
  * Attention of the nodes over their caches: node i of sequence b sees its cached
  * tokens, its ancestors and itself,
  *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j,
- * K and V read through the page table. lines is device memory, line_words 32-bit words
- * (1 .. 8) for each packed node: bit j of them is set when the node sees drafted slot j.
+ * K and V read through the page table. lines is device memory (16-byte aligned),
+ * line_words 32-bit words (4 or 8) for each packed node: bit j of them is set when the node
+ * sees drafted slot j.
  * Slots that no row of a tile sees, and the rest of a page, may hold any bits.
  * Plan and workspace (hy_tree_workspace_bytes(n_slots), NULL when 0) are those of
  * hy_plan_tree; max_rows as counted there. One call launches the attention and, when

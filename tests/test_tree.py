@@ -41,6 +41,8 @@ def check_plan(q_lens, kv_lens, hq=32, hkv=8, cus=256):
     for ch in chunks:
         assert ch[2] == steps[ch[0] : ch[1]].sum()
         assert (ch[8:] == pieces[ch[0]]).all()
+        mine = pieces[ch[0] : ch[1]]
+        assert ch[3] == (mine[:, 2] - mine[:, 1] == q[mine[:, 0]]).all()
     starts = np.concatenate([[0], np.cumsum(q)])
     at, used, merged, rows = 0, [], {}, 0
     for m in p.merge:
@@ -133,8 +135,8 @@ def test_batch_metadata(sizes):
     assert isinstance(batch, PagedTreeBatch) and batch.varlen and not batch.decode_only
     assert batch.logit_rows() is None
     words = batch.line_words
-    assert words == -(-max(sizes) // 32)
-    lines = batch._extra[batch.total_tokens :].numpy().view(np.uint32).reshape(-1, words)
+    assert words == 4 * -(-max(sizes) // 128) and batch._lines_ptr % 16 == 0
+    lines = batch.lines.numpy().view(np.uint32).reshape(-1, words)
     row = 0
     for h, tree in zip(handles, trees):
         assert len(h.pages) == -(-(h.length + len(tree)) // 128)
@@ -312,7 +314,7 @@ def test_c_copies_are_checked_before_any_launch(src, dst, tokens):
 def test_c_tree_attention_is_checked():
     lib = _native.lib()
     good = dict(q=4096, qs=0, qt=4096, qh=128, out=4096, os=0, ot=4096, oh=128, k=4096, v=4096,
-                hs=128 * 1000, pt=4096, pts=4, lines=4096, words=1, items=4096, chunks=1, rows=32,
+                hs=128 * 1000, pt=4096, pts=4, lines=4096, words=4, items=4096, chunks=1, rows=32,
                 merge=None, merges=0, slots=0, ws=None, wsb=0, hq=32, hkv=8, dim=128, page=128,
                 scale=0.1, stream=None)
 
@@ -321,10 +323,10 @@ def test_c_tree_attention_is_checked():
         return lib.hy_paged_tree(*args.values())
 
     for kw in (dict(scale=0.0), dict(scale=float("nan")), dict(hq=30), dict(chunks=-1),
-               dict(chunks=65536), dict(rows=0), dict(rows=257), dict(words=0), dict(words=9),
+               dict(chunks=65536), dict(rows=0), dict(rows=257), dict(words=0), dict(words=5), dict(words=12),
                dict(q=None), dict(out=None), dict(k=None), dict(v=None), dict(pt=None),
                dict(lines=None), dict(items=None), dict(merges=1, slots=2, ws=4096, wsb=1 << 30),
-               dict(q=4098), dict(qh=100), dict(ot=4), dict(hs=1001)):
+               dict(q=4098), dict(lines=4100), dict(qh=100), dict(ot=4), dict(hs=1001)):
         assert call(**kw) == _native.HY_EINVAL, kw
     for kw in (dict(dim=64), dict(page=96), dict(page=16), dict(hq=24), dict(hq=256)):
         assert call(**kw) == _native.HY_EUNSUPPORTED, kw
