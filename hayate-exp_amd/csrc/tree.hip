@@ -42,10 +42,6 @@ constexpr int kStage = 2 * kTile * kHeadDim;  // halfs per stage: K tile, then V
 constexpr int kStages = 4;
 constexpr int kMaskWords = kTreeMaxNodes / 32;
 
-// Instruction classes for __builtin_amdgcn_sched_group_barrier.
-constexpr int kSchedMfma = 0x008;
-constexpr int kSchedValu = 0x002 | 0x400;  // VALU incl. transcendentals
-constexpr int kSchedDsRead = 0x100;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -148,12 +144,11 @@ __device__ __forceinline__ Piece load_piece(const int32_t *r) {
   return Piece{r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};
 }
 
-// RW waves side by side hold 32 rows each; KS of them hold the same rows and share the
-// 32-key blocks of a tile (KS == 2: one block each). LW more waves do nothing but load; with
-// LW == 0 the others load as well.
+// RW waves side by side hold 32 rows each; KS of them hold the same rows and share the 32-key
+// blocks of a tile (KS == 2: one block each). LW more waves do nothing but load; with LW == 0
+// the others load as well.
 template <int RW, int KS, int LW>
-__global__ __launch_bounds__(64 * (RW * KS + LW))
-    __attribute__((amdgpu_waves_per_eu(RW * KS + LW > 4 ? 2 : 1, RW * KS + LW > 4 ? 2 : 1)))
+__global__ __launch_bounds__(64 * (RW * KS + LW)) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
                  uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
                  const uint16_t *__restrict__ k_pool, const uint16_t *__restrict__ v_pool,
@@ -165,14 +160,17 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   constexpr int W = RW * KS + LW;
   constexpr int kLoaders = LW > 0 ? LW : W;
   constexpr int kLoads = 32 / kLoaders;       // load instructions of a loading wave per stage
-  constexpr int kQStages = (RW + 3) / 4;      // 128 rows a stage
-  constexpr int kLineWords = kLoaders * 256;  // one load instruction of every loading wave
-  static_assert(kLineWords >= RW * 32 * kMaskWords, "a line for every row");
+  constexpr int kRows = 32 * RW;
+  constexpr int kQStages = (kRows + 127) / 128;
+  // load instructions of a loading wave for the rows' lines
+  constexpr int kLineLoads = (kRows * kMaskWords + kLoaders * 256 - 1) / (kLoaders * 256);
+  constexpr int kLineWords = kLineLoads * kLoaders * 256;
+  static_assert(KS == 1 || RW <= 2, "finish() joins two waves' rows in one stage");
   __shared__ __attribute__((aligned(1024))) uint16_t ring[kStages * kStage];
   // A piece has two stages at least, so the one issued three stages ahead belongs at most to
   // the piece after the next.
   __shared__ __attribute__((aligned(1024))) uint32_t line[3][kLineWords];
-  __shared__ float2 other_ml[RW * 32];
+  __shared__ float2 other_ml[kRows];
   __shared__ uint32_t sick[kMaskWords];  // drafted slots with an infinity or NaN in V
 
   const int32_t *ch = items + kTreeChunkInts * blockIdx.y;
@@ -267,10 +265,14 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
       }
       if (ip_step == -kQStages) {
         const int last = (ip.q1 - ip.q0) * line_words - 4;
-        load_to_lds(reinterpret_cast<const uint16_t *>(
-                        lines + static_cast<int64_t>(ip.q_row + ip.q0) * line_words +
-                        min(256 * loader + 4 * lane_, last)),
-                    reinterpret_cast<uint16_t *>(line[ip_index % 3] + 256 * loader));
+#pragma unroll
+        for (int j = 0; j < kLineLoads; ++j) {
+          const int at = 256 * (loader * kLineLoads + j);
+          load_to_lds(reinterpret_cast<const uint16_t *>(
+                          lines + static_cast<int64_t>(ip.q_row + ip.q0) * line_words +
+                          min(at + 4 * lane_, last)),
+                      reinterpret_cast<uint16_t *>(line[ip_index % 3] + at));
+        }
       }
       return;
     }
@@ -285,11 +287,12 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   const uint32_t *own_line = line[0];
   const int rw = wave % RW;
   const int ks = wave / RW;
-  const int r = 32 * rw + c;
-  bool wave_live = false, live = false;
-  bf16x8 qop[2][4];  // row c of Q^T
-  f32x16 acc[4];  // O^T[32 db + 8 (i / 4) + 4 h + i % 4][row c]
-  float base = -INFINITY, shift = 0.f, l_run = 0.f;
+  bool wave_live = false;
+  const int r = 32 * rw + c;  // this lane's row
+  bool live = false;
+  bf16x8 qop[2][4];  // the row of Q^T
+  f32x16 acc[4];     // O^T[32 db + 8 (i / 4) + 4 h + i % 4][row]
+  float base, shift, l_run;
 
   // LDS read bases (u16 units).
   const int r16 = lane & 15;
@@ -311,41 +314,40 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
     for (int kk = 0; kk < 4; ++kk)
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[kk], qop[half][kk], s, 0, 0, 0);
   };
-  auto first_scores = [&](f32x16 &s, const uint16_t *rows) __attribute__((always_inline)) {
-    s = f32x16{};
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      bf16x8 kop[4];
-      read_rows(kop, rows, half);
-      scores(s, kop, half);
-    }
-  };
   auto start = [&]() __attribute__((always_inline)) {
+    const int rows = (cp.q1 - cp.q0) << group_shift;
+    wave_live = wave < RW * KS && 32 * rw < rows;
+    live = r < rows;
     base = -INFINITY;
     shift = 0.f;
     l_run = 0.f;
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < 4; ++db) acc[db] = f32x16{};
+  };
+
+  // Drafted slots among the 32 keys from kb0 on: the rows' lines mask their scores. A line's
+  // bits for them (bit j: slot of key kb0 + j is seen); slots before the drafted ones are
+  // all seen.
+  auto mask = [&](f32x16 &s, int kb0) __attribute__((always_inline)) {
+    const int d = kb0 - cp.cache;
+    if (d <= -32) return;
+    uint32_t bits = 0u;
+    if (live) {
+      const int lane_ = here(lane);
+      const uint32_t *words =
+          own_line + ((32 * rw + (lane_ & 31)) >> group_shift) * line_words;
+      if (d < 0) {
+        bits = words[0] << -d | ((1u << -d) - 1);
+      } else {
+        const int w = d >> 5;  // the slot lies in the tree: below line_words
+        const uint32_t hi = w + 1 < line_words ? words[w + 1] : 0u;
+        bits = static_cast<uint32_t>((static_cast<uint64_t>(hi) << 32 | words[w]) >> (d & 31));
+      }
+      bits >>= 4 * (lane_ >> 5);
+    }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
-    const int rows = (cp.q1 - cp.q0) << group_shift;
-    wave_live = wave < RW * KS && 32 * rw < rows;
-    live = r < rows;
+    for (int i = 0; i < 16; ++i) s[i] = bits >> (8 * (i >> 2) + (i & 3)) & 1 ? s[i] : -INFINITY;
   };
-
-  // The line bits of the 32 slots from key kb0 on (bit j: slot kb0 + j is seen);
-  // slots before the drafted ones are all seen.
-  auto line_bits = [&](int kb0) __attribute__((always_inline)) -> uint32_t {
-    if (!live) return 0u;
-    const int row = 32 * rw + (here(lane) & 31);
-    const uint32_t *words = own_line + (row >> group_shift) * line_words;
-    const int d = kb0 - cp.cache;  // > -32, and below the tree's size
-    if (d < 0) return words[0] << -d | ((1u << -d) - 1);
-    const int w = d >> 5;
-    const uint32_t hi = w + 1 < line_words ? words[w + 1] : 0u;
-    return static_cast<uint32_t>((static_cast<uint64_t>(hi) << 32 | words[w]) >> (d & 31));
-  };
-
   // Online softmax on raw scores: p = exp2(s scale log2(e) - shift), shift the row's
   // exponent base (0 while it has none).
   auto probs = [&](const f32x16 &s, bf16x8(&pop)[2]) __attribute__((always_inline)) {
@@ -388,78 +390,39 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   // V^T operands of a block, dims 64 half .. 64 half + 63, and their product.
   auto read_v = [&](s16x8(&vop)[4], const uint16_t *kb, int half) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const uint16_t *vb = kb + v_base + 128 * (2 * half + (x >> 1)) + 2048 * (x & 1);
-      vop[x] = __builtin_shufflevector(tr_read(vb), tr_read(vb + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t *vb = kb + v_base + 128 * (2 * half + (i >> 1)) + 2048 * (i & 1);
+      vop[i] = __builtin_shufflevector(tr_read(vb), tr_read(vb + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
     }
   };
   auto pv = [&](const s16x8(&vop)[4], const bf16x8(&pop)[2], int half) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      f32x16 &a = acc[2 * half + (x >> 1)];
-      a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vop[x]), pop[x & 1],
-                                                  a, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) {
+      f32x16 &a = acc[2 * half + (i >> 1)];
+      a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vop[i]), pop[i & 1], a,
+                                                  0, 0, 0);
     }
   };
 
-  // Drafted slots among the 32 keys from kb0 on: the rows' lines mask their scores.
-  auto mask = [&](f32x16 &s, int kb0) __attribute__((always_inline)) {
-    if (kb0 + 32 <= cp.cache) return;
-    const uint32_t mine = line_bits(kb0) >> (4 * (here(lane) >> 5));
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? s[i] : -INFINITY;
-  };
-  // One block of 32 keys from kb0 on at kb (K rows; V behind), by itself: with up to 128 rows the
-  // loads take longer than a wave's blocks one after the other.
+  // One block of 32 keys from kb0 on at kb (K rows; V behind). The scores of a wave's next block
+  // are not computed beside this one's softmax: with 256 rows (two waves a SIMD, which cover
+  // each other) that gave 315 against 317 us on 8 x 64 nodes over 32k keys, two row blocks a
+  // wave to pair 314, and with fewer rows the loads take longer than the blocks.
   auto block = [&](const uint16_t *kb, int kb0) __attribute__((always_inline)) {
-    bf16x8 pop[2];
+    bf16x8 kop[4], pop[2];
     s16x8 v0[4], v1[4];
-    f32x16 s;
-    first_scores(s, kb);
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      read_rows(kop, kb, half);
+      scores(s, kop, half);
+    }
     read_v(v0, kb, 0);
     read_v(v1, kb, 1);
     mask(s, kb0);
     rebase(s, pop, probs(s, pop));
     pv(v0, pop, 0);
     pv(v1, pop, 1);
-  };
-  // The same with the wave's next blocks behind it (two blocks a tile, products near the time of
-  // the loads): s holds the block's scores, kop the K operands of the next, whose scores
-  // s_next takes from the matrix core while the VALU turns s into probabilities; kop then
-  // takes those of the block after, at kb_after. Past the piece there are no such blocks, and
-  // what comes of them is dropped.
-  bf16x8 kop[2][4];
-  auto piped_block = [&](f32x16 &s, f32x16 &s_next, const uint16_t *kb, const uint16_t *kb_after,
-                         int kb0) __attribute__((always_inline)) {
-    bf16x8 pop[2];
-    s16x8 v0[4], v1[4];
-    mask(s, kb0);
-    read_v(v0, kb, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    // the two waves of a SIMD take turns: the one here goes before the other's
-    // second product and reads
-    __builtin_amdgcn_s_setprio(1);
-    s_next = f32x16{};
-    scores(s_next, kop[0], 0);
-    scores(s_next, kop[1], 1);
-    read_v(v1, kb, 1);
-    const float psum = probs(s, pop);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kSchedValu, 7, 0);
-    }
-    // counts as used here, so that the probabilities stay in this region
-    __asm__ volatile("" ::"v"(psum), "v"(pop[0]), "v"(pop[1]));
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(0);
-    rebase(s, pop, psum);
-    pv(v0, pop, 0);
-    pv(v1, pop, 1);
-    read_rows(kop[0], kb_after, 0);
-    read_rows(kop[1], kb_after, 1);
   };
 
   // V rows of drafted slots in the stage `cur`, keys from `key` on, before they meet the
@@ -496,17 +459,15 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   // wave's rows are joined first, through the stage of the tile just used: it is
   // free once every wave has left it, until the loads that follow the next barrier.
   auto finish = [&](uint16_t *stage) __attribute__((always_inline)) {
-    float l = halves_sum(l_run);
-    const int lane_ = here(lane), r_ = 32 * rw + (lane_ & 31), h_ = lane_ >> 5;
+    const int lane_ = here(lane), c_ = lane_ & 31, h_ = lane_ >> 5, r_ = 32 * rw + c_;
     if (ks == 0 && wave_live) {
       // infinities and NaN of marked slots (none, as a rule), from the pool
       for (int w = 0; w < line_words; ++w) {
         uint32_t marks = __builtin_amdgcn_readfirstlane(sick[w]);
         while (marks != 0) {
-          const int key = cp.cache + 32 * w + __builtin_ctz(marks);
+          const int bit = __builtin_ctz(marks), key = cp.cache + 32 * w + bit;
           marks &= marks - 1;
-          const bool sees = live && own_line[(r_ >> group_shift) * line_words + w] >>
-                                        ((key - cp.cache) & 31) & 1;
+          const bool sees = live && own_line[(r_ >> group_shift) * line_words + w] >> bit & 1;
           const int64_t row =
               (static_cast<int64_t>(page_table[cp.seq * pt_stride + (key >> page_shift)]) << page_shift) +
               (key & page_mask);
@@ -523,73 +484,62 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
         }
       }
     }
+    float l = halves_sum(l_run);
     if constexpr (KS == 2) {
-      constexpr int kParts = RW > 2 ? 2 : 1;  // 16 KiB a wave, 32 KiB a stage
-      constexpr int kDb = 4 / kParts;
-      float *box = reinterpret_cast<float *>(stage) + rw * (kDb * 1024) + 4 * lane_;
-      float2 *ml = other_ml + r_;
-      float mine = 1.f, theirs = 0.f;
+      float *box = reinterpret_cast<float *>(stage) + 4096 * rw + 4 * lane_;
+      barrier();
+      if (ks == 1 && wave_live) {
+        if (h_ == 0) other_ml[r_] = make_float2(base, l);
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        barrier();
-        if (ks == 1 && wave_live) {
-          if (part == 0 && h == 0) *ml = make_float2(base, l);
-#pragma unroll
-          for (int j = 0; j < 4 * kDb; ++j) {
-            const f32x16 &a = acc[kDb * part + (j >> 2)];
-            const int i = 4 * (j & 3);
-            *reinterpret_cast<f32x4 *>(box + 256 * j) = f32x4{a[i], a[i + 1], a[i + 2], a[i + 3]};
-          }
-        }
-        barrier();
-        if (ks == 0 && wave_live) {
-          if (part == 0) {
-            const float2 o = *ml;
-            const float top = fmaxf(base, o.x);
-            // a wave that saw nothing adds nothing (its sums are 0)
-            mine = base == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - top);
-            theirs = o.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(o.x - top);
-            l = l * mine + o.y * theirs;
-            base = top;
-          }
-#pragma unroll
-          for (int j = 0; j < 4 * kDb; ++j) {
-            f32x16 &a = acc[kDb * part + (j >> 2)];
-            const int i = 4 * (j & 3);
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(box + 256 * j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[i + e] = a[i + e] * mine + x[e] * theirs;
-          }
+        for (int j = 0; j < 16; ++j) {
+          const f32x16 &a = acc[j >> 2];
+          const int i = 4 * (j & 3);
+          *reinterpret_cast<f32x4 *>(box + 256 * j) = f32x4{a[i], a[i + 1], a[i + 2], a[i + 3]};
         }
       }
-      if (ks != 0) return;
+      barrier();
+      if (ks == 0 && wave_live) {
+        const float2 o = other_ml[r_];
+        const float top = fmaxf(base, o.x);
+        // a wave that saw nothing adds nothing (its sums are 0)
+        const float mine = base == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - top);
+        const float theirs = o.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(o.x - top);
+        l = l * mine + o.y * theirs;
+        base = top;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          f32x16 &a = acc[j >> 2];
+          const int i = 4 * (j & 3);
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(box + 256 * j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[i + e] = a[i + e] * mine + x[e] * theirs;
+        }
+      }
     }
-    if (!wave_live) return;
+    if (ks != 0 || !wave_live || !live) return;
     if (cp.slot < 0) {
       const float inv = 1.0f / l;
       const int64_t tok = cp.q_row + cp.q0 + (r_ >> group_shift);
       uint16_t *dst = out + cp.seq * o_ss + tok * o_st + (h0 + (r_ & group_mask)) * o_sh + 4 * h_;
-      if (live)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int db = j >> 2, i = 4 * (j & 3);
-          *reinterpret_cast<uint2 *>(dst + 8 * j) =
-              make_uint2(pack_bf16x2_rne(acc[db][i] * inv, acc[db][i + 1] * inv),
-                         pack_bf16x2_rne(acc[db][i + 2] * inv, acc[db][i + 3] * inv));
-        }
-      return;
-    }
-    const int64_t block = static_cast<int64_t>(kvh) * n_slots + cp.slot + rw;
-    float *dst = ws_acc + block * 32 * kHeadDim + 4 * lane_;
-    if (live) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const int db = j >> 2, i = 4 * (j & 3);
-        *reinterpret_cast<f32x4 *>(dst + 256 * j) =
-            f32x4{acc[db][i], acc[db][i + 1], acc[db][i + 2], acc[db][i + 3]};
+        const f32x16 &a = acc[j >> 2];
+        const int i = 4 * (j & 3);
+        *reinterpret_cast<uint2 *>(dst + 8 * j) =
+            make_uint2(pack_bf16x2_rne(a[i] * inv, a[i + 1] * inv),
+                       pack_bf16x2_rne(a[i + 2] * inv, a[i + 3] * inv));
       }
-      if (h == 0) *reinterpret_cast<float2 *>(ws_ml + (block * 32 + (lane_ & 31)) * 2) = make_float2(base, l);
+      return;
     }
+    const int64_t at = static_cast<int64_t>(kvh) * n_slots + cp.slot + rw;
+    float *dst = ws_acc + at * 32 * kHeadDim + 4 * lane_;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const f32x16 &a = acc[j >> 2];
+      const int i = 4 * (j & 3);
+      *reinterpret_cast<f32x4 *>(dst + 256 * j) = f32x4{a[i], a[i + 1], a[i + 2], a[i + 3]};
+    }
+    if (h_ == 0) *reinterpret_cast<float2 *>(ws_ml + (at * 32 + c_) * 2) = make_float2(base, l);
   };
 
   // ---- the chunk ---------------------------------------------------------
@@ -601,18 +551,17 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   if (n_stages > 3) advance();
   int t = 0;  // stages computed
   uint16_t *cur;
-  const uint16_t *nxt;
   auto next_stage = [&]() __attribute__((always_inline)) {
     // The page ids of the next loads are read here and waited for with the stage: a scalar
     // load outstanding would make every wait for an LDS read in a block wait for it too.
     if ((LW == 0 || loader >= 0) && t > 0 && t + 3 < n_stages) advance();
-    // stage t (with KS == 1, whose blocks read ahead, t + 1 too) has arrived in every wave,
-    // and every wave is done with stage t - 1, which stage t + 3 takes
+    // stage t has arrived in every wave, and every wave is done with stage t - 1, which
+    // stage t + 3 takes
     if (LW > 0 && loader < 0) {
       // (nothing of its own in flight)
     } else if (t + 2 < n_stages) {
-      wait_loads<KS * kLoads>();
-    } else if (KS == 2 && t + 1 < n_stages) {
+      wait_loads<2 * kLoads>();
+    } else if (t + 1 < n_stages) {
       wait_loads<kLoads>();
     } else {
       wait_loads<0>();
@@ -620,7 +569,6 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
     barrier();
     if (t + 3 < n_stages) issue(t + 3);
     cur = ring + (t % kStages) * kStage;
-    nxt = ring + ((t + 1) % kStages) * kStage;
     ++t;
   };
   for (int cp_index = ch[0]; cp_index < p_end; ++cp_index) {
@@ -630,21 +578,14 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
     for (int part = 0; part < kQStages; ++part) {
       next_stage();
       if (part == 0 && wave == 0 && lane < kMaskWords) sick[lane] = 0;
-      if (part == rw >> 2) {
+      if (part != rw >> 2) continue;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          read_rows(qop[half], cur + 4096 * (rw & 3), half);
+      for (int half = 0; half < 2; ++half) {
+        read_rows(qop[half], cur + 4096 * (rw & 3), half);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            if (!live) qop[half][kk] = bf16x8{};
-        }
+        for (int kk = 0; kk < 4; ++kk)
+          if (!live) qop[half][kk] = bf16x8{};
       }
-    }
-    f32x16 s_a, s_b;  // scores of the wave's current and next block
-    if (KS == 1 && wave_live) {
-      first_scores(s_a, nxt);
-      read_rows(kop[0], nxt + 4096, 0);
-      read_rows(kop[1], nxt + 4096, 1);
     }
     for (int key = cp.kv0; key < cp.kv1; key += kTile) {
       next_stage();
@@ -653,8 +594,8 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
       if constexpr (KS == 2) {
         if (key + 32 * ks < cp.kv1) block(cur + 4096 * ks, key + 32 * ks);
       } else {
-        piped_block(s_a, s_b, cur, nxt, key);
-        if (key + 32 < cp.kv1) piped_block(s_b, s_a, cur + 4096, nxt + 4096, key + 32);
+        block(cur, key);
+        if (key + 32 < cp.kv1) block(cur + 4096, key + 32);
       }
     }
     finish(cur);
@@ -805,7 +746,7 @@ extern "C" int hy_paged_tree(
   else if (max_rows <= 64)
     launch(hy::tree_kernel<2, 2, 4>, 8);
   else if (max_rows <= 128)
-    launch(hy::tree_kernel<4, 2, 0>, 8);
+    launch(hy::tree_kernel<4, 1, 4>, 8);
   else
     launch(hy::tree_kernel<8, 1, 0>, 8);
   if (int rc = hy::launch_status("hy_paged_tree")) return rc;
