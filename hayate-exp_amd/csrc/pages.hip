@@ -159,30 +159,25 @@ int check_pool(const void *k_pool, const void *v_pool, int64_t layer_stride, int
 using hy::kHeadDim;
 
 extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
-                          int64_t pool_head_stride, int64_t pool_tokens, const int32_t *src,
-                          const int32_t *dst, int32_t n, int32_t num_layers, int32_t num_kv_heads,
-                          int32_t head_dim, void *stream) {
+                          int64_t pool_head_stride, int32_t num_pages, const int32_t *pages,
+                          const int32_t *page_start, const int32_t *first_page, const int32_t *src,
+                          const int32_t *src_start, const int32_t *first, int32_t num_seqs,
+                          int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t page_size, void *stream) {
   hy::clear_error();
-  HY_REQUIRE(n >= 0, "hy_kv_move: n must be non-negative");
+  HY_REQUIRE(num_seqs >= 0, "hy_kv_move: num_seqs must be non-negative");
+  HY_REQUIRE(num_pages >= 1 && page_size >= 1, "hy_kv_move: pages must be positive");
+  const int64_t tokens = static_cast<int64_t>(num_pages) * page_size;
   if (int rc = hy::check_pool(k_pool, v_pool, pool_layer_stride, pool_head_stride, num_layers,
-                              num_kv_heads, head_dim, pool_tokens, "hy_kv_move"))
+                              num_kv_heads, head_dim, tokens, "hy_kv_move"))
     return rc;
-  if (n == 0) return HY_OK;
-  HY_REQUIRE(src && dst, "hy_kv_move: null pointer argument");
-  hy::Marks written(pool_tokens);
+  if (num_seqs == 0) return HY_OK;
+  HY_REQUIRE(pages && page_start && first_page && src && src_start && first,
+             "hy_kv_move: null pointer argument");
+  hy::Marks written(tokens);
   if (!written.ok()) {
-    hy::set_error("hy_kv_move: no host memory to check %lld tokens",
-                  static_cast<long long>(pool_tokens));
+    hy::set_error("hy_kv_move: no host memory to check %lld tokens", static_cast<long long>(tokens));
     return HY_ENOSPACE;
-  }
-  for (int32_t i = 0; i < n; ++i) {
-    HY_REQUIRE(src[i] >= 0 && src[i] < pool_tokens && dst[i] >= 0 && dst[i] < pool_tokens,
-               "hy_kv_move: move %d (%d to %d) leaves the pool of %lld tokens", i, src[i], dst[i],
-               static_cast<long long>(pool_tokens));
-    HY_REQUIRE(!written.has(src[i]), "hy_kv_move: move %d reads token %d, which an earlier one wrote",
-               i, src[i]);
-    HY_REQUIRE(!written.has(dst[i]), "hy_kv_move: two moves write token %d", dst[i]);
-    if (src[i] != dst[i]) written.set(dst[i]);
   }
   hy::Runs runs;
   int n_runs = 0, n_rows = 0;
@@ -194,16 +189,49 @@ extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
     n_runs = n_rows = 0;
     return hy::launch_status("hy_kv_move");
   };
-  for (int32_t i = 0; i < n;) {
-    int32_t j = i + 1;
-    if (src[i] != dst[i]) {
-      while (j < n && src[j] == src[j - 1] + 1 && dst[j] == dst[j - 1] + 1) ++j;
-      runs.r[n_runs++] = {src[i], dst[i], n_rows};
-      n_rows += j - i;
+  // Every move is checked before the first launch: once to check, once to enqueue.
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t last_src = -1, last_dst = -1;  // of the run being built
+    for (int32_t b = 0; b < num_seqs; ++b) {
+      const int64_t held = static_cast<int64_t>(page_start[b + 1]) - page_start[b];
+      const int64_t base = static_cast<int64_t>(first_page[b]) * page_size;
+      if (pass == 0) {
+        HY_REQUIRE(held >= 0 && first_page[b] >= 0 && src_start[b + 1] >= src_start[b],
+                   "hy_kv_move: sequence %d has a negative count", b);
+        for (int32_t i = page_start[b]; i < page_start[b + 1]; ++i)
+          HY_REQUIRE(pages[i] >= 0 && pages[i] < num_pages,
+                     "hy_kv_move: page %d is not in the pool of %d", pages[i], num_pages);
+      }
+      for (int32_t i = src_start[b]; i < src_start[b + 1]; ++i) {
+        const int64_t from = src[i] - base;
+        const int64_t to = static_cast<int64_t>(first[b]) + (i - src_start[b]) - base;
+        if (pass == 0)
+          HY_REQUIRE(to >= 0 && from >= to && from < held * page_size &&
+                         (i == src_start[b] || src[i] > src[i - 1]),
+                     "hy_kv_move: sequence %d cannot take its token %d to position %lld (sources "
+                     "ascend, none before the position it fills, all in the given pages)",
+                     b, src[i], static_cast<long long>(to + base));
+        if (from == to) continue;
+        const int32_t *list = pages + page_start[b];
+        const int64_t s = static_cast<int64_t>(list[from / page_size]) * page_size + from % page_size;
+        const int64_t d = static_cast<int64_t>(list[to / page_size]) * page_size + to % page_size;
+        if (pass == 0) {
+          HY_REQUIRE(!written.has(s) && !written.has(d),
+                     "hy_kv_move: sequence %d shares pages that are written", b);
+          written.set(d);
+          continue;
+        }
+        if (n_runs > 0 && s == last_src + 1 && d == last_dst + 1) {
+          ++n_rows;
+        } else {
+          if (n_runs == hy::kRuns)
+            if (int rc = launch()) return rc;
+          runs.r[n_runs++] = {static_cast<int32_t>(s), static_cast<int32_t>(d), n_rows++};
+        }
+        last_src = s;
+        last_dst = d;
+      }
     }
-    i = j;
-    if (n_runs == hy::kRuns)
-      if (int rc = launch()) return rc;
   }
   return n_runs ? launch() : HY_OK;
 }

@@ -464,47 +464,75 @@ namespace {
 
 // Cost of a piece of drafted-tree attention after a chunk's first, in key steps.
 constexpr int64_t kTreePieceCost = 1;
+// Cost of the merge launch in key steps: 4-5 us and a second launch's host time, against
+// 0.55 us for a step while few compute units run.
+constexpr int64_t kTreeMergeCost = 8;
 
 struct TreePieceRec {
   int32_t tile, step0, step1;  // query tile, and its key steps
 };
+// Chunk i holds pieces [ends[i - 1], ends[i]).
+struct TreeCut {
+  std::vector<TreePieceRec> pieces;
+  std::vector<int32_t> ends;
+  int64_t worst = 0;  // the costliest chunk
+  bool split = false;
+};
 
-// Cuts the key steps of the query tiles, in order, into at most n_chunks
-// chunks of equal cost: chunk i holds pieces [ends[i - 1], ends[i]). Returns
-// the costliest chunk's cost. `total` is what the whole stream is taken to cost.
-int64_t cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total,
-                 std::vector<TreePieceRec> &pieces, std::vector<int32_t> &ends) {
-  pieces.clear();
-  ends.clear();
-  int64_t spent = 0, in_chunk = 0, worst = 0;
+// Cuts the key steps of the query tiles, in order, into at most n_chunks chunks of
+// equal cost; `total` is what the whole stream is taken to cost.
+void cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total, TreeCut &cut) {
+  cut = TreeCut();
+  int64_t spent = 0, in_chunk = 0;
   int32_t first = 0;
+  auto size = [&]() { return static_cast<int32_t>(cut.pieces.size()); };
   auto close = [&]() {
-    worst = std::max(worst, in_chunk);
+    cut.worst = std::max(cut.worst, in_chunk);
     spent += in_chunk;
     in_chunk = 0;
-    first = static_cast<int32_t>(pieces.size());
-    ends.push_back(first);
+    first = size();
+    cut.ends.push_back(first);
   };
   for (size_t t = 0; t < steps.size(); ++t) {
     int32_t at = 0;
     while (at < steps[t]) {
-      const int64_t left = n_chunks - static_cast<int64_t>(ends.size());  // this one included
-      const int64_t share = left > 1 ? (std::max<int64_t>(total - spent, 1) + left - 1) / left : INT64_MAX;
-      const int64_t extra = static_cast<int32_t>(pieces.size()) > first ? kTreePieceCost : 0;
+      const int64_t left = n_chunks - static_cast<int64_t>(cut.ends.size());  // this one included
+      const int64_t share =
+          left > 1 ? (std::max<int64_t>(total - spent, 1) + left - 1) / left : INT64_MAX;
+      const int64_t extra = size() > first ? kTreePieceCost : 0;
       const int64_t room = share - in_chunk - extra;
-      if (room <= 0 && static_cast<int32_t>(pieces.size()) > first) {
+      if (room <= 0 && size() > first) {
         close();
         continue;
       }
       const int32_t n = static_cast<int32_t>(
           std::min<int64_t>(steps[t] - at, std::max<int64_t>(room, 1)));
-      pieces.push_back({static_cast<int32_t>(t), at, at + n});
+      cut.pieces.push_back({static_cast<int32_t>(t), at, at + n});
+      cut.split = cut.split || n < steps[t];
       in_chunk += n + extra;
       at += n;
     }
   }
-  if (static_cast<int32_t>(pieces.size()) > first) close();
-  return worst;
+  if (size() > first) close();
+}
+
+// The query tiles whole, in order, in at most n_chunks chunks of at most `most`; false if they
+// do not fit.
+bool whole_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t most, TreeCut &cut) {
+  cut = TreeCut();
+  int64_t in_chunk = 0;
+  for (size_t t = 0; t < steps.size(); ++t) {
+    if (steps[t] > most) return false;
+    if (in_chunk > 0 && in_chunk + kTreePieceCost + steps[t] > most) {
+      cut.ends.push_back(static_cast<int32_t>(t));
+      in_chunk = 0;
+    }
+    in_chunk += steps[t] + (in_chunk > 0 ? kTreePieceCost : 0);
+    cut.pieces.push_back({static_cast<int32_t>(t), 0, steps[t]});
+    cut.worst = std::max(cut.worst, in_chunk);
+  }
+  if (!steps.empty()) cut.ends.push_back(static_cast<int32_t>(steps.size()));
+  return static_cast<int64_t>(cut.ends.size()) <= n_chunks;
 }
 
 int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t G,
@@ -535,19 +563,29 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   const int64_t n_chunks =
       std::max<int64_t>(1, std::min<int64_t>((cus + num_kv_heads - 1) / num_kv_heads, all));
-  std::vector<TreePieceRec> pieces, trial;
-  std::vector<int32_t> ends, trial_ends;
-  int64_t worst = cut_tree(steps, n_chunks, all, pieces, ends);
-  for (int pass = 0; pass < 3 && !pieces.empty(); ++pass) {
-    const int64_t total = all + kTreePieceCost * static_cast<int64_t>(
-        (pass ? trial : pieces).size() - (pass ? trial_ends : ends).size());
-    const int64_t w = cut_tree(steps, n_chunks, total, trial, trial_ends);
-    if (w < worst) {
-      worst = w;
-      pieces = trial;
-      ends = trial_ends;
+  TreeCut best, trial;
+  cut_tree(steps, n_chunks, all, best);
+  int64_t total = all;
+  for (int pass = 0; pass < 3; ++pass) {
+    const TreeCut &last = pass ? trial : best;
+    total = all + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
+    cut_tree(steps, n_chunks, total, trial);
+    if (trial.worst < best.worst) best = trial;
+  }
+  // Tiles that need no merge are worth a longer chunk; the shortest such chunk by bisection.
+  if (best.split) {
+    int64_t fits = best.worst + kTreeMergeCost, low = 0;
+    while (low < fits && whole_tree(steps, n_chunks, fits, trial)) {
+      best = trial;
+      const int64_t mid = low + (fits - low) / 2;
+      if (whole_tree(steps, n_chunks, mid, trial))
+        fits = mid;
+      else
+        low = mid + 1;
     }
   }
+  const std::vector<TreePieceRec> &pieces = best.pieces;
+  const std::vector<int32_t> &ends = best.ends;
   const int64_t need = 2 * static_cast<int64_t>(ends.size()) + static_cast<int64_t>(pieces.size());
   if (need > item_capacity) {
     hy::set_error("hy_plan_tree: item capacity %d too small (need %lld)", item_capacity,

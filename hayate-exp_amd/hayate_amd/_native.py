@@ -132,7 +132,7 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "hy_kv_move": (
-        [_P, _P, _I64, _I64, _I64, _P, _P, _I32, _I32, _I32, _I32, _P],
+        [_P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P],
         ctypes.c_int,
     ),
     "hy_page_copy": (

@@ -132,7 +132,7 @@ def _int_array(values, what: str) -> np.ndarray:
 
 def _current_device(device: torch.device):
     """Makes `device` current for a launch, which goes to its current stream."""
-    if device.index is None or torch.cuda.current_device() == device.index:
+    if device.type != "cuda" or torch.cuda.current_device() == device.index:
         return contextlib.nullcontext()
     return torch.cuda.device(device)
 
@@ -715,7 +715,7 @@ class PagedTreeBatch(PagedKVBatch):
                 np.asarray(self.q_lens, dtype=np.int32),
                 np.asarray(self.kv_lens_host, dtype=np.int32), num_q_heads, self.num_kv_heads,
                 self._num_cus)
-            cached = _DeviceTreePlan(host, self.num_kv_heads, self.head_dim, self.device)
+            cached = _DeviceTreePlan(host, self, num_q_heads)
             self._tree_plans[num_q_heads] = cached
         return cached
 
@@ -742,18 +742,27 @@ class PagedTreeBatch(PagedKVBatch):
             raise ValueError("query heads must be a multiple of kv heads")
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):  # the launch goes to its current stream
+                return self.attend_layer(q, layer_idx, scale)
         plan = self.plan(num_q_heads)
         out = torch.empty((self.total_tokens, num_q_heads, self.head_dim), dtype=q.dtype,
                           device=q.device)
-        k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
+        stream = _stream_handle(self.device)
+        plan.used_on(stream)
         self._launch("hy_paged_tree", _native.lib().hy_paged_tree,
-            q.data_ptr(), *qs, out.data_ptr(), 0, out.stride(0), out.stride(1), k_ptr, v_ptr, hs,
-            self._pt_ptr, self._pt_stride, self._lines_ptr, self.line_words, plan.items_ptr,
-            plan.n_chunks, plan.max_rows, plan.merge_ptr, plan.n_merge, plan.n_slots,
-            plan.workspace_ptr, plan.workspace_bytes, num_q_heads, self.num_kv_heads,
-            self.head_dim, self.page_size, float(scale), _stream_handle(self.device),
+            q.data_ptr(), *qs, out.data_ptr(), 0, num_q_heads * self.head_dim, self.head_dim,
+            *self._layer_pools(layer_idx), *plan.args, float(scale), stream,
         )
         return out
+
+    def norm_rope_write_layer(self, *args, **kwargs) -> torch.Tensor:
+        """As in a ``begin_tick`` batch, with every node rotated at its ``positions``
+        entry instead of its slot's."""
+        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return super().norm_rope_write_layer(*args, **kwargs)
+        return super().norm_rope_write_layer(*args, **kwargs)
 
     def check_path(self, seq: int, path: Sequence[int]) -> list[int]:
         """`path` as ints, if it is one: nodes of request `seq` from a child of the
@@ -773,24 +782,32 @@ class PagedTreeBatch(PagedKVBatch):
 class _DeviceTreePlan:
     """One tree tick's work lists on the device plus its split workspace."""
 
-    def __init__(self, host: "_native.TreePlan", num_kv_heads: int, head_dim: int,
-                 device: torch.device):
+    def __init__(self, host: "_native.TreePlan", batch: PagedTreeBatch, num_q_heads: int):
+        device, kv_heads, dim = batch.device, batch.num_kv_heads, batch.head_dim
         self.host = host
-        self.n_chunks = host.n_chunks
-        self.n_merge = len(host.merge)
-        self.n_slots = host.n_slots
-        self.max_rows = host.max_rows
+        self.batch_meta = batch._meta
         packed = np.concatenate([host.items.reshape(-1), host.merge.reshape(-1)])
         self.lists = torch.from_numpy(packed).to(device)
-        self.items_ptr = self.lists.data_ptr()
-        self.merge_ptr = self.items_ptr + 4 * host.items.size if self.n_merge else None
-        self.workspace_bytes = _native.tree_workspace_bytes(self.n_slots, num_kv_heads, head_dim)
-        self.workspace = (
-            torch.empty(self.workspace_bytes // 4, dtype=torch.float32, device=device)
-            if self.workspace_bytes
-            else None
-        )
-        self.workspace_ptr = None if self.workspace is None else self.workspace.data_ptr()
+        items = self.lists.data_ptr()
+        size = _native.tree_workspace_bytes(host.n_slots, kv_heads, dim)
+        self.workspace = (torch.empty(size // 4, dtype=torch.float32, device=device)
+                          if size else None)
+        self.stream = _stream_handle(device)
+        n_merge = len(host.merge)
+        # the call's arguments between the pools and the scale
+        self.args = (
+            batch._pt_ptr, batch._pt_stride, batch._lines_ptr, batch.line_words, items,
+            host.n_chunks, host.max_rows, items + 4 * host.items.size if n_merge else None, n_merge,
+            host.n_slots, None if self.workspace is None else self.workspace.data_ptr(), size,
+            num_q_heads, kv_heads, dim, batch.page_size)
+
+    def used_on(self, stream: int) -> None:
+        """Keeps the lists' and the workspace's memory from reuse while `stream`, the current
+        one, may still read them, if it is not the one they were made on."""
+        if stream != self.stream:
+            for t in (self.batch_meta, self.lists, self.workspace):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(t.device))
 
 
 class PagedKVCacheManager:
@@ -1157,39 +1174,60 @@ class PagedKVCacheManager:
             raise RuntimeError("cannot move tokens of a released cache handle")
         if len({id(h) for h in handles}) != len(handles):
             raise ValueError("the same cache handle is given twice")
-        moves, spans = [], []
+        lists, firsts, wanted = [], [], []
         for h, source, start in zip(handles, sources, starts):
             src, start = _int_array(source, "sources"), _index(start, "a start")
             if start < 0:
                 raise ValueError("starts must be non-negative")
-            if not len(src):
+            n = len(src)
+            if n == 0 or (src[n - 1] == start + n - 1 and src[0] == start):
+                # nothing moves if they ascend, which alone is left to check
+                if n > 1 and (np.diff(src) <= 0).any():
+                    raise ValueError("sources must ascend, none before the position it fills")
+                if n and src[n - 1] >= len(h.pages) * self.page_size:
+                    raise ValueError(f"position {src[n - 1]} is past the cache's reserved space")
                 continue
-            dst = np.arange(start, start + len(src))
-            if (np.diff(src) <= 0).any() or src[0] < start:
-                raise ValueError("sources must ascend, none before the position it fills")
-            if src[-1] >= len(h.pages) * self.page_size:
-                raise ValueError(f"position {src[-1]} is past the cache's reserved space")
-            # ascending on both sides, so the tokens that stay are the first ones
-            stay = int(np.count_nonzero(src == dst))
-            if stay < len(src):
-                moves.append((h, src[stay:], dst[stay:]))
+            lists.append(src)
+            firsts.append(start)
+            wanted.append(h)
+        if not lists:
+            return
+        ps, refs = self.page_size, self._refs
+        ends = [start + len(src) for start, src in zip(firsts, lists)]
+        if any(refs[p] > 1 for h, a, b in zip(wanted, firsts, ends)
+               for p in h.pages[a // ps : -(-b // ps)]):
+            spans = []
+            for h, src, start in zip(wanted, lists, firsts):
+                dst = np.arange(start, start + len(src))
+                if ((np.diff(src) <= 0).any() or src[0] < start
+                        or src[-1] >= len(h.pages) * ps):
+                    raise ValueError("sources must ascend, none before the position it fills, "
+                                     "all in the cache's reserved space")
+                # ascending on both sides, so the tokens that stay are the first ones
+                stay = int(np.count_nonzero(src == dst))
                 spans.append((h, start + stay, start + len(src),
                               max(h.length, int(src[-1]) + 1)))
-        if not moves:
-            return
-        self._make_all_private(spans)
-        rows = []
-        for h, *ends in moves:
-            pages = np.asarray(h.pages, dtype=np.int64)
-            rows.append([pages[x // self.page_size] * self.page_size + x % self.page_size
-                         for x in ends])
-        src, dst = (np.ascontiguousarray(np.concatenate(x), dtype=np.int32) for x in zip(*rows))
+            self._make_all_private(spans)
+        # the pages from the first written to the last read
+        pages, page_start, src_start = [], [0], [0]
+        first_page = [start // ps for start in firsts]
+        for h, src, page in zip(wanted, lists, first_page):
+            pages += h.pages[page : int(src[-1]) // ps + 1]
+            page_start.append(len(pages))
+            src_start.append(src_start[-1] + len(src))
+        lists = np.concatenate(lists)
+        if lists.min() < 0 or lists.max() >= self.capacity_tokens:
+            raise ValueError(f"positions lie in 0 .. {self.capacity_tokens - 1}")
+        n = len(wanted)
+        meta = np.array(page_start + src_start + first_page + firsts + pages, dtype=np.int32)
+        src, at = lists.astype(np.int32), meta.ctypes.data
         with _current_device(self.device):
             rc = _native.lib().hy_kv_move(
                 self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_cache.stride(0),
-                self.k_cache.stride(2), self.capacity_tokens, src.ctypes.data, dst.ctypes.data,
-                len(src), self.num_layers, self.num_kv_heads, self.head_dim,
-                _stream_handle(self.device),
+                self.k_cache.stride(2), self.num_pages, at + 4 * (4 * n + 2), at,
+                at + 4 * (2 * n + 2), src.ctypes.data, at + 4 * (n + 1), at + 4 * (3 * n + 2), n,
+                self.num_layers, self.num_kv_heads, self.head_dim, ps,
+                _stream_handle(self.device) if self.device.type == "cuda" else None,
             )
         _native.check(rc, "hy_kv_move")
 

@@ -508,19 +508,22 @@ int hy_paged_tree(const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
                   int32_t page_size, float scale, void *stream);
 
 /*
- * Token moves: for i in order, pool[l, h, dst[i]] = pool[l, h, src[i]] for every layer
- * l and kv head h of the K and the V pool. src and dst are host arrays of n physical
- * tokens (page * page_size + offset), read before the call returns and checked:
- * indexes below pool_tokens, no token written twice, none read after an earlier
- * move wrote it (a token may be written after it was read, so a sequence can be moved
- * forward over itself); otherwise HY_EINVAL and nothing is enqueued. Consecutive moves
- * of consecutive tokens are taken together.
+ * Token moves: position first[b] + i of sequence b takes the K and V of its position
+ * src[src_start[b] + i], in every layer and kv head, as if all were read before any is
+ * written. Its logical pages first_page[b], first_page[b] + 1, ... are pages[page_start[b]
+ * .. page_start[b + 1]); page_start and src_start have num_seqs + 1 entries. All arrays are
+ * host memory, read before the call returns and checked: positions inside the given
+ * pages, page ids below num_pages, sources ascending and none before the position it fills,
+ * no written token read or written for another sequence; otherwise HY_EINVAL and nothing
+ * is enqueued. Tokens that stay cost nothing; runs of tokens are moved together.
  * No reference counterpart (its caches only grow or are cut, paged_cache.py:168-178).
  */
 int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
-               int64_t pool_head_stride, int64_t pool_tokens,
-               const int32_t *src, const int32_t *dst, int32_t n,
-               int32_t num_layers, int32_t num_kv_heads, int32_t head_dim,
+               int64_t pool_head_stride, int32_t num_pages, const int32_t *pages,
+               const int32_t *page_start, const int32_t *first_page,
+               const int32_t *src, const int32_t *src_start,
+               const int32_t *first, int32_t num_seqs, int32_t num_layers,
+               int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                void *stream);
 
 /*

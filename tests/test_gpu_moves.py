@@ -257,14 +257,14 @@ def test_a_refused_call_enqueues_nothing():
     before = [bits(p).clone() for p in (m.k_cache, m.v_cache)]
     lib = _native.lib()
 
-    def move(src, dst, tokens=m.capacity_tokens):
-        src, dst = np.array(src, dtype=np.int32), np.array(dst, dtype=np.int32)
+    def move(src, first):
+        a = [np.array(x, dtype=np.int32) for x in
+             (h.pages, [0, len(h.pages)], [0], src, [0, len(src)], [first])]
         return lib.hy_kv_move(m.k_cache.data_ptr(), m.v_cache.data_ptr(), m.k_cache.stride(0),
-                              m.k_cache.stride(2), tokens, src.ctypes.data, dst.ctypes.data,
-                              len(src), 2, 8, D, None)
+                              m.k_cache.stride(2), m.num_pages, *(x.ctypes.data for x in a), 1, 2,
+                              8, D, m.page_size, None)
 
-    for src, dst in (([5, 6], [4, -1]), ([m.capacity_tokens], [0]), ([5, 4], [4, 3]),
-                     ([5, 6], [9, 9])):
-        assert move(src, dst) == _native.HY_EINVAL
+    for src, first in (([5, 384], 4), ([5, 4], 0), ([7, 9, 9], 1), ([3, 4], 4)):
+        assert move(src, first) == _native.HY_EINVAL
     torch.cuda.synchronize()
     assert same([bits(m.k_cache), bits(m.v_cache)], before)

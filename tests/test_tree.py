@@ -272,32 +272,49 @@ def c_arrays(*lists):
     return [(ctypes.c_int32 * max(1, len(x)))(*x) for x in lists]
 
 
-@pytest.mark.parametrize("src,dst", [([0, 1], [5, 5]), ([0, 5], [5, 6]), ([-1], [3]), ([3], [-1]),
-                                     ([1000], [3]), ([3], [1000]), ([2, 1], [1, 0])])
-def test_c_moves_are_checked_before_any_launch(src, dst):
-    lib = _native.lib()
-    a, b = c_arrays(src, dst)
-    call = lambda **kw: lib.hy_kv_move(4096, 4096, 8 * 1000 * 128, 1000 * 128, 1000, a, b,  # noqa: E731
-                                       len(src), kw.get("layers", 2), 8, kw.get("dim", 128), None)
-    assert call() == _native.HY_EINVAL and _native.last_error()
-    assert call(layers=0) == _native.HY_EINVAL
-    assert call(dim=64) == _native.HY_EUNSUPPORTED
+def c_move(pages, src, first, page_start=None, src_start=None, first_page=None, **kw):
+    """hy_kv_move on a pool of 8 pages of 128 that is never touched."""
+    n = len(first)
+    args = c_arrays(pages, page_start or [0, len(pages)], first_page or [0] * n, src,
+                    src_start or [0, len(src)], first)
+    args = {**dict(k=4096, v=4096, ls=8 * 1024 * 128, hs=1024 * 128, num_pages=8),
+            **dict(zip(("p_pages", "p_start", "p_first", "p_src", "p_ss", "p_to"), args)),
+            **dict(n=n, layers=2, heads=8, dim=128, page=128, stream=None), **kw}
+    return _native.lib().hy_kv_move(*args.values())
+
+
+def test_c_moves_are_checked_before_any_launch():
+    bad = [
+        ([0, 1], [5, 5], [0]), ([0, 1], [6, 5], [0]), ([0, 1], [3], [4]), ([0, 1], [256], [0]),
+        ([0, 1], [-1], [-2]), ([0, 8], [200], [0]), ([0, -1], [200], [0]), ([], [1], [0]),
+    ]
+    for pages, src, first in bad:
+        assert c_move(pages, src, first) == _native.HY_EINVAL, (pages, src, first)
+        assert _native.last_error()
+    # one page twice: position 128 is position 0, which the first of these moves wrote
+    assert c_move([0, 0], [2, 128], [0]) == _native.HY_EINVAL
+    # two sequences that write one page, or one that reads what the other wrote
+    two = dict(page_start=[0, 1, 2], src_start=[0, 1, 2])
+    assert c_move([3, 3], [5, 5], [1, 1], **two) == _native.HY_EINVAL
+    assert c_move([3, 3], [5, 1], [1, 0], **two) == _native.HY_EINVAL
+    assert c_move([3, 4], [5, 5], [1, 1], page_start=[0, 1, 0], src_start=[0, 1, 2]) == _native.HY_EINVAL
+    assert c_move([3, 4], [5, 5], [1, 1], page_start=[0, 1, 2], src_start=[0, 2, 1]) == _native.HY_EINVAL
+    # positions count from the first page given
+    assert c_move([3], [5], [1], first_page=[1]) == _native.HY_EINVAL
+    assert c_move([3], [5], [1], first_page=[-1]) == _native.HY_EINVAL
+    # tokens that stay need no launch
+    assert c_move([0, 1], [7, 8, 130][:2], [7]) == _native.HY_OK
+    assert c_move([3], [130, 131], [130], first_page=[1]) == _native.HY_OK
+    assert c_move([], [], []) == _native.HY_OK
 
 
 def test_c_pools_are_checked():
-    lib = _native.lib()
-    a, b = c_arrays([1], [0])
-    good = [4096, 4096, 8 * 1000 * 128, 1000 * 128, 1000, a, b, 1, 2, 8, 128, None]
-    for at, bad in ((0, None), (1, None), (0, 4098), (2, 1000 * 128), (3, 128), (3, 1000 * 128 + 4),
-                    (4, 0), (4, 1 << 31), (5, None), (6, None), (7, -1), (9, 0)):
-        args = list(good)
-        args[at] = bad
-        assert lib.hy_kv_move(*args) == _native.HY_EINVAL, (at, bad)
-    assert lib.hy_kv_move(*good[:7], 0, *good[8:]) == _native.HY_OK  # nothing to move
-    # a token that stays is no write: reading it afterwards is allowed, so only the range is at fault
-    a, b = c_arrays([1, 1, 2000], [1, 0, 3])
-    assert lib.hy_kv_move(*good[:5], a, b, 3, *good[8:]) == _native.HY_EINVAL
-    assert "move 2" in _native.last_error()
+    for kw in (dict(k=None), dict(v=None), dict(k=4098), dict(ls=1024 * 128), dict(hs=128),
+               dict(hs=1024 * 128 + 4), dict(num_pages=0), dict(num_pages=1 << 24), dict(p_pages=None),
+               dict(p_start=None), dict(p_first=None), dict(p_src=None), dict(p_ss=None), dict(p_to=None),
+               dict(n=-1), dict(layers=0), dict(heads=0), dict(page=0), dict(layers=1 << 23)):
+        assert c_move([0, 1], [5], [3], **kw) == _native.HY_EINVAL, kw
+    assert c_move([0, 1], [5], [3], dim=64) == _native.HY_EUNSUPPORTED
 
 
 @pytest.mark.parametrize("src,dst,tokens", [([0, 1], [2, 2], None), ([0, 1], [1, 2], None),
