@@ -41,7 +41,8 @@ __device__ __forceinline__ uint16_t *unit_base(uint16_t *k_pool, uint16_t *v_poo
 // kRowsPerPass rows a step: a step's rows are all loaded before the first of them is
 // stored (a row may be the target of a later row of the same step), and the
 // host has checked that no row is read after it was written, so the next step's
-// loads go out before this step's stores.
+// loads go out before this step's stores. 5,999 tokens of 36 layers (1.77 GB): 378 us,
+// 4.7 TB/s, 95 % of what a large copy reaches; 2 or 8 passes a step 394 and 415 us.
 constexpr int kMovePasses = 4;
 constexpr int kStepRows = kMovePasses * kRowsPerPass;
 
@@ -54,7 +55,19 @@ __global__ __launch_bounds__(kThreads) void move_kernel(uint16_t *k_pool, uint16
   uint16_t *base = unit_base(k_pool, v_pool, ls, hs, blockIdx.x, num_kv_heads) +
                    8 * (threadIdx.x & 15);
   const int group = threadIdx.x >> 4;
-  int at = 0;  // run of this lane group's latest row
+  // Run of a row: the last one that begins at or before it, by bisection (single tokens make
+  // as many runs as rows).
+  auto run_of = [&](int row) {
+    int lo = 0, hi = n_runs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (run[mid].n <= row)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return run[lo];
+  };
   u32x4 cur[kMovePasses], nxt[kMovePasses];
   int64_t cur_dst[kMovePasses], nxt_dst[kMovePasses];
   auto load = [&](int row0, u32x4(&x)[kMovePasses], int64_t(&dst)[kMovePasses]) {
@@ -63,10 +76,9 @@ __global__ __launch_bounds__(kThreads) void move_kernel(uint16_t *k_pool, uint16
       const int row = row0 + j * kRowsPerPass + group;
       dst[j] = -1;
       if (row >= n_rows) continue;
-      while (at + 1 < n_runs && run[at + 1].n <= row) ++at;
-      const int o = row - run[at].n;
-      dst[j] = static_cast<int64_t>(run[at].dst + o) * kHeadDim;
-      x[j] = load16(base + static_cast<int64_t>(run[at].src + o) * kHeadDim);
+      const Run at = run_of(row);
+      dst[j] = static_cast<int64_t>(at.dst + row - at.n) * kHeadDim;
+      x[j] = load16(base + static_cast<int64_t>(at.src + row - at.n) * kHeadDim);
     }
   };
   load(0, cur, cur_dst);
@@ -88,7 +100,10 @@ __global__ __launch_bounds__(kThreads) void move_kernel(uint16_t *k_pool, uint16
 }
 
 // Copies. Sources and targets are distinct pages, so nothing is ordered: one
-// workgroup per (unit, record), 128 rows (32 KiB) in flight.
+// workgroup per (unit, record), 128 rows (32 KiB) in flight. Nontemporal on both
+// sides: 15 pages of 77 tokens in 36 layers (341 MB read and written) 65.9 us against 70.4, 32
+// pages 232 against 238; a large torch copy moves 4.94 TB/s, these 5.1. (In the moves it
+// gave nothing.)
 constexpr int kCopyPasses = 8;
 
 __global__ __launch_bounds__(kThreads) void copy_kernel(uint16_t *k_pool, uint16_t *v_pool,
@@ -104,11 +119,12 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(uint16_t *k_pool, uint16
 #pragma unroll
     for (int j = 0; j < kCopyPasses; ++j)
       if (row0 + j * kRowsPerPass < r.n)
-        x[j] = load16(src + (row0 + j * kRowsPerPass) * kHeadDim);
+        x[j] = load16_stream(src + (row0 + j * kRowsPerPass) * kHeadDim);
 #pragma unroll
     for (int j = 0; j < kCopyPasses; ++j)
       if (row0 + j * kRowsPerPass < r.n)
-        store16(dst + (row0 + j * kRowsPerPass) * kHeadDim, x[j]);
+        __builtin_nontemporal_store(
+            x[j], reinterpret_cast<u32x4 *>(dst + (row0 + j * kRowsPerPass) * kHeadDim));
   }
 }
 

@@ -658,6 +658,38 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
 
 }  // namespace
 
+extern "C" int hy_tree_lines(const int32_t *parents, const int32_t *q_lens, int32_t num_seqs,
+                             int32_t line_words, uint32_t *lines, int32_t *depths) {
+  hy::clear_error();
+  if (num_seqs < 0 || (num_seqs > 0 && (!parents || !q_lens || !lines || !depths)) ||
+      (line_words != 4 && line_words != 8)) {
+    hy::set_error("hy_tree_lines: invalid arrays");
+    return HY_EINVAL;
+  }
+  int64_t row = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    if (q_lens[b] < 1 || q_lens[b] > 32 * line_words) {
+      hy::set_error("hy_tree_lines: tree %d has %d nodes, not 1 to %d", b, q_lens[b],
+                    32 * line_words);
+      return HY_EINVAL;
+    }
+    const int64_t first = row;
+    for (int32_t i = 0; i < q_lens[b]; ++i, ++row) {
+      const int32_t p = parents[row];
+      if (p < -1 || p >= i) {
+        hy::set_error("hy_tree_lines: tree %d: the parent of node %d is %d, not an earlier node or -1",
+                      b, i, p);
+        return HY_EINVAL;
+      }
+      for (int32_t w = 0; w < line_words; ++w)
+        lines[row * line_words + w] = p < 0 ? 0u : lines[(first + p) * line_words + w];
+      lines[row * line_words + (i >> 5)] |= 1u << (i & 31);
+      depths[row] = p < 0 ? 0 : depths[first + p] + 1;
+    }
+  }
+  return HY_OK;
+}
+
 extern "C" int32_t hy_tree_max_nodes(void) { return hy::kTreeMaxNodes; }
 
 extern "C" int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs,

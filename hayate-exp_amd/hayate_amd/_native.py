@@ -121,6 +121,7 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "hy_tree_max_nodes": ([], ctypes.c_int32),
+    "hy_tree_lines": ([_P, _P, _I32, _I32, _P, _P], ctypes.c_int),
     "hy_plan_tree": (
         [_P, _P, _I32, _I32, _I32, _I32, _P, _I32, _P, _I32, _P],
         ctypes.c_int,
@@ -268,6 +269,17 @@ def decode_workspace_bytes(n_slots: int, num_q_heads: int, head_dim: int) -> int
 
 def prefill_workspace_bytes(n_slots: int, num_kv_heads: int, head_dim: int) -> int:
     return int(lib().hy_prefill_workspace_bytes(n_slots, num_kv_heads, head_dim))
+
+
+def tree_lines(parents: np.ndarray, q_lens: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """Lines (nodes, words) and depths of packed trees; the words are whole 16-byte units."""
+    words = 4 * -(-int(q_lens.max()) // 128)
+    lines = np.empty((len(parents), words), dtype=np.uint32)
+    depths = np.empty(len(parents), dtype=np.int32)
+    rc = lib().hy_tree_lines(parents.ctypes.data, q_lens.ctypes.data, len(q_lens), words,
+                             lines.ctypes.data, depths.ctypes.data)
+    check(rc, "hy_tree_lines")
+    return lines, depths
 
 
 class TreePlan:

@@ -675,31 +675,24 @@ class PagedTreeBatch(PagedKVBatch):
     included, are not run at the same time on two streams.
     """
 
-    def __init__(self, manager: "PagedKVCacheManager", parents: list[list[int]],
+    def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],
-                 num_q_heads: Optional[int]):
-        q_lens = [len(p) for p in parents]
-        self.parents = parents
-        # a node's line: a bit for each drafted slot, in whole 16-byte units
-        self.line_words = 4 * -(-max(q_lens) // 128)
-        depths, lines = [], np.zeros((sum(q_lens), self.line_words), dtype=np.uint32)
-        row = 0
-        for tree in parents:
-            first = row
-            for i, p in enumerate(tree):
-                if p >= 0:
-                    lines[row] = lines[first + p]
-                lines[row, i >> 5] |= np.uint32(1 << (i & 31))
-                depths.append(depths[first + p] + 1 if p >= 0 else 0)
-                row += 1
-        positions = np.repeat(np.asarray(cache_lens_host, dtype=np.int32), q_lens)
-        positions += np.asarray(depths, dtype=np.int32)
+                 num_q_heads: Optional[int], lines: Optional[tuple] = None):
+        self.parents = [np.asarray(p) for p in parents]
+        q_lens = [len(p) for p in self.parents]
+        # a node's line: a bit for each drafted slot it sees
+        lines, depths = lines or _native.tree_lines(
+            np.concatenate(self.parents).astype(np.int32), np.array(q_lens, dtype=np.int32))
+        self.line_words = lines.shape[1]
+        positions = depths + np.repeat(np.asarray(cache_lens_host, dtype=np.int32), q_lens)
         self._tree_plans: dict[int, _DeviceTreePlan] = {}
         super().__init__(manager, q_lens, cache_lens_host, page_lists, varlen=True,
                          num_q_heads=None,
                          extra=np.concatenate([lines.reshape(-1).view(np.int32), positions]))
         # every tree goes through the tree kernel, requests with one node included
         self.decode_only = False
+        # rope positions go by depth, so a wide tree needs fewer than its slots
+        self._max_kv = int(positions.max()) + 1
         self.lines = self._extra[: lines.size]
         self.positions = self._extra[lines.size :]
         self._lines_ptr = self.lines.data_ptr()
@@ -767,7 +760,7 @@ class PagedTreeBatch(PagedKVBatch):
     def check_path(self, seq: int, path: Sequence[int]) -> list[int]:
         """`path` as ints, if it is one: nodes of request `seq` from a child of the
         cached context down, each the parent of the next (empty: nothing accepted)."""
-        tree, last, nodes = self.parents[seq], -1, []
+        tree, last, nodes = self.parents[seq].tolist(), -1, []
         for i in path:
             i = _index(i, "a node")
             if not 0 <= i < len(tree) or tree[i] != last:
@@ -1263,15 +1256,20 @@ class PagedKVCacheManager:
         most = int(_native.lib().hy_tree_max_nodes())
         trees = []
         for tree in parents:
-            tree = _int_array(tree, "a tree's parents").tolist()
-            if not 1 <= len(tree) <= most:
-                raise ValueError(f"a tree has 1 to {most} nodes, not {len(tree)}")
-            if any(not -1 <= p < i for i, p in enumerate(tree)):
-                raise ValueError("a node's parent is an earlier node, or -1")
+            tree = _int_array(tree, "a tree's parents")
+            n = len(tree)
+            if not 1 <= n <= most:
+                raise ValueError(f"a tree has 1 to {most} nodes, not {n}")
             trees.append(tree)
+        nodes = np.concatenate(trees)
+        if nodes.min() < -1 or nodes.max() >= most:
+            raise ValueError("a node's parent is an earlier node, or -1")
+        # (finds the other bad parents, before anything is reserved)
+        lines = _native.tree_lines(nodes.astype(np.int32),
+                                   np.array([len(t) for t in trees], dtype=np.int32))
         self.reserve_tick(handles, [len(t) for t in trees])
         return PagedTreeBatch(self, trees, [h.length for h in handles],
-                              [list(h.pages) for h in handles], self.num_q_heads)
+                              [list(h.pages) for h in handles], self.num_q_heads, lines)
 
     def commit_tree(self, handles: Sequence[PagedCacheHandle], batch: PagedTreeBatch,
                     accepted: Sequence[Sequence[int]]) -> None:

@@ -453,6 +453,16 @@ int hy_qknorm_rope_append_at(
 int32_t hy_tree_max_nodes(void);
 
 /*
+ * The lines and depths of trees (host only): parents holds, for each packed node, its
+ * parent's index within its own tree (an earlier node) or -1 for a child of the cached context.
+ * lines (line_words 32-bit words, 4 or 8, a node) receives the ancestors and the node
+ * itself as bits, depths the number of ancestors. HY_EINVAL for a parent that is no earlier
+ * node or a tree of more nodes than a line has bits.
+ */
+int hy_tree_lines(const int32_t *parents, const int32_t *q_lens, int32_t num_seqs,
+                  int32_t line_words, uint32_t *lines, int32_t *depths);
+
+/*
  * Planner of hy_paged_tree (host only): q_lens[b] >= 1 nodes on kv_lens[b] -
  * q_lens[b] cached tokens. The (node, query head) rows of a sequence form query
  * tiles of at most 256 rows per kv head; the 64-key steps of all tiles, in order,

@@ -124,6 +124,22 @@ def test_plan_refusals():
     assert call([3], [10000], merges=0) == _native.HY_ENOSPACE
 
 
+def test_lines_refusals():
+    def call(parents, q_lens, words=4):
+        p, q = np.array(parents, np.int32), np.array(q_lens, np.int32)
+        lines, depths = np.zeros((len(p), 8), np.uint32), np.zeros(len(p), np.int32)
+        return _native.lib().hy_tree_lines(p.ctypes.data, q.ctypes.data, len(q), words,
+                                           lines.ctypes.data, depths.ctypes.data)
+
+    assert call([-1, 0, 0], [3]) == _native.HY_OK
+    assert call([-1, 0, -1, 0], [2, 2]) == _native.HY_OK
+    for parents, q, words in (([-1, 1], [2], 4), ([0], [1], 4), ([-1, -2], [2], 4),
+                              ([-1, 0, 1], [2, 1], 4), (chain(129), [129], 4), ([], [0], 4),
+                              ([-1], [1], 3), ([-1], [1], 12)):
+        assert call(parents, q, words) == _native.HY_EINVAL
+    assert call(chain(256), [256], 8) == _native.HY_OK
+
+
 # ---------------------------------------------------------------- metadata
 @pytest.mark.parametrize("sizes", [[1], [3, 40], [256, 1, 33]])
 def test_batch_metadata(sizes):
