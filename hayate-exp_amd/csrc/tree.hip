@@ -42,7 +42,6 @@ constexpr int kStage = 2 * kTile * kHeadDim;  // halfs per stage: K tile, then V
 constexpr int kStages = 4;
 constexpr int kMaskWords = kTreeMaxNodes / 32;
 
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -51,12 +50,11 @@ __device__ __forceinline__ s16x4 tr_read(const uint16_t *p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(const_cast<uint16_t *>(p)));
 }
 
-// 16 bytes from each lane's own address straight into LDS: lane l's land at lds + 16 l
-// (lds wave-uniform, through M0, with the wait state the ISA asks for between
-// its write and the load). The caller waits (wait_loads) before it reads them.
-// Four of them with the instruction's offset, which counts on both sides: 4 KiB (16 rows)
-// from rows + off[i] + 1024 i to lds + 1024 i + 16 l, for one M0. kStream:
-// nontemporal, for lines that no other workgroup reads.
+// 16 rows of 256 bytes (4 KiB) from rows + off[i] + 1024 i (lane l's own off) straight to LDS at
+// lds + 1024 i + 16 l, four instructions for one M0: the instruction's offset counts on both
+// sides. lds is wave-uniform, through M0, with the wait state the ISA asks for between its write
+// and the load. The caller waits (wait_loads) before it reads them. kStream: nontemporal, for
+// lines that no other workgroup reads.
 template <bool kStream>
 __device__ __forceinline__ void load_rows_to_lds(const uint16_t *rows, const uint32_t (&off)[4],
                                                  const uint16_t *lds) {
@@ -91,6 +89,7 @@ __device__ __forceinline__ void load_rows_to_lds(const uint16_t *rows, const uin
         : "memory");
 }
 
+// 16 bytes from each lane's own address to lds + 16 l.
 __device__ __forceinline__ void load_to_lds(const uint16_t *g, const uint16_t *lds) {
   const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (const __attribute__((address_space(3))) uint16_t *)lds));
@@ -460,30 +459,6 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
   // free once every wave has left it, until the loads that follow the next barrier.
   auto finish = [&](uint16_t *stage) __attribute__((always_inline)) {
     const int lane_ = here(lane), c_ = lane_ & 31, h_ = lane_ >> 5, r_ = 32 * rw + c_;
-    if (ks == 0 && wave_live) {
-      // infinities and NaN of marked slots (none, as a rule), from the pool
-      for (int w = 0; w < line_words; ++w) {
-        uint32_t marks = __builtin_amdgcn_readfirstlane(sick[w]);
-        while (marks != 0) {
-          const int bit = __builtin_ctz(marks), key = cp.cache + 32 * w + bit;
-          marks &= marks - 1;
-          const bool sees = live && own_line[(r_ >> group_shift) * line_words + w] >> bit & 1;
-          const int64_t row =
-              (static_cast<int64_t>(page_table[cp.seq * pt_stride + (key >> page_shift)]) << page_shift) +
-              (key & page_mask);
-          const uint16_t *v = vh + row * kHeadDim + 4 * h_;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(v + 8 * j);
-            const float value[4] = {bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (sees && (__float_as_uint(value[e]) & 0x7f800000u) == 0x7f800000u)
-                acc[j >> 2][4 * (j & 3) + e] += value[e];
-          }
-        }
-      }
-    }
     float l = halves_sum(l_run);
     if constexpr (KS == 2) {
       float *box = reinterpret_cast<float *>(stage) + 4096 * rw + 4 * lane_;
@@ -516,7 +491,30 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
         }
       }
     }
-    if (ks != 0 || !wave_live || !live) return;
+    if (ks != 0 || !wave_live) return;
+    // infinities and NaN of marked slots (none, as a rule), from the pool
+    for (int w = 0; w < line_words; ++w) {
+      uint32_t marks = __builtin_amdgcn_readfirstlane(sick[w]);
+      while (marks != 0) {
+        const int bit = __builtin_ctz(marks), key = cp.cache + 32 * w + bit;
+        marks &= marks - 1;
+        const bool sees = live && own_line[(r_ >> group_shift) * line_words + w] >> bit & 1;
+        const int64_t row =
+            (static_cast<int64_t>(page_table[cp.seq * pt_stride + (key >> page_shift)]) << page_shift) +
+            (key & page_mask);
+        const uint16_t *v = vh + row * kHeadDim + 4 * h_;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(v + 8 * j);
+          const float value[4] = {bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sees && (__float_as_uint(value[e]) & 0x7f800000u) == 0x7f800000u)
+              acc[j >> 2][4 * (j & 3) + e] += value[e];
+        }
+      }
+    }
+    if (!live) return;
     if (cp.slot < 0) {
       const float inv = 1.0f / l;
       const int64_t tok = cp.q_row + cp.q0 + (r_ >> group_shift);
@@ -531,6 +529,8 @@ void tree_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int
       }
       return;
     }
+    // a sum that is NaN counts as seen (the merge drops rows that saw nothing)
+    if (base == -INFINITY && l != l) base = 0.f;
     const int64_t at = static_cast<int64_t>(kvh) * n_slots + cp.slot + rw;
     float *dst = ws_acc + at * 32 * kHeadDim + 4 * lane_;
 #pragma unroll
@@ -709,6 +709,7 @@ extern "C" int hy_paged_tree(
              "%d chunks and %d merge items: the grid takes 65535", n_chunks, n_merge);
   HY_REQUIRE(max_rows >= 1 && max_rows <= hy::kTreeRows, "max_rows %d is not within 1 .. %d",
              max_rows, hy::kTreeRows);
+  HY_REQUIRE(n_merge == 0 || n_slots > 0, "%d merge items without partials", n_merge);
   HY_REQUIRE(line_words == 4 || line_words == 8, "line_words is %d, not 4 or 8", line_words);
   HY_REQUIRE(q && out && k_pool && v_pool && page_table && lines && items &&
                  (merge_items || n_merge == 0),

@@ -212,8 +212,11 @@ class Qwen3Model(nn.Module):
         for layer_idx, block in enumerate(self.layers):
             x, _, _ = block(x, self.cos, self.sin, None, None, None, None, paged_cache, layer_idx)
         if paged_cache.varlen:
-            rows = paged_cache.logit_rows()
-            x = (x[0] if rows is None else x[0].index_select(0, rows)).unsqueeze(1)
+            x = x[0]
+            if not getattr(paged_cache, "every_logit", False):
+                # each sequence's last packed token
+                x = x.index_select(0, paged_cache.q_start[1:].to(torch.long) - 1)
+            x = x.unsqueeze(1)
         else:
             x = x[:, -1:, :]
         if (linear.few_rows(x) and linear.plain(x, norms=(self.norm,), linears=(self.out_head,))

@@ -429,10 +429,8 @@ class PagedKVBatch:
     # the append entry point, and what it takes behind the rope tables
     _append_call: tuple = ("hy_qknorm_rope_append", ())
 
-    def logit_rows(self) -> Optional[torch.Tensor]:
-        """Packed rows whose logits a varlen tick is run for: each sequence's
-        last token."""
-        return self.q_start[1:].to(torch.long) - 1
+    # whether a tick is run for every token's logits, not each sequence's last one's
+    every_logit = False
 
     def _append_inputs(self, what, q, k, v, q_norm_weight, k_norm_weight, cos, sin):
         """Checked, 16-byte-aligned inputs of the fused norm + rope + append
@@ -675,6 +673,8 @@ class PagedTreeBatch(PagedKVBatch):
     included, are not run at the same time on two streams.
     """
 
+    every_logit = True
+
     def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],
                  num_q_heads: Optional[int], lines: Optional[tuple] = None):
@@ -712,10 +712,6 @@ class PagedTreeBatch(PagedKVBatch):
             self._tree_plans[num_q_heads] = cached
         return cached
 
-    def logit_rows(self) -> None:
-        """Every node's logits are wanted."""
-        return None
-
     def attend_layer(
         self, q: torch.Tensor, layer_idx: int, scale: Optional[float] = None
     ) -> torch.Tensor:
@@ -723,8 +719,8 @@ class PagedTreeBatch(PagedKVBatch):
         itself in this layer's pages: q packed (tokens, Hq, D), returns the same."""
         _require_hip(q, "attend_layer")
         q = _aligned_rows(q)
-        if q.dtype != self.k_cache.dtype:
-            raise TypeError("q dtype must match the pool dtype")
+        if q.dtype != torch.bfloat16 or self.k_cache.dtype != torch.bfloat16:
+            raise TypeError("q and the pool must be bfloat16")
         qs = self._layout(q, "thd")
         num_q_heads = q.shape[1]
         if q.shape[2] != self.head_dim:
@@ -1109,8 +1105,9 @@ class PagedKVCacheManager:
 
     # ----------------------------------------------------------- moved data
     def _copy_pages(self, src: Sequence[int], dst: Sequence[int], tokens: Sequence[int]) -> None:
-        if self.device.type != "cuda":
-            # a pool in host memory, for its bookkeeping: callers that compute refuse it
+        if self.device.type != "cuda" or not self._rows_of_256_bytes():
+            # other rows than the kernels' (a pool in host memory is for bookkeeping only:
+            # callers that compute refuse it)
             for a, b, n in zip(src, dst, tokens):
                 a, b = a * self.page_size, b * self.page_size
                 for pool in (self.k_cache, self.v_cache):
@@ -1125,6 +1122,10 @@ class PagedKVCacheManager:
                 self.page_size, _stream_handle(self.device),
             )
         _native.check(rc, "hy_page_copy")
+
+    def _rows_of_256_bytes(self) -> bool:
+        """Rows as the kernels move them: 128 values of two bytes."""
+        return self.head_dim == 128 and self.k_cache.element_size() == 2
 
     def copy_pages(self, src: Sequence[int], dst: Sequence[int],
                    tokens: Optional[Sequence[int]] = None) -> None:
@@ -1161,6 +1162,8 @@ class PagedKVCacheManager:
         change. Shared pages that would be written are copied first."""
         handles = list(handles)
         _require_hip(self.k_cache, "move_tokens")
+        if not self._rows_of_256_bytes():
+            raise NotImplementedError("move_tokens moves rows of 128 two-byte values")
         if len(sources) != len(handles) or len(starts) != len(handles):
             raise ValueError("one source list and one start per handle is required")
         if any(h.released for h in handles):

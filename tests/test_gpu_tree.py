@@ -170,6 +170,51 @@ def test_other_branches_may_hold_anything(bad, where):
         at += len(tree)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 8), (32, 8), (64, 8)])
+def test_a_row_that_sees_one_bad_key_in_a_part(q_heads, kv_heads):
+    """Forty roots: each sees, of the drafted slots, its own only. With no cached tokens an
+    infinite value there is the row's result; a key that is NaN makes the row NaN also where the
+    last part of a split request holds no other key that it sees."""
+    n = 40
+    tree = [-1] * n
+    m, handles = make_pool([0], [n], q_heads=q_heads, kv_heads=kv_heads, seed=4)
+    batch = m.begin_tree(handles, [tree])
+    q, k, v = normal(n, q_heads, D, seed=1), normal(n, kv_heads, D, seed=2), normal(n, kv_heads, D, seed=3)
+    v[35, :, 7] = float("inf")
+    v[3, :, 9] = -float("inf")
+    batch.write_layer(0, k, v)
+    out = batch.attend_layer(q, 0)
+    # a row that sees one key takes its value as it is
+    assert torch.equal(out, v.repeat_interleave(q_heads // kv_heads, dim=1))
+
+    from hayate_amd import _native
+
+    cached = next(c for c in range(64, 1 << 20, 64) if any(
+        r[3] == c for r in _native.plan_tree(np.array([n]), np.array([c + n]), q_heads, kv_heads,
+                                             m.num_cus).items[2:].tolist()))
+    m, handles = make_pool([cached], [n], q_heads=q_heads, kv_heads=kv_heads, seed=4)
+    batch = m.begin_tree(handles, [tree])
+    k[11] = float("nan")
+    v = v.nan_to_num(0, 0, 0)
+    batch.write_layer(0, k, v)
+    out = batch.attend_layer(q, 0)
+    assert torch.isnan(out[11]).all()
+    rows = physical(m, handles[0], cached + n)
+    others = [i for i in range(n) if i != 11]
+    ref, size = attention64(q[others], m.k_cache[0, 0][:, rows], m.v_cache[0, 0][:, rows],
+                            seen(cached, tree)[others])
+    assert_attention(out[others], ref, size)
+
+
+def test_pools_of_other_types_are_refused():
+    from hayate_amd import PagedKVCacheManager
+
+    m = PagedKVCacheManager(1, 8, D, 512, 128, 2, torch.float16, "cuda")
+    batch = m.begin_tree([m.allocate()], [[-1]])
+    with pytest.raises(TypeError):
+        batch.attend_layer(torch.zeros(1, 32, D, dtype=torch.float16, device="cuda"), 0)
+
+
 def test_strided_rows():
     """q, k and v as views of one projection, as the model has them."""
     m, handles = make_pool([150, 20], [12, 5], seed=4)

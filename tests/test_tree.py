@@ -145,11 +145,11 @@ def test_lines_refusals():
 def test_batch_metadata(sizes):
     rng = random.Random(sum(sizes))
     trees = [wide_tree(rng, n) for n in sizes]
-    m = pool(pages=20)
+    m = pool(pages=22)
     handles = [handle(m, rng.randint(1, 300)) for _ in sizes]
     batch = m.begin_tree(handles, trees)
     assert isinstance(batch, PagedTreeBatch) and batch.varlen and not batch.decode_only
-    assert batch.logit_rows() is None
+    assert batch.every_logit and not m.begin_tick([handle(m, 5)], [1]).every_logit
     words = batch.line_words
     assert words == 4 * -(-max(sizes) // 128) and batch._lines_ptr % 16 == 0
     lines = batch.lines.numpy().view(np.uint32).reshape(-1, words)
@@ -284,6 +284,27 @@ def test_move_and_copy_refusals(monkeypatch):
             call()
 
 
+def test_pools_of_other_rows(monkeypatch):
+    """The copy-on-write of a pool whose rows the kernels do not move copies as before; moving
+    tokens in one is refused."""
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    for dtype, dim in ((torch.float32, 128), (torch.bfloat16, 64)):
+        m = PagedKVCacheManager(2, 3, dim, 6 * 128, 128, 4, dtype, "cpu")
+        m.k_cache.normal_()
+        m.v_cache.normal_()
+        h = handle(m, 200)
+        child = m.fork(h)
+        want = [p[:, :, :, 128 * h.pages[1] : 128 * h.pages[1] + 72].clone() for p in (m.k_cache, m.v_cache)]
+        m.begin_batch([child], 1)
+        assert child.pages[1] != h.pages[1]
+        for p, x in zip((m.k_cache, m.v_cache), want):
+            assert torch.equal(p[:, :, :, 128 * child.pages[1] : 128 * child.pages[1] + 72], x)
+        with pytest.raises(NotImplementedError):
+            m.move_tokens([h], [[5]], [3])
+
+
 def c_arrays(*lists):
     return [(ctypes.c_int32 * max(1, len(x)))(*x) for x in lists]
 
@@ -359,6 +380,7 @@ def test_c_tree_attention_is_checked():
                dict(chunks=65536), dict(rows=0), dict(rows=257), dict(words=0), dict(words=5), dict(words=12),
                dict(q=None), dict(out=None), dict(k=None), dict(v=None), dict(pt=None),
                dict(lines=None), dict(items=None), dict(merges=1, slots=2, ws=4096, wsb=1 << 30),
+               dict(merge=4096, merges=1),
                dict(q=4098), dict(lines=4100), dict(qh=100), dict(ot=4), dict(hs=1001)):
         assert call(**kw) == _native.HY_EINVAL, kw
     for kw in (dict(dim=64), dict(page=96), dict(page=16), dict(hq=24), dict(hq=256)):
