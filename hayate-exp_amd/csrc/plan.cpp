@@ -724,6 +724,11 @@ extern "C" int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32
                     q_lens[b], hy::kTreeMaxNodes);
       return HY_EUNSUPPORTED;
     }
+    // the kernel counts keys to the end of the next tile in 32 bits
+    if (kv_lens[b] > INT32_MAX - 2 * hy::kTreeTileKeys) {
+      hy::set_error("hy_plan_tree: sequence %d has kv_len %d, too long", b, kv_lens[b]);
+      return HY_EUNSUPPORTED;
+    }
     rows += q_lens[b];
   }
   if (rows > INT32_MAX) {

@@ -674,6 +674,8 @@ class PagedTreeBatch(PagedKVBatch):
     """
 
     every_logit = True
+    # the handles that begin_tree made the batch for
+    handles: Sequence[PagedCacheHandle] = ()
 
     def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],
@@ -1271,20 +1273,24 @@ class PagedKVCacheManager:
         lines = _native.tree_lines(nodes.astype(np.int32),
                                    np.array([len(t) for t in trees], dtype=np.int32))
         self.reserve_tick(handles, [len(t) for t in trees])
-        return PagedTreeBatch(self, trees, [h.length for h in handles],
-                              [list(h.pages) for h in handles], self.num_q_heads, lines)
+        batch = PagedTreeBatch(self, trees, [h.length for h in handles],
+                               [list(h.pages) for h in handles], self.num_q_heads, lines)
+        batch.handles = handles
+        return batch
 
     def commit_tree(self, handles: Sequence[PagedCacheHandle], batch: PagedTreeBatch,
                     accepted: Sequence[Sequence[int]]) -> None:
         """Keep of each handle's tree the nodes accepted[b] (a path from a child of the
         cached context down, possibly empty): their K and V move to the positions behind the
-        cached tokens in every layer, the length grows by as many and the other nodes'
-        pages are returned."""
+        cached tokens in every layer, the length grows by as many and the pages behind it are
+        returned."""
         handles = list(handles)
         if len(handles) != batch.num_seqs or len(accepted) != batch.num_seqs:
             raise ValueError("one handle and one path per tree is required")
         if batch.k_cache is not self.k_cache:
             raise ValueError("the batch belongs to another pool")
+        if any(a is not b for a, b in zip(handles, batch.handles)):
+            raise ValueError("the handles are not those the batch began with, in their order")
         if any(h.released for h in handles):
             raise RuntimeError("cannot commit a released cache handle")
         if [h.length for h in handles] != batch.cache_lens_host:

@@ -385,6 +385,22 @@ def test_positions_past_the_rope_tables_are_refused():
         batch.norm_rope_write_layer(0, q, k, k, None, None, 1e-6, cos, sin)
 
 
+def test_a_wide_tree_needs_its_depths_positions_only():
+    """Slots 100 .. 139, positions 100 and 101: tables of 102 positions are enough."""
+    m, handles = make_pool([100], [40])
+    tree = [-1] * 20 + list(range(20))
+    batch = m.begin_tree(handles, [tree])
+    q, k = normal(40, 32, D), normal(40, 8, D)
+    full = compute_rope_params(D, 10_000, 200, device="cuda")
+    want = batch.norm_rope_write_layer(0, q, k, k, None, None, 1e-6, *full)
+    got = batch.norm_rope_write_layer(0, q, k, k, None, None, 1e-6,
+                                      *(t[:102].contiguous() for t in full))
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError):
+        batch.norm_rope_write_layer(0, q, k, k, None, None, 1e-6,
+                                    *(t[:101].contiguous() for t in full))
+
+
 def test_refusals():
     m, handles = make_pool([10], [4])
     batch = m.begin_tree(handles, [chain(4)])

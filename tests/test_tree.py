@@ -122,6 +122,7 @@ def test_plan_refusals():
     assert call([3], [10], hq=30) == _native.HY_EINVAL
     assert call([3], [10000], items=4) == _native.HY_ENOSPACE
     assert call([3], [10000], merges=0) == _native.HY_ENOSPACE
+    assert call([3], [2**31 - 128]) == _native.HY_EUNSUPPORTED
 
 
 def test_lines_refusals():
@@ -225,6 +226,22 @@ def test_commit_tree_without_moves_is_bookkeeping(monkeypatch):
     assert [len(h.pages) for h in (a, b)] == [1, 3] and m.free_page_count == free + 1
     with pytest.raises(ValueError):  # committed already
         m.commit_tree([a, b], batch, [[0], [0]])
+
+
+def test_commit_tree_takes_the_batch_s_handles(monkeypatch):
+    """Handles of the same length in another order, or another handle of that length, would
+    commit one request's path to another."""
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    m = pool()
+    a, b, other = (handle(m, 100) for _ in range(3))
+    batch = m.begin_tree([a, b], [chain(3), chain(3)])
+    for handles in ([b, a], [a, other], [a, a]):
+        with pytest.raises(ValueError):
+            m.commit_tree(handles, batch, [[0], [0]])
+    m.commit_tree([a, b], batch, [[0], [0, 1]])
+    assert (a.length, b.length) == (101, 102)
 
 
 # ------------------------------------------------------------ moves, copies
