@@ -462,11 +462,18 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
 
 namespace {
 
-// Cost of a piece of drafted-tree attention after a chunk's first, in key steps.
-constexpr int64_t kTreePieceCost = 1;
-// Cost of the merge launch in key steps: 4-5 us and a second launch's host time, against
-// 0.55 us for a step while few compute units run.
-constexpr int64_t kTreeMergeCost = 8;
+// Costs of drafted-tree attention, in sixteenths of a key step.
+constexpr int64_t kTreeStep = 16;
+// A step of a tile of at most 128 rows in a launch of more: one wave a SIMD computes instead of
+// two. 32 trees of 4 to 64 nodes on 4 to 30 k tokens (16 to 256 rows) take 433 us at this
+// cost, 444 at 10 and 456 at 16; 4 of 200 nodes (three full tiles and one of 32 rows
+// each) 70.6, 75.8 and 71.5; four equal tiles each took 72.8.
+constexpr int64_t kTreeFewRowsStep = 12;
+// A piece after a chunk's first.
+constexpr int64_t kTreePieceCost = 16;
+// The merge launch: 4-5 us and a second launch's host time, against 0.55 us for a step while
+// few compute units run.
+constexpr int64_t kTreeMergeCost = 128;
 
 struct TreePieceRec {
   int32_t tile, step0, step1;  // query tile, and its key steps
@@ -480,8 +487,9 @@ struct TreeCut {
 };
 
 // Cuts the key steps of the query tiles, in order, into at most n_chunks chunks of
-// equal cost; `total` is what the whole stream is taken to cost.
-void cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total, TreeCut &cut) {
+// equal cost; `total` is what the whole stream is taken to cost, a step of tile t cost[t].
+void cut_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cost, int64_t n_chunks,
+              int64_t total, TreeCut &cut) {
   cut = TreeCut();
   int64_t spent = 0, in_chunk = 0;
   int32_t first = 0;
@@ -505,11 +513,11 @@ void cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total
         close();
         continue;
       }
-      const int32_t n = static_cast<int32_t>(
-          std::min<int64_t>(steps[t] - at, std::max<int64_t>(room, 1)));
+      const int64_t fit = (std::max<int64_t>(room, 1) - 1) / cost[t] + 1;
+      const int32_t n = static_cast<int32_t>(std::min<int64_t>(steps[t] - at, fit));
       cut.pieces.push_back({static_cast<int32_t>(t), at, at + n});
       cut.split = cut.split || n < steps[t];
-      in_chunk += n + extra;
+      in_chunk += n * static_cast<int64_t>(cost[t]) + extra;
       at += n;
     }
   }
@@ -518,16 +526,18 @@ void cut_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t total
 
 // The query tiles whole, in order, in at most n_chunks chunks of at most `most`; false if they
 // do not fit.
-bool whole_tree(const std::vector<int32_t> &steps, int64_t n_chunks, int64_t most, TreeCut &cut) {
+bool whole_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cost,
+                int64_t n_chunks, int64_t most, TreeCut &cut) {
   cut = TreeCut();
   int64_t in_chunk = 0;
   for (size_t t = 0; t < steps.size(); ++t) {
-    if (steps[t] > most) return false;
-    if (in_chunk > 0 && in_chunk + kTreePieceCost + steps[t] > most) {
+    const int64_t all = steps[t] * static_cast<int64_t>(cost[t]);
+    if (all > most) return false;
+    if (in_chunk > 0 && in_chunk + kTreePieceCost + all > most) {
       cut.ends.push_back(static_cast<int32_t>(t));
       in_chunk = 0;
     }
-    in_chunk += steps[t] + (in_chunk > 0 ? kTreePieceCost : 0);
+    in_chunk += all + (in_chunk > 0 ? kTreePieceCost : 0);
     cut.pieces.push_back({static_cast<int32_t>(t), 0, steps[t]});
     cut.worst = std::max(cut.worst, in_chunk);
   }
@@ -542,17 +552,15 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
     int32_t seq, q0, q1, kv_end;
   };
   std::vector<Tile> tiles;
-  std::vector<int32_t> q_begin(static_cast<size_t>(num_seqs) + 1, 0), steps;
-  int64_t all = 0;
+  std::vector<int32_t> q_begin(static_cast<size_t>(num_seqs) + 1, 0), steps, cost;
+  int64_t all = 0, all_cost = 0;
   int32_t max_rows = 0;
   for (int b = 0; b < num_seqs; ++b) {
     q_begin[b + 1] = q_begin[b] + q_lens[b];
-    // nodes beyond one workgroup's rows: tiles of equal size
+    // nodes beyond one workgroup's rows: full tiles, and the rest
     const int32_t per = hy::kTreeRows / G;
-    const int32_t n = (q_lens[b] + per - 1) / per;
-    for (int32_t i = 0; i < n; ++i) {
-      const int32_t q0 = static_cast<int32_t>(static_cast<int64_t>(q_lens[b]) * i / n);
-      const int32_t q1 = static_cast<int32_t>(static_cast<int64_t>(q_lens[b]) * (i + 1) / n);
+    for (int32_t q0 = 0; q0 < q_lens[b]; q0 += per) {
+      const int32_t q1 = std::min(q_lens[b], q0 + per);
       const int32_t end = kv_lens[b] - q_lens[b] + q1;
       tiles.push_back({b, q0, q1, end});
       steps.push_back((end + hy::kTreeTileKeys - 1) / hy::kTreeTileKeys);
@@ -560,25 +568,30 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
       max_rows = std::max(max_rows, (q1 - q0) * G);
     }
   }
+  for (size_t t = 0; t < tiles.size(); ++t) {
+    const bool few = max_rows > 128 && (tiles[t].q1 - tiles[t].q0) * G <= 128;
+    cost.push_back(static_cast<int32_t>(few ? kTreeFewRowsStep : kTreeStep));
+    all_cost += steps[t] * static_cast<int64_t>(cost[t]);
+  }
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   const int64_t n_chunks =
       std::max<int64_t>(1, std::min<int64_t>((cus + num_kv_heads - 1) / num_kv_heads, all));
   TreeCut best, trial;
-  cut_tree(steps, n_chunks, all, best);
-  int64_t total = all;
+  cut_tree(steps, cost, n_chunks, all_cost, best);
+  int64_t total = all_cost;
   for (int pass = 0; pass < 3; ++pass) {
     const TreeCut &last = pass ? trial : best;
-    total = all + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
-    cut_tree(steps, n_chunks, total, trial);
+    total = all_cost + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
+    cut_tree(steps, cost, n_chunks, total, trial);
     if (trial.worst < best.worst) best = trial;
   }
   // Tiles that need no merge are worth a longer chunk; the shortest such chunk by bisection.
   if (best.split) {
     int64_t fits = best.worst + kTreeMergeCost, low = 0;
-    while (low < fits && whole_tree(steps, n_chunks, fits, trial)) {
+    while (low < fits && whole_tree(steps, cost, n_chunks, fits, trial)) {
       best = trial;
       const int64_t mid = low + (fits - low) / 2;
-      if (whole_tree(steps, n_chunks, mid, trial))
+      if (whole_tree(steps, cost, n_chunks, mid, trial))
         fits = mid;
       else
         low = mid + 1;

@@ -26,6 +26,7 @@ Data operations need the pool on a HIP device; on any other device they raise
 from __future__ import annotations
 
 import contextlib
+import itertools
 import math
 import operator
 from dataclasses import dataclass, field
@@ -1172,53 +1173,55 @@ class PagedKVCacheManager:
             raise RuntimeError("cannot move tokens of a released cache handle")
         if len({id(h) for h in handles}) != len(handles):
             raise ValueError("the same cache handle is given twice")
-        lists, firsts, wanted = [], [], []
-        for h, source, start in zip(handles, sources, starts):
-            src, start = _int_array(source, "sources"), _index(start, "a start")
-            if start < 0:
-                raise ValueError("starts must be non-negative")
-            n = len(src)
-            if n == 0 or (src[n - 1] == start + n - 1 and src[0] == start):
-                # nothing moves if they ascend, which alone is left to check
-                if n > 1 and (np.diff(src) <= 0).any():
-                    raise ValueError("sources must ascend, none before the position it fills")
-                if n and src[n - 1] >= len(h.pages) * self.page_size:
-                    raise ValueError(f"position {src[n - 1]} is past the cache's reserved space")
-                continue
-            lists.append(src)
-            firsts.append(start)
-            wanted.append(h)
-        if not lists:
+        firsts = [start if type(start) is int else _index(start, "a start") for start in starts]
+        if firsts and min(firsts) < 0:
+            raise ValueError("starts must be non-negative")
+        if all(type(source) is list for source in sources):  # one conversion for all
+            src = _int_array(list(itertools.chain.from_iterable(sources)), "sources")
+        else:
+            sources = [source if type(source) is np.ndarray and source.dtype == np.int64
+                       and source.ndim == 1 else _int_array(source, "sources")
+                       for source in sources]
+            src = np.concatenate(sources)
+        lens = [len(source) for source in sources]
+        if not len(src):
             return
+        if not all(lens):  # without the requests that move nothing
+            handles, firsts, lens = zip(*[x for x in zip(handles, firsts, lens) if x[2]])
+        src_start = [0, *itertools.accumulate(lens)]
+        lasts = src[[at - 1 for at in src_start[1:]]].tolist()
         ps, refs = self.page_size, self._refs
-        ends = [start + len(src) for start, src in zip(firsts, lists)]
-        if any(refs[p] > 1 for h, a, b in zip(wanted, firsts, ends)
-               for p in h.pages[a // ps : -(-b // ps)]):
+        # the pages from the first written to the last read
+        first_page = [start // ps for start in firsts]
+        pages, page_start, shared = [], [0], False
+        for h, start, page, n, last in zip(handles, firsts, first_page, lens, lasts):
+            held = h.pages[page : last // ps + 1]
+            # (sources that ascend from `start` on reach the last page written)
+            for p in held[: (start + n - 1) // ps + 1 - page]:
+                shared |= refs[p] > 1
+            pages += held
+            page_start.append(len(pages))
+        if (src >> 31).any() or max(firsts) >= self.capacity_tokens:
+            raise ValueError(f"positions lie in 0 .. {self.capacity_tokens - 1}")
+        if shared:
             spans = []
-            for h, src, start in zip(wanted, lists, firsts):
-                dst = np.arange(start, start + len(src))
-                if ((np.diff(src) <= 0).any() or src[0] < start
-                        or src[-1] >= len(h.pages) * ps):
+            for i, (h, start) in enumerate(zip(handles, firsts)):
+                of_h = src[src_start[i] : src_start[i + 1]]
+                if ((np.diff(of_h) <= 0).any() or of_h[0] < start
+                        or of_h[-1] >= len(h.pages) * ps):
                     raise ValueError("sources must ascend, none before the position it fills, "
                                      "all in the cache's reserved space")
                 # ascending on both sides, so the tokens that stay are the first ones
-                stay = int(np.count_nonzero(src == dst))
-                spans.append((h, start + stay, start + len(src),
-                              max(h.length, int(src[-1]) + 1)))
+                end = start + len(of_h)
+                stay = int(np.count_nonzero(of_h == np.arange(start, end)))
+                spans.append((h, start + stay, end, max(h.length, int(of_h[-1]) + 1)))
             self._make_all_private(spans)
-        # the pages from the first written to the last read
-        pages, page_start, src_start = [], [0], [0]
-        first_page = [start // ps for start in firsts]
-        for h, src, page in zip(wanted, lists, first_page):
-            pages += h.pages[page : int(src[-1]) // ps + 1]
-            page_start.append(len(pages))
-            src_start.append(src_start[-1] + len(src))
-        lists = np.concatenate(lists)
-        if lists.min() < 0 or lists.max() >= self.capacity_tokens:
-            raise ValueError(f"positions lie in 0 .. {self.capacity_tokens - 1}")
-        n = len(wanted)
-        meta = np.array(page_start + src_start + first_page + firsts + pages, dtype=np.int32)
-        src, at = lists.astype(np.int32), meta.ctypes.data
+            pages = []
+            for h, page, last in zip(handles, first_page, lasts):
+                pages += h.pages[page : last // ps + 1]
+        n = len(handles)
+        meta = np.array([*page_start, *src_start, *first_page, *firsts, *pages], dtype=np.int32)
+        src, at = src.astype(np.int32), meta.ctypes.data
         with _current_device(self.device):
             rc = _native.lib().hy_kv_move(
                 self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_cache.stride(0),

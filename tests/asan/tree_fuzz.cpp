@@ -50,21 +50,20 @@ int plan(const std::vector<int32_t> &q, const std::vector<int32_t> &kv, int hq, 
   const int rc = hy_plan_tree(q.data(), kv.data(), static_cast<int32_t>(q.size()), hq, hkv, cus,
                               a.data(), items, b.data(), merges, counts);
   if (rc != HY_OK) return rc;
-  // every key of every tile once, in order
-  int64_t keys = 0, want = 0;
-  const int per = 256 / (hq / hkv);
-  for (size_t i = 0; i < q.size(); ++i) {
-    const int n = (q[i] + per - 1) / per;
-    for (int t = 1; t <= n; ++t) want += kv[i] - q[i] + static_cast<int64_t>(q[i]) * t / n;
-  }
+  // every node in one tile, and every key of every tile once
+  int64_t keys = 0, want = 0, nodes = 0;
   for (int p = 0; p < counts[1]; ++p) {
     const int32_t *r = a.data() + 16 * static_cast<size_t>(counts[0]) + 8 * static_cast<size_t>(p);
     CHECK(r[0] >= 0 && r[0] < static_cast<int32_t>(q.size()) && r[1] < r[2] && r[3] < r[4]);
     CHECK(r[3] % 64 == 0 && r[4] <= kv[r[0]] && (r[2] - r[1]) * (hq / hkv) <= counts[4]);
     CHECK(r[5] < counts[3]);
     keys += r[4] - r[3];
+    if (r[3] > 0) continue;
+    nodes += r[2] - r[1];
+    want += kv[r[0]] - q[r[0]] + r[2];
   }
-  CHECK(keys == want);
+  for (int32_t n : q) nodes -= n;
+  CHECK(keys == want && nodes == 0);
   return rc;
 }
 
