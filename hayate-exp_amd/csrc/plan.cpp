@@ -465,10 +465,11 @@ namespace {
 // Costs of drafted-tree attention, in sixteenths of a key step.
 constexpr int64_t kTreeStep = 16;
 // A step of a tile of at most 128 rows in a launch of more: one wave a SIMD computes instead of
-// two. 32 trees of 4 to 64 nodes on 4 to 30 k tokens (16 to 256 rows) take 433 us at this
-// cost, 444 at 10 and 456 at 16; 4 of 200 nodes (three full tiles and one of 32 rows
-// each) 70.6, 75.8 and 71.5; four equal tiles each took 72.8.
-constexpr int64_t kTreeFewRowsStep = 12;
+// two. Geometric means over 14 batches each: 4 trees of 200 nodes (three full tiles and one of
+// 32 rows each) on 1.5 to 4 k tokens 66.2 us at 16, 64.8 at 14, 64.6 at 13, 65.3 at 12, 66.3 at
+// 11; 2 to 32 trees of 5 to 100 nodes 66.2, 65.3, 64.6, 65.3 and 66.7. (With equal tiles, all at
+// 16: 67.0 and 66.2.)
+constexpr int64_t kTreeFewRowsStep = 13;
 // A piece after a chunk's first.
 constexpr int64_t kTreePieceCost = 16;
 // The merge launch: 4-5 us and a second launch's host time, against 0.55 us for a step while
