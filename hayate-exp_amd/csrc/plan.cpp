@@ -470,6 +470,13 @@ constexpr int64_t kTreeStep = 16;
 // 11; 2 to 32 trees of 5 to 100 nodes 66.2, 65.3, 64.6, 65.3 and 66.7. (With equal tiles, all at
 // 16: 67.0 and 66.2.)
 constexpr int64_t kTreeFewRowsStep = 13;
+// Tiles of 128 rows instead of 256 read keys twice but leave more of the work to units that
+// would idle, often without a merge: 5 to 100 nodes on up to 1,500 tokens 30 -> 22 us, 26 -> 20;
+// on long caches, where every unit is busy, 390 -> 440. A step of theirs is taken as 11 (9:
+// 67.0 us over the 14 mixed batches, 10: 62.9, 11: 62.6, 12: 62.8, only full tiles 65.4), the
+// merge as 8 full steps.
+constexpr int64_t kTreeHalfStep = 11;
+constexpr int64_t kTreeSplitCost = 128;
 // A piece after a chunk's first.
 constexpr int64_t kTreePieceCost = 16;
 // The merge launch: 4-5 us and a second launch's host time, against 0.55 us for a step while
@@ -546,43 +553,45 @@ bool whole_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &c
   return static_cast<int64_t>(cut.ends.size()) <= n_chunks;
 }
 
-int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t G,
-              int32_t num_kv_heads, int32_t num_cus, int32_t *items, int32_t item_capacity,
-              int32_t *merge_items, int32_t merge_capacity, int32_t *counts_out) {
-  struct Tile {
-    int32_t seq, q0, q1, kv_end;
-  };
-  std::vector<Tile> tiles;
-  std::vector<int32_t> q_begin(static_cast<size_t>(num_seqs) + 1, 0), steps, cost;
-  int64_t all = 0, all_cost = 0;
+struct TreeTile {
+  int32_t seq, q0, q1, kv_end;
+};
+struct TreeTiling {
+  std::vector<TreeTile> tiles;
+  std::vector<int32_t> steps;  // a tile's key steps
   int32_t max_rows = 0;
+  TreeCut cut;
+};
+
+// The requests' rows in tiles of at most tile_rows, and the chunks of their key steps.
+void tile_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t G,
+               int64_t n_units, int32_t tile_rows, TreeTiling &out) {
+  std::vector<int32_t> &steps = out.steps, cost;
+  int64_t all = 0, all_cost = 0;
   for (int b = 0; b < num_seqs; ++b) {
-    q_begin[b + 1] = q_begin[b] + q_lens[b];
     // nodes beyond one workgroup's rows: full tiles, and the rest
-    const int32_t per = hy::kTreeRows / G;
+    const int32_t per = tile_rows / G;
     for (int32_t q0 = 0; q0 < q_lens[b]; q0 += per) {
       const int32_t q1 = std::min(q_lens[b], q0 + per);
       const int32_t end = kv_lens[b] - q_lens[b] + q1;
-      tiles.push_back({b, q0, q1, end});
+      out.tiles.push_back({b, q0, q1, end});
       steps.push_back((end + hy::kTreeTileKeys - 1) / hy::kTreeTileKeys);
       all += steps.back();
-      max_rows = std::max(max_rows, (q1 - q0) * G);
+      out.max_rows = std::max(out.max_rows, (q1 - q0) * G);
     }
   }
-  for (size_t t = 0; t < tiles.size(); ++t) {
-    const bool few = max_rows > 128 && (tiles[t].q1 - tiles[t].q0) * G <= 128;
+  for (size_t t = 0; t < steps.size(); ++t) {
+    const bool few = out.max_rows > 128 && (out.tiles[t].q1 - out.tiles[t].q0) * G <= 128;
     cost.push_back(static_cast<int32_t>(few ? kTreeFewRowsStep : kTreeStep));
     all_cost += steps[t] * static_cast<int64_t>(cost[t]);
   }
-  const int64_t cus = num_cus > 0 ? num_cus : 256;
-  const int64_t n_chunks =
-      std::max<int64_t>(1, std::min<int64_t>((cus + num_kv_heads - 1) / num_kv_heads, all));
-  TreeCut best, trial;
+  const int64_t n_chunks = std::max<int64_t>(1, std::min<int64_t>(n_units, all));
+  TreeCut trial, &best = out.cut;
   cut_tree(steps, cost, n_chunks, all_cost, best);
-  int64_t total = all_cost;
   for (int pass = 0; pass < 3; ++pass) {
     const TreeCut &last = pass ? trial : best;
-    total = all_cost + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
+    const int64_t total =
+        all_cost + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
     cut_tree(steps, cost, n_chunks, total, trial);
     if (trial.worst < best.worst) best = trial;
   }
@@ -598,6 +607,29 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
         low = mid + 1;
     }
   }
+}
+
+int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t G,
+              int32_t num_kv_heads, int32_t num_cus, int32_t *items, int32_t item_capacity,
+              int32_t *merge_items, int32_t merge_capacity, int32_t *counts_out) {
+  std::vector<int32_t> q_begin(static_cast<size_t>(num_seqs) + 1, 0);
+  for (int b = 0; b < num_seqs; ++b) q_begin[b + 1] = q_begin[b] + q_lens[b];
+  const int64_t cus = num_cus > 0 ? num_cus : 256, n_units = (cus + num_kv_heads - 1) / num_kv_heads;
+  // the tiling whose costliest chunk, and merge, take the shorter time
+  TreeTiling full, half;
+  tile_tree(q_lens, kv_lens, num_seqs, G, n_units, hy::kTreeRows, full);
+  const TreeTiling *tiling = &full;
+  if (full.max_rows > 128) {
+    tile_tree(q_lens, kv_lens, num_seqs, G, n_units, 128, half);
+    auto time = [](const TreeTiling &t, int64_t step) {
+      return t.cut.worst * step / kTreeStep + (t.cut.split ? kTreeSplitCost : 0);
+    };
+    if (time(half, kTreeHalfStep) < time(full, kTreeStep)) tiling = &half;
+  }
+  const std::vector<TreeTile> &tiles = tiling->tiles;
+  const std::vector<int32_t> &steps = tiling->steps;
+  const TreeCut &best = tiling->cut;
+  const int32_t max_rows = tiling->max_rows;
   const std::vector<TreePieceRec> &pieces = best.pieces;
   const std::vector<int32_t> &ends = best.ends;
   const int64_t need = 2 * static_cast<int64_t>(ends.size()) + static_cast<int64_t>(pieces.size());
@@ -610,7 +642,7 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
   int64_t n_slots = 0;
   int32_t *rec = items + hy::kTreeChunkInts * static_cast<int64_t>(ends.size());
   for (size_t i = 0; i < pieces.size(); ++i) {
-    const Tile &t = tiles[pieces[i].tile];
+    const TreeTile &t = tiles[pieces[i].tile];
     const int32_t blocks = ((t.q1 - t.q0) * G + 31) / 32;
     const bool whole = pieces[i].step0 == 0 && pieces[i].step1 == steps[pieces[i].tile];
     if (!whole) {
@@ -656,7 +688,7 @@ int plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, i
     ch[2] = n;
     ch[3] = 1;
     for (int32_t p = first; p < ends[i]; ++p) {
-      const Tile &t = tiles[pieces[p].tile];
+      const TreeTile &t = tiles[pieces[p].tile];
       if (t.q1 - t.q0 < q_lens[t.seq]) ch[3] = 0;
     }
     for (int j = 4; j < 8; ++j) ch[j] = 0;

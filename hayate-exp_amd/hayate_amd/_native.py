@@ -305,9 +305,9 @@ def plan_tree(
     q_lens = np.ascontiguousarray(q_lens, dtype=np.int32)
     kv_lens = np.ascontiguousarray(kv_lens, dtype=np.int32)
     n = int(q_lens.shape[0])
-    # at most 16 heads a group, so a tree has at most 16 tiles of 256 rows, and every
+    # at most 16 heads a group, so a tree has at most 32 tiles of 128 rows, and every
     # cut between chunks adds one piece
-    tiles = n * 16
+    tiles = n * 32
     chunks = -(-(num_cus if num_cus > 0 else 256) // max(1, num_kv_heads)) + 1
     items = np.zeros((3 * chunks + tiles, 8), dtype=np.int32)
     merge = np.zeros((tiles + 1, 8), dtype=np.int32)

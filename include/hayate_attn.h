@@ -465,8 +465,9 @@ int hy_tree_lines(const int32_t *parents, const int32_t *q_lens, int32_t num_seq
 /*
  * Planner of hy_paged_tree (host only): q_lens[b] >= 1 nodes on kv_lens[b] -
  * q_lens[b] cached tokens. The (node, query head) rows of a sequence form query
- * tiles of 256 rows per kv head, the last with the rest; the 64-key steps of all tiles, in
- * order, are cut into chunks of equal cost, one per CU and kv head. items:
+ * tiles of 256 rows per kv head (or all of 128, whichever takes less time), the last with
+ * the rest; the 64-key steps of all tiles, in order, are cut into chunks of equal cost, one per
+ * CU and kv head. items:
  *   n_chunks chunk records int32[16] = {piece_begin, piece_end, n_steps, alone, 0, 0, 0,
  *   0, the first piece's record} (alone: 1 when its sequences have one tile each, so
  *   that their keys are read once), then the piece records int32[8] = {seq, q_begin, q_end,

@@ -98,7 +98,7 @@ int main(int argc, char **argv) {
       parents[at] = 300;
       CHECK(hy_tree_lines(parents.data(), q.data(), n, words, lines.data(), depths.data()) == HY_EINVAL);
     }
-    const int tiles = 16 * n, chunks = (cus > 0 ? cus : 256) / hkv + 1;
+    const int tiles = 32 * n, chunks = (cus > 0 ? cus : 256) / hkv + 1;
     int32_t counts[5], again[5];
     CHECK(plan(q, kv, hkv * group, hkv, cus, 3 * (chunks + tiles), tiles, counts) == HY_OK);
     const int items = 2 * counts[0] + counts[1];
