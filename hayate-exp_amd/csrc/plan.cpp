@@ -477,8 +477,13 @@ constexpr int64_t kTreeFewRowsStep = 13;
 // merge as 8 full steps.
 constexpr int64_t kTreeHalfStep = 11;
 constexpr int64_t kTreeSplitCost = 128;
-// A piece after a chunk's first.
-constexpr int64_t kTreePieceCost = 16;
+// A piece after a chunk's first, in launches of at most 128 rows and of more: the rows of Q come
+// and the partials go between its steps and the others'. Geometric means over 16 batches each: 2
+// to 40 chains of 3 to 8 nodes 22.4 us at 16, 21.2 at 32, 20.7 at 64, 21.1 at 112; trees of 20
+// to 32 nodes 41.0, 40.0, 39.3 and 39.9; 4 of 200 nodes 63.7 at 16, 61.7 at 48, 61.8 at 64, 62.9
+// at 80.
+constexpr int64_t kTreeFewRowsPiece = 64;
+constexpr int64_t kTreePiece = 48;
 // The merge launch: 4-5 us and a second launch's host time, against 0.55 us for a step while
 // few compute units run.
 constexpr int64_t kTreeMergeCost = 128;
@@ -495,9 +500,10 @@ struct TreeCut {
 };
 
 // Cuts the key steps of the query tiles, in order, into at most n_chunks chunks of
-// equal cost; `total` is what the whole stream is taken to cost, a step of tile t cost[t].
+// equal cost; `total` is what the whole stream is taken to cost, a step of tile t cost[t] and a
+// piece after a chunk's first piece_cost.
 void cut_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cost, int64_t n_chunks,
-              int64_t total, TreeCut &cut) {
+              int64_t total, int64_t piece_cost, TreeCut &cut) {
   cut = TreeCut();
   int64_t spent = 0, in_chunk = 0;
   int32_t first = 0;
@@ -515,7 +521,7 @@ void cut_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cos
       const int64_t left = n_chunks - static_cast<int64_t>(cut.ends.size());  // this one included
       const int64_t share =
           left > 1 ? (std::max<int64_t>(total - spent, 1) + left - 1) / left : INT64_MAX;
-      const int64_t extra = size() > first ? kTreePieceCost : 0;
+      const int64_t extra = size() > first ? piece_cost : 0;
       const int64_t room = share - in_chunk - extra;
       if (room <= 0 && size() > first) {
         close();
@@ -535,17 +541,17 @@ void cut_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cos
 // The query tiles whole, in order, in at most n_chunks chunks of at most `most`; false if they
 // do not fit.
 bool whole_tree(const std::vector<int32_t> &steps, const std::vector<int32_t> &cost,
-                int64_t n_chunks, int64_t most, TreeCut &cut) {
+                int64_t n_chunks, int64_t most, int64_t piece_cost, TreeCut &cut) {
   cut = TreeCut();
   int64_t in_chunk = 0;
   for (size_t t = 0; t < steps.size(); ++t) {
     const int64_t all = steps[t] * static_cast<int64_t>(cost[t]);
     if (all > most) return false;
-    if (in_chunk > 0 && in_chunk + kTreePieceCost + all > most) {
+    if (in_chunk > 0 && in_chunk + piece_cost + all > most) {
       cut.ends.push_back(static_cast<int32_t>(t));
       in_chunk = 0;
     }
-    in_chunk += all + (in_chunk > 0 ? kTreePieceCost : 0);
+    in_chunk += all + (in_chunk > 0 ? piece_cost : 0);
     cut.pieces.push_back({static_cast<int32_t>(t), 0, steps[t]});
     cut.worst = std::max(cut.worst, in_chunk);
   }
@@ -586,22 +592,23 @@ void tile_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, 
     all_cost += steps[t] * static_cast<int64_t>(cost[t]);
   }
   const int64_t n_chunks = std::max<int64_t>(1, std::min<int64_t>(n_units, all));
+  const int64_t piece = out.max_rows > 128 ? kTreePiece : kTreeFewRowsPiece;
   TreeCut trial, &best = out.cut;
-  cut_tree(steps, cost, n_chunks, all_cost, best);
+  cut_tree(steps, cost, n_chunks, all_cost, piece, best);
   for (int pass = 0; pass < 3; ++pass) {
     const TreeCut &last = pass ? trial : best;
     const int64_t total =
-        all_cost + kTreePieceCost * static_cast<int64_t>(last.pieces.size() - last.ends.size());
-    cut_tree(steps, cost, n_chunks, total, trial);
+        all_cost + piece * static_cast<int64_t>(last.pieces.size() - last.ends.size());
+    cut_tree(steps, cost, n_chunks, total, piece, trial);
     if (trial.worst < best.worst) best = trial;
   }
   // Tiles that need no merge are worth a longer chunk; the shortest such chunk by bisection.
   if (best.split) {
     int64_t fits = best.worst + kTreeMergeCost, low = 0;
-    while (low < fits && whole_tree(steps, cost, n_chunks, fits, trial)) {
+    while (low < fits && whole_tree(steps, cost, n_chunks, fits, piece, trial)) {
       best = trial;
       const int64_t mid = low + (fits - low) / 2;
-      if (whole_tree(steps, cost, n_chunks, mid, trial))
+      if (whole_tree(steps, cost, n_chunks, mid, piece, trial))
         fits = mid;
       else
         low = mid + 1;

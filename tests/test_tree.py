@@ -74,7 +74,9 @@ def check_plan(q_lens, kv_lens, hq=32, hkv=8, cus=256):
             node = q1
     assert at == len(pieces) and not merged
     assert sorted(used) == list(range(p.n_slots)) and p.max_rows == rows
-    cost = chunks[:, 2] + (chunks[:, 1] - chunks[:, 0] - 1)
+    # in key steps: the planner counts a piece after the chunk's first as 4, 3 in launches of
+    # more than 128 rows
+    cost = chunks[:, 2] + (4 if p.max_rows <= 128 else 3) * (chunks[:, 1] - chunks[:, 0] - 1)
     return p, cost
 
 
@@ -94,7 +96,8 @@ def test_plan_shares_the_steps_evenly():
     _, cost = check_plan(q, q + rng.integers(200, 4000, size=20))
     assert len(cost) == 32 and cost.max() <= cost.mean() + 2
     _, cost = check_plan([64] * 8, [32064] * 8)
-    assert len(cost) == 32 and cost.max() - cost.min() <= 1
+    # a chunk is closed when another piece would not pay: at most a piece's cost short
+    assert len(cost) == 32 and cost.max() - cost.min() <= 3
 
 
 def test_plan_of_small_work_and_few_units():
