@@ -484,9 +484,16 @@ constexpr int64_t kTreeSplitCost = 128;
 // at 80.
 constexpr int64_t kTreeFewRowsPiece = 64;
 constexpr int64_t kTreePiece = 48;
-// The merge launch: 4-5 us and a second launch's host time, against 0.55 us for a step while
-// few compute units run.
+// The merge launch, in launches of at most 32 rows (a step takes 0.45 us there while few units
+// run) and of more (1.1 us): 8 nodes on 500 tokens 12.6 us in one piece, 11.8 in two and a merge,
+// but then the host takes 13.2; 26 nodes 17.6 and 12.4. Where all units run a merge reads
+// more: 9 large trees 31 us whole, 35 at 40 and 32 at 72.
 constexpr int64_t kTreeMergeCost = 128;
+constexpr int64_t kTreeMergeCostRows = 72;
+// Key steps of a chunk at least, on average: more chunks add partials. 8 nodes on 2,000 tokens in
+// one launch take 16.0 us at 1, 13.7 at 2, 13.6 at 3 and 13.4 at 4, 64 nodes 24.1, 18.3, 17.4
+// and 17.1, on 800 tokens 15.0, 15.0, 14.7 and 14.9; 8 nodes there 12.6, 12.0, 12.0 and 15.7.
+constexpr int64_t kTreeChunkSteps = 3;
 
 struct TreePieceRec {
   int32_t tile, step0, step1;  // query tile, and its key steps
@@ -591,7 +598,7 @@ void tile_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, 
     cost.push_back(static_cast<int32_t>(few ? kTreeFewRowsStep : kTreeStep));
     all_cost += steps[t] * static_cast<int64_t>(cost[t]);
   }
-  const int64_t n_chunks = std::max<int64_t>(1, std::min<int64_t>(n_units, all));
+  const int64_t n_chunks = std::max<int64_t>(1, std::min<int64_t>(n_units, all / kTreeChunkSteps));
   const int64_t piece = out.max_rows > 128 ? kTreePiece : kTreeFewRowsPiece;
   TreeCut trial, &best = out.cut;
   cut_tree(steps, cost, n_chunks, all_cost, piece, best);
@@ -604,7 +611,7 @@ void tile_tree(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, 
   }
   // Tiles that need no merge are worth a longer chunk; the shortest such chunk by bisection.
   if (best.split) {
-    int64_t fits = best.worst + kTreeMergeCost, low = 0;
+    int64_t fits = best.worst + (out.max_rows > 32 ? kTreeMergeCostRows : kTreeMergeCost), low = 0;
     while (low < fits && whole_tree(steps, cost, n_chunks, fits, piece, trial)) {
       best = trial;
       const int64_t mid = low + (fits - low) / 2;

@@ -189,15 +189,22 @@ def test_a_row_that_sees_one_bad_key_in_a_part(q_heads, kv_heads):
 
     from hayate_amd import _native
 
-    cached = next(c for c in range(64, 1 << 20, 64) if any(
-        r[3] == c for r in _native.plan_tree(np.array([n]), np.array([c + n]), q_heads, kv_heads,
-                                             m.num_cus).items[2:].tolist()))
-    m, handles = make_pool([cached], [n], q_heads=q_heads, kv_heads=kv_heads, seed=4)
-    batch = m.begin_tree(handles, [tree])
+    # a request before another one, cut where its drafted slots begin
+    def cut_there(cached, other):
+        plan = _native.plan_tree(np.array([n, 1]), np.array([cached + n, other + 1]), q_heads, kv_heads,
+                                 m.num_cus)
+        pieces = plan.items[2 * plan.n_chunks :]
+        return any(r[0] == 0 and r[3] == cached for r in pieces.tolist())
+
+    cached, other = next((c, x) for c in range(64, 1 << 16, 64) for x in range(0, 4096, 64)
+                         if cut_there(c, x))
+    m, handles = make_pool([cached, other], [n, 1], q_heads=q_heads, kv_heads=kv_heads, seed=4)
+    batch = m.begin_tree(handles, [tree, [-1]])
     k[11] = float("nan")
     v = v.nan_to_num(0, 0, 0)
-    batch.write_layer(0, k, v)
-    out = batch.attend_layer(q, 0)
+    last = normal(1, q_heads, D, seed=5)
+    batch.write_layer(0, torch.cat([k, last[:, :kv_heads]]), torch.cat([v, last[:, :kv_heads]]))
+    out = batch.attend_layer(torch.cat([q, last]), 0)[:n]
     assert torch.isnan(out[11]).all()
     rows = physical(m, handles[0], cached + n)
     others = [i for i in range(n) if i != 11]
