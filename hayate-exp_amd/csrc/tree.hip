@@ -7,10 +7,16 @@
 //
 // Work split: as in the decode kernel, the key steps (64 keys) of all requests, in
 // order, form one stream per kv head that the planner cuts into one chunk per
-// compute unit; a chunk holds pieces (the part of one request inside it). All
-// rows (node, head of the group) of a request read each K/V row once: up to 256
-// rows in W waves of 32. A piece that is not a request's whole stream leaves
-// fp32 partials that tree_merge_kernel joins.
+// compute unit (fewer in small ticks); a chunk holds pieces (the part of one
+// request inside it). All rows (node, head of the group) of a request read each
+// K/V row once, up to 256 of them, 32 a wave; more go into further tiles. A piece
+// that is not a tile's whole stream leaves fp32 partials that tree_merge_kernel joins.
+//
+// What bounds it: up to about 128 rows HBM (32 chains of 5 nodes, 233 MB: 42.6 us, 5.5 TB/s,
+// and 4.6 for the merge); with 256 the matrix cores at the clock that the power limit leaves
+// (8 trees of 64 nodes on 32 k tokens: 303 us, 861 TFLOP/s, MFMAs busy in 51 % of the cycles at
+// 1.63 GHz; a large library product reaches 1,209 TFLOP/s); in small ticks the latency
+// of the steps and the launch (8 nodes on 500 tokens: 12.6 us, 8 steps of 0.45).
 //
 // A chunk's tiles (64 keys of K and V, 32 KiB) go through a ring of four LDS
 // stages by direct-to-LDS loads, three tiles ahead of the one being used and
@@ -761,6 +767,12 @@ extern "C" int hy_paged_tree(
                        line_words, ws_acc, ws_ml, n_slots, group_shift,
                        __builtin_ctz(static_cast<unsigned>(page_size)), scale * hy::kLog2e);
   };
+  // The narrowest variant that holds the largest tile. Up to 128 rows, four waves only load: one
+  // wave issues such a load every 130 cycles or so, and the others' would wait behind products
+  // (32 chains: 54 us without them, 42 with); up to 64 rows two waves share a row block's keys.
+  // With 256 rows the eight waves are needed for the products. Geometric means over 16
+  // batches in the next wider variant: 8 nodes (32 rows) 27.9 us against 27.2, 16 nodes 23.4
+  // against 22.2, 32 nodes 35.4 against 32.5.
   if (max_rows <= 32)
     launch(hy::tree_kernel<1, 2, 4>, 6);
   else if (max_rows <= 64)
