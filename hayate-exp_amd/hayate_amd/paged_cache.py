@@ -704,9 +704,12 @@ class PagedTreeBatch(PagedKVBatch):
             self.plan(num_q_heads)
 
     def plan(self, num_q_heads: int) -> "_DeviceTreePlan":
-        """Work lists of this tick (built once per query-head count)."""
+        """Work lists of this tick (built once per query-head count, not during a graph
+        capture: they are copied from the host)."""
         cached = self._tree_plans.get(num_q_heads)
         if cached is None:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"plan({num_q_heads}) must be called before the capture")
             host = _native.plan_tree(
                 np.asarray(self.q_lens, dtype=np.int32),
                 np.asarray(self.kv_lens_host, dtype=np.int32), num_q_heads, self.num_kv_heads,
@@ -747,6 +750,10 @@ class PagedTreeBatch(PagedKVBatch):
             *self._layer_pools(layer_idx), *plan.args, float(scale), stream,
         )
         return out
+
+    def write_layer(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        with _current_device(self.device):
+            super().write_layer(layer_idx, k, v)
 
     def norm_rope_write_layer(self, *args, **kwargs) -> torch.Tensor:
         """As in a ``begin_tick`` batch, with every node rotated at its ``positions``
@@ -1275,9 +1282,16 @@ class PagedKVCacheManager:
         # (finds the other bad parents, before anything is reserved)
         lines = _native.tree_lines(nodes.astype(np.int32),
                                    np.array([len(t) for t in trees], dtype=np.int32))
+        held = [len(h.pages) for h in handles]
         self.reserve_tick(handles, [len(t) for t in trees])
-        batch = PagedTreeBatch(self, trees, [h.length for h in handles],
-                               [list(h.pages) for h in handles], self.num_q_heads, lines)
+        try:
+            batch = PagedTreeBatch(self, trees, [h.length for h in handles],
+                                   [list(h.pages) for h in handles], self.num_q_heads, lines)
+        except Exception:
+            for h, n in zip(handles, held):
+                self._drop_pages(h.pages[n:])
+                del h.pages[n:]
+            raise
         batch.handles = handles
         return batch
 

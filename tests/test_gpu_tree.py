@@ -297,6 +297,28 @@ def test_captured_and_replayed():
         assert torch.equal(m.v_cache.view(torch.int16), pools[1].view(torch.int16))
 
 
+def test_an_unplanned_batch_is_refused_in_a_capture():
+    m, handles = make_pool([100], [8], q_heads=None)
+    batch = m.begin_tree(handles, [chain(8)])
+    q, k = normal(8, 32, D), normal(8, 8, D)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.write_layer(0, k, k)
+        with pytest.raises(RuntimeError):
+            batch.attend_layer(q, 0)
+    graph.replay()
+    assert batch.attend_layer(q, 0).isfinite().all()
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(32, 8), (16, 1), (4, 4)])
+@pytest.mark.parametrize("sizes,cached", [([200], [130]), ([200] * 8, [3000] * 8),
+                                          ([256, 3, 70], [900, 40, 2000])])
+def test_tiles_of_128_and_of_256_rows(sizes, cached, q_heads, kv_heads):
+    """Trees of more rows than a tile holds, in tiles of both sizes."""
+    trees = [wide_tree(random.Random(i), n) for i, n in enumerate(sizes)]
+    attend(cached, trees, q_heads, kv_heads, nodes=[0, 31, 32, 63, 64, 65, 127, 150, 199, 255])
+
+
 def test_pages_past_2_31_elements():
     """A head of over 2^31 elements, its last pages in use."""
     from hayate_amd import PagedKVCacheManager

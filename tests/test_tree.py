@@ -247,6 +247,21 @@ def test_commit_tree_takes_the_batch_s_handles(monkeypatch):
     assert (a.length, b.length) == (101, 102)
 
 
+def test_a_tree_that_cannot_be_planned_reserves_nothing(monkeypatch):
+    import hayate_amd.paged_cache as pc
+
+    def refuse(self, *args):
+        raise NotImplementedError
+
+    m = pool()
+    h = handle(m, 100)
+    free, pages = m.free_page_count, list(h.pages)
+    monkeypatch.setattr(pc.PagedTreeBatch, "__init__", refuse)
+    with pytest.raises(NotImplementedError):
+        m.begin_tree([h], [chain(200)])
+    assert m.free_page_count == free and h.pages == pages
+
+
 # ------------------------------------------------------------ moves, copies
 def test_data_operations_need_a_gpu():
     m = pool()
