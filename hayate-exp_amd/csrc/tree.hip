@@ -77,7 +77,7 @@ __device__ __forceinline__ void load_rows_to_lds(const uint16_t *rows, const uin
         "global_load_lds_dwordx4 %0, %4 nt\n\t"
         "global_load_lds_dwordx4 %1, %4 offset:1024 nt\n\t"
         "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\t"
-        "global_load_lds_dwordx4 %3, %4 offset:3072 nt"
+        "global_load_lds_dwordx4 %3, %4 offset:3*1024 nt"
         :
         : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base),
           "s"(__builtin_amdgcn_readfirstlane(m0))
@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_rows_to_lds(const uint16_t *rows, const uin
         "global_load_lds_dwordx4 %0, %4\n\t"
         "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
         "global_load_lds_dwordx4 %2, %4 offset:2048\n\t"
-        "global_load_lds_dwordx4 %3, %4 offset:3072"
+        "global_load_lds_dwordx4 %3, %4 offset:3*1024"
         :
         : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base),
           "s"(__builtin_amdgcn_readfirstlane(m0))
