@@ -105,6 +105,9 @@ class PagedPrefix:
 
 
 def _stream_handle(device: torch.device) -> int:
+    """Handle of the device's current stream (0 for a pool in host memory)."""
+    if device.type != "cuda":
+        return 0
     return _native.stream_of(torch.cuda.current_device() if device.index is None
                              else device.index)
 
@@ -235,6 +238,7 @@ class _DevicePlan:
         self.prefill_merge_ptr = addr(self.prefill_merge)
         self.workspace_ptr = addr(self.workspace)
         self.prefill_workspace_ptr = addr(self.prefill_workspace)
+        self.memory = (dev, self.workspace, self.prefill_workspace)
 
 
 class PagedKVBatch:
@@ -315,6 +319,8 @@ class PagedKVBatch:
         self._extra = meta[n_meta:]
         self.cache_lens = self.cache_lens_i32.to(torch.long)
         self._meta = meta
+        self._owned = []
+        self._own(meta)
         self._pt_ptr = self.page_table.data_ptr()
         self._pt_stride = self.page_table.stride(0)
         self._q_start_ptr = self.q_start.data_ptr()
@@ -323,6 +329,23 @@ class PagedKVBatch:
         self._plans: dict[int, tuple] = {}
         if num_q_heads is not None and self.device.type == "cuda":
             self.plan(num_q_heads)
+
+    # (stream, tensor): device memory that the calls read, and the stream it was made on
+    # (none where the memory outlives every call)
+    _owned: Sequence[tuple[int, torch.Tensor]] = ()
+
+    def _own(self, *tensors: Optional[torch.Tensor]) -> None:
+        stream = _stream_handle(self.device)
+        self._owned += [(stream, t) for t in tensors if t is not None]
+
+    def _stream(self) -> int:
+        """The stream that a call goes to. The allocator takes memory to be done with when
+        the stream it was made on is, so it is told of any other."""
+        stream = _stream_handle(self.device)
+        for made_on, t in self._owned:
+            if made_on != stream:
+                t.record_stream(torch.cuda.current_stream(self.device))
+        return stream
 
     # ------------------------------------------------------------------ plan
     def plan(self, num_q_heads: int) -> "_DevicePlan":
@@ -340,6 +363,7 @@ class PagedKVBatch:
             self.tokens_per_split,
         )
         plan = _DevicePlan(host, num_q_heads, self.num_kv_heads, self.head_dim, self.device)
+        self._own(*plan.memory)
         self._plans[num_q_heads] = plan
         return plan
 
@@ -390,7 +414,7 @@ class PagedKVBatch:
             k.data_ptr(), *ks, v.data_ptr(), *vs,
             self._q_start_ptr, self._cache_lens_ptr, self._pt_ptr, self._pt_stride,
             self.num_seqs, self.total_tokens, self.num_kv_heads, self.head_dim,
-            self.page_size, _stream_handle(self.device),
+            self.page_size, self._stream(),
         )
         _native.check(rc, "hy_kv_append")
 
@@ -422,7 +446,7 @@ class PagedKVBatch:
             k_ptr, v_ptr, hs,
             self._q_start_ptr, self._cache_lens_ptr, self._pt_ptr, self._pt_stride,
             self.num_seqs, self.total_tokens, a.num_q_heads, self.num_kv_heads,
-            self.head_dim, self.page_size, _stream_handle(self.device),
+            self.head_dim, self.page_size, self._stream(),
         )
         _native.check(rc, name)
         return a.q_out
@@ -528,7 +552,7 @@ class PagedKVBatch:
             scale = 1.0 / math.sqrt(self.head_dim)
         plan = self.plan(num_q_heads)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
-        stream = _stream_handle(self.device)
+        stream = self._stream()
         lib = _native.lib()
         eps_pair = (float(eps), float(eps if k_eps is None else k_eps))
         if no_alloc:
@@ -616,7 +640,7 @@ class PagedKVBatch:
             scale = 1.0 / math.sqrt(self.head_dim)
         plan = self.plan(num_q_heads)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
-        stream = _stream_handle(self.device)
+        stream = self._stream()
         lib = _native.lib()
         if plan.n_decode:
             self._launch("hy_paged_decode", lib.hy_paged_decode,
@@ -715,6 +739,7 @@ class PagedTreeBatch(PagedKVBatch):
                 np.asarray(self.kv_lens_host, dtype=np.int32), num_q_heads, self.num_kv_heads,
                 self._num_cus)
             cached = _DeviceTreePlan(host, self, num_q_heads)
+            self._own(cached.lists, cached.workspace)
             self._tree_plans[num_q_heads] = cached
         return cached
 
@@ -743,11 +768,9 @@ class PagedTreeBatch(PagedKVBatch):
         plan = self.plan(num_q_heads)
         out = torch.empty((self.total_tokens, num_q_heads, self.head_dim), dtype=q.dtype,
                           device=q.device)
-        stream = _stream_handle(self.device)
-        plan.used_on(stream)
         self._launch("hy_paged_tree", _native.lib().hy_paged_tree,
             q.data_ptr(), *qs, out.data_ptr(), 0, num_q_heads * self.head_dim, self.head_dim,
-            *self._layer_pools(layer_idx), *plan.args, float(scale), stream,
+            *self._layer_pools(layer_idx), *plan.args, float(scale), self._stream(),
         )
         return out
 
@@ -784,14 +807,12 @@ class _DeviceTreePlan:
     def __init__(self, host: "_native.TreePlan", batch: PagedTreeBatch, num_q_heads: int):
         device, kv_heads, dim = batch.device, batch.num_kv_heads, batch.head_dim
         self.host = host
-        self.batch_meta = batch._meta
         packed = np.concatenate([host.items.reshape(-1), host.merge.reshape(-1)])
         self.lists = torch.from_numpy(packed).to(device)
         items = self.lists.data_ptr()
         size = _native.tree_workspace_bytes(host.n_slots, kv_heads, dim)
         self.workspace = (torch.empty(size // 4, dtype=torch.float32, device=device)
                           if size else None)
-        self.stream = _stream_handle(device)
         n_merge = len(host.merge)
         # the call's arguments between the pools and the scale
         self.args = (
@@ -799,14 +820,6 @@ class _DeviceTreePlan:
             host.n_chunks, host.max_rows, items + 4 * host.items.size if n_merge else None, n_merge,
             host.n_slots, None if self.workspace is None else self.workspace.data_ptr(), size,
             num_q_heads, kv_heads, dim, batch.page_size)
-
-    def used_on(self, stream: int) -> None:
-        """Keeps the lists' and the workspace's memory from reuse while `stream`, the current
-        one, may still read them, if it is not the one they were made on."""
-        if stream != self.stream:
-            for t in (self.batch_meta, self.lists, self.workspace):
-                if t is not None:
-                    t.record_stream(torch.cuda.current_stream(t.device))
 
 
 class PagedKVCacheManager:
@@ -1235,7 +1248,7 @@ class PagedKVCacheManager:
                 self.k_cache.stride(2), self.num_pages, at + 4 * (4 * n + 2), at,
                 at + 4 * (2 * n + 2), src.ctypes.data, at + 4 * (n + 1), at + 4 * (3 * n + 2), n,
                 self.num_layers, self.num_kv_heads, self.head_dim, ps,
-                _stream_handle(self.device) if self.device.type == "cuda" else None,
+                _stream_handle(self.device),
             )
         _native.check(rc, "hy_kv_move")
 
