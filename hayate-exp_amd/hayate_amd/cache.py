@@ -6,15 +6,30 @@ Tensors have shape (layers, kv_heads, tokens, head_dim).
 
 from __future__ import annotations
 
+from typing import Optional
+
+import numpy as np
 import torch
 
 
+def positions_below(positions: Optional[np.ndarray], length: int) -> Optional[np.ndarray]:
+    """Rope positions of a cache cut to `length` tokens, None if they are the slots."""
+    if positions is None:
+        return None
+    p = positions[:length]
+    return p if len(p) and p[-1] != len(p) - 1 else None
+
+
 class Cache:
-    __slots__ = ("k", "v", "_length")
+    """``positions``: rope positions of the first tokens where some were dropped between
+    them (as ``PagedCacheHandle.positions``), else None."""
+
+    __slots__ = ("k", "v", "positions", "_length")
 
     def __init__(self):
         self.k: torch.Tensor | None = None
         self.v: torch.Tensor | None = None
+        self.positions: Optional[np.ndarray] = None
         self._length = 0
 
     @classmethod
@@ -45,9 +60,12 @@ class Cache:
         if clone:
             k = k.contiguous().clone()
             v = v.contiguous().clone()
-        return Cache.from_tensors(k, v)
+        cache = Cache.from_tensors(k, v)
+        cache.positions = positions_below(self.positions, end)
+        return cache
 
     def reset(self) -> None:
         self.k = None
         self.v = None
+        self.positions = None
         self._length = 0

@@ -36,19 +36,28 @@ import numpy as np
 import torch
 
 from . import _native
-from .cache import Cache
+from .cache import Cache, positions_below
 from .constants import MIN_KV_PAGE_SIZE
 
 
 @dataclass
 class PagedCacheHandle:
     """One request's physical KV pages and logical cache length
-    (paged_cache.py:23-30)."""
+    (paged_cache.py:23-30). ``positions`` holds the rope positions of the first
+    cached tokens where ``compact`` dropped some between them (None: a token's
+    position is its slot); tokens behind those go on one by one."""
 
     slot: int
     pages: list[int] = field(default_factory=list)
     length: int = 0
     released: bool = False
+    positions: Optional[np.ndarray] = field(default=None, compare=False)
+
+    @property
+    def next_position(self) -> int:
+        """Rope position of the next token: behind the last cached one's."""
+        p = self.positions
+        return self.length if p is None else int(p[-1]) + 1 + self.length - len(p)
 
 
 class PagedPrefix:
@@ -65,12 +74,14 @@ class PagedPrefix:
     ``slice``, ``reset``); ``to_cache()`` gathers a compact Cache copy.
     """
 
-    __slots__ = ("manager", "pages", "_length")
+    __slots__ = ("manager", "pages", "positions", "_length")
 
-    def __init__(self, manager: "PagedKVCacheManager", pages: list[int], length: int):
+    def __init__(self, manager: "PagedKVCacheManager", pages: list[int], length: int,
+                 positions: Optional[np.ndarray] = None):
         # the caller has already taken one reference per page for this object
         self.manager = manager
         self.pages = pages
+        self.positions = positions  # as a handle's
         self._length = length
 
     @property
@@ -90,18 +101,21 @@ class PagedPrefix:
             raise ValueError(f"cache slice end {end} exceeds cache length {self._length}")
         pages = self.pages[: -(-end // self.manager.page_size)]
         self.manager._ref_pages(pages)
-        return PagedPrefix(self.manager, list(pages), end)
+        return PagedPrefix(self.manager, list(pages), end, positions_below(self.positions, end))
 
     def reset(self) -> None:
         """Drop the page references (idempotent)."""
         if self.pages:
             self.manager._drop_pages(self.pages)
         self.pages = []
+        self.positions = None
         self._length = 0
 
     def to_cache(self) -> Cache:
         """A compact (layers, Hkv, length, D) copy gathered from the pages."""
-        return self.manager._gather(self.pages, self._length)
+        cache = self.manager._gather(self.pages, self._length)
+        cache.positions = self.positions
+        return cache
 
 
 def _stream_handle(device: torch.device) -> int:
@@ -253,7 +267,12 @@ class PagedKVBatch:
     Uniform batches (``begin_batch``) use the reference's tensor shapes:
     k/v (B, Hkv, T, D) for ``write_layer``, q (B, Hq, T, D) for
     ``attend_layer``. Varlen ticks (``begin_tick``) use packed (N, H, D).
+
+    ``positions`` holds every packed token's rope position (int32) where one of the
+    caches dropped tokens (``compact``); it is None where they are cache_lens + index.
     """
+
+    positions: Optional[torch.Tensor] = None
 
     def __init__(
         self,
@@ -265,6 +284,7 @@ class PagedKVBatch:
         num_q_heads: Optional[int],
         tokens_per_split: int = 0,
         extra: Optional[np.ndarray] = None,
+        first_positions: Optional[list[int]] = None,
     ):
         self.k_cache = manager.k_cache
         self.v_cache = manager.v_cache
@@ -305,8 +325,13 @@ class PagedKVBatch:
             ]
         )
         n_meta = self._meta_np.size
+        if first_positions is not None:
+            # each sequence's first token is rotated there, not at its slot
+            extra = (np.arange(self.total_tokens, dtype=np.int32)
+                     + np.repeat(np.asarray(first_positions, dtype=np.int32) - q_start[:-1], q_lens))
         if extra is not None:
-            # a subclass's own metadata travels in the same copy, from 16 bytes on
+            # more metadata, a subclass's own or the positions, travels in the same
+            # copy, from 16 bytes on
             n_meta += -n_meta % 4
             self._meta_np = np.concatenate(
                 [self._meta_np, np.zeros(n_meta - self._meta_np.size, dtype=np.int32), extra])
@@ -327,8 +352,17 @@ class PagedKVBatch:
         self._cache_lens_ptr = self.cache_lens_i32.data_ptr()
         self._kv_lens_ptr = self.kv_lens.data_ptr()
         self._plans: dict[int, tuple] = {}
+        if first_positions is not None:
+            self._rotate_at(self._extra, extra)
         if num_q_heads is not None and self.device.type == "cuda":
             self.plan(num_q_heads)
+
+    def _rotate_at(self, positions: torch.Tensor, host: np.ndarray) -> None:
+        """Has the append rotate each packed token at its entry of `positions`."""
+        self.positions = positions
+        # what the rope tables have to hold
+        self._max_kv = int(host.max()) + 1
+        self._append_call = ("hy_qknorm_rope_append_at", (positions.data_ptr(),))
 
     # (stream, tensor): device memory that the calls read, and the stream it was made on
     # (none where the memory outlives every call)
@@ -434,7 +468,7 @@ class PagedKVBatch:
         """Fused q/k RMSNorm + RoPE + paged append of k and v
         (attention.py:62-75 with rope.py:31-47). Inputs are the projection
         outputs, (B, T, H, D) (or packed (N, H, D) for a varlen tick); positions
-        are cache_lens + token index. `eps` is the q norm's epsilon and
+        are cache_lens + token index, or the batch's ``positions``. `eps` is the q norm's epsilon and
         `k_eps` the k norm's (default: `eps`). Returns the rotated q in the
         same layout; k and v go to the pool only."""
         a = self._append_inputs("norm_rope_write_layer", q, k, v, q_norm_weight,
@@ -529,9 +563,19 @@ class PagedKVBatch:
         no_alloc=True runs both launches through
         hy_paged_decode_append_noalloc, whose partials live in the library's
         static device scratch instead of the plan's workspace (same
-        results; raises MemoryError if the tick's partials do not fit)."""
+        results; raises MemoryError if the tick's partials do not fit).
+
+        The launch rotates at cache_lens; a batch with ``positions`` of its own
+        makes the two calls (and refuses no_alloc)."""
         if not self.decode_only:
             raise ValueError("decode_layer needs q_len == 1 for every sequence")
+        if self.positions is not None:
+            if no_alloc:
+                raise NotImplementedError("no_alloc rotates at the slots, not at `positions`")
+            q_rot = self.norm_rope_write_layer(layer_idx, q, k, v, q_norm_weight, k_norm_weight,
+                                               eps, cos, sin, k_eps=k_eps)
+            return q_rot, self.attend_layer(q_rot if self.varlen else q_rot.transpose(1, 2),
+                                            layer_idx, scale)
         a = self._append_inputs("decode_layer", q, k, v, q_norm_weight, k_norm_weight, cos,
                                 sin)
         num_q_heads = a.num_q_heads
@@ -682,7 +726,7 @@ class PagedTreeBatch(PagedKVBatch):
     """A tick that checks drafted tokens: each request's tokens form a tree.
 
     Node i of a request with c cached tokens holds slot c + i of its cache, is
-    rotated at position c + depth(i) and sees the c cached tokens, its ancestors and
+    rotated at position c + depth(i) (from the handle's ``next_position`` on) and sees the c cached tokens, its ancestors and
     itself, so one forward pass gives every node the states it would have at the end
     of its own branch. ``parents[b][i]`` is node i's parent, an earlier node of the
     request, or -1 for a child of the cached context (several nodes may be). A node
@@ -704,26 +748,27 @@ class PagedTreeBatch(PagedKVBatch):
 
     def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],
-                 num_q_heads: Optional[int], lines: Optional[tuple] = None):
+                 num_q_heads: Optional[int], lines: Optional[tuple] = None,
+                 first_positions: Optional[list[int]] = None):
         self.parents = [np.asarray(p) for p in parents]
         q_lens = [len(p) for p in self.parents]
         # a node's line: a bit for each drafted slot it sees
         lines, depths = lines or _native.tree_lines(
             np.concatenate(self.parents).astype(np.int32), np.array(q_lens, dtype=np.int32))
         self.line_words = lines.shape[1]
-        positions = depths + np.repeat(np.asarray(cache_lens_host, dtype=np.int32), q_lens)
+        # a tree's roots follow the cached tokens
+        roots = cache_lens_host if first_positions is None else first_positions
+        positions = depths + np.repeat(np.asarray(roots, dtype=np.int32), q_lens)
         self._tree_plans: dict[int, _DeviceTreePlan] = {}
         super().__init__(manager, q_lens, cache_lens_host, page_lists, varlen=True,
                          num_q_heads=None,
                          extra=np.concatenate([lines.reshape(-1).view(np.int32), positions]))
         # every tree goes through the tree kernel, requests with one node included
         self.decode_only = False
-        # rope positions go by depth, so a wide tree needs fewer than its slots
-        self._max_kv = int(positions.max()) + 1
         self.lines = self._extra[: lines.size]
-        self.positions = self._extra[lines.size :]
         self._lines_ptr = self.lines.data_ptr()
-        self._append_call = ("hy_qknorm_rope_append_at", (self.positions.data_ptr(),))
+        # (by depth, so a wide tree needs fewer rope positions than its slots)
+        self._rotate_at(self._extra[lines.size :], positions)
         if num_q_heads is not None and self.device.type == "cuda":
             self.plan(num_q_heads)
 
@@ -944,6 +989,7 @@ class PagedKVCacheManager:
                     self._ref_pages(cache.pages)
                     handle.pages = list(cache.pages)
                     handle.length = cache.length
+                    handle.positions = cache.positions
             elif cache is not None and cache.length:
                 self.import_cache(handle, cache)
         except Exception:
@@ -972,6 +1018,7 @@ class PagedKVCacheManager:
             )
             _native.check(rc, "hy_page_scatter")
         handle.length = cache.length
+        handle.positions = getattr(cache, "positions", None)
 
     def truncate(self, handle: PagedCacheHandle, length: int) -> None:
         """Shorten a cache, returning whole pages past the end (168-178)."""
@@ -984,6 +1031,7 @@ class PagedKVCacheManager:
         handle.pages = handle.pages[:keep]
         self._drop_pages(released)
         handle.length = length
+        handle.positions = positions_below(handle.positions, length)
 
     def snapshot(self, handle: PagedCacheHandle, length: int | None = None) -> Cache:
         """Gather the first `length` positions into a compact Cache with
@@ -993,7 +1041,9 @@ class PagedKVCacheManager:
         snapshot_len = handle.length if length is None else length
         if snapshot_len < 0 or snapshot_len > handle.length:
             raise ValueError("snapshot length must be within the current cache length")
-        return self._gather(handle.pages, snapshot_len)
+        cache = self._gather(handle.pages, snapshot_len)
+        cache.positions = positions_below(handle.positions, snapshot_len)
+        return cache
 
     def share(self, handle: PagedCacheHandle, length: int | None = None) -> PagedPrefix:
         """Zero-copy snapshot: the first `length` tokens (default: all) as a
@@ -1006,7 +1056,8 @@ class PagedKVCacheManager:
             raise ValueError("snapshot length must be within the current cache length")
         pages = handle.pages[: -(-share_len // self.page_size)]
         self._ref_pages(pages)
-        return PagedPrefix(self, list(pages), share_len)
+        return PagedPrefix(self, list(pages), share_len,
+                           positions_below(handle.positions, share_len))
 
     def _gather(self, page_list: Sequence[int], snapshot_len: int) -> Cache:
         _require_hip(self.k_cache, "snapshot")
@@ -1032,6 +1083,7 @@ class PagedKVCacheManager:
         self._drop_pages(handle.pages)
         handle.pages.clear()
         handle.length = 0
+        handle.positions = None
         handle.released = True
         self._free_slots.append(handle.slot)
 
@@ -1073,6 +1125,7 @@ class PagedKVCacheManager:
             self._ref_pages(shared)
             child.pages = list(shared)
             child.length = length
+            child.positions = positions_below(handle.positions, length)
             return child
         if shared:
             _require_hip(self.k_cache, "fork with copies")
@@ -1085,6 +1138,7 @@ class PagedKVCacheManager:
             self.release(child)
             raise
         child.length = length
+        child.positions = positions_below(handle.positions, length)
         return child
 
     def _make_private(self, handle: PagedCacheHandle, start: int, end: int) -> None:
@@ -1182,7 +1236,9 @@ class PagedKVCacheManager:
         tokens at positions sources[b] (ascending, none before the position it fills),
         K and V of every layer, as if all were read before any is written. Positions
         may lie past the handle's length, in space reserved for it; lengths do not
-        change. Shared pages that would be written are copied first."""
+        change, nor does the rope position that a later tick goes on from (``compact``
+        keeps that of the last kept token). Shared pages that would be written are
+        copied first."""
         handles = list(handles)
         _require_hip(self.k_cache, "move_tokens")
         if not self._rows_of_256_bytes():
@@ -1260,16 +1316,24 @@ class PagedKVCacheManager:
 
     def compact(self, handle: PagedCacheHandle, keep: Sequence[int]) -> None:
         """Keep only the tokens at positions `keep` (ascending), closed up in every
-        layer, and return the pages that this empties. Keys stay rotated at the positions they
-        were written for."""
+        layer, and return the pages that this empties. Keys stay rotated at the rope positions
+        they were written for, and the next token follows the last kept one's
+        (``handle.next_position``)."""
         if handle.released:
             raise RuntimeError("cannot compact a released cache handle")
         kept = _int_array(keep, "keep")
         if len(kept) and (kept[0] < 0 or kept[-1] >= handle.length or (np.diff(kept) <= 0).any()):
             raise ValueError("keep must be ascending positions within the cache's length")
+        positions = None
         if len(kept) and kept[-1] != len(kept) - 1:
             self.move_tokens([handle], [kept], [0])
+            positions = kept.copy()
+        if handle.positions is not None:
+            old = handle.positions
+            after = np.arange(old[-1] + 1, handle.next_position)
+            positions = positions_below(np.concatenate([old, after])[kept], len(kept))
         self._set_length(handle, len(kept))
+        handle.positions = positions
 
     # ---------------------------------------------------------- drafted trees
     def begin_tree(self, handles: Sequence[PagedCacheHandle],
@@ -1299,7 +1363,8 @@ class PagedKVCacheManager:
         self.reserve_tick(handles, [len(t) for t in trees])
         try:
             batch = PagedTreeBatch(self, trees, [h.length for h in handles],
-                                   [list(h.pages) for h in handles], self.num_q_heads, lines)
+                                   [list(h.pages) for h in handles], self.num_q_heads, lines,
+                                   self._first_positions(handles))
         except Exception:
             for h, n in zip(handles, held):
                 self._drop_pages(h.pages[n:])
@@ -1390,6 +1455,13 @@ class PagedKVCacheManager:
         self._make_all_private([(h, h.length, h.length + q, h.length)
                                 for h, q in zip(handles, q_lens)])
 
+    @staticmethod
+    def _first_positions(handles: Sequence[PagedCacheHandle]) -> Optional[list[int]]:
+        """Every handle's next rope position, None if all are at their slots."""
+        if all(h.positions is None for h in handles):
+            return None
+        return [h.next_position for h in handles]
+
     def begin_batch(
         self, handles: Sequence[PagedCacheHandle], query_len: int
     ) -> PagedKVBatch:
@@ -1408,6 +1480,7 @@ class PagedKVCacheManager:
             self, q_lens, [h.length for h in handles], [list(h.pages) for h in handles],
             varlen=False, num_q_heads=self.num_q_heads,
             tokens_per_split=self.tokens_per_split,
+            first_positions=self._first_positions(handles),
         )
 
     def begin_tick(
@@ -1421,6 +1494,7 @@ class PagedKVCacheManager:
             self, q_lens, [h.length for h in handles], [list(h.pages) for h in handles],
             varlen=True, num_q_heads=self.num_q_heads,
             tokens_per_split=self.tokens_per_split,
+            first_positions=self._first_positions(handles),
         )
 
     def reserve_tick(self, handles: Sequence[PagedCacheHandle],

@@ -154,7 +154,8 @@ class PrefixCache:
     def put(self, tokens: Sequence[int], cache) -> None:
         """Store the first min(len(tokens), cache.length, max_tokens) tokens.
         A paged entry takes its own page references (no copy); a Cache entry
-        is cloned, as in the reference."""
+        is cloned, as in the reference. Not for tokens of which the cache dropped
+        some: the rest was computed behind those."""
         if self.max_tokens == 0 or not tokens or cache.length == 0:
             return
         n = min(len(tokens), cache.length, self.max_tokens)
@@ -162,6 +163,9 @@ class PrefixCache:
             return
         key = tuple(tokens[:n])
         stored = cache.slice(n, clone=True)
+        if getattr(stored, "positions", None) is not None:
+            _release(stored)
+            raise ValueError("the cache dropped some of the prompt's tokens")
         old = self._ids.get(key)
         if old is not None:
             self._drop(old)

@@ -226,7 +226,8 @@ class StaticTickBatch(PagedKVBatch):
         """Rewrites the metadata and work lists for `handles` (whose append
         space is reserved) and enqueues the copy on the current stream.
         Returns False, changing nothing, when the tick does not fit the
-        buffers (more pages per sequence, records or slots than sized); if
+        buffers (more pages per sequence, records or slots than sized) or a
+        cache dropped tokens (the tick rotates at the slots); if
         only the prefill partial slots ran short, ``prefill_slots_needed``
         then says how many the plan needs. `host` is the plan of `handles`
         when the caller already has it."""
@@ -235,7 +236,7 @@ class StaticTickBatch(PagedKVBatch):
             raise ValueError(f"static tick batch holds {B} sequences, got {len(handles)}")
         cache = [h.length for h in handles]
         kv = [c + q for c, q in zip(cache, self.q_lens)]
-        if any(len(h.pages) > self.max_pages for h in handles):
+        if any(len(h.pages) > self.max_pages or h.positions is not None for h in handles):
             return False
         if host is None:
             host = _plan_for(self._manager, self.q_lens, self.num_q_heads, handles)
@@ -306,7 +307,8 @@ class TickGraphRunner:
     ``run(handles, q_lens, token_ids)`` returns the logits of each sequence's
     last token (B, 1, vocab) for handles whose append space the caller has
     reserved, or None when the tick must run eagerly (a prompt shape seen
-    for the first time, or a tick that does not fit the static buffers)."""
+    for the first time, a tick that does not fit the static buffers, or a
+    cache that dropped tokens)."""
 
     def __init__(self, model, manager: PagedKVCacheManager, max_tokens: int,
                  max_graphs: int = 8):
@@ -349,6 +351,8 @@ class TickGraphRunner:
         key = tuple(int(q) for q in q_lens)
         if len(key) != len(handles) or len(token_ids) != sum(key):
             raise ValueError("one query length per handle and one token id per query row")
+        if any(h.positions is not None for h in handles):
+            return None
         st = self._states.get(key)
         host = None
         if st is None:
