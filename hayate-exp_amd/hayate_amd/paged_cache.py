@@ -1290,7 +1290,8 @@ class PagedKVCacheManager:
                 # ascending on both sides, so the tokens that stay are the first ones
                 end = start + len(of_h)
                 stay = int(np.count_nonzero(of_h == np.arange(start, end)))
-                spans.append((h, start + stay, end, max(h.length, int(of_h[-1]) + 1)))
+                # (copies hold whole pages: reserved tokens may be moved by a later call)
+                spans.append((h, start + stay, end, len(h.pages) * ps))
             self._make_all_private(spans)
             pages = []
             for h, page, last in zip(handles, first_page, lasts):

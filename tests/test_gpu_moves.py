@@ -268,3 +268,19 @@ def test_a_refused_call_enqueues_nothing():
         assert move(src, first) == _native.HY_EINVAL
     torch.cuda.synchronize()
     assert same([bits(m.k_cache), bits(m.v_cache)], before)
+
+
+def test_two_moves_of_drafted_tokens_out_of_a_shared_page():
+    """The second move reads a drafted token behind the first one's, in the copy that the first
+    one made of the shared page."""
+    m, (h,) = make_pool([100], [28], layers=2, spare=6)
+    scramble(m)
+    before = logical(m, h, 128)
+    child = m.fork(h)
+    m.move_tokens([h], [[105]], [100])
+    m.move_tokens([h], [[110, 120]], [101])
+    want = [x.clone() for x in before]
+    for x, old in zip(want, before):
+        x[:, :, 100:103] = old[:, :, [105, 110, 120]]
+    assert h.pages[0] != child.pages[0] and same(logical(m, h, 128), want)
+    assert same(logical(m, child, 128), before)

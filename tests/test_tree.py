@@ -424,3 +424,19 @@ def test_c_tree_attention_is_checked():
     assert call(chunks=0) == _native.HY_OK
     assert lib.hy_tree_workspace_bytes(0, 8, 128) == 0
     assert lib.hy_tree_workspace_bytes(3, 8, 128) == 3 * 8 * 32 * (128 + 2) * 4
+
+def test_moves_into_a_shared_page_keep_what_is_reserved_in_it(monkeypatch):
+    """Drafted tokens sit past the handle's length. A move that gives the handle its own copy of
+    a page takes all of them over: a later move may still read them."""
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    m = pool()
+    h = handle(m, 100)
+    m.begin_tree([h], [chain(20)])
+    m.fork(h)
+    copied = []
+    monkeypatch.setattr(m, "_copy_pages", lambda src, dst, tokens: copied.append(list(tokens)))
+    monkeypatch.setattr(pc._native, "lib", lambda: type("", (), {"hy_kv_move": lambda *a: 0}))
+    m.move_tokens([h], [[105]], [100])
+    assert copied == [[128]]
