@@ -750,7 +750,7 @@ class PagedTreeBatch(PagedKVBatch):
                  cache_lens_host: list[int], page_lists: list[list[int]],
                  num_q_heads: Optional[int], lines: Optional[tuple] = None,
                  first_positions: Optional[list[int]] = None):
-        self.parents = [np.asarray(p) for p in parents]
+        self.parents = [np.asarray(p).copy() for p in parents]  # a caller may reuse its arrays
         q_lens = [len(p) for p in self.parents]
         # a node's line: a bit for each drafted slot it sees
         lines, depths = lines or _native.tree_lines(

@@ -440,3 +440,20 @@ def test_moves_into_a_shared_page_keep_what_is_reserved_in_it(monkeypatch):
     monkeypatch.setattr(pc._native, "lib", lambda: type("", (), {"hy_kv_move": lambda *a: 0}))
     m.move_tokens([h], [[105]], [100])
     assert copied == [[128]]
+
+@pytest.mark.parametrize("make", [lambda x: np.array(x, dtype=np.int64), torch.tensor,
+                                  lambda x: np.array(x, dtype=np.int32)])
+def test_a_batch_keeps_its_own_trees(make):
+    """A caller may write the next tick's parents into the same arrays."""
+    m = pool()
+    h = handle(m, 5)
+    tree = make([-1, 0, 1, 0])
+    batch = m.begin_tree([h], [tree])
+    tree[:] = -1
+    assert batch.check_path(0, [0, 1, 2]) == [0, 1, 2]
+    with pytest.raises(ValueError):
+        batch.check_path(0, [2])
+    tree = make([-1, 0, 1, 0])
+    batch = PagedTreeBatch(m, [tree], [5], [list(h.pages)], None)
+    tree[:] = -1
+    assert batch.check_path(0, [0, 1, 2]) == [0, 1, 2]
