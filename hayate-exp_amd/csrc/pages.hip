@@ -190,8 +190,11 @@ extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
   if (num_seqs == 0) return HY_OK;
   HY_REQUIRE(pages && page_start && first_page && src && src_start && first,
              "hy_kv_move: null pointer argument");
-  hy::Marks written(tokens);
-  if (!written.ok()) {
+  // Of the tokens: moved to; filled by a token that stays; read for a move; read for moves of
+  // two sequences. (Only other sequences' reads matter, so the last two go with several.)
+  hy::Marks written(tokens), stays(tokens), read(num_seqs > 1 ? tokens : 1),
+      shared(num_seqs > 1 ? tokens : 1);
+  if (!written.ok() || !stays.ok() || !read.ok() || !shared.ok()) {
     hy::set_error("hy_kv_move: no host memory to check %lld tokens", static_cast<long long>(tokens));
     return HY_ENOSPACE;
   }
@@ -218,6 +221,7 @@ extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
           HY_REQUIRE(pages[i] >= 0 && pages[i] < num_pages,
                      "hy_kv_move: page %d is not in the pool of %d", pages[i], num_pages);
       }
+      int32_t own = src_start[b];  // the first source not before the position being filled
       for (int32_t i = src_start[b]; i < src_start[b + 1]; ++i) {
         const int64_t from = src[i] - base;
         const int64_t to = static_cast<int64_t>(first[b]) + (i - src_start[b]) - base;
@@ -227,13 +231,23 @@ extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
                      "hy_kv_move: sequence %d cannot take its token %d to position %lld (sources "
                      "ascend, none before the position it fills, all in the given pages)",
                      b, src[i], static_cast<long long>(to + base));
-        if (from == to) continue;
+        if (from == to && pass == 1) continue;
         const int32_t *list = pages + page_start[b];
-        const int64_t s = static_cast<int64_t>(list[from / page_size]) * page_size + from % page_size;
         const int64_t d = static_cast<int64_t>(list[to / page_size]) * page_size + to % page_size;
+        if (from == to) {
+          HY_REQUIRE(!written.has(d), "hy_kv_move: sequence %d shares pages that are written", b);
+          stays.set(d);
+          continue;
+        }
+        const int64_t s = static_cast<int64_t>(list[from / page_size]) * page_size + from % page_size;
         if (pass == 0) {
-          HY_REQUIRE(!written.has(s) && !written.has(d),
-                     "hy_kv_move: sequence %d shares pages that are written", b);
+          bool clash = written.has(s) || written.has(d) || stays.has(d);
+          if (num_seqs > 1) {
+            (read.has(s) ? shared : read).set(s);
+            while (src[own] - base < to) ++own;  // ends at i at the latest
+            clash = clash || shared.has(d) || (read.has(d) && src[own] - base != to);
+          }
+          HY_REQUIRE(!clash, "hy_kv_move: sequence %d shares pages that are written", b);
           written.set(d);
           continue;
         }

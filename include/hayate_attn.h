@@ -525,8 +525,9 @@ int hy_paged_tree(const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
  * .. page_start[b + 1]); page_start and src_start have num_seqs + 1 entries. All arrays are
  * host memory, read before the call returns and checked: positions inside the given
  * pages, page ids below num_pages, sources ascending and none before the position it fills,
- * no written token read or written for another sequence; otherwise HY_EINVAL and nothing
- * is enqueued. Tokens that stay cost nothing; runs of tokens are moved together.
+ * no written token read, written or kept in place for another sequence, in whichever order the
+ * two come; otherwise HY_EINVAL and nothing is enqueued. Tokens that stay cost nothing; runs of
+ * tokens are moved together.
  * No reference counterpart (its caches only grow or are cut, paged_cache.py:168-178).
  */
 int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,

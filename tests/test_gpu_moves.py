@@ -284,3 +284,26 @@ def test_two_moves_of_drafted_tokens_out_of_a_shared_page():
         x[:, :, 100:103] = old[:, :, [105, 110, 120]]
     assert h.pages[0] != child.pages[0] and same(logical(m, h, 128), want)
     assert same(logical(m, child, 128), before)
+
+
+def test_one_sequence_keeps_what_another_reads():
+    """Two sequences over one shared page, in C: tokens that stay for one may be read for the
+    other's moves, and both may read a token."""
+    m, (h, g) = make_pool([128, 128], [0, 0], layers=2, kv_heads=3)
+    scramble(m)
+    a, b = logical(m, h, 128), logical(m, g, 128)
+    arrays = [np.array(x, dtype=np.int32) for x in (
+        [h.pages[0], g.pages[0], h.pages[0]], [0, 1, 3], [0, 0],
+        [5, 6, 90, 129, 133, 134, 218], [0, 3, 7], [5, 10])]
+    rc = _native.lib().hy_kv_move(
+        m.k_cache.data_ptr(), m.v_cache.data_ptr(), m.k_cache.stride(0), m.k_cache.stride(2),
+        m.num_pages, *(x.ctypes.data for x in arrays), 2, 2, 3, D, m.page_size, None)
+    assert rc == _native.HY_OK, _native.last_error()
+    torch.cuda.synchronize()
+    # the first sequence: 5 and 6 stay, 90 goes to 7; the second, whose positions from 128 on
+    # are the first one's page: its 1, 5, 6 and 90 to 10 .. 13
+    want = [x.clone() for x in a], [x.clone() for x in b]
+    for x, y, old in zip(*want, a):
+        x[:, :, 7] = old[:, :, 90]
+        y[:, :, 10:14] = old[:, :, [1, 5, 6, 90]]
+    assert same(logical(m, h, 128), want[0]) and same(logical(m, g, 128), want[1])

@@ -457,3 +457,28 @@ def test_a_batch_keeps_its_own_trees(make):
     batch = PagedTreeBatch(m, [tree], [5], [list(h.pages)], None)
     tree[:] = -1
     assert batch.check_path(0, [0, 1, 2]) == [0, 1, 2]
+
+
+def test_c_moves_of_sequences_that_share_a_page():
+    """A position that a sequence fills, by a move or by a token that stays, is written for no
+    other one, and a written token is read for no other one, in whichever order they come."""
+    two = dict(page_start=[0, 1, 2], src_start=[0, 1, 2])
+    for moves in (((5, 1), (9, 5)),    # the second writes what the first read
+                  ((9, 5), (5, 1)),    # the first writes what the second reads
+                  ((5, 5), (9, 5)),    # ... or what stays for the first
+                  ((9, 5), (5, 5)),
+                  ((9, 5), (9, 5))):   # both write it
+        src, first = [m[0] for m in moves], [m[1] for m in moves]
+        assert c_move([3, 3], src, first, **two) == _native.HY_EINVAL, moves
+        assert "share" in _native.last_error()
+    # read for two others, then written for itself
+    assert c_move([3, 3, 3], [5, 5, 9], [1, 2, 5], page_start=[0, 1, 2, 3],
+                  src_start=[0, 1, 2, 3]) == _native.HY_EINVAL
+    # both read it, and the second, which reads it in front of the token that it fills it with
+    assert c_move([3, 3], [5, 5, 6, 7, 8], [1, 2], page_start=[0, 1, 2],
+                  src_start=[0, 1, 5]) == _native.HY_EINVAL
+    # one page twice in a sequence: position 130 is position 2, which stays
+    assert c_move([0, 0], [*range(2, 130), 140], [2]) == _native.HY_EINVAL
+    # a shared page whose tokens stay for both
+    assert c_move([3, 3], [5, 6, 5, 6, 7], [5, 5], page_start=[0, 1, 2],
+                  src_start=[0, 2, 5]) == _native.HY_OK
