@@ -215,8 +215,9 @@ extern "C" int hy_kv_move(void *k_pool, void *v_pool, int64_t pool_layer_stride,
       const int64_t held = static_cast<int64_t>(page_start[b + 1]) - page_start[b];
       const int64_t base = static_cast<int64_t>(first_page[b]) * page_size;
       if (pass == 0) {
-        HY_REQUIRE(held >= 0 && first_page[b] >= 0 && src_start[b + 1] >= src_start[b],
-                   "hy_kv_move: sequence %d has a negative count", b);
+        HY_REQUIRE(held >= 0 && first_page[b] >= 0 && src_start[b + 1] >= src_start[b] &&
+                       page_start[b] >= 0 && src_start[b] >= 0,
+                   "hy_kv_move: sequence %d has a negative start or count", b);
         for (int32_t i = page_start[b]; i < page_start[b + 1]; ++i)
           HY_REQUIRE(pages[i] >= 0 && pages[i] < num_pages,
                      "hy_kv_move: page %d is not in the pool of %d", pages[i], num_pages);

@@ -482,3 +482,9 @@ def test_c_moves_of_sequences_that_share_a_page():
     # a shared page whose tokens stay for both
     assert c_move([3, 3], [5, 6, 5, 6, 7], [5, 5], page_start=[0, 1, 2],
                   src_start=[0, 2, 5]) == _native.HY_OK
+
+
+def test_c_moves_begin_inside_their_arrays():
+    for kw in (dict(page_start=[-1, 1]), dict(src_start=[-2, 1])):
+        assert c_move([3], [5], [1], **kw) == _native.HY_EINVAL
+        assert "negative" in _native.last_error()
