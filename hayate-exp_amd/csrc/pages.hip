@@ -119,12 +119,13 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(uint16_t *k_pool, uint16
 #pragma unroll
     for (int j = 0; j < kCopyPasses; ++j)
       if (row0 + j * kRowsPerPass < r.n)
-        x[j] = load16_stream(src + (row0 + j * kRowsPerPass) * kHeadDim);
+        x[j] = load16_stream(src + static_cast<int64_t>(row0 + j * kRowsPerPass) * kHeadDim);
 #pragma unroll
     for (int j = 0; j < kCopyPasses; ++j)
       if (row0 + j * kRowsPerPass < r.n)
         __builtin_nontemporal_store(
-            x[j], reinterpret_cast<u32x4 *>(dst + (row0 + j * kRowsPerPass) * kHeadDim));
+            x[j], reinterpret_cast<u32x4 *>(
+                      dst + static_cast<int64_t>(row0 + j * kRowsPerPass) * kHeadDim));
   }
 }
 

@@ -307,3 +307,23 @@ def test_one_sequence_keeps_what_another_reads():
         x[:, :, 7] = old[:, :, 90]
         y[:, :, 10:14] = old[:, :, [1, 5, 6, 90]]
     assert same(logical(m, h, 128), want[0]) and same(logical(m, g, 128), want[1])
+
+
+def test_a_page_past_2_31_elements():
+    """Pages of 2^25 tokens: a row's offset inside one passes 32 bits."""
+    from hayate_amd import PagedKVCacheManager
+
+    page = 1 << 25
+    m = PagedKVCacheManager(1, 1, D, 2 * page, page, 2, torch.bfloat16, "cuda")
+    h = m.allocate()
+    m.claim_pages(h, [1])
+    h.length = page
+    rows = torch.tensor([0, 1, (1 << 24) - 1, 1 << 24, (1 << 24) + 5, page - 1], device="cuda")
+    for p in (m.k_cache, m.v_cache):
+        bits(p)[:, :, :, rows] = -1
+        bits(p)[:, :, :, page + rows] = torch.arange(6 * D, device="cuda",
+                                                     dtype=torch.int16).view(1, 1, 1, 6, D)
+    child = m.fork(h, copy=True)
+    assert child.pages == [0]
+    for p in (m.k_cache, m.v_cache):
+        assert torch.equal(bits(p)[:, :, :, rows], bits(p)[:, :, :, page + rows])
