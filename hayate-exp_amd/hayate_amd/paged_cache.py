@@ -421,14 +421,22 @@ class PagedKVBatch:
         return hit
 
     def _layout(self, t: torch.Tensor, uniform_layout: str) -> tuple:
+        """Row strides of t, whose rows the kernels take as many and as long as the batch's."""
+        shape = t.shape
+        if t.device != self.device:
+            raise ValueError(f"rows are on {t.device}, the pool on {self.device}")
+        if shape[-1] != self.head_dim:
+            raise ValueError(f"rows of {shape[-1]} values do not match the pool's {self.head_dim}")
         if self.varlen:
-            if t.dim() != 3 or t.shape[0] != self.total_tokens:
+            if len(shape) != 3 or shape[0] != self.total_tokens:
                 raise ValueError(
                     f"varlen batch expects packed (tokens={self.total_tokens}, heads, dim)"
                 )
             return _row_strides(t, "thd", 0)
-        if t.dim() != 4:
+        if len(shape) != 4:
             raise ValueError("uniform batch expects 4-D tensors")
+        if shape[0] != self.num_seqs or shape[2 if uniform_layout == "bhtd" else 1] != self.query_len:
+            raise ValueError(f"uniform batch expects {self.num_seqs} sequences of {self.query_len} rows")
         return _row_strides(t, uniform_layout, self.query_len)
 
     # ----------------------------------------------------------- write path
@@ -505,7 +513,7 @@ class PagedKVBatch:
         num_q_heads = q.shape[-2]
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qs = self._layout(q, "bthd")
-        qos = self._layout(q_out, "bthd")
+        qos = (0, num_q_heads * self.head_dim, self.head_dim)  # contiguous, whatever the layout
         ks = self._layout(k, "bthd")
         vs = self._layout(v, "bthd")
         if (cos is None) != (sin is None):
@@ -513,6 +521,10 @@ class PagedKVBatch:
         if cos is not None:
             if cos.dtype != torch.float32 or sin.dtype != torch.float32:
                 raise TypeError("rope tables must be float32")
+            if cos.device != self.device or sin.device != self.device:
+                raise ValueError(f"rope tables must be on the pool's device, {self.device}")
+            if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != self.head_dim:
+                raise ValueError(f"rope tables must both be (positions, {self.head_dim})")
             cos = cos.contiguous()
             sin = sin.contiguous()
             max_pos = cos.shape[0]
@@ -528,6 +540,8 @@ class PagedKVBatch:
         for w in (qw, kw):
             if w is not None and (w.dtype != torch.bfloat16 or w.numel() != self.head_dim):
                 raise TypeError("norm weights must be bfloat16 (head_dim,)")
+            if w is not None and w.device != self.device:
+                raise ValueError(f"norm weights must be on the pool's device, {self.device}")
         return _AppendInputs(
             q=q, q_out=q_out, num_q_heads=num_q_heads, keep=(k, v, qw, kw, cos, sin),
             head=(q.data_ptr(), *qs, q_out.data_ptr(), *qos, k.data_ptr(), *ks,
@@ -628,8 +642,6 @@ class PagedKVBatch:
             raise ValueError("k and v must have the same shape")
         if k.dtype != self.k_cache.dtype or v.dtype != self.v_cache.dtype:
             raise TypeError("k/v dtype must match the pool dtype")
-        if k.shape[-1] != self.head_dim:
-            raise ValueError("k/v head_dim does not match the pool")
         if self.varlen:
             head_axis = 1
         if k.shape[head_axis] != self.num_kv_heads:
@@ -799,10 +811,6 @@ class PagedTreeBatch(PagedKVBatch):
             raise TypeError("q and the pool must be bfloat16")
         qs = self._layout(q, "thd")
         num_q_heads = q.shape[1]
-        if q.shape[2] != self.head_dim:
-            raise ValueError("q head_dim does not match the pool")
-        if q.device != self.device:
-            raise ValueError(f"q is on {q.device}, the pool on {self.device}")
         if num_q_heads == 0 or num_q_heads % self.num_kv_heads:
             raise ValueError("query heads must be a multiple of kv heads")
         if scale is None:
