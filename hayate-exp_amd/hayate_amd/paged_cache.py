@@ -1369,14 +1369,14 @@ class PagedKVCacheManager:
         lines = _native.tree_lines(nodes.astype(np.int32),
                                    np.array([len(t) for t in trees], dtype=np.int32))
         held = [len(h.pages) for h in handles]
-        self.reserve_tick(handles, [len(t) for t in trees])
         try:
+            self.reserve_tick(handles, [len(t) for t in trees])
             batch = PagedTreeBatch(self, trees, [h.length for h in handles],
                                    [list(h.pages) for h in handles], self.num_q_heads, lines,
                                    self._first_positions(handles))
         except Exception:
-            for h, n in zip(handles, held):
-                self._drop_pages(h.pages[n:])
+            for h, n in reversed(list(zip(handles, held))):
+                self._drop_pages(reversed(h.pages[n:]))
                 del h.pages[n:]
             raise
         batch.handles = handles

@@ -488,3 +488,27 @@ def test_c_moves_begin_inside_their_arrays():
     for kw in (dict(page_start=[-1, 1]), dict(src_start=[-2, 1])):
         assert c_move([3], [5], [1], **kw) == _native.HY_EINVAL
         assert "negative" in _native.last_error()
+
+
+def test_a_tree_on_small_pages_reserves_nothing():
+    """Pages below what ticks take are refused before any is reserved."""
+    m = PagedKVCacheManager(1, 8, 128, 12 * 64, 64, 2, torch.bfloat16, "cpu", num_q_heads=32)
+    h = m.allocate()
+    m.reserve(h, 60)
+    h.length = 60
+    free = list(m._free_pages)
+    with pytest.raises(ValueError):
+        m.begin_tree([h], [chain(100)])
+    assert m._free_pages == free and len(h.pages) == 1
+
+
+def test_pages_of_a_refused_tree_return_in_their_order(monkeypatch):
+    import hayate_amd.paged_cache as pc
+
+    m = pool()
+    handles = [handle(m, 100), handle(m, 100)]
+    free = list(m._free_pages)
+    monkeypatch.setattr(pc.PagedTreeBatch, "__init__", lambda *args: 1 // 0)
+    with pytest.raises(ZeroDivisionError):
+        m.begin_tree(handles, [chain(200), chain(200)])
+    assert m._free_pages == free
