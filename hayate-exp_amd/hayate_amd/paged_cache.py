@@ -757,6 +757,8 @@ class PagedTreeBatch(PagedKVBatch):
     every_logit = True
     # the handles that begin_tree made the batch for
     handles: Sequence[PagedCacheHandle] = ()
+    # whether commit_tree took its nodes over already
+    committed = False
 
     def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],
@@ -1387,12 +1389,14 @@ class PagedKVCacheManager:
         """Keep of each handle's tree the nodes accepted[b] (a path from a child of the
         cached context down, possibly empty): their K and V move to the positions behind the
         cached tokens in every layer, the length grows by as many and the pages behind it are
-        returned."""
+        returned. Once per batch."""
         handles = list(handles)
         if len(handles) != batch.num_seqs or len(accepted) != batch.num_seqs:
             raise ValueError("one handle and one path per tree is required")
         if batch.k_cache is not self.k_cache:
             raise ValueError("the batch belongs to another pool")
+        if batch.committed:
+            raise ValueError("the batch was committed already")
         if any(a is not b for a, b in zip(handles, batch.handles)):
             raise ValueError("the handles are not those the batch began with, in their order")
         if any(h.released for h in handles):
@@ -1407,6 +1411,7 @@ class PagedKVCacheManager:
                          [h.length for h in handles])
         for h, path in zip(handles, paths):
             self._set_length(h, h.length + len(path))
+        batch.committed = True
 
     # ---------------------------------------------------------- tick setup
     def _validate_handles(self, handles: Sequence[PagedCacheHandle]) -> None:

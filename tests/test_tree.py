@@ -512,3 +512,21 @@ def test_pages_of_a_refused_tree_return_in_their_order(monkeypatch):
     with pytest.raises(ZeroDivisionError):
         m.begin_tree(handles, [chain(200), chain(200)])
     assert m._free_pages == free
+
+
+def test_a_batch_is_committed_once(monkeypatch):
+    """Also where nothing was accepted: the slots may hold the next tick's tokens by then."""
+    import hayate_amd.paged_cache as pc
+
+    monkeypatch.setattr(pc, "_require_hip", lambda t, what: None)
+    m = pool()
+    h = handle(m, 100)
+    batch = m.begin_tree([h], [chain(3)])
+    with pytest.raises(ValueError):
+        m.commit_tree([h], batch, [[1]])
+    m.commit_tree([h], batch, [[]])
+    other = m.begin_tree([h], [chain(3)])
+    with pytest.raises(ValueError):
+        m.commit_tree([h], batch, [[0]])
+    m.commit_tree([h], other, [[0]])
+    assert h.length == 101
