@@ -523,3 +523,72 @@ def test_draft_check_commit_and_go_on(nodes):
         # projections' rows were summed in another order
         for pool, alone in ((m.k_cache, one.k_cache), (m.v_cache, one.v_cache)):
             assert cosine(pool[0, 0][:, rows], alone[0, 0][:, other]).min().item() > 0.9999
+
+
+@pytest.mark.parametrize("n,cached", [(20, 900), (1, 40), (70, 3000), (200, 500)])
+def test_a_request_alone_and_among_sick_neighbours(n, cached):
+    """The plan cuts a request by the whole batch, so its bits may differ; what its neighbours
+    hold, NaN in every key and value, reaches none of them."""
+    tree = wide_tree(random.Random(n), n)
+    q, k, v = normal(n, 32, D, seed=1), normal(n, 8, D, seed=2), normal(n, 8, D, seed=3)
+    m, (h,) = make_pool([cached], [n], seed=7)
+    rows = physical(m, h, cached)
+    own = [p[0, 0][:, rows].clone() for p in (m.k_cache, m.v_cache)]
+    batch = m.begin_tree([h], [tree])
+    batch.write_layer(0, k, v)
+    rows = physical(m, h, cached + n)
+    ref, size = attention64(q, m.k_cache[0, 0][:, rows], m.v_cache[0, 0][:, rows], seen(cached, tree))
+    assert_attention(batch.attend_layer(q, 0), ref, size, "alone")
+    for before, after in (([700, 64], [33]), ([5], [2000, 1, 130]), ([3] * 40, [90] * 40)):
+        rng = random.Random(len(before))
+        others = [wide_tree(rng, rng.randint(1, 60)) for _ in before + after]
+        trees = others[: len(before)] + [tree] + others[len(before) :]
+        m, handles = make_pool([*before, cached, *after], [len(t) for t in trees], seed=7)
+        mine = len(before)
+        m.k_cache.fill_(float("nan"))
+        m.v_cache.fill_(float("nan"))
+        rows = physical(m, handles[mine], cached)
+        for p, x in zip((m.k_cache, m.v_cache), own):
+            p[0, 0][:, rows] = x
+        batch = m.begin_tree(handles, trees)
+        at = sum(len(t) for t in trees[:mine])
+        every = [torch.full((sum(len(t) for t in trees), x.shape[1], D), float("nan"),
+                            dtype=torch.bfloat16, device="cuda") for x in (q, k, v)]
+        for x, y in zip(every, (q, k, v)):
+            x[at : at + n] = y
+        batch.write_layer(0, *every[1:])
+        out = batch.attend_layer(every[0], 0)
+        assert_attention(out[at : at + n], ref, size, (before, after))
+
+
+@pytest.mark.parametrize("sizes,cached", [([9], [500]), ([20, 5, 33], [900, 10, 3000]),
+                                          ([200, 60], [2500, 800])])
+def test_lists_padded_with_empty_records(sizes, cached):
+    """A caller with a fixed launch size pads the chunk and the merge records: the same bits."""
+    from hayate_amd import _native
+
+    m, handles = make_pool(cached, sizes, seed=3)
+    batch = m.begin_tree(handles, [wide_tree(random.Random(i), n) for i, n in enumerate(sizes)])
+    n = sum(sizes)
+    q, k, v = normal(n, 32, D, seed=1), normal(n, 8, D, seed=2), normal(n, 8, D, seed=3)
+    batch.write_layer(0, k, v)
+    want = batch.attend_layer(q, 0)
+    plan = batch.plan(32).host
+    chunks, merges = plan.n_chunks + 7, len(plan.merge) + 5
+    items = np.zeros((2 * chunks + len(plan.items) - 2 * plan.n_chunks, 8), dtype=np.int32)
+    items[: 2 * plan.n_chunks] = plan.items[: 2 * plan.n_chunks]
+    items[2 * chunks :] = plan.items[2 * plan.n_chunks :]
+    merge = np.zeros((merges, 8), dtype=np.int32)
+    merge[: len(plan.merge)] = plan.merge
+    slots = max(1, plan.n_slots)
+    size = _native.tree_workspace_bytes(slots, 8, D)
+    items, merge = torch.from_numpy(items).cuda(), torch.from_numpy(merge).cuda()
+    space, out = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.full_like(q, float("nan"))
+    rc = _native.lib().hy_paged_tree(
+        q.data_ptr(), 0, 32 * D, D, out.data_ptr(), 0, 32 * D, D, m.k_cache.data_ptr(),
+        m.v_cache.data_ptr(), m.k_cache.stride(2), batch.page_table.data_ptr(),
+        batch.page_table.stride(0), batch.lines.data_ptr(), batch.line_words, items.data_ptr(),
+        chunks, plan.max_rows, merge.data_ptr(), merges, slots, space.data_ptr(), size, 32, 8, D,
+        m.page_size, D**-0.5, torch.cuda.current_stream().cuda_stream)
+    assert rc == _native.HY_OK, _native.last_error()
+    assert torch.equal(out, want)
