@@ -163,29 +163,6 @@ def _require_hip(t: torch.Tensor, what: str) -> None:
         )
 
 
-def _row_strides(t: torch.Tensor, layout: str, q_len: int):
-    """(stride_seq, stride_tok, stride_head) for the kernels' addressing
-    base + b*seq + (q_start[b] + i)*tok + h*head with q_start[b] = b * q_len.
-
-    layout "bhtd": (B, H, T, D); "bthd": (B, T, H, D); "thd": packed (N, H, D).
-    """
-    st = t.stride()
-    if layout == "thd":
-        s_tok, s_head, s_el = st
-        s_seq = 0
-    elif layout == "bhtd":
-        s_b, s_head, s_tok, s_el = st
-        s_seq = s_b - q_len * s_tok
-    elif layout == "bthd":
-        s_b, s_tok, s_head, s_el = st
-        s_seq = s_b - q_len * s_tok
-    else:
-        raise ValueError(layout)
-    if s_el != 1 or (s_tok | s_head | s_seq) & 7 or t.data_ptr() & 15:
-        raise ValueError("rows must be contiguous in the last dim and 16-byte aligned")
-    return s_seq, s_tok, s_head
-
-
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     st = t.stride()
     if t.data_ptr() & 15:  # contiguous() would return contiguous rows as they are
@@ -420,24 +397,35 @@ class PagedKVBatch:
         self._pool_ptrs[layer_idx] = hit
         return hit
 
-    def _layout(self, t: torch.Tensor, uniform_layout: str) -> tuple:
-        """Row strides of t, whose rows the kernels take as many and as long as the batch's."""
-        shape = t.shape
+    def _rows(self, t: torch.Tensor, uniform_layout: str) -> tuple[torch.Tensor, tuple]:
+        """Checks t's rows against the batch's, which the kernels go by, and returns them
+        16-byte aligned (a copy where they are not) with (stride_seq, stride_tok, stride_head) for
+        the kernels' addressing base + b*seq + (q_start[b] + i)*tok + h*head: q_start[b] = b *
+        query_len in a uniform batch, (B, H, T, D) for layout "bhtd" or (B, T, H, D) for
+        "bthd"; a varlen batch's rows are packed (N, H, D)."""
+        shape, st = t.shape, t.stride()
         if t.device != self.device:
             raise ValueError(f"rows are on {t.device}, the pool on {self.device}")
         if shape[-1] != self.head_dim:
             raise ValueError(f"rows of {shape[-1]} values do not match the pool's {self.head_dim}")
+        tok, head = (0, 1) if self.varlen else (2, 1) if uniform_layout == "bhtd" else (1, 2)
         if self.varlen:
             if len(shape) != 3 or shape[0] != self.total_tokens:
                 raise ValueError(
                     f"varlen batch expects packed (tokens={self.total_tokens}, heads, dim)"
                 )
-            return _row_strides(t, "thd", 0)
-        if len(shape) != 4:
+        elif len(shape) != 4:
             raise ValueError("uniform batch expects 4-D tensors")
-        if shape[0] != self.num_seqs or shape[2 if uniform_layout == "bhtd" else 1] != self.query_len:
+        elif shape[0] != self.num_seqs or shape[tok] != self.query_len:
             raise ValueError(f"uniform batch expects {self.num_seqs} sequences of {self.query_len} rows")
-        return _row_strides(t, uniform_layout, self.query_len)
+        if st[-1] != 1 or (st[0] | st[1] | st[-2]) & 7 or t.data_ptr() & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = t.stride()
+        return t, (0 if self.varlen else st[0] - self.query_len * st[tok], st[tok], st[head])
+
+    def _packed(self, num_heads: int) -> tuple:
+        """The strides of contiguous rows (tokens, heads, D), sequences one after the other."""
+        return 0, num_heads * self.head_dim, self.head_dim
 
     # ----------------------------------------------------------- write path
     def write_layer(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -445,12 +433,10 @@ class PagedKVBatch:
         (paged_cache.py:44-60): k, v are (B, Hkv, T, D), or packed (N, Hkv, D)
         for a varlen tick."""
         _require_hip(k, "write_layer")
-        k = _aligned_rows(k)
-        v = _aligned_rows(v)
         self._check_kv(k, v, head_axis=1)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
-        ks = self._layout(k, "bhtd")
-        vs = self._layout(v, "bhtd")
+        k, ks = self._rows(k, "bhtd")
+        v, vs = self._rows(v, "bhtd")
         rc = _native.lib().hy_kv_append(
             k_ptr, v_ptr, hs,
             k.data_ptr(), *ks, v.data_ptr(), *vs,
@@ -504,18 +490,15 @@ class PagedKVBatch:
         and the C arguments they map to (shared by norm_rope_write_layer and
         decode_layer)."""
         _require_hip(q, what)
-        q = _aligned_rows(q)
-        k = _aligned_rows(k)
-        v = _aligned_rows(v)
         self._check_kv(k, v, head_axis=2)
         if q.dtype != torch.bfloat16:
             raise TypeError("q must be bfloat16")
+        q, qs = self._rows(q, "bthd")
+        k, ks = self._rows(k, "bthd")
+        v, vs = self._rows(v, "bthd")
         num_q_heads = q.shape[-2]
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        qs = self._layout(q, "bthd")
-        qos = (0, num_q_heads * self.head_dim, self.head_dim)  # contiguous, whatever the layout
-        ks = self._layout(k, "bthd")
-        vs = self._layout(v, "bthd")
+        qos = self._packed(num_q_heads)
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin rope tables go together (both or neither)")
         if cos is not None:
@@ -599,13 +582,12 @@ class PagedKVBatch:
             out = torch.empty((self.total_tokens, num_q_heads, self.head_dim),
                               dtype=q.dtype, device=q.device)
             result = out
-            os_ = self._layout(out, "thd")
         else:
             B, T = self.num_seqs, self.query_len
             buf = torch.empty((B, T, num_q_heads, self.head_dim), dtype=q.dtype,
                               device=q.device)
             result = buf.transpose(1, 2)
-            os_ = self._layout(result, "bhtd")
+        os_ = self._packed(num_q_heads)
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
         plan = self.plan(num_q_heads)
@@ -672,24 +654,19 @@ class PagedKVBatch:
         transpose + reshape is free) or packed (N, Hq, D) for a varlen tick.
         """
         _require_hip(q, "attend_layer")
-        q = _aligned_rows(q)
         if q.dtype != self.k_cache.dtype:
             raise TypeError("q dtype must match the pool dtype")
+        q, qs = self._rows(q, "bhtd")
+        num_q_heads = q.shape[1]
+        os_ = self._packed(num_q_heads)
         if self.varlen:
-            num_q_heads = q.shape[1]
             out = torch.empty((self.total_tokens, num_q_heads, self.head_dim),
                               dtype=q.dtype, device=q.device)
-            qs = self._layout(q, "thd")
-            os_ = self._layout(out, "thd")
             result = out
         else:
-            B, num_q_heads, T, D = q.shape
-            if B != self.num_seqs or T != self.query_len:
-                raise ValueError("q does not match the batch shape")
-            buf = torch.empty((B, T, num_q_heads, D), dtype=q.dtype, device=q.device)
+            buf = torch.empty((self.num_seqs, self.query_len, num_q_heads, self.head_dim),
+                              dtype=q.dtype, device=q.device)
             result = buf.transpose(1, 2)
-            qs = self._layout(q, "bhtd")
-            os_ = self._layout(result, "bhtd")
         if num_q_heads % self.num_kv_heads:
             raise ValueError("query heads must be a multiple of kv heads")
         if scale is None:
@@ -808,10 +785,9 @@ class PagedTreeBatch(PagedKVBatch):
         """Attention of every node over its request's cached tokens, its ancestors and
         itself in this layer's pages: q packed (tokens, Hq, D), returns the same."""
         _require_hip(q, "attend_layer")
-        q = _aligned_rows(q)
         if q.dtype != torch.bfloat16 or self.k_cache.dtype != torch.bfloat16:
             raise TypeError("q and the pool must be bfloat16")
-        qs = self._layout(q, "thd")
+        q, qs = self._rows(q, "thd")
         num_q_heads = q.shape[1]
         if num_q_heads == 0 or num_q_heads % self.num_kv_heads:
             raise ValueError("query heads must be a multiple of kv heads")
@@ -824,7 +800,7 @@ class PagedTreeBatch(PagedKVBatch):
         out = torch.empty((self.total_tokens, num_q_heads, self.head_dim), dtype=q.dtype,
                           device=q.device)
         self._launch("hy_paged_tree", _native.lib().hy_paged_tree,
-            q.data_ptr(), *qs, out.data_ptr(), 0, num_q_heads * self.head_dim, self.head_dim,
+            q.data_ptr(), *qs, out.data_ptr(), *self._packed(num_q_heads),
             *self._layer_pools(layer_idx), *plan.args, float(scale), self._stream(),
         )
         return out
