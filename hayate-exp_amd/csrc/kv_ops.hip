@@ -112,7 +112,8 @@ __device__ __forceinline__ void load_half_rows(const float *__restrict__ row, in
 }
 
 // kAt: tokens are rotated at positions[tok] instead of the position of the slot
-// they are written to (drafted tokens: depth in their tree against place in it).
+// they are written to (drafted tokens: depth in their tree against place in it; a cache
+// that dropped tokens: behind the last kept one's position).
 template <bool kSeqStride, bool kAt>
 __global__ __launch_bounds__(256) void qknorm_rope_append_kernel(
     const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
@@ -161,9 +162,9 @@ __global__ __launch_bounds__(256) void qknorm_rope_append_kernel(
   };
   if (tok >= total_tokens) return;  // the whole wave
   if (!kSeqStride && live) issue_loads(0);
-  // Every load is issued before the first use of any: rows, weights, the
-  // token's sequence and position (one search round), the cos/sin row and
-  // the page (scalar).
+  // Rows, weights and the token's sequence (one search round) are loaded before the first
+  // use of any; the page (scalar) and the cos/sin row follow from the sequence or, with
+  // kAt, the row from positions[tok], which is read behind the search.
   const uint16_t *w = is_q ? q_w : k_w;
   const float eps = is_q ? q_eps : k_eps;
   u32x4 w_lo, w_hi;

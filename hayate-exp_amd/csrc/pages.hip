@@ -41,8 +41,10 @@ __device__ __forceinline__ uint16_t *unit_base(uint16_t *k_pool, uint16_t *v_poo
 // kRowsPerPass rows a step: a step's rows are all loaded before the first of them is
 // stored (a row may be the target of a later row of the same step), and the
 // host has checked that no row is read after it was written, so the next step's
-// loads go out before this step's stores. 5,999 tokens of 36 layers (1.77 GB): 378 us,
-// 4.7 TB/s, 95 % of what a large copy reaches; 2 or 8 passes a step 394 and 415 us.
+// loads go out before this step's stores. 5,999 tokens of 36 layers of 8 heads (1.77 GB): 376
+// us, 4.7 TB/s, 95 % of what a large copy reaches; 2 or 8 passes a step 394 and 415 us. That
+// is 576 units; with fewer than the GPU has compute units the steps' latency bounds it (1 us
+// each): 93 us for 1 layer of 8 heads (0.5 TB/s), 96 for 36 layers of one (2.3 TB/s).
 constexpr int kMovePasses = 4;
 constexpr int kStepRows = kMovePasses * kRowsPerPass;
 
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void move_kernel(uint16_t *k_pool, uint16
 // Copies. Sources and targets are distinct pages, so nothing is ordered: one
 // workgroup per (unit, record), 128 rows (32 KiB) in flight. Nontemporal on both
 // sides: 15 pages of 77 tokens in 36 layers (341 MB read and written) 65.9 us against 70.4, 32
-// pages 232 against 238; a large torch copy moves 4.94 TB/s, these 5.1. (In the moves it
+// pages 232 against 238; a large torch copy moves 4.93 TB/s, these 5.1 to 5.2. (In the moves it
 // gave nothing.)
 constexpr int kCopyPasses = 8;
 

@@ -12,11 +12,15 @@
 // K/V row once, up to 256 of them, 32 a wave; more go into further tiles. A piece
 // that is not a tile's whole stream leaves fp32 partials that tree_merge_kernel joins.
 //
-// What bounds it: up to about 128 rows HBM (32 chains of 5 nodes, 233 MB: 42.6 us, 5.5 TB/s,
-// and 4.6 for the merge); with 256 the matrix cores at the clock that the power limit leaves
-// (8 trees of 64 nodes on 32 k tokens: 303 us, 861 TFLOP/s, MFMAs busy in 51 % of the cycles at
-// 1.63 GHz; a large library product reaches 1,209 TFLOP/s); in small ticks the latency
-// of the steps and the launch (8 nodes on 500 tokens: 12.6 us, 8 steps of 0.45).
+// What bounds it: up to about 128 rows HBM (32 chains of 5 nodes, 233 MB: 42.3 us, 5.5 TB/s,
+// and 4.6 for the merge); with 256 the matrix cores, in part by the clock that the power limit
+// leaves and in part by what stands between the products (8 trees of 64 nodes on 32 k tokens:
+// 290 us a call with the merge, 902 TFLOP/s, 305 and 9.4 traced kernel by kernel; MFMAs are busy
+// in 51 % of the cycles at 1.63 GHz; with all keys in L2 1,000 TFLOP/s, a large library product
+// 1,415 to 1,649 by the layout of its right operand); in small ticks the latency of the steps and
+// the launch (8 nodes on 500 tokens: 13.0 us, 8 steps of 0.45). The variants keep 37 to 67
+// scalars, strides and bases above all, in lanes of vector registers, most of them in those
+// with waves that only load.
 //
 // A chunk's tiles (64 keys of K and V, 32 KiB) go through a ring of four LDS
 // stages by direct-to-LDS loads, three tiles ahead of the one being used and

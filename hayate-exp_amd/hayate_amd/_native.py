@@ -289,8 +289,8 @@ class TreePlan:
 
     def __init__(self, items, n_chunks, merge, n_slots, max_rows):
         # int32 (2 n_chunks + n_pieces, 8): chunk records of two rows {piece_begin,
-        # piece_end, n_steps, 0..} and the first piece, then piece records {seq, q_begin,
-        # q_end, kv_begin, kv_end, slot, q_row, cache_len}
+        # piece_end, n_steps, alone, 0..} and the first piece, then piece records {seq,
+        # q_begin, q_end, kv_begin, kv_end, slot, q_row, cache_len}
         self.items = items
         self.n_chunks = n_chunks
         self.merge = merge  # int32 (n, 8) {seq, q_begin, q_end, first_slot, splits, q_row, blocks, 0}

@@ -121,7 +121,9 @@ class GroupedQueryAttention(nn.Module):
         """x (B, T, d_in) -> (o_proj(context), None, None).
 
         Positions are the batch's cache_lens + token index, which is what the
-        reference's position_ids hold in paged mode (qwen.py:89-109).
+        reference's position_ids hold in paged mode (qwen.py:89-109), or the
+        batch's ``positions`` where it has them (drafted trees, caches that dropped
+        tokens).
         """
         if paged_cache is None:
             raise NotImplementedError(

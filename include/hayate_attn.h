@@ -427,7 +427,8 @@ int64_t hy_sample_workspace_bytes(int32_t n_rows, int32_t vocab);
  *
  * hy_qknorm_rope_append_at is hy_qknorm_rope_append with the rotation of token tok
  * (packed index q_start[b] + i) taken at positions[tok] (>= 0, device memory)
- * instead of the position of its slot: the node's depth in the sequence. A token whose
+ * instead of the position of its slot: the node's depth in the sequence, or for a sequence
+ * that dropped cached tokens the position behind its last one's. A token whose
  * position is its slot's gets the same bits from both. positions[tok] <
  * max_positions is the caller's guarantee, as there.
  * With hayate/model/attention.py:62-75 as the reference for one linear sequence.
