@@ -462,9 +462,9 @@ class PagedKVBatch:
         """Fused q/k RMSNorm + RoPE + paged append of k and v
         (attention.py:62-75 with rope.py:31-47). Inputs are the projection
         outputs, (B, T, H, D) (or packed (N, H, D) for a varlen tick); positions
-        are cache_lens + token index, or the batch's ``positions``. `eps` is the q norm's epsilon and
-        `k_eps` the k norm's (default: `eps`). Returns the rotated q in the
-        same layout; k and v go to the pool only."""
+        are cache_lens + token index, or the batch's ``positions``. `eps` is
+        the q norm's epsilon and `k_eps` the k norm's (default: `eps`).
+        Returns the rotated q in the same layout; k and v go to the pool only."""
         a = self._append_inputs("norm_rope_write_layer", q, k, v, q_norm_weight,
                                 k_norm_weight, cos, sin)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
@@ -715,11 +715,11 @@ class PagedTreeBatch(PagedKVBatch):
     """A tick that checks drafted tokens: each request's tokens form a tree.
 
     Node i of a request with c cached tokens holds slot c + i of its cache, is
-    rotated at position c + depth(i) (from the handle's ``next_position`` on) and sees the c cached tokens, its ancestors and
-    itself, so one forward pass gives every node the states it would have at the end
-    of its own branch. ``parents[b][i]`` is node i's parent, an earlier node of the
-    request, or -1 for a child of the cached context (several nodes may be). A node
-    alone is a decode token. Tensors are packed (tokens, heads, dim) in handle order,
+    rotated at position c + depth(i) (from the handle's ``next_position`` on) and sees
+    the c cached tokens, its ancestors and itself, so one forward pass gives every
+    node the states it would have at the end of its own branch. ``parents[b][i]`` is
+    node i's parent, an earlier node of the request, or -1 for a child of the cached
+    context (several nodes may be). A node alone is a decode token. Tensors are packed (tokens, heads, dim) in handle order,
     as in a ``begin_tick`` batch; ``write_layer``, ``norm_rope_write_layer`` and
     ``attend_layer`` are called as there. ``positions`` holds each packed node's rope
     position (int32). No reference counterpart: the reference decodes one token at a
