@@ -45,12 +45,17 @@
 // double buffered: slice k + W is in flight while slice k is consumed. Rows
 // past the end of a context may hold any bits; their scores are masked and
 // their V values zeroed before the MFMA so that 0 * NaN never occurs.
+//
+// With a window (kWindow) the stream holds only the keys in sight, numbered as window.h says:
+// the planner cuts those numbers, a slice's K and V rows lie at its number or `gap` keys
+// further, and a slice at the edge of the sinks or the window is masked as the last one is.
 
 #include <mutex>
 
 #include "decode_shape.h"
 #include "hy_common.h"
 #include "qknorm.h"
+#include "window.h"
 
 namespace hy {
 namespace {
@@ -120,11 +125,15 @@ __device__ __forceinline__ s16x4 read_vt(const uint16_t *lane_base, int key0, in
 
 // Scores, online softmax and PV for one slice whose V rows are already in
 // `vbuf`. vt_base is this lane's transposed-read base in that buffer.
-template <int G>
+// With a window, tokens of [sinks, low) are masked as those from tok_end on are; every slice
+// that is issued holds one that is not.
+// kScores: the raw scores of head n < G go to score_row (this lane's four tokens of every 16).
+template <int G, bool kWindow, bool kScores>
 __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t *vt_base,
                                               const bf16x8 (&qop)[4], int t0, int tok_end,
-                                              int lane, float scale_log2, float &m_run,
-                                              float &l_run, f32x4 (&acc)[8]) {
+                                              int sinks, int low, float *score_row, int lane,
+                                              float scale_log2, float &m_run, float &l_run,
+                                              f32x4 (&acc)[8]) {
   const int g = lane >> 4;
   f32x4 sc[2];
 #pragma unroll
@@ -135,16 +144,24 @@ __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t
       sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
           __builtin_bit_cast(bf16x8, r.k[b][kk]), qop[kk], sc[b], 0, 0, 0);
   }
+  if constexpr (kScores) {
+    if ((lane & 15) < G) {
+      *reinterpret_cast<f32x4 *>(score_row) = sc[0];
+      *reinterpret_cast<f32x4 *>(score_row + 16) = sc[1];
+    }
+  }
 
   // Online softmax in the exp2 domain on raw scores: max first, then
   // p = exp2(s * c - m * c) with c = scale * log2(e) > 0.
-  const bool partial = t0 + kSlice > tok_end;
+  const bool partial =
+      t0 + kSlice > tok_end || (kWindow && t0 < low && t0 + kSlice > sinks);
+  auto hidden = [&](int tok) { return tok >= tok_end || (kWindow && tok >= sinks && tok < low); };
   float mloc = -INFINITY;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (partial && t0 + 16 * b + 4 * g + i >= tok_end) sc[b][i] = -INFINITY;
+      if (partial && hidden(t0 + 16 * b + 4 * g + i)) sc[b][i] = -INFINITY;
       mloc = fmaxf(mloc, sc[b][i]);
     }
   mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
@@ -187,12 +204,12 @@ __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t
                                                         acc[db], 0, 0, 0);
     }
   } else {
-    // Keys past the end: zero their V values (the rows may hold any bits).
+    // Masked keys: zero their V values (the rows may hold any bits).
     s16x8 keep;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      keep[k] = t0 + 4 * g + k < tok_end ? -1 : 0;
-      keep[4 + k] = t0 + 16 + 4 * g + k < tok_end ? -1 : 0;
+      keep[k] = hidden(t0 + 4 * g + k) ? 0 : -1;
+      keep[4 + k] = hidden(t0 + 16 + 4 * g + k) ? 0 : -1;
     }
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
@@ -210,9 +227,19 @@ __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t
 // q_tok, 0, 0}.
 struct Piece {
   int seq, t0, t1, slot, sb, qt, nsl, ends;
+  int ns, gap, low;  // with a window: its keys, and the first number in sight behind the sinks
 };
 
-__device__ __forceinline__ Piece load_piece(const int32_t *pieces, int p) {
+// Adds the window's part to piece x, whose sequence's token is at position pos.
+__device__ __forceinline__ void set_window(Piece &x, int pos, int window, int sinks) {
+  const WindowKeys w = window_keys<kSlice>(pos, window, sinks);
+  x.ns = w.ns;
+  x.gap = w.gap;
+  x.low = pos - window + 1 - w.gap;
+}
+
+template <bool kWindow>
+__device__ __forceinline__ Piece load_piece(const int32_t *pieces, int p, int window, int sinks) {
   const int32_t *r = pieces + 8 * p;
   Piece x;
   x.seq = r[0];
@@ -223,6 +250,7 @@ __device__ __forceinline__ Piece load_piece(const int32_t *pieces, int p) {
   x.qt = r[5];
   x.ends = r[7];
   x.nsl = (x.t1 - x.t0 + kSlice - 1) / kSlice;
+  if constexpr (kWindow) set_window(x, r[6], window, sinks);
   return x;
 }
 
@@ -230,6 +258,17 @@ __device__ __forceinline__ Piece load_piece(const int32_t *pieces, int p) {
 // newrow is the slice row of its sequence's query token, or -1.
 struct SliceMeta {
   int piece, t0, tend, newrow;
+  int low;    // with a window, as in Piece
+  int score;  // where the slice's scores go in every head's row
+};
+
+// What the variants take: the window, or where the raw scores go, row by query head
+// (sequence b's from score_start[b], a multiple of 4, with room for whole slices).
+struct DecodeExtra {
+  int window, sinks;
+  float *scores;
+  const int32_t *score_start;
+  int64_t score_stride;
 };
 
 // Inputs of the fused append (hy_paged_decode_append): the raw q, k, v
@@ -260,14 +299,14 @@ struct AppendArgs {
 // their page; the workgroup's barrier publishes them before any wave loads
 // that slice (only the one workgroup that owns the row reads it). The
 // values are those of qknorm_rope_append_kernel, bit for bit.
-template <int G, bool kFused>
+template <int G, bool kFused, bool kWindow, bool kScores>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void decode_kernel(
     const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
     uint16_t *__restrict__ k_pool, uint16_t *__restrict__ v_pool,
     int64_t pool_hs, const int32_t *__restrict__ page_table, int64_t pt_stride,
     const int32_t *__restrict__ items, int n_chunks, float *__restrict__ ws_acc,
     float *__restrict__ ws_ml, int num_q_heads, int page_shift, float scale_log2,
-    AppendArgs ap) {
+    AppendArgs ap, DecodeExtra ex) {
   // One V transpose buffer per wave and the query rows (G heads) of every
   // piece of the chunk.
   constexpr int kMaxPieces = decode_max_pieces(G);
@@ -310,19 +349,34 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   ipc.qt = ch[7];
   ipc.nsl = (ipc.t1 - ipc.t0 + kSlice - 1) / kSlice;
   ipc.ends = pieces[8 * pb + 7];
+  if constexpr (kWindow) set_window(ipc, pieces[8 * pb + 6], ex.window, ex.sinks);
   // Loads slice k of the chunk (k-th 32-token slice in piece order) into r.
   // locate() moves the cursor to slice k and describes it; issue() also
   // loads it.
   auto locate = [&](SliceMeta &m, int k) {
-    while (k >= ipc.sb + ipc.nsl) ipc = load_piece(pieces, ++ip);
+    while (k >= ipc.sb + ipc.nsl) ipc = load_piece<kWindow>(pieces, ++ip, ex.window, ex.sinks);
     m.piece = ip;
     m.t0 = ipc.t0 + (k - ipc.sb) * kSlice;
     m.tend = ipc.t1;
     m.newrow = ipc.ends && m.t0 + kSlice >= ipc.t1 ? ipc.t1 - 1 - m.t0 : -1;
+    if constexpr (kWindow) m.low = ipc.low;
+    if constexpr (kScores) m.score = ex.score_start[ipc.seq] + m.t0;
+  };
+  // The first token of the located slice in its cache.
+  auto first_token = [&](const SliceMeta &m) {
+    return kWindow && m.t0 >= ipc.ns ? m.t0 + ipc.gap : m.t0;
   };
   auto issue = [&](SliceRegs &r, SliceMeta &m, int k) {
     locate(m, k);
-    issue_slice(r, kh, vh, page_table + ipc.seq * pt_stride, m.t0, page_shift, lane);
+    issue_slice(r, kh, vh, page_table + ipc.seq * pt_stride, first_token(m), page_shift, lane);
+  };
+  auto consume = [&](const SliceRegs &r, const SliceMeta &m, const bf16x8 (&qop)[4], float &m_run,
+                     float &l_run, f32x4 (&acc)[8]) __attribute__((always_inline)) {
+    float *row = nullptr;
+    if constexpr (kScores)
+      row = ex.scores + (h0 + n) * ex.score_stride + m.score + 4 * g;
+    consume_slice<G, kWindow, kScores>(r, vt_base, qop, m.t0, m.tend, ex.sinks, kWindow ? m.low : 0,
+                                       row, lane, scale_log2, m_run, l_run, acc);
   };
 
   // Online-softmax state of the piece being accumulated (cp).
@@ -395,7 +449,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
     locate(ma, k);
     deferred = kFused && ma.newrow >= 0;
     if (!deferred)
-      issue_slice(ra, kh, vh, page_table + ipc.seq * pt_stride, ma.t0, page_shift, lane);
+      issue_slice(ra, kh, vh, page_table + ipc.seq * pt_stride, first_token(ma), page_shift, lane);
   }
   const int n_p = min(pe - pb, kMaxPieces);
   if constexpr (!kFused) {
@@ -458,7 +512,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
     }
   }
   __syncthreads();
-  if (deferred) issue_slice(ra, kh, vh, page_table + ipc.seq * pt_stride, ma.t0, page_shift, lane);
+  if (deferred) issue_slice(ra, kh, vh, page_table + ipc.seq * pt_stride, first_token(ma), page_shift, lane);
   load_q(pb);
 
   // Wave w takes slices w, w + 4, ... of the chunk. Double-buffered: the
@@ -471,24 +525,24 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       stage_v(ra, vbuf, lane);
       issue(rb, mb, k + kWaves);
       if (ma.piece != cp) move_to(ma.piece);
-      consume_slice<G>(ra, vt_base, qop, ma.t0, ma.tend, lane, scale_log2, m_run, l_run, acc);
+      consume(ra, ma, qop, m_run, l_run, acc);
       stage_v(rb, vbuf, lane);
       issue(ra, ma, k + 2 * kWaves);
       if (mb.piece != cp) move_to(mb.piece);
-      consume_slice<G>(rb, vt_base, qop, mb.t0, mb.tend, lane, scale_log2, m_run, l_run, acc);
+      consume(rb, mb, qop, m_run, l_run, acc);
       k += 2 * kWaves;
     }
     stage_v(ra, vbuf, lane);
     if (k + kWaves < n_sl) {
       issue(rb, mb, k + kWaves);
       if (ma.piece != cp) move_to(ma.piece);
-      consume_slice<G>(ra, vt_base, qop, ma.t0, ma.tend, lane, scale_log2, m_run, l_run, acc);
+      consume(ra, ma, qop, m_run, l_run, acc);
       stage_v(rb, vbuf, lane);
       if (mb.piece != cp) move_to(mb.piece);
-      consume_slice<G>(rb, vt_base, qop, mb.t0, mb.tend, lane, scale_log2, m_run, l_run, acc);
+      consume(rb, mb, qop, m_run, l_run, acc);
     } else {
       if (ma.piece != cp) move_to(ma.piece);
-      consume_slice<G>(ra, vt_base, qop, ma.t0, ma.tend, lane, scale_log2, m_run, l_run, acc);
+      consume(ra, ma, qop, m_run, l_run, acc);
     }
   }
   // Close the last piece and any later ones this wave had no slice of.
@@ -504,11 +558,13 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // partial (the split index is clamped to the last one) and the ones past
 // num_partials are then replaced by the empty partial, so no load sits
 // behind a branch. A lane whose head is past num_q_heads computes on a
-// clamped head and does not store.
+// clamped head and does not store. row_ml (if given) gets each row's maximum, in the exp2
+// domain, and sum, by packed row and query head.
 __global__ __launch_bounds__(128) void decode_merge_kernel(
     uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
     const int32_t *__restrict__ q_start, const int32_t *__restrict__ items,
-    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_q_heads) {
+    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_q_heads,
+    float2 *__restrict__ row_ml) {
   const int4 it = *reinterpret_cast<const int4 *>(items + 4 * blockIdx.x);
   const int seq = it.x;
   const int first = it.y;
@@ -552,20 +608,21 @@ __global__ __launch_bounds__(128) void decode_merge_kernel(
     mx = cmx;
   }
   if (hq_lane >= num_q_heads) return;
+  if (row_ml != nullptr && d == 0) row_ml[qs * num_q_heads + hq] = make_float2(mx, lsum);
   uint16_t *dst = out + seq * o_ss + qs * o_st + hq * o_sh + d;
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2_rne(a[0] / lsum, a[1] / lsum),
                                                pack_bf16x2_rne(a[2] / lsum, a[3] / lsum));
 }
 
-template <int G, bool kFused>
+template <int G, bool kFused, bool kWindow, bool kScores>
 void launch_decode(hipStream_t st, dim3 grid, const uint16_t *q, int64_t q_ss, int64_t q_st,
                    int64_t q_sh, uint16_t *k_pool, uint16_t *v_pool, int64_t pool_hs,
                    const int32_t *page_table, int64_t pt_stride, const int32_t *items,
                    int n_chunks, float *ws_acc, float *ws_ml, int num_q_heads, int page_shift,
-                   float scale_log2, const AppendArgs &ap) {
-  hipLaunchKernelGGL((decode_kernel<G, kFused>), grid, dim3(kWaves * 64), 0, st, q, q_ss, q_st,
-                     q_sh, k_pool, v_pool, pool_hs, page_table, pt_stride, items, n_chunks, ws_acc,
-                     ws_ml, num_q_heads, page_shift, scale_log2, ap);
+                   float scale_log2, const AppendArgs &ap, const DecodeExtra &ex) {
+  hipLaunchKernelGGL((decode_kernel<G, kFused, kWindow, kScores>), grid, dim3(kWaves * 64), 0, st,
+                     q, q_ss, q_st, q_sh, k_pool, v_pool, pool_hs, page_table, pt_stride, items,
+                     n_chunks, ws_acc, ws_ml, num_q_heads, page_shift, scale_log2, ap, ex);
 }
 
 // Workspace layout: [acc fp32 n_slots*Hq*D][max,sum fp32 n_slots*Hq*2],
@@ -595,7 +652,8 @@ int paged_decode_impl(const char *name, const void *q, int64_t q_stride_seq,
                       const int32_t *decode_items, int32_t n_decode, int32_t n_slots,
                       void *workspace, int64_t workspace_bytes, int32_t num_seqs,
                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                      int32_t page_size, float scale, void *stream, const hy::AppendArgs *ap) {
+                      int32_t page_size, float scale, void *stream, const hy::AppendArgs *ap,
+                      const hy::DecodeExtra *ex = nullptr) {
   HY_REQUIRE(num_seqs >= 1, "num_seqs must be positive");
   HY_REQUIRE(scale > 0.f, "softmax scale must be positive");
   HY_REQUIRE(num_kv_heads >= 1 && num_q_heads >= num_kv_heads &&
@@ -633,18 +691,24 @@ int paged_decode_impl(const char *name, const void *q, int64_t q_stride_seq,
   uint16_t *kp = static_cast<uint16_t *>(const_cast<void *>(k_pool));
   uint16_t *vp = static_cast<uint16_t *>(const_cast<void *>(v_pool));
   const hy::AppendArgs none{};
-#define HY_DECODE_CASE(GG)                                                                     \
-  case GG:                                                                                     \
-    if (ap)                                                                                    \
-      hy::launch_decode<GG, true>(st, grid, qq, q_stride_seq, q_stride_tok, q_stride_head, kp, \
-                                  vp, pool_head_stride, page_table, page_table_stride,         \
-                                  decode_items, n_decode, ws_acc, ws_ml, num_q_heads,          \
-                                  page_shift, scale_log2, *ap);                                \
-    else                                                                                       \
-      hy::launch_decode<GG, false>(st, grid, qq, q_stride_seq, q_stride_tok, q_stride_head,    \
-                                   kp, vp, pool_head_stride, page_table, page_table_stride,    \
-                                   decode_items, n_decode, ws_acc, ws_ml, num_q_heads,         \
-                                   page_shift, scale_log2, none);                              \
+  const hy::DecodeExtra plain{};
+#define HY_DECODE_LAUNCH(GG, FUSED, WINDOW, SCORES)                                             \
+  hy::launch_decode<GG, FUSED, WINDOW, SCORES>(                                                 \
+      st, grid, qq, q_stride_seq, q_stride_tok, q_stride_head, kp, vp, pool_head_stride,        \
+      page_table, page_table_stride, decode_items, n_decode, ws_acc, ws_ml, num_q_heads,        \
+      page_shift, scale_log2, ap ? *ap : none, ex ? *ex : plain)
+#define HY_DECODE_CASE(GG)                             \
+  case GG:                                             \
+    if (ex && ex->scores)                              \
+      HY_DECODE_LAUNCH(GG, false, false, true);        \
+    else if (ex && ap)                                 \
+      HY_DECODE_LAUNCH(GG, true, true, false);         \
+    else if (ex)                                       \
+      HY_DECODE_LAUNCH(GG, false, true, false);        \
+    else if (ap)                                       \
+      HY_DECODE_LAUNCH(GG, true, false, false);        \
+    else                                               \
+      HY_DECODE_LAUNCH(GG, false, false, false);       \
     break;
   switch (G) {
     HY_DECODE_CASE(1)
@@ -654,6 +718,7 @@ int paged_decode_impl(const char *name, const void *q, int64_t q_stride_seq,
     HY_DECODE_CASE(16)
   }
 #undef HY_DECODE_CASE
+#undef HY_DECODE_LAUNCH
   return hy::launch_status(name);
 }
 
@@ -726,7 +791,7 @@ int decode_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t
                       int64_t o_stride_head, const int32_t *q_start, const int32_t *merge_items,
                       int32_t n_merge, int32_t n_slots, const void *workspace,
                       int64_t workspace_bytes, int32_t num_q_heads, int32_t head_dim,
-                      void *stream) {
+                      void *stream, float *row_ml = nullptr) {
   HY_REQUIRE(n_merge >= 0 && n_slots >= 0, "item counts must be non-negative");
   if (n_merge == 0) return HY_OK;
   HY_REQUIRE_SUPPORTED(head_dim == kHeadDim, "head_dim %d unsupported (need %d)", head_dim,
@@ -747,7 +812,7 @@ int decode_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t
   hipLaunchKernelGGL(hy::decode_merge_kernel, dim3(n_merge, (num_q_heads + 3) / 4), dim3(128), 0,
                      static_cast<hipStream_t>(stream), static_cast<uint16_t *>(out),
                      o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc,
-                     ws_ml, num_q_heads);
+                     ws_ml, num_q_heads, reinterpret_cast<float2 *>(row_ml));
   return hy::launch_status(name);
 }
 
@@ -792,6 +857,97 @@ extern "C" int hy_paged_decode_merge(void *out, int64_t o_stride_seq, int64_t o_
   return decode_merge_impl("hy_paged_decode_merge", out, o_stride_seq, o_stride_tok,
                            o_stride_head, q_start, merge_items, n_merge, n_slots, workspace,
                            workspace_bytes, num_q_heads, head_dim, stream);
+}
+
+namespace {
+
+int check_window(const char *name, int32_t window, int32_t sinks) {
+  HY_REQUIRE(window >= 1 && sinks >= 0 && sinks <= hy::kMaxSinks,
+             "%s: window %d (at least 1), sinks %d (0 to %d)", name, window, sinks, hy::kMaxSinks);
+  return HY_OK;
+}
+
+}  // namespace
+
+extern "C" int hy_paged_decode_window(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head, void *out,
+    const void *k_pool, const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
+    int64_t page_table_stride, const int32_t *q_start, const int32_t *decode_items,
+    int32_t n_decode, int32_t n_slots, void *workspace, int64_t workspace_bytes,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, float scale, int32_t window, int32_t sinks, void *stream) {
+  hy::clear_error();
+  if (int rc = check_window("hy_paged_decode_window", window, sinks)) return rc;
+  const hy::DecodeExtra ex{window, sinks, nullptr, nullptr, 0};
+  return paged_decode_impl("hy_paged_decode_window", q, q_stride_seq, q_stride_tok, q_stride_head,
+                           out, k_pool, v_pool, pool_head_stride, page_table, page_table_stride,
+                           q_start, decode_items, n_decode, n_slots, workspace, workspace_bytes,
+                           num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
+                           stream, nullptr, &ex);
+}
+
+extern "C" int hy_paged_decode_append_window(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
+    void *q_out, int64_t qo_stride_seq, int64_t qo_stride_tok, int64_t qo_stride_head,
+    const void *k, int64_t k_stride_seq, int64_t k_stride_tok, int64_t k_stride_head,
+    const void *v, int64_t v_stride_seq, int64_t v_stride_tok, int64_t v_stride_head,
+    const void *q_norm_weight, const void *k_norm_weight, float q_eps, float k_eps,
+    const float *cos_table, const float *sin_table, int32_t max_positions, void *out,
+    void *k_pool, void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
+    int64_t page_table_stride, const int32_t *q_start, const int32_t *cache_lens,
+    const int32_t *decode_items, int32_t n_decode, int32_t n_slots, void *workspace,
+    int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, float scale, int32_t window, int32_t sinks,
+    void *stream) {
+  hy::clear_error();
+  if (int rc = check_window("hy_paged_decode_append_window", window, sinks)) return rc;
+  hy::AppendArgs ap;
+  if (int rc = fill_append_args("hy_paged_decode_append_window", ap, q_out, qo_stride_seq,
+                                qo_stride_tok, qo_stride_head, k, k_stride_seq, k_stride_tok,
+                                k_stride_head, v, v_stride_seq, v_stride_tok, v_stride_head,
+                                q_norm_weight, k_norm_weight, q_eps, k_eps, cos_table,
+                                sin_table, max_positions, cache_lens))
+    return rc;
+  const hy::DecodeExtra ex{window, sinks, nullptr, nullptr, 0};
+  return paged_decode_impl("hy_paged_decode_append_window", q, q_stride_seq, q_stride_tok,
+                           q_stride_head, out, k_pool, v_pool, pool_head_stride, page_table,
+                           page_table_stride, q_start, decode_items, n_decode, n_slots,
+                           workspace, workspace_bytes, num_seqs, num_q_heads, num_kv_heads,
+                           head_dim, page_size, scale, stream, &ap, &ex);
+}
+
+extern "C" int hy_paged_decode_weigh(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head, void *out,
+    const void *k_pool, const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
+    int64_t page_table_stride, const int32_t *q_start, const int32_t *decode_items,
+    int32_t n_decode, int32_t n_slots, void *workspace, int64_t workspace_bytes,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, float scale, float *scores, const int32_t *score_start,
+    int64_t score_stride, void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(n_decode == 0 || (scores && score_start), "hy_paged_decode_weigh: null pointer argument");
+  HY_REQUIRE((reinterpret_cast<uintptr_t>(scores) & 15) == 0 && score_stride >= 0 &&
+                 score_stride % 4 == 0,
+             "hy_paged_decode_weigh: score rows lie on 16 bytes");
+  const hy::DecodeExtra ex{0, 0, scores, score_start, score_stride};
+  return paged_decode_impl("hy_paged_decode_weigh", q, q_stride_seq, q_stride_tok, q_stride_head,
+                           out, k_pool, v_pool, pool_head_stride, page_table, page_table_stride,
+                           q_start, decode_items, n_decode, n_slots, workspace, workspace_bytes,
+                           num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
+                           stream, nullptr, &ex);
+}
+
+extern "C" int hy_paged_decode_merge_weigh(void *out, int64_t o_stride_seq, int64_t o_stride_tok,
+                                           int64_t o_stride_head, const int32_t *q_start,
+                                           const int32_t *merge_items, int32_t n_merge,
+                                           int32_t n_slots, const void *workspace,
+                                           int64_t workspace_bytes, int32_t num_q_heads,
+                                           int32_t head_dim, float *row_ml, void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(n_merge == 0 || row_ml, "hy_paged_decode_merge_weigh: null pointer argument");
+  return decode_merge_impl("hy_paged_decode_merge_weigh", out, o_stride_seq, o_stride_tok,
+                           o_stride_head, q_start, merge_items, n_merge, n_slots, workspace,
+                           workspace_bytes, num_q_heads, head_dim, stream, row_ml);
 }
 
 // ---------------------------------------------------------------------------

@@ -28,6 +28,8 @@
 #include "decode_shape.h"
 #include "prefill_shape.h"
 #include "tree_shape.h"
+#include "weigh_shape.h"
+#include "window.h"
 
 namespace hy {
 void set_error(const char *fmt, ...);
@@ -146,18 +148,15 @@ struct PrefillSim {
   }
 };
 
-}  // namespace
-
-extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
-                            int32_t num_seqs, int32_t num_q_heads,
-                            int32_t num_kv_heads, int32_t page_size,
-                            int32_t num_cus, int32_t target_tokens_per_split,
-                            int32_t *decode_items, int32_t decode_capacity,
-                            int32_t *merge_items, int32_t merge_capacity,
-                            int32_t *prefill_items, int32_t prefill_capacity,
-                            int32_t *prefill_merge_items, int32_t prefill_merge_capacity,
-                            int32_t *counts_out) {
-  hy::clear_error();
+// window 0: none. Otherwise decode pieces and prefill ranges are cut from the numbers of the
+// keys in sight (window.h), for the sequence's token and for a tile's first one.
+int plan_tick(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs,
+              int32_t num_q_heads, int32_t num_kv_heads, int32_t page_size, int32_t num_cus,
+              int32_t target_tokens_per_split, int32_t window, int32_t sinks,
+              int32_t *decode_items, int32_t decode_capacity, int32_t *merge_items,
+              int32_t merge_capacity, int32_t *prefill_items, int32_t prefill_capacity,
+              int32_t *prefill_merge_items, int32_t prefill_merge_capacity,
+              int32_t *counts_out) {
   if (num_seqs < 0 || (num_seqs > 0 && (q_lens == nullptr || kv_lens == nullptr)) ||
       counts_out == nullptr) {
     hy::set_error("hy_plan_tick: invalid sequence arrays");
@@ -177,6 +176,14 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
     hy::set_error("hy_plan_tick: GQA group size %d unsupported", G);
     return HY_EUNSUPPORTED;
   }
+  // Keys of a decode sequence's stream, and those a tile from token q0 on leaves out.
+  auto decode_keys = [&](int b) {
+    return window > 0 ? kv_lens[b] - hy::window_keys<kSlice>(kv_lens[b] - 1, window, sinks).gap
+                      : kv_lens[b];
+  };
+  auto tile_gap = [&](int32_t first_pos) {
+    return window > 0 ? hy::window_keys<kPrefillKeys>(first_pos, window, sinks).gap : 0;
+  };
   int64_t decode_tokens = 0;
   for (int b = 0; b < num_seqs; ++b) {
     if (q_lens[b] < 0 || kv_lens[b] < q_lens[b]) {
@@ -184,7 +191,7 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
                     kv_lens[b]);
       return HY_EINVAL;
     }
-    if (q_lens[b] == 1) decode_tokens += kv_lens[b];
+    if (q_lens[b] == 1) decode_tokens += decode_keys(b);
   }
 
   // Decode: the K/V rows of all decode sequences, concatenated in sequence
@@ -245,7 +252,7 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
     };
     for (int b = 0; b < num_seqs; ++b) {
       if (q_lens[b] != 1) continue;
-      const int64_t kv = kv_lens[b];
+      const int64_t kv = decode_keys(b);
       int64_t t = 0;
       while (t < kv) {
         // stream cost at token t once the piece's own cost is paid
@@ -350,7 +357,7 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
     it[4] = pieces[i].slice_begin;
     it[5] = q_begin[pieces[i].seq];
     it[6] = kv_lens[pieces[i].seq] - 1;  // position of the sequence's query token
-    it[7] = pieces[i].t1 == kv_lens[pieces[i].seq];  // the piece holds that token
+    it[7] = pieces[i].t1 == decode_keys(pieces[i].seq);  // the piece holds that token
   }
 
   // Prefill: query tiles of kPrefillRows / G tokens; the key range of a tile is
@@ -369,8 +376,9 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
     const int cache = kv_lens[b] - ql;
     for (int q0 = 0; q0 < ql; q0 += tile) {
       const int q1 = std::min(ql, q0 + tile);
-      const int64_t st = (cache + q1 + kPrefillKeys - 1) / kPrefillKeys;
-      tiles.push_back({b, q0, q1, cache + q1, st});
+      const int32_t end = cache + q1 - tile_gap(cache + q0);
+      const int64_t st = (end + kPrefillKeys - 1) / kPrefillKeys;
+      tiles.push_back({b, q0, q1, end, st});
       max_tile_steps = std::max(max_tile_steps, st);
     }
   }
@@ -458,6 +466,48 @@ extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
   counts_out[5] = n_pslots;
   counts_out[6] = n_pieces;
   return HY_OK;
+}
+
+}  // namespace
+
+extern "C" int hy_plan_tick(const int32_t *q_lens, const int32_t *kv_lens,
+                            int32_t num_seqs, int32_t num_q_heads,
+                            int32_t num_kv_heads, int32_t page_size,
+                            int32_t num_cus, int32_t target_tokens_per_split,
+                            int32_t *decode_items, int32_t decode_capacity,
+                            int32_t *merge_items, int32_t merge_capacity,
+                            int32_t *prefill_items, int32_t prefill_capacity,
+                            int32_t *prefill_merge_items, int32_t prefill_merge_capacity,
+                            int32_t *counts_out) {
+  hy::clear_error();
+  return plan_tick(q_lens, kv_lens, num_seqs, num_q_heads, num_kv_heads, page_size, num_cus,
+                   target_tokens_per_split, 0, 0, decode_items, decode_capacity, merge_items,
+                   merge_capacity, prefill_items, prefill_capacity, prefill_merge_items,
+                   prefill_merge_capacity, counts_out);
+}
+
+extern "C" int hy_plan_tick_window(
+    const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t page_size, int32_t num_cus, int32_t target_tokens_per_split,
+    int32_t window, int32_t sinks, int32_t *decode_items, int32_t decode_capacity,
+    int32_t *merge_items, int32_t merge_capacity, int32_t *prefill_items,
+    int32_t prefill_capacity, int32_t *prefill_merge_items, int32_t prefill_merge_capacity,
+    int32_t *counts_out) {
+  hy::clear_error();
+  if (window < 1 || sinks < 0 || sinks > hy::kMaxSinks) {
+    hy::set_error("hy_plan_tick_window: window %d (at least 1), sinks %d (0 to %d)", window, sinks,
+                  hy::kMaxSinks);
+    return HY_EINVAL;
+  }
+  try {
+    return plan_tick(q_lens, kv_lens, num_seqs, num_q_heads, num_kv_heads, page_size, num_cus,
+                     target_tokens_per_split, window, sinks, decode_items, decode_capacity,
+                     merge_items, merge_capacity, prefill_items, prefill_capacity,
+                     prefill_merge_items, prefill_merge_capacity, counts_out);
+  } catch (const std::bad_alloc &) {
+    hy::set_error("hy_plan_tick_window: out of host memory");
+    return HY_ENOSPACE;
+  }
 }
 
 namespace {
@@ -802,4 +852,120 @@ extern "C" int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32
     hy::set_error("hy_plan_tree: out of host memory");
     return HY_ENOSPACE;
   }
+}
+
+namespace {
+
+// Rows (token, head) of a weigh item at least, and items a compute unit should get: more items
+// fill the GPU, each loads its 256 keys again. (Chosen by measurement, see weigh.hip.)
+constexpr int64_t kWeighMinRows = 256;
+constexpr int64_t kWeighPerCu = 4;
+
+int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
+               int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
+               int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds,
+               int32_t add_capacity, int64_t *counts_out) {
+  constexpr int64_t keys = hy::kWeighKeys;
+  const int64_t G = num_q_heads / num_kv_heads;
+  const int64_t cus = num_cus > 0 ? num_cus : 256;
+  // row ranges of the same length for all chunks, as long as the GPU stays filled
+  int64_t tiles_rows = 0;
+  for (int b = 0; b < num_seqs; ++b)
+    if (q_lens[b] > 1) tiles_rows += (kv_lens[b] + keys - 1) / keys * q_lens[b] * G;
+  int64_t range = tiles_rows * num_kv_heads / (cus * kWeighPerCu);
+  range = std::max(kWeighMinRows, (range + hy::kWeighRows - 1) / hy::kWeighRows * hy::kWeighRows);
+  const int64_t range_tokens = std::max<int64_t>(1, range / G);
+  int64_t scores = 0, partials = 0, q_row = 0, n_items = 0, n_adds = 0, parts_max = 0;
+  for (int b = 0; b < num_seqs; ++b) {
+    const int64_t kv = kv_lens[b], ql = q_lens[b], cache = kv - ql;
+    const bool chunk = ql > 1;
+    const int64_t parts = (ql + range_tokens - 1) / range_tokens;
+    const int64_t per = (ql + parts - 1) / parts;  // tokens of a part
+    const int64_t n_parts = (ql + per - 1) / per;
+    score_start[b] = chunk ? 0 : static_cast<int32_t>(scores);
+    for (int64_t t0 = 0; t0 < kv; t0 += keys) {
+      // parts whose last token sees the first key
+      const int64_t first = !chunk || t0 <= cache ? 0 : (t0 - cache) / per;
+      if (n_adds >= add_capacity) {
+        hy::set_error("hy_plan_weigh: addition capacity %d too small", add_capacity);
+        return HY_ENOSPACE;
+      }
+      int32_t *a = adds + 8 * n_adds++;
+      a[0] = rows[b];
+      a[1] = static_cast<int32_t>(t0);
+      a[2] = static_cast<int32_t>(std::min(kv, t0 + keys));
+      a[3] = static_cast<int32_t>(chunk ? (n_parts - first) * num_kv_heads : num_q_heads);
+      a[4] = static_cast<int32_t>(chunk ? first * num_kv_heads : 0);
+      a[5] = static_cast<int32_t>(chunk ? -1 : q_row);
+      a[6] = static_cast<int32_t>(chunk ? partials : scores);
+      a[7] = 0;
+      for (int64_t p = first; chunk && p < n_parts; ++p) {
+        if (n_items >= item_capacity) {
+          hy::set_error("hy_plan_weigh: item capacity %d too small", item_capacity);
+          return HY_ENOSPACE;
+        }
+        int32_t *it = items + 8 * n_items++;
+        it[0] = b;
+        it[1] = static_cast<int32_t>(t0);
+        it[2] = static_cast<int32_t>(p * per);
+        it[3] = static_cast<int32_t>(std::min(ql, (p + 1) * per));
+        it[4] = static_cast<int32_t>(p);
+        it[5] = static_cast<int32_t>(q_row);
+        it[6] = static_cast<int32_t>(cache);
+        it[7] = static_cast<int32_t>(partials);
+      }
+    }
+    if (chunk) {
+      partials += (kv + keys - 1) / keys * keys;
+      parts_max = std::max(parts_max, n_parts);
+    } else {
+      scores += (kv + hy::kWeighPad - 1) / hy::kWeighPad * hy::kWeighPad;
+    }
+    q_row += ql;
+    if (scores > INT32_MAX - 2 * keys || partials > INT32_MAX - 2 * keys || q_row > INT32_MAX) {
+      hy::set_error("hy_plan_weigh: too many keys in one batch");
+      return HY_EUNSUPPORTED;
+    }
+  }
+  counts_out[0] = n_items;
+  counts_out[1] = n_adds;
+  counts_out[2] = scores;
+  counts_out[3] = partials;
+  counts_out[4] = parts_max;
+  return HY_OK;
+}
+
+}  // namespace
+
+extern "C" int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
+                             int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                             int32_t num_cus, int32_t *score_start, int32_t *items,
+                             int32_t item_capacity, int32_t *adds, int32_t add_capacity,
+                             int64_t *counts_out) {
+  hy::clear_error();
+  if (num_seqs < 0 || counts_out == nullptr ||
+      (num_seqs > 0 && (!q_lens || !kv_lens || !rows || !score_start)) ||
+      (item_capacity > 0 && items == nullptr) || (add_capacity > 0 && adds == nullptr)) {
+    hy::set_error("hy_plan_weigh: invalid arrays");
+    return HY_EINVAL;
+  }
+  if (num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads % num_kv_heads) {
+    hy::set_error("hy_plan_weigh: num_q_heads (%d) must be a multiple of num_kv_heads (%d)",
+                  num_q_heads, num_kv_heads);
+    return HY_EINVAL;
+  }
+  const int32_t G = num_q_heads / num_kv_heads;
+  if (G > 16 || (G & (G - 1))) {
+    hy::set_error("hy_plan_weigh: GQA group size %d unsupported (1, 2, 4, 8, 16)", G);
+    return HY_EUNSUPPORTED;
+  }
+  for (int b = 0; b < num_seqs; ++b) {
+    if (q_lens[b] < 1 || kv_lens[b] < q_lens[b] || rows[b] < 0) {
+      hy::set_error("hy_plan_weigh: sequence %d has q_len %d, kv_len %d, row %d", b, q_lens[b],
+                    kv_lens[b], rows[b]);
+      return HY_EINVAL;
+    }
+  }
+  return plan_weigh(q_lens, kv_lens, rows, num_seqs, num_q_heads, num_kv_heads, num_cus,
+                    score_start, items, item_capacity, adds, add_capacity, counts_out);
 }

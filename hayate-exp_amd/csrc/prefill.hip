@@ -69,11 +69,18 @@
 // multiples of the 64-key tile), so the rows one wave loads of a tile lie
 // in one page (pages hold at least 32 keys) and their page-table entry is a
 // scalar load.
+//
+// With a window (kWindow) an item's keys are the numbers of window.h for the tile's first
+// token, in units of the 64-key tile: a tile of numbers from ns on lies `gap` keys further.
+// Blocks that hold a key between the sinks and some row's window are masked like those on the
+// diagonal. A masked key's V may be infinite or NaN, which 0 times is NaN: masked blocks are
+// looked through for such values on the way to the second product (see clean_v).
 
 #include <type_traits>
 
 #include "hy_common.h"
 #include "prefill_shape.h"
+#include "window.h"
 
 namespace hy {
 namespace {
@@ -86,6 +93,7 @@ constexpr float kLazyP = 256.0f;  // 2^kLazy
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16 &s, int base) {
@@ -170,7 +178,10 @@ constexpr int kSchedMfma = 0x008;
 constexpr int kSchedValu = 0x002 | 0x400;  // VALU incl. transcendentals
 constexpr int kSchedDsRead = 0x100;
 
-template <int G>
+// What a launch adds to causal attention: a window, or the rows' maxima and sums.
+enum class Extra { kNone, kWindow, kRowMl };
+
+template <int G, Extra kExtra>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void prefill_kernel(
     const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
@@ -178,8 +189,10 @@ void prefill_kernel(
     const uint16_t *__restrict__ k_pool, const uint16_t *__restrict__ v_pool,
     int64_t pool_hs, const int32_t *__restrict__ page_table, int64_t pt_stride,
     const int32_t *__restrict__ items, float *__restrict__ ws_acc, float *__restrict__ ws_ml,
-    int num_kv_heads, int page_shift, float scale_log2, bool q_aligned) {
+    int num_kv_heads, int page_shift, float scale_log2, bool q_aligned, int window, int sinks,
+    float2 *__restrict__ row_ml) {
   static_assert(kThreads == 512, "eight waves");
+  constexpr bool kWindow = kExtra == Extra::kWindow;
   __shared__ __attribute__((aligned(1024))) uint16_t smem[kStages * kStage];
 
   const int32_t *it = items + 8 * blockIdx.y;
@@ -194,10 +207,18 @@ void prefill_kernel(
   // so the Q loads and page-table reads issue one dependent read after
   // the kernel starts
   const int qs = it[6];
-  const int cache_len = it[7];
+  int cache_len = it[7];
   const int h0 = kvh * G;
   // an empty record (q_end <= q_begin) pads a list to a fixed launch size
   if (q_end <= q_begin) return;
+  // with a window, positions of tokens count in the item's key numbers too
+  int ns = 0, gap = 0;
+  if constexpr (kWindow) {
+    const WindowKeys w = window_keys<kTile>(cache_len + q_begin, window, sinks);
+    ns = w.ns;
+    gap = w.gap;
+    cache_len -= gap;
+  }
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -249,6 +270,14 @@ void prefill_kernel(
   // cross its rows' diagonal and are masked.
   const int nb = wave_live && wave_hi >= kv_begin ? (wave_hi - kv_begin) / 32 + 1 : 0;
   const int jm = wave_lo >= kv_begin ? (wave_lo - kv_begin + 1) / 32 : 0;
+  // First number in the row's window, and in that of the wave's last row.
+  const int low = kWindow ? cache_len + row_tok - window + 1 : 0;
+  const int wave_low = kWindow ? cache_len + tw1 - window + 1 : 0;
+  auto masked = [&](int j) {
+    const int b0 = kv_begin + 32 * j;
+    return j >= jm || (kWindow && b0 < wave_low && b0 + 32 > sinks);
+  };
+  auto hidden = [&](int key) { return key > limit || (kWindow && key >= sinks && key < low); };
 
   const uint16_t *kh = k_pool + kvh * pool_hs;
   const uint16_t *vh = v_pool + kvh * pool_hs;
@@ -271,24 +300,31 @@ void prefill_kernel(
   };
   auto fetch_pages = [&](int kt) __attribute__((always_inline)) {
     Pages pg;
-    pg.k = static_cast<uint32_t>(pt[max(min(kt + 16 * (wave >> 1), last_key), 0) >> page_shift]);
-    pg.v = static_cast<uint32_t>(pt[max(min(kt + 8 * wave, last_key), 0) >> page_shift]);
+    int kk = max(min(kt + 16 * (wave >> 1), last_key), 0);
+    int kv = max(min(kt + 8 * wave, last_key), 0);
+    if constexpr (kWindow) {
+      kk += kk >= ns ? gap : 0;
+      kv += kv >= ns ? gap : 0;
+    }
+    pg.k = static_cast<uint32_t>(pt[kk >> page_shift]);
+    pg.v = static_cast<uint32_t>(pt[kv >> page_shift]);
     return pg;
   };
   // First element of this lane's chunk within its row.
   const int k_chunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
   const int v_chunk = 32 * (lane >> 4) + 8 * (lane & 3);
   auto issue_tile = [&](int kt, const Pages &pg, uint16_t *dst) __attribute__((always_inline)) {
+    const int far = kWindow && kt >= ns ? gap : 0;  // a tile lies on one side of ns
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int i = 2 * wave + j;
       {
-        const int key = min(kt + 16 * (i >> 2) + (lane >> 2), last_key);
+        const int key = min(kt + 16 * (i >> 2) + (lane >> 2), last_key) + far;
         const int64_t p = (static_cast<int64_t>(pg.k) << page_shift) + (key & page_mask);
         load_to_lds(kh + p * kHeadDim + 32 * (i & 3) + k_chunk, dst + i * 512);
       }
       {
-        const int key = min(kt + 4 * i + ((lane >> 2) & 3), last_key);
+        const int key = min(kt + 4 * i + ((lane >> 2) & 3), last_key) + far;
         const int64_t p = (static_cast<int64_t>(pg.v) << page_shift) + (key & page_mask);
         load_to_lds(vh + p * kHeadDim + v_chunk, dst + kTile * kHeadDim + i * 512);
       }
@@ -360,7 +396,7 @@ void prefill_kernel(
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int key = kb0 + 8 * (i >> 2) + 4 * h + (i & 3);
-      s[i] = key > limit ? -INFINITY : s[i];
+      s[i] = hidden(key) ? -INFINITY : s[i];
     }
   };
   auto probs = [&](const f32x16 &s, bf16x8 &pop0, bf16x8 &pop1, float &psum)
@@ -432,6 +468,63 @@ void prefill_kernel(
             __builtin_bit_cast(bf16x8, vop[2 * db + kh2]), kh2 ? pop1 : pop0, acc[db], 0, 0, 0);
   };
 
+  // Infinities and NaN among block j's V operands, where block j is masked, become 0 (0 times
+  // one of them is NaN); as a rule there are none. restore_v() gives them to the rows that see
+  // them.
+  bool sick = false;
+  auto clean_v = [&](int j) __attribute__((always_inline)) {
+    if (!kWindow || !masked(j)) return;
+    uint32_t top = 0;  // the largest magnitudes, two to a word
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const u32x4 w = __builtin_bit_cast(u32x4, vop[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t mag = w[e] & 0x7fff7fffu;
+        top = __builtin_bit_cast(uint32_t,
+                                 __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                           __builtin_bit_cast(u16x2, mag)));
+      }
+    }
+    const bool found = (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u;
+    if (__builtin_expect(!__any(found), 1)) return;
+    sick = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u32x4 w = __builtin_bit_cast(u32x4, vop[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] &= ((w[e] & 0x7f80u) == 0x7f80u ? 0xffff0000u : 0xffffffffu) &
+                ((w[e] & 0x7f800000u) == 0x7f800000u ? 0xffffu : 0xffffffffu);
+      vop[i] = __builtin_bit_cast(s16x8, w);
+    }
+  };
+  // The sums of rows that see an infinity or NaN of a masked block, from the pool. (In whole
+  // numbers: this file is built without regard for NaN.)
+  auto restore_v = [&]() __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int key = kv_begin; key < min(kv_begin + 32 * nb, kv_end); ++key) {
+      if (!masked((key - kv_begin) / 32)) continue;
+      const bool sees = !hidden(key);
+      const int at = key >= ns ? key + gap : key;
+      const int64_t p = (static_cast<int64_t>(pt[at >> page_shift]) << page_shift) + (at & page_mask);
+      const uint16_t *v = vh + p * kHeadDim + 4 * h;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(v + 8 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bits = e & 1 ? (e & 2 ? x.y : x.x) & 0xffff0000u : (e & 2 ? x.y : x.x) << 16;
+          const uint32_t was = __float_as_uint(acc[j >> 2][4 * (j & 3) + e]);
+          // the other infinity, or a NaN, makes it NaN
+          const bool clash = (was & 0x7f800000u) == 0x7f800000u && was != bits;
+          if (sees && (bits & 0x7f800000u) == 0x7f800000u)
+            acc[j >> 2][4 * (j & 3) + e] = __uint_as_float(clash ? 0x7fc00000u : bits);
+        }
+      }
+    }
+  };
+
   // One block (with kLatePv): half of block j - 1's V reads go out first (the LDS counter
   // holds at most 15 outstanding reads, so the first MFMA's wait for the K
   // operands cannot leave all 16 in flight); then QK^T of block j + 1 on the
@@ -442,10 +535,10 @@ void prefill_kernel(
   // the scores do.
   f32x16 s_a, s_b;
   bf16x8 pa0, pa1, pb0, pb1;
-  auto body = [&](bool masked, int j, f32x16 &s_cur, f32x16 &s_nxt, bf16x8 &pop0, bf16x8 &pop1,
+  auto body = [&](bool cut, int j, f32x16 &s_cur, f32x16 &s_nxt, bf16x8 &pop0, bf16x8 &pop1,
                   const bf16x8 &prev0, const bf16x8 &prev1) __attribute__((always_inline)) {
     float psum;
-    if (masked) mask(s_cur, kv_begin + 32 * j);  // blocks on the diagonal
+    if (cut) mask(s_cur, kv_begin + 32 * j);  // blocks on the diagonal or a window's edge
     // V of the block whose P V runs in this body; for j = 0 with kLatePv
     // block 0's stage is read and the values are unused
     const int jv = kLatePv ? (j > 0 ? j - 1 : 0) : j;
@@ -471,9 +564,15 @@ void prefill_kernel(
     __asm__ volatile("" ::"v"(psum), "v"(pop0), "v"(pop1));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
-    if (kLatePv && j > 0) pv(prev0, prev1);  // block j - 1's, before block j's rebase
+    if (kLatePv && j > 0) {
+      clean_v(j - 1);
+      pv(prev0, prev1);  // block j - 1's, before block j's rebase
+    }
     rebase(s_cur, pop0, pop1, psum);
-    if (!kLatePv) pv(pop0, pop1);
+    if (!kLatePv) {
+      clean_v(j);
+      pv(pop0, pop1);
+    }
     read_k(j + 2);
   };
 
@@ -526,8 +625,8 @@ void prefill_kernel(
       issue_tile(kv_begin + (t + 2) * kTile, pg_next, smem + ((t + 2) % kStages) * kStage);
     // two bodies per tile with the score registers swapped, so the
     // next block's scores never have to be copied into place
-    if (2 * t < nb) body(2 * t >= jm, 2 * t, s_a, s_b, pa0, pa1, pb0, pb1);
-    if (2 * t + 1 < nb) body(2 * t + 1 >= jm, 2 * t + 1, s_b, s_a, pb0, pb1, pa0, pa1);
+    if (2 * t < nb) body(masked(2 * t), 2 * t, s_a, s_b, pa0, pa1, pb0, pb1);
+    if (2 * t + 1 < nb) body(masked(2 * t + 1), 2 * t + 1, s_b, s_a, pb0, pb1, pa0, pa1);
     if (t + 1 < n_tiles) {
       // tile t + 3's page ids; the wait below covers them too
       if (t + 3 < n_tiles) pg_next = fetch_pages(kv_begin + (t + 3) * kTile);
@@ -541,13 +640,18 @@ void prefill_kernel(
   if (kLatePv && nb > 0) {
     read_v(nb - 1, 0);
     read_v(nb - 1, 1);
+    clean_v(nb - 1);
     if ((nb - 1) & 1)
       pv(pb0, pb1);
     else
       pv(pa0, pa1);
   }
+  if (kWindow && sick) restore_v();
   // Epilogue: full row sums, then the output or the split's partial.
   const float lsum = halves_sum(l_run);
+  if (kExtra == Extra::kRowMl && slot < 0 && live && h == 0)  // the exponent base and sum
+    row_ml[static_cast<int64_t>(qs + row_tok) * num_kv_heads * G + h0 + r % G] =
+        make_float2(base, lsum);
   if (slot < 0) {
     // The output rows go through LDS so that 16 lanes store a row: a lane
     // holds 8-byte pieces of one row, and 64 lanes storing to 32 rows keep a
@@ -617,7 +721,8 @@ template <int G>
 __global__ __launch_bounds__(512) void prefill_merge_kernel(
     uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
     const int32_t *__restrict__ q_start, const int32_t *__restrict__ items,
-    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_kv_heads) {
+    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_kv_heads,
+    float2 *__restrict__ row_ml) {
   const int4 it0 = *reinterpret_cast<const int4 *>(items + 8 * blockIdx.y);
   const int4 it1 = *reinterpret_cast<const int4 *>(items + 8 * blockIdx.y + 4);
   const int kvh = blockIdx.x;
@@ -682,34 +787,39 @@ __global__ __launch_bounds__(512) void prefill_merge_kernel(
   const int chunk = threadIdx.x & 15;
   const int row = 32 * blockIdx.z + r;
   const int i = q_begin + row / G;
+  // (the thread with the row's first dims has its maximum and sum)
+  const int own = 32 * blockIdx.z + c;
+  if (row_ml != nullptr && j8 == 0 && q_begin + own / G < q_end)
+    row_ml[(qs + q_begin + own / G) * num_kv_heads * G + kvh * G + own % G] = make_float2(mx, lsum);
   if (i >= q_end) return;
   store16(out + seq * o_ss + (qs + i) * o_st + (kvh * G + row % G) * o_sh + 8 * chunk,
           *reinterpret_cast<const u32x4 *>(rows + r * kHeadDim + 8 * (chunk ^ (r & 15))));
 }
 
-template <int G>
+template <int G, Extra kExtra>
 void launch_prefill(hipStream_t st, int num_kv_heads, int n_items, const uint16_t *q,
                     int64_t q_ss, int64_t q_st, int64_t q_sh, uint16_t *out, int64_t o_ss,
                     int64_t o_st, int64_t o_sh, const uint16_t *k_pool, const uint16_t *v_pool,
                     int64_t pool_hs, const int32_t *page_table, int64_t pt_stride,
                     const int32_t *items, float *ws_acc, float *ws_ml, int page_shift,
-                    float scale_log2) {
+                    float scale_log2, int window, int sinks, float *row_ml) {
   const bool q_aligned =
       (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ((q_ss | q_st | q_sh) & 7) == 0;
-  hipLaunchKernelGGL((prefill_kernel<G>), dim3(num_kv_heads, n_items), dim3(kThreads), 0,
+  hipLaunchKernelGGL((prefill_kernel<G, kExtra>), dim3(num_kv_heads, n_items), dim3(kThreads), 0,
                      st, q, q_ss,
                      q_st, q_sh, out, o_ss, o_st, o_sh, k_pool, v_pool, pool_hs, page_table,
                      pt_stride, items, ws_acc, ws_ml, num_kv_heads, page_shift, scale_log2,
-                     q_aligned);
+                     q_aligned, window, sinks, reinterpret_cast<float2 *>(row_ml));
 }
 
 template <int G>
 void launch_prefill_merge(hipStream_t st, int num_kv_heads, int n_merge, uint16_t *out,
                           int64_t o_ss, int64_t o_st, int64_t o_sh, const int32_t *q_start,
-                          const int32_t *merge_items, const float *ws_acc, const float *ws_ml) {
+                          const int32_t *merge_items, const float *ws_acc, const float *ws_ml,
+                          float *row_ml) {
   hipLaunchKernelGGL(prefill_merge_kernel<G>, dim3(num_kv_heads, n_merge, kRows / 32), dim3(512),
                      0, st, out, o_ss, o_st, o_sh, q_start, merge_items, ws_acc, ws_ml,
-                     num_kv_heads);
+                     num_kv_heads, reinterpret_cast<float2 *>(row_ml));
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -728,15 +838,18 @@ extern "C" int64_t hy_prefill_workspace_bytes(int32_t n_slots, int32_t num_kv_he
   return hy::align256(rows * head_dim * 4) + hy::align256(rows * 2 * 4);
 }
 
-extern "C" int hy_paged_prefill(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
+namespace {
+
+// window > 0: with a window; row_ml (may be null): every row's maximum and sum.
+int paged_prefill_impl(
+    const char *name, const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
     void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
     const void *k_pool, const void *v_pool, int64_t pool_head_stride,
     const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
     const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
     void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, void *stream) {
-  hy::clear_error();
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, int32_t window,
+    int32_t sinks, float *row_ml, void *stream) {
   HY_REQUIRE(num_seqs >= 1, "num_seqs must be positive");
   HY_REQUIRE(scale > 0.f, "softmax scale must be positive");
   HY_REQUIRE(num_kv_heads >= 1 && num_q_heads >= num_kv_heads &&
@@ -751,7 +864,7 @@ extern "C" int hy_paged_prefill(
   if (n_prefill == 0) return HY_OK;
   HY_REQUIRE(n_prefill <= 65535, "%d prefill items exceed the grid limit of 65535", n_prefill);
   HY_REQUIRE(q && out && k_pool && v_pool && page_table && q_start && kv_lens && prefill_items,
-             "hy_paged_prefill: null pointer argument");
+             "%s: null pointer argument", name);
   const int64_t need = hy_prefill_workspace_bytes(n_slots, num_kv_heads, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     hy::set_error("workspace too small: need %lld bytes, got %lld",
@@ -775,10 +888,13 @@ extern "C" int hy_paged_prefill(
   const uint16_t *vp = static_cast<const uint16_t *>(v_pool);
 #define HY_PREFILL_CASE(GG)                                                                   \
   case GG:                                                                                    \
-    hy::launch_prefill<GG>(st, num_kv_heads, n_prefill, qq, q_stride_seq, q_stride_tok,       \
-                           q_stride_head, oo, o_stride_seq, o_stride_tok, o_stride_head, kp,  \
-                           vp, pool_head_stride, page_table, page_table_stride,               \
-                           prefill_items, ws_acc, ws_ml, page_shift, scale_log2);             \
+    (window > 0 ? hy::launch_prefill<GG, hy::Extra::kWindow>                                  \
+     : row_ml   ? hy::launch_prefill<GG, hy::Extra::kRowMl>                                   \
+                : hy::launch_prefill<GG, hy::Extra::kNone>)(                                  \
+        st, num_kv_heads, n_prefill, qq, q_stride_seq, q_stride_tok, q_stride_head, oo,       \
+        o_stride_seq, o_stride_tok, o_stride_head, kp, vp, pool_head_stride, page_table,      \
+        page_table_stride, prefill_items, ws_acc, ws_ml, page_shift, scale_log2, window,      \
+        sinks, row_ml);                                                                       \
     break;
   switch (G) {
     HY_PREFILL_CASE(1)
@@ -791,16 +907,75 @@ extern "C" int hy_paged_prefill(
       return HY_EUNSUPPORTED;
   }
 #undef HY_PREFILL_CASE
-  return hy::launch_status("hy_paged_prefill");
+  return hy::launch_status(name);
 }
 
-extern "C" int hy_paged_prefill_merge(void *out, int64_t o_stride_seq, int64_t o_stride_tok,
-                                      int64_t o_stride_head, const int32_t *q_start,
-                                      const int32_t *merge_items, int32_t n_merge,
-                                      int32_t n_slots, const void *workspace,
-                                      int64_t workspace_bytes, int32_t num_q_heads,
-                                      int32_t num_kv_heads, int32_t head_dim, void *stream) {
+}  // namespace
+
+extern "C" int hy_paged_prefill(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
+    const void *k_pool, const void *v_pool, int64_t pool_head_stride,
+    const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
+    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
+    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, void *stream) {
   hy::clear_error();
+  return paged_prefill_impl("hy_paged_prefill", q, q_stride_seq, q_stride_tok, q_stride_head, out,
+                            o_stride_seq, o_stride_tok, o_stride_head, k_pool, v_pool,
+                            pool_head_stride, page_table, page_table_stride, q_start, kv_lens,
+                            prefill_items, n_prefill, n_slots, workspace, workspace_bytes,
+                            num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
+                            0, 0, nullptr, stream);
+}
+
+extern "C" int hy_paged_prefill_window(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
+    const void *k_pool, const void *v_pool, int64_t pool_head_stride,
+    const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
+    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
+    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, int32_t window,
+    int32_t sinks, void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(window >= 1 && sinks >= 0 && sinks <= hy::kMaxSinks,
+             "hy_paged_prefill_window: window %d (at least 1), sinks %d (0 to %d)", window, sinks,
+             hy::kMaxSinks);
+  return paged_prefill_impl("hy_paged_prefill_window", q, q_stride_seq, q_stride_tok, q_stride_head, out,
+                            o_stride_seq, o_stride_tok, o_stride_head, k_pool, v_pool,
+                            pool_head_stride, page_table, page_table_stride, q_start, kv_lens,
+                            prefill_items, n_prefill, n_slots, workspace, workspace_bytes,
+                            num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
+                            window, sinks, nullptr, stream);
+}
+
+extern "C" int hy_paged_prefill_weigh(
+    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
+    const void *k_pool, const void *v_pool, int64_t pool_head_stride,
+    const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
+    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
+    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, float *row_ml,
+    void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(n_prefill == 0 || row_ml, "hy_paged_prefill_weigh: null pointer argument");
+  return paged_prefill_impl("hy_paged_prefill_weigh", q, q_stride_seq, q_stride_tok, q_stride_head, out,
+                            o_stride_seq, o_stride_tok, o_stride_head, k_pool, v_pool,
+                            pool_head_stride, page_table, page_table_stride, q_start, kv_lens,
+                            prefill_items, n_prefill, n_slots, workspace, workspace_bytes,
+                            num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
+                            0, 0, row_ml, stream);
+}
+
+namespace {
+
+int prefill_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t o_stride_tok,
+                       int64_t o_stride_head, const int32_t *q_start, const int32_t *merge_items,
+                       int32_t n_merge, int32_t n_slots, const void *workspace,
+                       int64_t workspace_bytes, int32_t num_q_heads, int32_t num_kv_heads,
+                       int32_t head_dim, float *row_ml, void *stream) {
   HY_REQUIRE(n_merge >= 0 && n_slots >= 0, "item counts must be non-negative");
   if (n_merge == 0) return HY_OK;
   HY_REQUIRE(n_merge <= 65535, "%d merge items exceed the grid limit of 65535", n_merge);
@@ -811,7 +986,7 @@ extern "C" int hy_paged_prefill_merge(void *out, int64_t o_stride_seq, int64_t o
   HY_REQUIRE_SUPPORTED(head_dim == kHeadDim, "head_dim %d unsupported (need %d)", head_dim,
                        kHeadDim);
   HY_REQUIRE(out && q_start && merge_items && workspace,
-             "hy_paged_prefill_merge: null pointer argument");
+             "%s: null pointer argument", name);
   const int64_t need = hy_prefill_workspace_bytes(n_slots, num_kv_heads, head_dim);
   if (workspace_bytes < need) {
     hy::set_error("workspace too small: need %lld bytes, got %lld",
@@ -825,14 +1000,39 @@ extern "C" int hy_paged_prefill_merge(void *out, int64_t o_stride_seq, int64_t o
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint16_t *oo = static_cast<uint16_t *>(out);
   switch (num_q_heads / num_kv_heads) {
-    case 1: hy::launch_prefill_merge<1>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml); break;
-    case 2: hy::launch_prefill_merge<2>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml); break;
-    case 4: hy::launch_prefill_merge<4>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml); break;
-    case 8: hy::launch_prefill_merge<8>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml); break;
-    case 16: hy::launch_prefill_merge<16>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml); break;
+    case 1: hy::launch_prefill_merge<1>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml, row_ml); break;
+    case 2: hy::launch_prefill_merge<2>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml, row_ml); break;
+    case 4: hy::launch_prefill_merge<4>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml, row_ml); break;
+    case 8: hy::launch_prefill_merge<8>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml, row_ml); break;
+    case 16: hy::launch_prefill_merge<16>(st, num_kv_heads, n_merge, oo, o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc, ws_ml, row_ml); break;
     default:
       hy::set_error("GQA group size %d unsupported (1, 2, 4, 8, 16)", num_q_heads / num_kv_heads);
       return HY_EUNSUPPORTED;
   }
-  return hy::launch_status("hy_paged_prefill_merge");
+  return hy::launch_status(name);
+}
+
+}  // namespace
+
+extern "C" int hy_paged_prefill_merge(
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
+    const int32_t *q_start, const int32_t *merge_items, int32_t n_merge, int32_t n_slots,
+    const void *workspace, int64_t workspace_bytes, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, void *stream) {
+  hy::clear_error();
+  return prefill_merge_impl("hy_paged_prefill_merge", out, o_stride_seq, o_stride_tok, o_stride_head, q_start,
+                            merge_items, n_merge, n_slots, workspace, workspace_bytes,
+                            num_q_heads, num_kv_heads, head_dim, nullptr, stream);
+}
+
+extern "C" int hy_paged_prefill_merge_weigh(
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
+    const int32_t *q_start, const int32_t *merge_items, int32_t n_merge, int32_t n_slots,
+    const void *workspace, int64_t workspace_bytes, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, float *row_ml, void *stream) {
+  hy::clear_error();
+  HY_REQUIRE(n_merge == 0 || row_ml, "hy_paged_prefill_merge_weigh: null pointer argument");
+  return prefill_merge_impl("hy_paged_prefill_merge_weigh", out, o_stride_seq, o_stride_tok, o_stride_head, q_start,
+                            merge_items, n_merge, n_slots, workspace, workspace_bytes,
+                            num_q_heads, num_kv_heads, head_dim, row_ml, stream);
 }

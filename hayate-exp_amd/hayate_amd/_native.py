@@ -140,6 +140,54 @@ _SIGNATURES = {
         [_P, _P, _I64, _I64, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P],
         ctypes.c_int,
     ),
+    "hy_plan_tick_window": (
+        [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32, _P, _I32, _P, _I32, _P,
+         _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_decode_window": (
+        [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _I32,
+         _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_decode_append_window": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64,
+         _I64, _P, _P, _F32, _F32, _P, _P, _I32, _P, _P, _P, _I64, _P, _I64, _P, _P, _P, _I32,
+         _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_prefill_window": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
+         _P, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_plan_weigh": (
+        [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_decode_weigh": (
+        [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _I32,
+         _I32, _I32, _I32, _I32, _F32, _P, _P, _I64, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_decode_merge_weigh": (
+        [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _P, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_prefill_weigh": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
+         _P, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _P, _P],
+        ctypes.c_int,
+    ),
+    "hy_paged_prefill_merge_weigh": (
+        [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P, _P],
+        ctypes.c_int,
+    ),
+    "hy_token_weights": (
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _P,
+         _I64, _I32, _I32, _I32, _I32, _F32, _P],
+        ctypes.c_int,
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -223,8 +271,10 @@ def plan_tick(
     page_size: int,
     num_cus: int,
     tokens_per_split: int = 0,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> TickPlan:
-    """Run the native tick planner."""
+    """Run the native tick planner, with a `window` the one for windowed attention."""
     q_lens = np.ascontiguousarray(q_lens, dtype=np.int32)
     kv_lens = np.ascontiguousarray(kv_lens, dtype=np.int32)
     n = int(q_lens.shape[0])
@@ -251,13 +301,15 @@ def plan_tick(
     pre = np.zeros((pre_cap, 8), dtype=np.int32)
     pmrg = np.zeros((n_tiles + 1, 8), dtype=np.int32)
     counts = np.zeros(7, dtype=np.int32)
-    rc = lib().hy_plan_tick(
+    name, extra = ("hy_plan_tick", ()) if window is None else ("hy_plan_tick_window",
+                                                               (window, sinks))
+    rc = getattr(lib(), name)(
         q_lens.ctypes.data, kv_lens.ctypes.data, n, num_q_heads, num_kv_heads,
-        page_size, num_cus, tokens_per_split, dec.ctypes.data, dec_cap,
+        page_size, num_cus, tokens_per_split, *extra, dec.ctypes.data, dec_cap,
         mrg.ctypes.data, n + 1, pre.ctypes.data, pre_cap, pmrg.ctypes.data, n_tiles + 1,
         counts.ctypes.data,
     )
-    check(rc, "hy_plan_tick")
+    check(rc, name)
     nd, nm, ns, npf, npm, nps, npc = (int(x) for x in counts)
     return TickPlan(dec[: nd + npc].copy(), nd, mrg[:nm].copy(), ns, pre[:npf].copy(),
                     pmrg[:npm].copy(), nps)
@@ -324,3 +376,38 @@ def plan_tree(
 
 def tree_workspace_bytes(n_slots: int, num_kv_heads: int, head_dim: int) -> int:
     return int(lib().hy_tree_workspace_bytes(n_slots, num_kv_heads, head_dim))
+
+
+class WeighPlan:
+    """Host copy of the lists that add up one tick's attention weights (hy_plan_weigh)."""
+
+    __slots__ = ("score_start", "items", "adds", "scores", "partials", "parts")
+
+    def __init__(self, score_start, items, adds, scores, partials, parts):
+        self.score_start = score_start  # int32 (sequences): its scores' first place in a row
+        self.items = items  # int32 (n, 8) {seq, key0, token0, token1, part, q_row, cache, offset}
+        self.adds = adds  # int32 (n, 8) {row, t0, t1, sources, first, q_row or -1, offset, 0}
+        self.scores = scores  # places a row of scores has
+        self.partials = partials  # and a row of partial sums
+        self.parts = parts
+
+
+def plan_weigh(q_lens: np.ndarray, kv_lens: np.ndarray, rows: np.ndarray, num_q_heads: int,
+               num_kv_heads: int, num_cus: int) -> WeighPlan:
+    """Run the native planner of attention weights."""
+    q_lens, kv_lens, rows = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, kv_lens, rows))
+    n = len(q_lens)
+    blocks = -(-kv_lens.astype(np.int64) // 256)
+    # a range holds 256 rows at least, of at most 16 heads a token
+    ranges = -(-q_lens.astype(np.int64) // 16)
+    items = np.zeros((int((blocks * ranges)[q_lens > 1].sum()) + 1, 8), dtype=np.int32)
+    adds = np.zeros((int(blocks.sum()) + 1, 8), dtype=np.int32)
+    starts, counts = np.zeros(n, dtype=np.int32), np.zeros(5, dtype=np.int64)
+    rc = lib().hy_plan_weigh(
+        q_lens.ctypes.data, kv_lens.ctypes.data, rows.ctypes.data, n, num_q_heads, num_kv_heads,
+        num_cus, starts.ctypes.data, items.ctypes.data, len(items), adds.ctypes.data, len(adds),
+        counts.ctypes.data,
+    )
+    check(rc, "hy_plan_weigh")
+    n_items, n_adds, scores, partials, parts = counts.tolist()
+    return WeighPlan(starts, items[:n_items].copy(), adds[:n_adds].copy(), scores, partials, parts)

@@ -250,6 +250,11 @@ class PagedKVBatch:
     """
 
     positions: Optional[torch.Tensor] = None
+    # attention sees the last `window` slots up to a token's own, and the first `sinks`
+    window: Optional[int] = None
+    sinks: int = 0
+    # where attention adds up the weight of every cached token: row handle.slot, entry slot
+    weights: Optional[torch.Tensor] = None
 
     def __init__(
         self,
@@ -262,7 +267,16 @@ class PagedKVBatch:
         tokens_per_split: int = 0,
         extra: Optional[np.ndarray] = None,
         first_positions: Optional[list[int]] = None,
+        window: Optional[int] = None,
+        sinks: int = 0,
+        weights: Optional[torch.Tensor] = None,
+        weight_rows: Sequence[int] = (),
     ):
+        if window is not None:
+            self.window, self.sinks = window, sinks
+        if weights is not None:
+            self.weights, self._weight_rows = weights, list(weight_rows)
+            self._weigh_plans: dict[int, _DeviceWeighPlan] = {}
         self.k_cache = manager.k_cache
         self.v_cache = manager.v_cache
         self.page_size = manager.page_size
@@ -372,11 +386,26 @@ class PagedKVBatch:
             self.page_size,
             self._num_cus,
             self.tokens_per_split,
+            self.window,
+            self.sinks,
         )
         plan = _DevicePlan(host, num_q_heads, self.num_kv_heads, self.head_dim, self.device)
         self._own(*plan.memory)
         self._plans[num_q_heads] = plan
+        if self.weights is not None:
+            self._weigh_plan(num_q_heads)
         return plan
+
+    def _weigh_plan(self, num_q_heads: int) -> "_DeviceWeighPlan":
+        cached = self._weigh_plans.get(num_q_heads)
+        if cached is None:
+            host = _native.plan_weigh(
+                np.asarray(self.q_lens), np.asarray(self.kv_lens_host),
+                np.asarray(self._weight_rows), num_q_heads, self.num_kv_heads, self._num_cus)
+            cached = _DeviceWeighPlan(host, self, num_q_heads)
+            self._own(*cached.memory)
+            self._weigh_plans[num_q_heads] = cached
+        return cached
 
     def _layer_pools(self, layer_idx: int):
         """(k_ptr, v_ptr, head_stride) of one layer's pool slice, cached
@@ -562,11 +591,14 @@ class PagedKVBatch:
         static device scratch instead of the plan's workspace (same
         results; raises MemoryError if the tick's partials do not fit).
 
-        The launch rotates at cache_lens; a batch with ``positions`` of its own
-        makes the two calls (and refuses no_alloc)."""
+        The launch rotates at cache_lens; a batch with ``positions`` of its own, or
+        with ``weights``, makes the two calls (and refuses no_alloc, as one with a window
+        does)."""
         if not self.decode_only:
             raise ValueError("decode_layer needs q_len == 1 for every sequence")
-        if self.positions is not None:
+        if no_alloc and (self.window is not None or self.weights is not None):
+            raise NotImplementedError("no_alloc has no form with a window or weights")
+        if self.positions is not None or self.weights is not None:
             if no_alloc:
                 raise NotImplementedError("no_alloc rotates at the slots, not at `positions`")
             q_rot = self.norm_rope_write_layer(layer_idx, q, k, v, q_norm_weight, k_norm_weight,
@@ -604,12 +636,14 @@ class PagedKVBatch:
                 float(scale), stream,
             )
             return a.q_out, result
-        self._launch("hy_paged_decode_append", lib.hy_paged_decode_append,
+        name, windowed = ("hy_paged_decode_append", ()) if self.window is None else (
+            "hy_paged_decode_append_window", (self.window, self.sinks))
+        self._launch(name, getattr(lib, name),
             *a.head, *eps_pair, *a.tables, result.data_ptr(), k_ptr, v_ptr, hs,
             self._pt_ptr, self._pt_stride, self._q_start_ptr, self._cache_lens_ptr,
             plan.decode_ptr, plan.n_decode, plan.n_slots, plan.workspace_ptr,
             plan.workspace_bytes, self.num_seqs, num_q_heads, self.num_kv_heads,
-            self.head_dim, self.page_size, float(scale), stream,
+            self.head_dim, self.page_size, float(scale), *windowed, stream,
         )
         self._launch("hy_paged_decode_merge", lib.hy_paged_decode_merge,
             result.data_ptr(), *os_, self._q_start_ptr,
@@ -652,10 +686,16 @@ class PagedKVBatch:
         q is (B, Hq, T, D) for a uniform batch (returns (B, Hq, T, D), a
         transposed view of a (B, T, Hq, D) buffer so the caller's
         transpose + reshape is free) or packed (N, Hq, D) for a varlen tick.
+        With the batch's ``window`` a token sees no other slots than the last ones and
+        the sinks; with ``weights`` the call also adds to them.
         """
         _require_hip(q, "attend_layer")
         if q.dtype != self.k_cache.dtype:
             raise TypeError("q dtype must match the pool dtype")
+        if ((self.window is not None or self.weights is not None)
+                and torch.cuda.current_device() != self.device.index):
+            with torch.cuda.device(self.device):  # the launches go to its current stream
+                return self.attend_layer(q, layer_idx, scale)
         q, qs = self._rows(q, "bhtd")
         num_q_heads = q.shape[1]
         os_ = self._packed(num_q_heads)
@@ -675,40 +715,89 @@ class PagedKVBatch:
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
         stream = self._stream()
         lib = _native.lib()
+        # the calls' variants and what they take besides
+        kind, merge_kind, window, scores, row_ml = "", "", (), (), ()
+        weigh = None
+        if self.window is not None:
+            kind, window = "_window", (self.window, self.sinks)
+        elif self.weights is not None:
+            weigh = self._weigh_plan(num_q_heads)
+            kind = merge_kind = "_weigh"
+            scores, row_ml = weigh.scores_args, (weigh.row_ml_ptr,)
         if plan.n_decode:
-            self._launch("hy_paged_decode", lib.hy_paged_decode,
-                q.data_ptr(), *qs, result.data_ptr(), *os_,
+            name = "hy_paged_decode" + kind
+            self._launch(name, getattr(lib, name),
+                q.data_ptr(), *qs, result.data_ptr(), *(() if kind else os_),
                 k_ptr, v_ptr, hs,
                 self._pt_ptr, self._pt_stride, self._q_start_ptr, plan.decode_ptr,
                 plan.n_decode, plan.n_slots, plan.workspace_ptr, plan.workspace_bytes, self.num_seqs, num_q_heads,
-                self.num_kv_heads, self.head_dim, self.page_size, float(scale),
+                self.num_kv_heads, self.head_dim, self.page_size, float(scale), *window, *scores,
                 stream,
             )
         if plan.n_merge:
-            self._launch("hy_paged_decode_merge", lib.hy_paged_decode_merge,
+            name = "hy_paged_decode_merge" + merge_kind
+            self._launch(name, getattr(lib, name),
                 result.data_ptr(), *os_, self._q_start_ptr,
                 plan.merge_ptr, plan.n_merge, plan.n_slots,
                 plan.workspace_ptr, plan.workspace_bytes, num_q_heads,
-                self.head_dim, stream,
+                self.head_dim, *row_ml, stream,
             )
         if plan.n_prefill:
-            self._launch("hy_paged_prefill", lib.hy_paged_prefill,
+            name = "hy_paged_prefill" + kind
+            self._launch(name, getattr(lib, name),
                 q.data_ptr(), *qs, result.data_ptr(), *os_,
                 k_ptr, v_ptr, hs,
                 self._pt_ptr, self._pt_stride, self._q_start_ptr, self._kv_lens_ptr,
                 plan.prefill_ptr, plan.n_prefill, plan.n_prefill_slots,
                 plan.prefill_workspace_ptr, plan.prefill_workspace_bytes, self.num_seqs, num_q_heads,
-                self.num_kv_heads, self.head_dim, self.page_size, float(scale),
+                self.num_kv_heads, self.head_dim, self.page_size, float(scale), *window, *row_ml,
                 stream,
             )
         if plan.n_prefill_merge:
-            self._launch("hy_paged_prefill_merge", lib.hy_paged_prefill_merge,
+            name = "hy_paged_prefill_merge" + merge_kind
+            self._launch(name, getattr(lib, name),
                 result.data_ptr(), *os_, self._q_start_ptr,
                 plan.prefill_merge_ptr, plan.n_prefill_merge, plan.n_prefill_slots,
                 plan.prefill_workspace_ptr, plan.prefill_workspace_bytes,
-                num_q_heads, self.num_kv_heads, self.head_dim, stream,
+                num_q_heads, self.num_kv_heads, self.head_dim, *row_ml, stream,
+            )
+        if weigh is not None:
+            self._launch("hy_token_weights", lib.hy_token_weights,
+                q.data_ptr(), *qs, k_ptr, hs, self._pt_ptr, self._pt_stride, *weigh.args,
+                self.weights.data_ptr(), self.weights.stride(0), num_q_heads, self.num_kv_heads,
+                self.head_dim, self.page_size, float(scale), stream,
             )
         return result
+
+
+class _DeviceWeighPlan:
+    """The lists that add up one tick's attention weights, on the device, and the room for what
+    the calls leave between them."""
+
+    def __init__(self, host: "_native.WeighPlan", batch: PagedKVBatch, num_q_heads: int):
+        self.host = host
+        kv_heads, device = batch.num_kv_heads, batch.device
+        starts = np.zeros(len(host.score_start) + -len(host.score_start) % 4, dtype=np.int32)
+        starts[: len(host.score_start)] = host.score_start
+        packed = np.concatenate([starts, host.items.reshape(-1), host.adds.reshape(-1)])
+        lists = torch.from_numpy(packed).to(device)
+        # (row_ml first, then the scores and the partial sums on 16 bytes)
+        row_ml = 2 * batch.total_tokens * num_q_heads
+        row_ml += -row_ml % 4
+        scores = num_q_heads * host.scores
+        room = torch.empty(row_ml + scores + host.parts * kv_heads * host.partials,
+                           dtype=torch.float32, device=device)
+        self.memory = (lists, room)
+        at = lists.data_ptr()
+        items = at + 4 * starts.size
+        self.row_ml_ptr = room.data_ptr()
+        scores_ptr = self.row_ml_ptr + 4 * row_ml if scores else None
+        partials_ptr = self.row_ml_ptr + 4 * (row_ml + scores) if host.parts else None
+        self.scores_args = (scores_ptr, at, host.scores)
+        # hy_token_weights' arguments between the page table and the table of weights
+        self.args = (items if len(host.items) else None, len(host.items),
+                     items + 4 * host.items.size, len(host.adds), scores_ptr, host.scores,
+                     partials_ptr, host.partials, self.row_ml_ptr)
 
 
 class PagedTreeBatch(PagedKVBatch):
@@ -1452,15 +1541,62 @@ class PagedKVCacheManager:
             return None
         return [h.next_position for h in handles]
 
+    def _attention_form(self, handles: Sequence[PagedCacheHandle], query_lens: Sequence[int],
+                        window: Optional[int], sinks: int,
+                        weights: Optional[torch.Tensor]) -> dict:
+        """Checks how a tick is to attend, and what PagedKVBatch takes for it."""
+        if window is None:
+            if _index(sinks, "sinks"):
+                raise ValueError("sinks go with a window")
+        else:
+            window, sinks = _index(window, "window"), _index(sinks, "sinks")
+            if window < 1:
+                raise ValueError("window must be positive")
+            if sinks < 0:
+                raise ValueError("sinks must be non-negative")
+            if weights is not None:
+                raise NotImplementedError("weights are of attention to the whole cache, "
+                                          "without a window")
+            # (no cache is longer)
+            most = self.capacity_tokens
+            return {"window": min(window, most), "sinks": min(sinks, most)}
+        if weights is None:
+            return {}
+        if self.k_cache.dtype != torch.bfloat16:
+            raise TypeError("weights need a bfloat16 pool")
+        rows = [h.slot for h in handles]
+        self._check_weights(weights, rows, [h.length + q for h, q in zip(handles, query_lens)])
+        return {"weights": weights, "weight_rows": rows}
+
+    def _check_weights(self, weights: torch.Tensor, rows: Sequence[int],
+                       lengths: Sequence[int]) -> None:
+        """A table of weights: fp32 (rows, tokens), a row for every handle's slot."""
+        if not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32:
+            raise TypeError("weights must be a float32 tensor")
+        if weights.device != self.device:
+            raise ValueError(f"weights are on {weights.device}, the pool on {self.device}")
+        if weights.dim() != 2 or weights.shape[0] <= max(rows):
+            raise ValueError("weights must be (rows, tokens), with a row for every handle's slot")
+        if weights.shape[1] < max(lengths):
+            raise ValueError(f"weights have {weights.shape[1]} tokens a row, a cache {max(lengths)}")
+        if weights.stride(1) != 1 or (weights.shape[0] > 1
+                                      and weights.stride(0) < weights.shape[1]):
+            raise ValueError("weights' rows must be contiguous and apart")
+        if weights.requires_grad:
+            raise ValueError("weights are written in place and take no gradient")
+
     def begin_batch(
-        self, handles: Sequence[PagedCacheHandle], query_len: int
+        self, handles: Sequence[PagedCacheHandle], query_len: int, *,
+        window: Optional[int] = None, sinks: int = 0, weights: Optional[torch.Tensor] = None,
     ) -> PagedKVBatch:
         """Reserve append space for `query_len` tokens per request and build
-        the tick metadata (paged_cache.py:202-293)."""
+        the tick metadata (paged_cache.py:202-293). `window`, `sinks` and `weights`
+        as in ``begin_tick``."""
         self._validate_handles(handles)
         if query_len < 1:
             raise ValueError("query_len must be positive")
         q_lens = [query_len] * len(handles)
+        form = self._attention_form(handles, q_lens, window, sinks, weights)
         self._reserve_all(handles, q_lens)
         if self.page_size < MIN_KV_PAGE_SIZE:
             raise ValueError(
@@ -1470,21 +1606,34 @@ class PagedKVCacheManager:
             self, q_lens, [h.length for h in handles], [list(h.pages) for h in handles],
             varlen=False, num_q_heads=self.num_q_heads,
             tokens_per_split=self.tokens_per_split,
-            first_positions=self._first_positions(handles),
+            first_positions=self._first_positions(handles), **form,
         )
 
     def begin_tick(
-        self, handles: Sequence[PagedCacheHandle], query_lens: Sequence[int]
+        self, handles: Sequence[PagedCacheHandle], query_lens: Sequence[int], *,
+        window: Optional[int] = None, sinks: int = 0, weights: Optional[torch.Tensor] = None,
     ) -> PagedKVBatch:
         """One varlen batch mixing prefill chunks (q_len > 1) and decode
         tokens (q_len == 1); tensors are packed (total_tokens, heads, dim)
-        in handle order. Commit with ``commit_tick``."""
+        in handle order. Commit with ``commit_tick``.
+
+        `window`: in every layer a token sees the last `window` slots up to its own, and
+        the first `sinks` slots, instead of the whole cache (slots, not rope positions: the
+        two differ where ``compact`` dropped tokens).
+
+        `weights`, fp32 (rows, tokens): every layer's attention adds to
+        weights[handle.slot, j] what weight the tick's tokens give the token in slot j, all
+        query heads together; entries past a cache's length stay. The caller clears the
+        row of a new request. A tick's weights pass through memory of the batch, so calls of
+        one such batch are not run on two streams at once."""
+        self._validate_handles(handles)
+        form = self._attention_form(handles, query_lens, window, sinks, weights)
         q_lens = self.reserve_tick(handles, query_lens)
         return PagedKVBatch(
             self, q_lens, [h.length for h in handles], [list(h.pages) for h in handles],
             varlen=True, num_q_heads=self.num_q_heads,
             tokens_per_split=self.tokens_per_split,
-            first_positions=self._first_positions(handles),
+            first_positions=self._first_positions(handles), **form,
         )
 
     def reserve_tick(self, handles: Sequence[PagedCacheHandle],

@@ -1,0 +1,161 @@
+"""Host side of windowed and weighed attention, without a GPU: the planners' lists against the
+definition, token by token, and the refusals of the entry points."""
+
+import numpy as np
+import pytest
+import torch
+
+from hayate_amd import PagedKVCacheManager, _native
+
+
+def keys_of(first_pos, window, sinks, unit):
+    """(ns, gap) of a range of rows from first_pos on, from the definition."""
+    low = max(0, first_pos - window + 1)
+    ns = -(-sinks // unit) * unit
+    gap = max(0, low // unit * unit - ns)
+    return ns, gap
+
+
+def in_sight(pos, window, sinks):
+    return {j for j in range(pos + 1) if pos - j < window or j < sinks}
+
+
+CASES = [(1, 0), (1, 5), (33, 1), (64, 64), (100, 31), (500, 4), (10_000, 0), (2**31 - 1, 3),
+         (7, 2**30)]
+
+
+@pytest.mark.parametrize("window,sinks", CASES)
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (8, 8), (16, 1)])
+def test_every_key_in_sight_is_planned_once(window, sinks, hq, hkv):
+    rng = np.random.default_rng(window % 1000 + sinks % 1000)
+    q = np.array([1, 1, 1, 1, 2, 70, 130, 1, 33, 1], dtype=np.int32)
+    kv = q + np.concatenate([[0, 30, 31, 1500], rng.integers(0, 900, 6)]).astype(np.int32)
+    plan = _native.plan_tick(q, kv, hq, hkv, 128, 256, 0, window, sinks)
+    pieces = plan.decode[plan.n_chunks :]
+    for b in np.flatnonzero(q == 1):
+        ns, gap = keys_of(kv[b] - 1, window, sinks, 32)
+        of = pieces[pieces[:, 0] == b]
+        numbers = [x for p in of for x in range(p[1], p[2])]
+        assert numbers == list(range(kv[b] - gap))  # in order, without a hole
+        keys = [x if x < ns else x + gap for x in numbers]
+        sight = in_sight(kv[b] - 1, window, sinks)
+        assert sight <= set(keys)
+        assert max(keys) == kv[b] - 1 and len(set(keys)) == len(keys)
+        # a slice of 32 without a key in sight would leave a wave without a maximum
+        for p in of:
+            for x in range(p[1], p[2], 32):
+                assert sight & {y if y < ns else y + gap for y in range(x, min(x + 32, p[2]))}
+        assert of[-1][7] == 1 and not of[:-1, 7].any() and (of[:, 6] == kv[b] - 1).all()
+    for b in np.flatnonzero(q > 1):
+        cache = kv[b] - q[b]
+        of = plan.prefill[plan.prefill[:, 0] == b]
+        for q0, q1 in {(x[1], x[2]) for x in of.tolist()}:
+            ns, gap = keys_of(cache + q0, window, sinks, 64)
+            ranges = sorted((x[3], x[4]) for x in of.tolist() if x[1] == q0)
+            assert ranges[0][0] == 0 and ranges[-1][1] == cache + q1 - gap
+            assert all(a[1] == z[0] and z[0] % 64 == 0 for a, z in zip(ranges, ranges[1:]))
+            sight = set().union(*(in_sight(cache + t, window, sinks) for t in range(q0, q1)))
+            keys = {x if x < ns else x + gap for x in range(cache + q1 - gap)}
+            assert sight <= keys and max(keys) == cache + q1 - 1
+        tokens = sorted({t for x in of for t in range(x[1], x[2])})
+        assert tokens == list(range(q[b]))
+
+
+def test_a_plan_without_a_window_is_the_plan_of_a_wide_one():
+    q, kv = np.array([1, 40, 1, 300]), np.array([700, 900, 1, 300])
+    a = _native.plan_tick(q, kv, 32, 8, 128, 256)
+    b = _native.plan_tick(q, kv, 32, 8, 128, 256, 0, 1000, 0)
+    for name in ("decode", "merge", "prefill", "prefill_merge"):
+        assert np.array_equal(getattr(a, name), getattr(b, name))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (-1, 0), (1, -1), (1, 2**30 + 1)])
+def test_the_planner_refuses(window, sinks):
+    with pytest.raises(ValueError):
+        _native.plan_tick(np.array([1]), np.array([5]), 32, 8, 128, 256, 0, window, sinks)
+
+
+@pytest.mark.parametrize("hq,hkv,cus", [(32, 8, 256), (8, 8, 4), (16, 1, 256), (1, 1, 1)])
+def test_weigh_lists_cover_every_pair_once(hq, hkv, cus):
+    rng = np.random.default_rng(hq + cus)
+    q = np.array([1, 2, 300, 1, 512, 17, 1], dtype=np.int32)
+    kv = q + rng.integers(0, 900, len(q)).astype(np.int32)
+    rows = np.array([4, 0, 2, 9, 1, 3, 7], dtype=np.int32)
+    p = _native.plan_weigh(q, kv, rows, hq, hkv, cus)
+    start = np.cumsum(q) - q
+    taken = np.zeros(p.scores, dtype=bool)
+    for b in range(len(q)):
+        adds = p.adds[p.adds[:, 0] == rows[b]]
+        assert [t for a in adds for t in range(a[1], a[2])] == list(range(kv[b]))
+        assert (adds[:, 2] - adds[:, 1] <= 256).all() and (adds[:, 1] % 256 == 0).all()
+        if q[b] == 1:
+            assert (adds[:, 3] == hq).all() and (adds[:, 4] == 0).all()
+            assert (adds[:, 5] == start[b]).all() and (adds[:, 6] == p.score_start[b]).all()
+            assert p.score_start[b] % 4 == 0
+            # whole slices of 32 scores, none of another sequence's
+            room = slice(p.score_start[b], p.score_start[b] + -(-kv[b] // 32) * 32)
+            assert room.stop <= p.scores and not taken[room].any()
+            taken[room] = True
+            continue
+        cache = kv[b] - q[b]
+        items = p.items[p.items[:, 0] == b]
+        assert (items[:, 5] == start[b]).all() and (items[:, 6] == cache).all()
+        assert len({x for x in items[:, 7]}) == 1 and (adds[:, 6] == items[0, 7]).all()
+        for a in adds:
+            of = items[items[:, 1] == a[1]]
+            # the parts that the addition reads, and each of them written
+            assert a[4] == of[0, 4] * hkv and a[3] == len(of) * hkv and a[5] == -1
+            assert [x for x in of[:, 4]] == list(range(of[0, 4], of[0, 4] + len(of)))
+            assert of[-1, 4] < p.parts and of[0, 7] + a[1] + 256 <= p.partials
+            tokens = [t for x in of for t in range(x[2], x[3])]
+            assert tokens == list(range(tokens[0], q[b]))
+            # tokens before them see none of the block's keys
+            assert tokens[0] == 0 or cache + tokens[0] - 1 < a[1]
+
+
+def manager(**kw):
+    return PagedKVCacheManager(2, 8, 128, 1024, 128, 4, torch.bfloat16, "cpu", num_q_heads=32, **kw)
+
+
+def test_refusals_of_a_tick():
+    m = manager()
+    h = m.allocate()
+    good = torch.zeros(4, 200)
+    for kw, error in [
+        ({"window": 0}, ValueError), ({"window": -3}, ValueError), ({"window": 2.0}, TypeError),
+        ({"window": True}, TypeError), ({"window": 5, "sinks": -1}, ValueError),
+        ({"window": 5, "sinks": 1.5}, TypeError), ({"sinks": 4}, ValueError),
+        ({"window": 5, "weights": good}, NotImplementedError),
+        ({"weights": good.double()}, TypeError), ({"weights": [[0.0]]}, TypeError),
+        ({"weights": torch.zeros(200)}, ValueError), ({"weights": torch.zeros(0, 200)}, ValueError),
+        ({"weights": torch.zeros(4, 2)}, ValueError),
+        ({"weights": torch.zeros(200, 4).T}, ValueError),
+        ({"weights": torch.zeros(1, 200).expand(4, 200)}, ValueError),
+        ({"weights": torch.zeros(4, 200, requires_grad=True)}, ValueError),
+    ]:
+        for begin in (lambda: m.begin_tick([h], [3], **kw), lambda: m.begin_batch([h], 3, **kw)):
+            with pytest.raises(error):
+                begin()
+        assert not h.pages, kw  # nothing is reserved for a refused tick
+    for _ in range(2):
+        other = m.allocate()
+    with pytest.raises(ValueError, match="slot"):
+        m.begin_tick([other], [1], weights=torch.zeros(2, 200))
+    m16 = PagedKVCacheManager(1, 8, 128, 256, 128, 1, torch.float16, "cpu", num_q_heads=32)
+    with pytest.raises(TypeError):
+        m16.begin_tick([m16.allocate()], [1], weights=good)
+
+
+def test_a_tick_with_a_form_of_its_own():
+    m = manager()
+    h = m.allocate()
+    batch = m.begin_tick([h], [3], window=7, sinks=2)
+    assert (batch.window, batch.sinks, batch.weights) == (7, 2, None)
+    batch = m.begin_batch([h], 3, window=10**12)
+    assert batch.window == m.capacity_tokens
+    weights = torch.zeros(4, 200)
+    assert m.begin_tick([h], [1], weights=weights).weights is weights
+    batch = m.begin_tick([h], [1])
+    assert batch.window is None and batch.weights is None
+    with pytest.raises(NotImplementedError):
+        m.begin_tick([h], [1], window=3).decode_layer(0, *[None] * 8, no_alloc=True)
