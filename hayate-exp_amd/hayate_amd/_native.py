@@ -188,6 +188,16 @@ _SIGNATURES = {
          _I64, _I32, _I32, _I32, _I32, _F32, _P],
         ctypes.c_int,
     ),
+    "hy_keep_positions": (
+        [_P, _I64, _P, _P, _I32, _I32, _I32, _I32, _P, _P],
+        ctypes.c_int,
+    ),
+    "hy_verify_workspace_bytes": ([_I32, _I32, _I32], ctypes.c_int64),
+    "hy_verify_tree": (
+        [_P, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _I64, _P, _I32, _P, _P, _P, _P,
+         _I64, _P],
+        ctypes.c_int,
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -840,15 +840,19 @@ class PagedTreeBatch(PagedKVBatch):
         roots = cache_lens_host if first_positions is None else first_positions
         positions = depths + np.repeat(np.asarray(roots, dtype=np.int32), q_lens)
         self._tree_plans: dict[int, _DeviceTreePlan] = {}
+        packed = np.concatenate(self.parents).astype(np.int32)
         super().__init__(manager, q_lens, cache_lens_host, page_lists, varlen=True,
                          num_q_heads=None,
-                         extra=np.concatenate([lines.reshape(-1).view(np.int32), positions]))
+                         extra=np.concatenate([lines.reshape(-1).view(np.int32), positions, packed]))
         # every tree goes through the tree kernel, requests with one node included
         self.decode_only = False
         self.lines = self._extra[: lines.size]
         self._lines_ptr = self.lines.data_ptr()
         # (by depth, so a wide tree needs fewer rope positions than its slots)
-        self._rotate_at(self._extra[lines.size :], positions)
+        at = lines.size + len(positions)
+        self._rotate_at(self._extra[lines.size : at], positions)
+        self.packed_parents = self._extra[at:]  # of every node, in its request
+        self.levels = int(depths.max()) + 1
         if num_q_heads is not None and self.device.type == "cuda":
             self.plan(num_q_heads)
 
@@ -1400,9 +1404,14 @@ class PagedKVCacheManager:
         kept = _int_array(keep, "keep")
         if len(kept) and (kept[0] < 0 or kept[-1] >= handle.length or (np.diff(kept) <= 0).any()):
             raise ValueError("keep must be ascending positions within the cache's length")
-        positions = None
         if len(kept) and kept[-1] != len(kept) - 1:
             self.move_tokens([handle], [kept], [0])
+        self._keep(handle, kept)
+
+    def _keep(self, handle: PagedCacheHandle, kept: np.ndarray) -> None:
+        """The handle's side of ``compact``, once the tokens have moved."""
+        positions = None
+        if len(kept) and kept[-1] != len(kept) - 1:
             positions = kept.copy()
         if handle.positions is not None:
             old = handle.positions
@@ -1410,6 +1419,62 @@ class PagedKVCacheManager:
             positions = positions_below(np.concatenate([old, after])[kept], len(kept))
         self._set_length(handle, len(kept))
         handle.positions = positions
+
+    # ------------------------------------------------------------- eviction
+    def keep_positions(self, handles: Sequence[PagedCacheHandle], weights: torch.Tensor,
+                       budget: int, *, sinks: int = 4, recent: int = 32) -> torch.Tensor:
+        """The positions that stay when every handle's cache is cut to `budget` tokens: its
+        first `sinks`, its last `recent`, and of those between the ones with the largest
+        weights[handle.slot] (as ``begin_tick`` adds them up; equal ones by their
+        position, NaN as the largest). int32 (handles, budget), ascending; a cache of at most
+        `budget` tokens keeps all, followed by -1."""
+        handles = list(handles)
+        if any(h.released for h in handles):
+            raise RuntimeError("cannot choose tokens of a released cache handle")
+        budget, sinks, recent = (_index(budget, "budget"), _index(sinks, "sinks"),
+                                 _index(recent, "recent"))
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError("budget must be positive and hold the first and the last tokens")
+        _require_hip(self.k_cache, "keep_positions")
+        if not handles:
+            return torch.empty((0, budget), dtype=torch.int32, device=self.device)
+        self._check_weights(weights, [h.slot for h in handles], [h.length for h in handles])
+        rows = np.array([[h.slot for h in handles], [h.length for h in handles]], dtype=np.int32)
+        out = torch.empty((len(handles), budget), dtype=torch.int32, device=self.device)
+        with _current_device(self.device):
+            rc = _native.lib().hy_keep_positions(
+                weights.data_ptr(), weights.stride(0), rows.ctypes.data,
+                rows.ctypes.data + rows.strides[0], len(handles), budget, sinks, recent,
+                out.data_ptr(), _stream_handle(self.device),
+            )
+        _native.check(rc, "hy_keep_positions")
+        return out
+
+    def evict(self, handles: Sequence[PagedCacheHandle], weights: torch.Tensor, budget: int, *,
+              sinks: int = 4, recent: int = 32) -> list[list[int]]:
+        """Cut every handle's cache to `budget` tokens, those of ``keep_positions``: their K and
+        V move up in every layer, as does their weight in the handle's row of `weights` (the
+        rest of the row is cleared), the emptied pages return, and the next token follows the
+        last kept one (as after ``compact``). Returns the kept positions. Waits for the GPU:
+        pages are bookkept on the host. All handles, or with an exception none, are cut."""
+        handles = list(handles)
+        if len({id(h) for h in handles}) != len(handles):
+            raise ValueError("the same cache handle is given twice")
+        if handles and not self._rows_of_256_bytes():
+            raise NotImplementedError("evict moves rows of 128 two-byte values")
+        chosen = self.keep_positions(handles, weights, budget, sinks=sinks, recent=recent)
+        kept = [row[: min(budget, h.length)] for h, row in zip(handles, chosen.tolist())]
+        cut = [(h, at, row) for h, at, row in zip(handles, chosen, kept) if len(row) < h.length]
+        if not cut:
+            return kept
+        self.move_tokens([h for h, _, _ in cut], [row for _, _, row in cut], [0] * len(cut))
+        for h, at, row in cut:
+            self._keep(h, np.asarray(row, dtype=np.int64))
+        with torch.inference_mode():  # (a table made under it takes no other updates)
+            rows = torch.tensor([h.slot for h, _, _ in cut], device=self.device)
+            moved = weights[rows[:, None], torch.stack([at for _, at, _ in cut]).long()]
+            weights[rows] = torch.nn.functional.pad(moved, (0, weights.shape[1] - budget))
+        return kept
 
     # ---------------------------------------------------------- drafted trees
     def begin_tree(self, handles: Sequence[PagedCacheHandle],

@@ -26,6 +26,7 @@ import numpy as np
 import torch
 
 from . import _native, linear
+from .paged_cache import PagedTreeBatch
 
 
 def validate_parameters(temperature, top_k, top_p) -> None:
@@ -148,6 +149,101 @@ def _sample_native(logits, temperature, top_k, top_p, generator):
     return out
 
 
+def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tensor,
+                temperature: Sequence[float], top_k: Sequence[Optional[int]],
+                top_p: Sequence[Optional[float]], uniforms: torch.Tensor,
+                draft_probs: Optional[torch.Tensor] = None,
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens of a ``begin_tree`` batch stand, and each request's next token, so
+    that both are distributed as tokens sampled one by one from the target.
+
+    Every tree has one root, node 0: the request's last token, which is not cached yet. logits
+    (nodes, vocab), or (nodes, 1, vocab) as Qwen3Model returns them, 16-bit; tokens (nodes,)
+    int64; both packed as the batch. temperature, top_k and top_p have an entry per request, as
+    for ``sample_batch``. uniforms: fp32 (nodes + requests,) of [0, 1), a number for every
+    node's test and one for every request's draw.
+
+    Without draft_probs the drafts are taken as given, a node's children tried in index
+    order: child x stands if u (1 - R) < p(x), R the mass of its refused earlier siblings' tokens;
+    where none stands, the next token is drawn from p without the refused tokens. draft_probs
+    (nodes, vocab) fp32 are the distributions that the nodes' tokens were drawn from (a root's
+    row is not read); then no node may have two children, x stands if u q(x) < p(x), and the
+    draw is from max(p - q, 0). At temperature 0 a child stands if it is the first largest
+    logit's token, which is also the next token.
+
+    Returns paths (requests, levels) int32, nodes from node 0 on, then -1: what
+    ``commit_tree`` takes once cut to its length; lengths (requests,) int32, at least 1; and the
+    next tokens (requests, 1) int64. Enqueues only; a row on a path that holds NaN or has no
+    finite maximum fails a device-side assertion, as in ``sample_batch``."""
+    if not isinstance(batch, PagedTreeBatch):
+        raise TypeError("verify_tree takes a begin_tree batch")
+    n, requests = batch.total_tokens, batch.num_seqs
+    if not len(temperature) == len(top_k) == len(top_p) == requests:
+        raise ValueError("one temperature, top_k and top_p per request is required")
+    for t, k, p in zip(temperature, top_k, top_p):
+        validate_parameters(t, k, p)
+        if t and not 1e-30 <= t <= 1e30:
+            raise ValueError("verification takes temperatures of 0 or 1e-30 to 1e30")
+    for parents in batch.parents:
+        if (parents[1:] < 0).any():
+            raise ValueError("a tree to verify has one root, node 0")
+        if draft_probs is not None and len(np.unique(parents)) != len(parents):
+            raise NotImplementedError("with draft_probs a node has at most one child")
+    if logits.dim() == 3 and logits.shape[1] == 1:
+        logits = logits[:, 0]
+    if logits.dtype not in _DTYPES:
+        raise TypeError("logits must be bfloat16 or float16")
+    if logits.dim() != 2 or logits.shape[0] != n or not 0 < logits.shape[1] <= MAX_VOCAB:
+        raise ValueError(f"logits must be ({n} nodes, vocab), vocab at most {MAX_VOCAB}")
+    vocab = logits.shape[1]
+    if tokens.dtype != torch.int64 or uniforms.dtype != torch.float32:
+        raise TypeError("tokens must be int64, uniforms float32")
+    if tokens.shape != (n,) or uniforms.shape != (n + requests,):
+        raise ValueError(f"tokens must be ({n},), uniforms ({n + requests},)")
+    given = [logits, tokens, uniforms]
+    if draft_probs is not None:
+        if draft_probs.dtype != torch.float32:
+            raise TypeError("draft_probs must be float32")
+        if draft_probs.shape != (n, vocab):
+            raise ValueError(f"draft_probs must be ({n}, {vocab})")
+        given.append(draft_probs)
+    if any(t.device != batch.device for t in given):
+        raise ValueError(f"logits, tokens and uniforms must be on the pool's device, {batch.device}")
+    if batch.device.type != "cuda":
+        raise RuntimeError("verify_tree runs only on a HIP device; there is no CPU implementation")
+    if torch.cuda.current_device() != batch.device.index:
+        with torch.cuda.device(batch.device):
+            return verify_tree(batch, logits, tokens, temperature, top_k, top_p, uniforms,
+                               draft_probs)
+    logits, tokens, uniforms = (t if t.stride(-1) == 1 else t.contiguous()
+                                for t in (logits, tokens, uniforms))
+    if draft_probs is not None and draft_probs.stride(1) != 1:
+        draft_probs = draft_probs.contiguous()
+    dev, lib = batch.device, _native.lib()
+    temp = np.asarray(list(map(float, temperature)), dtype=np.float32)
+    k = np.asarray([vocab if v is None else min(v, vocab) for v in top_k], dtype=np.int32)
+    p = np.asarray([1.0 if v is None else max(float(v), _TINY) for v in top_p], dtype=np.float32)
+    q_lens = np.asarray(batch.q_lens, dtype=np.int32)
+    paths = torch.empty((requests, batch.levels), dtype=torch.int32, device=dev)
+    lengths = torch.empty(requests, dtype=torch.int32, device=dev)
+    drawn = torch.empty((requests, 1), dtype=torch.int64, device=dev)
+    valid = torch.empty((), dtype=torch.bool, device=dev)
+    work = torch.empty(lib.hy_verify_workspace_bytes(n, requests, vocab), dtype=torch.uint8,
+                       device=dev)
+    rc = lib.hy_verify_tree(
+        logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], vocab,
+        batch.packed_parents.data_ptr(), tokens.data_ptr(), q_lens.ctypes.data, requests,
+        temp.ctypes.data, k.ctypes.data, p.ctypes.data, uniforms.data_ptr(),
+        None if draft_probs is None else draft_probs.data_ptr(),
+        0 if draft_probs is None else draft_probs.stride(0), paths.data_ptr(), batch.levels,
+        lengths.data_ptr(), drawn.data_ptr(), valid.data_ptr(), work.data_ptr(), work.numel(),
+        batch._stream())
+    _native.check(rc, "hy_verify_tree")
+    if temp.any():
+        torch._assert_async(valid, "logits hold NaN or have no finite maximum")
+    return paths, lengths, drawn
+
+
 class Sampler:
     """Samples the next token of each request (sampler.py:8-93)."""
 
@@ -169,6 +265,20 @@ class Sampler:
         return sample_batch(logits, [r.temperature for r in requests],
                             [r.top_k for r in requests], [r.top_p for r in requests],
                             self.generator)
+
+    def verify(self, logits: torch.Tensor, tokens: torch.Tensor, batch: PagedTreeBatch, requests,
+               draft_probs: Optional[torch.Tensor] = None) -> tuple[list[list[int]], list[int]]:
+        """``verify_tree`` with the requests' own settings and numbers of this sampler's
+        generator: each request's path, as ``commit_tree`` takes it, and its next token."""
+        if len(requests) != batch.num_seqs:
+            raise ValueError("verification takes one request per tree")
+        uniforms = torch.rand(batch.total_tokens + batch.num_seqs, generator=self.generator,
+                              device=batch.device)
+        paths, lengths, drawn = verify_tree(
+            batch, logits, tokens, [r.temperature for r in requests],
+            [r.top_k for r in requests], [r.top_p for r in requests], uniforms, draft_probs)
+        got = torch.cat([lengths[:, None].long(), drawn, paths.long()], 1).tolist()
+        return [row[2 : 2 + row[0]] for row in got], [row[1] for row in got]
 
     def finalize(self, request, tok: int) -> None:
         request.tokens.append(tok)

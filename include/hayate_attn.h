@@ -700,6 +700,58 @@ int hy_token_weights(
     int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale,
     void *stream);
 
+/*
+ * Which tokens stay when caches are cut to `budget`: of sequence b with
+ * lens[b] > budget the first `sinks`, the last `recent` and, of those between,
+ * the ones with the largest weights[rows[b] * weights_stride + j] (fp32), equal
+ * ones by their position; NaN counts as the largest. out gets `budget` int32
+ * positions a sequence, ascending; a sequence of at most `budget` tokens keeps
+ * all, followed by -1. rows and lens are host arrays (lens at most 2^30).
+ * No reference counterpart.
+ */
+int hy_keep_positions(const float *weights, int64_t weights_stride,
+                      const int32_t *rows, const int32_t *lens,
+                      int32_t num_seqs, int32_t budget, int32_t sinks,
+                      int32_t recent, int32_t *out, void *stream);
+
+/*
+ * Verification of trees of drafted tokens against the target's probabilities.
+ * logits: a row of `vocab` 16-bit values (dtype 0: bf16, 1: fp16) per node,
+ * packed by request; parents (int32) and tokens (int64) likewise, on the
+ * device. Node 0 of a request is its last token, taken as it is; every other
+ * node's parent is an earlier one. temperature, top_k (>= vocab: none) and top_p
+ * (>= 1: none) are host arrays with an entry per request, as for hy_sample.
+ * uniforms: fp32 of [0, 1), one per node, then one per request (of roots and
+ * greedy requests they are not used).
+ * From node 0 on, the first child x in index order is taken for which
+ * u (1 - R) < p(x), p being the softmax of the node's logits over the
+ * temperature, cut by top-k and top-p, and R its mass in the refused earlier
+ * siblings' tokens, which count as 0 from then on; where none is, the next
+ * token is the first whose cumulative p without the refused tokens exceeds u
+ * times their total. With draft_probs (fp32 rows of draft_stride, row of
+ * node i the distribution its token was drawn from; at most one child a node)
+ * x is taken where u q(x) < p(x), and drawn from max(p - q, 0) otherwise. At
+ * temperature 0 x is taken where it is the first largest logit's token.
+ * Results: paths (int32, `levels` a request: its nodes from node 0 on, then
+ * -1), lengths, next_tokens, and *valid = 0 if a row on some path holds NaN or
+ * has no finite maximum (its request then draws token 0). Tokens outside the
+ * vocabulary are refused. Probabilities are those of 32-bit sums, the masses a
+ * draw goes through are summed in 64.
+ * Workspace: hy_verify_workspace_bytes(nodes in all, num_seqs, vocab).
+ * No reference counterpart: the reference decodes one token at a time.
+ */
+int64_t hy_verify_workspace_bytes(int32_t n_rows, int32_t num_seqs,
+                                  int32_t vocab);
+int hy_verify_tree(const void *logits, int64_t row_stride, int32_t dtype,
+                   int32_t vocab, const int32_t *parents,
+                   const int64_t *tokens, const int32_t *q_lens,
+                   int32_t num_seqs, const float *temperature,
+                   const int32_t *top_k, const float *top_p,
+                   const float *uniforms, const float *draft_probs,
+                   int64_t draft_stride, int32_t *paths, int32_t levels,
+                   int32_t *lengths, int64_t *next_tokens, uint8_t *valid,
+                   void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
