@@ -52,6 +52,7 @@
 
 #include <mutex>
 
+#include "attend.h"
 #include "decode_shape.h"
 #include "hy_common.h"
 #include "qknorm.h"
@@ -230,9 +231,11 @@ struct Piece {
   int ns, gap, low;  // with a window: its keys, and the first number in sight behind the sinks
 };
 
+static_assert(kWindowUnit == kSlice, "a slice lies on one side of the keys left out");
+
 // Adds the window's part to piece x, whose sequence's token is at position pos.
 __device__ __forceinline__ void set_window(Piece &x, int pos, int window, int sinks) {
-  const WindowKeys w = window_keys<kSlice>(pos, window, sinks);
+  const WindowKeys w = window_keys(pos, window, sinks);
   x.ns = w.ns;
   x.gap = w.gap;
   x.low = pos - window + 1 - w.gap;
@@ -271,6 +274,8 @@ struct DecodeExtra {
   int64_t score_stride;
 };
 
+}  // namespace
+
 // Inputs of the fused append (hy_paged_decode_append): the raw q, k, v
 // projections of the step's tokens, the norm weights and rope tables. The
 // kernel's q then points at the raw q rows.
@@ -287,6 +292,8 @@ struct AppendArgs {
   int max_pos;  // rows of cos_t / sin_t
   const int32_t *cache_lens;
 };
+
+namespace {
 
 // Two waves per SIMD: the double-buffered slice registers need about 240
 // VGPRs.
@@ -859,95 +866,69 @@ extern "C" int hy_paged_decode_merge(void *out, int64_t o_stride_seq, int64_t o_
                            workspace_bytes, num_q_heads, head_dim, stream);
 }
 
-namespace {
-
-int check_window(const char *name, int32_t window, int32_t sinks) {
-  HY_REQUIRE(window >= 1 && sinks >= 0 && sinks <= hy::kMaxSinks,
-             "%s: window %d (at least 1), sinks %d (0 to %d)", name, window, sinks, hy::kMaxSinks);
+int hy::check_window(const char *name, const Window &w) {
+  HY_REQUIRE(w.window >= 1 && w.sinks >= 0 && w.sinks <= kMaxSinks,
+             "%s: window %d (at least 1), sinks %d (0 to %d)", name, w.window, w.sinks, kMaxSinks);
   return HY_OK;
 }
 
-}  // namespace
-
-extern "C" int hy_paged_decode_window(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head, void *out,
-    const void *k_pool, const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start, const int32_t *decode_items,
-    int32_t n_decode, int32_t n_slots, void *workspace, int64_t workspace_bytes,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t page_size, float scale, int32_t window, int32_t sinks, void *stream) {
-  hy::clear_error();
-  if (int rc = check_window("hy_paged_decode_window", window, sinks)) return rc;
-  const hy::DecodeExtra ex{window, sinks, nullptr, nullptr, 0};
-  return paged_decode_impl("hy_paged_decode_window", q, q_stride_seq, q_stride_tok, q_stride_head,
-                           out, k_pool, v_pool, pool_head_stride, page_table, page_table_stride,
-                           q_start, decode_items, n_decode, n_slots, workspace, workspace_bytes,
-                           num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
-                           stream, nullptr, &ex);
+int hy::decode(const char *name, const Rows &q, const Rows &out, const Pools &pools,
+               const int32_t *q_start, const Items &items, const Workspace &ws, const Shape &s,
+               const Window &window, const Scores &scores, const AppendArgs *append,
+               void *stream) {
+  HY_REQUIRE(scores.at == nullptr ||
+                 (scores.start && (reinterpret_cast<uintptr_t>(scores.at) & 15) == 0 &&
+                  scores.stride >= 0 && scores.stride % 4 == 0),
+             "%s: score rows lie on 16 bytes", name);
+  const DecodeExtra ex{window.window, window.sinks, scores.at, scores.start, scores.stride};
+  const bool extra = window.window > 0 || scores.at;
+  return paged_decode_impl(name, q.at, q.seq, q.tok, q.head, out.at, pools.k, pools.v,
+                           pools.head_stride, pools.page_table, pools.page_table_stride, q_start,
+                           items.at, items.count, items.slots, ws.at, ws.bytes, s.num_seqs,
+                           s.num_q_heads, s.num_kv_heads, s.head_dim, s.page_size, s.scale, stream,
+                           append, extra ? &ex : nullptr);
 }
 
-extern "C" int hy_paged_decode_append_window(
+int hy::decode_merge(const char *name, const Rows &out, const int32_t *q_start, const Items &items,
+                     const Workspace &ws, const Shape &s, float *row_ml, void *stream) {
+  return decode_merge_impl(name, out.at, out.seq, out.tok, out.head, q_start, items.at, items.count,
+                           items.slots, ws.at, ws.bytes, s.num_q_heads, s.head_dim, stream, row_ml);
+}
+
+extern "C" int hy_paged_window_append(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
     void *q_out, int64_t qo_stride_seq, int64_t qo_stride_tok, int64_t qo_stride_head,
     const void *k, int64_t k_stride_seq, int64_t k_stride_tok, int64_t k_stride_head,
     const void *v, int64_t v_stride_seq, int64_t v_stride_tok, int64_t v_stride_head,
     const void *q_norm_weight, const void *k_norm_weight, float q_eps, float k_eps,
     const float *cos_table, const float *sin_table, int32_t max_positions, void *out,
-    void *k_pool, void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start, const int32_t *cache_lens,
-    const int32_t *decode_items, int32_t n_decode, int32_t n_slots, void *workspace,
-    int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, int32_t page_size, float scale, int32_t window, int32_t sinks,
-    void *stream) {
+    int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head, void *k_pool, void *v_pool,
+    int64_t pool_head_stride, const int32_t *page_table, int64_t page_table_stride,
+    const int32_t *q_start, const int32_t *cache_lens, const int32_t *decode_items,
+    int32_t n_decode, const int32_t *merge_items, int32_t n_merge, int32_t n_slots,
+    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, int32_t window,
+    int32_t sinks, void *stream) {
+  const char *name = "hy_paged_window_append";
   hy::clear_error();
-  if (int rc = check_window("hy_paged_decode_append_window", window, sinks)) return rc;
+  const hy::Window w{window, sinks};
+  if (int rc = hy::check_window(name, w)) return rc;
   hy::AppendArgs ap;
-  if (int rc = fill_append_args("hy_paged_decode_append_window", ap, q_out, qo_stride_seq,
-                                qo_stride_tok, qo_stride_head, k, k_stride_seq, k_stride_tok,
-                                k_stride_head, v, v_stride_seq, v_stride_tok, v_stride_head,
-                                q_norm_weight, k_norm_weight, q_eps, k_eps, cos_table,
-                                sin_table, max_positions, cache_lens))
+  if (int rc = fill_append_args(name, ap, q_out, qo_stride_seq, qo_stride_tok, qo_stride_head, k,
+                                k_stride_seq, k_stride_tok, k_stride_head, v, v_stride_seq,
+                                v_stride_tok, v_stride_head, q_norm_weight, k_norm_weight, q_eps,
+                                k_eps, cos_table, sin_table, max_positions, cache_lens))
     return rc;
-  const hy::DecodeExtra ex{window, sinks, nullptr, nullptr, 0};
-  return paged_decode_impl("hy_paged_decode_append_window", q, q_stride_seq, q_stride_tok,
-                           q_stride_head, out, k_pool, v_pool, pool_head_stride, page_table,
-                           page_table_stride, q_start, decode_items, n_decode, n_slots,
-                           workspace, workspace_bytes, num_seqs, num_q_heads, num_kv_heads,
-                           head_dim, page_size, scale, stream, &ap, &ex);
-}
-
-extern "C" int hy_paged_decode_weigh(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head, void *out,
-    const void *k_pool, const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start, const int32_t *decode_items,
-    int32_t n_decode, int32_t n_slots, void *workspace, int64_t workspace_bytes,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t page_size, float scale, float *scores, const int32_t *score_start,
-    int64_t score_stride, void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(n_decode == 0 || (scores && score_start), "hy_paged_decode_weigh: null pointer argument");
-  HY_REQUIRE((reinterpret_cast<uintptr_t>(scores) & 15) == 0 && score_stride >= 0 &&
-                 score_stride % 4 == 0,
-             "hy_paged_decode_weigh: score rows lie on 16 bytes");
-  const hy::DecodeExtra ex{0, 0, scores, score_start, score_stride};
-  return paged_decode_impl("hy_paged_decode_weigh", q, q_stride_seq, q_stride_tok, q_stride_head,
-                           out, k_pool, v_pool, pool_head_stride, page_table, page_table_stride,
-                           q_start, decode_items, n_decode, n_slots, workspace, workspace_bytes,
-                           num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
-                           stream, nullptr, &ex);
-}
-
-extern "C" int hy_paged_decode_merge_weigh(void *out, int64_t o_stride_seq, int64_t o_stride_tok,
-                                           int64_t o_stride_head, const int32_t *q_start,
-                                           const int32_t *merge_items, int32_t n_merge,
-                                           int32_t n_slots, const void *workspace,
-                                           int64_t workspace_bytes, int32_t num_q_heads,
-                                           int32_t head_dim, float *row_ml, void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(n_merge == 0 || row_ml, "hy_paged_decode_merge_weigh: null pointer argument");
-  return decode_merge_impl("hy_paged_decode_merge_weigh", out, o_stride_seq, o_stride_tok,
-                           o_stride_head, q_start, merge_items, n_merge, n_slots, workspace,
-                           workspace_bytes, num_q_heads, head_dim, stream, row_ml);
+  const hy::Rows rows{const_cast<void *>(q), q_stride_seq, q_stride_tok, q_stride_head};
+  const hy::Rows to{out, o_stride_seq, o_stride_tok, o_stride_head};
+  const hy::Workspace ws{workspace, workspace_bytes};
+  const hy::Shape shape{num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale};
+  if (int rc = hy::decode(name, rows, to, {k_pool, v_pool, pool_head_stride, page_table,
+                                           page_table_stride},
+                          q_start, {decode_items, n_decode, n_slots}, ws, shape, w, {}, &ap, stream))
+    return rc;
+  return hy::decode_merge(name, to, q_start, {merge_items, n_merge, n_slots}, ws, shape, nullptr,
+                          stream);
 }
 
 // ---------------------------------------------------------------------------

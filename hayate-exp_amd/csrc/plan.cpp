@@ -19,6 +19,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <array>
 #include <functional>
 #include <new>
 #include <queue>
@@ -178,11 +179,11 @@ int plan_tick(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs,
   }
   // Keys of a decode sequence's stream, and those a tile from token q0 on leaves out.
   auto decode_keys = [&](int b) {
-    return window > 0 ? kv_lens[b] - hy::window_keys<kSlice>(kv_lens[b] - 1, window, sinks).gap
+    return window > 0 ? kv_lens[b] - hy::window_keys(kv_lens[b] - 1, window, sinks).gap
                       : kv_lens[b];
   };
   auto tile_gap = [&](int32_t first_pos) {
-    return window > 0 ? hy::window_keys<kPrefillKeys>(first_pos, window, sinks).gap : 0;
+    return window > 0 ? hy::window_keys(first_pos, window, sinks).gap : 0;
   };
   int64_t decode_tokens = 0;
   for (int b = 0; b < num_seqs; ++b) {
@@ -856,10 +857,65 @@ extern "C" int hy_plan_tree(const int32_t *q_lens, const int32_t *kv_lens, int32
 
 namespace {
 
-// Rows (token, head) of a weigh item at least, and items a compute unit should get: more items
-// fill the GPU, each loads its 256 keys again. (Chosen by measurement, see weigh.hip.)
-constexpr int64_t kWeighMinRows = 256;
-constexpr int64_t kWeighPerCu = 4;
+// Weigh workgroups a compute unit holds, and what an item costs besides its row stages, in stages
+// (measured on MI355X, two a unit: 2.6 us a stage, about 5 us for the keys, the first rows and the
+// sums).
+constexpr int64_t kWeighPerCu = 2;
+constexpr double kWeighFixed = 2.0;
+// Items a slot beyond which no cut evens out more than it costs.
+constexpr int64_t kWeighItems = 6;
+
+// One sequence's chunk in row ranges ("parts") of equal length.
+struct WeighParts {
+  int64_t count, tokens;
+  WeighParts(int64_t ql, int64_t range) {
+    count = (ql + range - 1) / range;
+    tokens = (ql + count - 1) / count;
+    count = (ql + tokens - 1) / tokens;
+  }
+};
+
+// The range of tokens whose items, longest first, are done soonest.
+int64_t weigh_range(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_seqs, int64_t G,
+                    int64_t slots) {
+  constexpr int64_t keys = hy::kWeighKeys;
+  int64_t longest = 1;
+  for (int b = 0; b < num_seqs; ++b) longest = std::max<int64_t>(longest, q_lens[b]);
+  int64_t best_range = longest;
+  double best = HUGE_VAL;
+  std::vector<double> costs, free_at;
+  const int64_t least = std::max<int64_t>(1, hy::kWeighRows / G);  // one stage
+  for (int64_t n = 1; n <= 32; ++n) {
+    const int64_t range = (longest + n - 1) / n;
+    if (n > 1 && range < least) break;
+    costs.clear();
+    for (int b = 0; b < num_seqs; ++b) {
+      const int64_t ql = q_lens[b], cache = kv_lens[b] - ql;
+      if (ql <= 1) continue;
+      const WeighParts parts(ql, range);
+      for (int64_t t0 = 0; t0 < kv_lens[b]; t0 += keys)
+        for (int64_t p = t0 <= cache ? 0 : (t0 - cache) / parts.tokens; p < parts.count; ++p) {
+          const int64_t from = std::max(p * parts.tokens, t0 - cache);
+          const int64_t rows = (std::min(ql, (p + 1) * parts.tokens) - from) * G;
+          costs.push_back(kWeighFixed + static_cast<double>((rows + hy::kWeighRows - 1) / hy::kWeighRows));
+        }
+      if (n > 1 && static_cast<int64_t>(costs.size()) > kWeighItems * slots) return best_range;
+    }
+    std::sort(costs.begin(), costs.end(), std::greater<double>());
+    free_at.assign(static_cast<size_t>(slots), 0.0);
+    double end = 0;
+    for (double c : costs) {
+      std::pop_heap(free_at.begin(), free_at.end(), std::greater<double>());
+      end = std::max(end, free_at.back() += c);
+      std::push_heap(free_at.begin(), free_at.end(), std::greater<double>());
+    }
+    if (end < best) {
+      best = end;
+      best_range = range;
+    }
+  }
+  return best_range;
+}
 
 int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
                int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
@@ -868,20 +924,15 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
   constexpr int64_t keys = hy::kWeighKeys;
   const int64_t G = num_q_heads / num_kv_heads;
   const int64_t cus = num_cus > 0 ? num_cus : 256;
-  // row ranges of the same length for all chunks, as long as the GPU stays filled
-  int64_t tiles_rows = 0;
-  for (int b = 0; b < num_seqs; ++b)
-    if (q_lens[b] > 1) tiles_rows += (kv_lens[b] + keys - 1) / keys * q_lens[b] * G;
-  int64_t range = tiles_rows * num_kv_heads / (cus * kWeighPerCu);
-  range = std::max(kWeighMinRows, (range + hy::kWeighRows - 1) / hy::kWeighRows * hy::kWeighRows);
-  const int64_t range_tokens = std::max<int64_t>(1, range / G);
+  const int64_t slots =
+      std::max<int64_t>(1, (num_cus > 0 ? num_cus : 256) * kWeighPerCu / num_kv_heads);
+  const int64_t range = weigh_range(q_lens, kv_lens, num_seqs, G, slots);
   int64_t scores = 0, partials = 0, q_row = 0, n_items = 0, n_adds = 0, parts_max = 0;
   for (int b = 0; b < num_seqs; ++b) {
     const int64_t kv = kv_lens[b], ql = q_lens[b], cache = kv - ql;
     const bool chunk = ql > 1;
-    const int64_t parts = (ql + range_tokens - 1) / range_tokens;
-    const int64_t per = (ql + parts - 1) / parts;  // tokens of a part
-    const int64_t n_parts = (ql + per - 1) / per;
+    const WeighParts parts(ql, range);
+    const int64_t per = parts.tokens, n_parts = parts.count;
     score_start[b] = chunk ? 0 : static_cast<int32_t>(scores);
     for (int64_t t0 = 0; t0 < kv; t0 += keys) {
       // parts whose last token sees the first key
@@ -922,11 +973,19 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
       scores += (kv + hy::kWeighPad - 1) / hy::kWeighPad * hy::kWeighPad;
     }
     q_row += ql;
-    if (scores > INT32_MAX - 2 * keys || partials > INT32_MAX - 2 * keys || q_row > INT32_MAX) {
-      hy::set_error("hy_plan_weigh: too many keys in one batch");
+    if (scores > INT32_MAX - 2 * keys || partials > INT32_MAX - 2 * keys ||
+        q_row * num_q_heads > INT32_MAX) {
+      hy::set_error("hy_plan_weigh: too many keys or rows in one batch");
       return HY_EUNSUPPORTED;
     }
   }
+  // the longest first, as weigh_range() has them
+  std::vector<std::array<int32_t, 8>> order(static_cast<size_t>(n_items));
+  if (n_items > 0) std::copy_n(items, 8 * n_items, order[0].data());
+  auto tokens = [](const std::array<int32_t, 8> &x) { return x[3] - std::max(x[2], x[1] - x[6]); };
+  std::stable_sort(order.begin(), order.end(),
+                   [&](const auto &x, const auto &y) { return tokens(x) > tokens(y); });
+  for (size_t i = 0; i < order.size(); ++i) std::copy(order[i].begin(), order[i].end(), items + 8 * i);
   counts_out[0] = n_items;
   counts_out[1] = n_adds;
   counts_out[2] = scores;
@@ -966,6 +1025,11 @@ extern "C" int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, cons
       return HY_EINVAL;
     }
   }
-  return plan_weigh(q_lens, kv_lens, rows, num_seqs, num_q_heads, num_kv_heads, num_cus,
-                    score_start, items, item_capacity, adds, add_capacity, counts_out);
+  try {
+    return plan_weigh(q_lens, kv_lens, rows, num_seqs, num_q_heads, num_kv_heads, num_cus,
+                      score_start, items, item_capacity, adds, add_capacity, counts_out);
+  } catch (const std::bad_alloc &) {
+    hy::set_error("hy_plan_weigh: out of host memory");
+    return HY_ENOSPACE;
+  }
 }

@@ -71,13 +71,14 @@
 // scalar load.
 //
 // With a window (kWindow) an item's keys are the numbers of window.h for the tile's first
-// token, in units of the 64-key tile: a tile of numbers from ns on lies `gap` keys further.
+// token: the half of a tile whose numbers are from ns on lies `gap` keys further.
 // Blocks that hold a key between the sinks and some row's window are masked like those on the
 // diagonal. A masked key's V may be infinite or NaN, which 0 times is NaN: masked blocks are
 // looked through for such values on the way to the second product (see clean_v).
 
 #include <type_traits>
 
+#include "attend.h"
 #include "hy_common.h"
 #include "prefill_shape.h"
 #include "window.h"
@@ -214,7 +215,7 @@ void prefill_kernel(
   // with a window, positions of tokens count in the item's key numbers too
   int ns = 0, gap = 0;
   if constexpr (kWindow) {
-    const WindowKeys w = window_keys<kTile>(cache_len + q_begin, window, sinks);
+    const WindowKeys w = window_keys(cache_len + q_begin, window, sinks);
     ns = w.ns;
     gap = w.gap;
     cache_len -= gap;
@@ -314,7 +315,8 @@ void prefill_kernel(
   const int k_chunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
   const int v_chunk = 32 * (lane >> 4) + 8 * (lane & 3);
   auto issue_tile = [&](int kt, const Pages &pg, uint16_t *dst) __attribute__((always_inline)) {
-    const int far = kWindow && kt >= ns ? gap : 0;  // a tile lies on one side of ns
+    // (the rows of waves 0-3, and of 4-7, lie on one side of ns)
+    const int far = kWindow && kt + 32 * (wave >> 2) >= ns ? gap : 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int i = 2 * wave + j;
@@ -929,46 +931,6 @@ extern "C" int hy_paged_prefill(
                             0, 0, nullptr, stream);
 }
 
-extern "C" int hy_paged_prefill_window(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
-    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
-    const void *k_pool, const void *v_pool, int64_t pool_head_stride,
-    const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
-    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, int32_t window,
-    int32_t sinks, void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(window >= 1 && sinks >= 0 && sinks <= hy::kMaxSinks,
-             "hy_paged_prefill_window: window %d (at least 1), sinks %d (0 to %d)", window, sinks,
-             hy::kMaxSinks);
-  return paged_prefill_impl("hy_paged_prefill_window", q, q_stride_seq, q_stride_tok, q_stride_head, out,
-                            o_stride_seq, o_stride_tok, o_stride_head, k_pool, v_pool,
-                            pool_head_stride, page_table, page_table_stride, q_start, kv_lens,
-                            prefill_items, n_prefill, n_slots, workspace, workspace_bytes,
-                            num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
-                            window, sinks, nullptr, stream);
-}
-
-extern "C" int hy_paged_prefill_weigh(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
-    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
-    const void *k_pool, const void *v_pool, int64_t pool_head_stride,
-    const int32_t *page_table, int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill, int32_t n_slots,
-    void *workspace, int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale, float *row_ml,
-    void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(n_prefill == 0 || row_ml, "hy_paged_prefill_weigh: null pointer argument");
-  return paged_prefill_impl("hy_paged_prefill_weigh", q, q_stride_seq, q_stride_tok, q_stride_head, out,
-                            o_stride_seq, o_stride_tok, o_stride_head, k_pool, v_pool,
-                            pool_head_stride, page_table, page_table_stride, q_start, kv_lens,
-                            prefill_items, n_prefill, n_slots, workspace, workspace_bytes,
-                            num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, scale,
-                            0, 0, row_ml, stream);
-}
-
 namespace {
 
 int prefill_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t o_stride_tok,
@@ -1025,14 +987,21 @@ extern "C" int hy_paged_prefill_merge(
                             num_q_heads, num_kv_heads, head_dim, nullptr, stream);
 }
 
-extern "C" int hy_paged_prefill_merge_weigh(
-    void *out, int64_t o_stride_seq, int64_t o_stride_tok, int64_t o_stride_head,
-    const int32_t *q_start, const int32_t *merge_items, int32_t n_merge, int32_t n_slots,
-    const void *workspace, int64_t workspace_bytes, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, float *row_ml, void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(n_merge == 0 || row_ml, "hy_paged_prefill_merge_weigh: null pointer argument");
-  return prefill_merge_impl("hy_paged_prefill_merge_weigh", out, o_stride_seq, o_stride_tok, o_stride_head, q_start,
-                            merge_items, n_merge, n_slots, workspace, workspace_bytes,
-                            num_q_heads, num_kv_heads, head_dim, row_ml, stream);
+int hy::prefill(const char *name, const Rows &q, const Rows &out, const Pools &pools,
+                const int32_t *q_start, const int32_t *kv_lens, const Items &items,
+                const Workspace &ws, const Shape &s, const Window &window, float *row_ml,
+                void *stream) {
+  return paged_prefill_impl(name, q.at, q.seq, q.tok, q.head, out.at, out.seq, out.tok, out.head,
+                            pools.k, pools.v, pools.head_stride, pools.page_table,
+                            pools.page_table_stride, q_start, kv_lens, items.at, items.count,
+                            items.slots, ws.at, ws.bytes, s.num_seqs, s.num_q_heads,
+                            s.num_kv_heads, s.head_dim, s.page_size, s.scale, window.window,
+                            window.sinks, row_ml, stream);
+}
+
+int hy::prefill_merge(const char *name, const Rows &out, const int32_t *q_start, const Items &items,
+                      const Workspace &ws, const Shape &s, float *row_ml, void *stream) {
+  return prefill_merge_impl(name, out.at, out.seq, out.tok, out.head, q_start, items.at,
+                            items.count, items.slots, ws.at, ws.bytes, s.num_q_heads,
+                            s.num_kv_heads, s.head_dim, row_ml, stream);
 }

@@ -19,10 +19,15 @@
 //                 share of the logits (greedy: its largest logit).
 //   walk_kernel   the walk, in every workgroup of the request: its tests need the shares of its
 //                 rows and a logit a node, a few reads that all nodes make at once. Then the
-//                 masses of its share of the last node's row, in 64 bits: a border between
+//                 masses of its part of the last node's row, in 64 bits: a border between
 //                 two of 151,936 tokens is met by one draw in thousands of 32-bit sums.
-//   rest_kernel   (drafts drawn) the masses of max(p - q, 0).
-//   pick_kernel   the share that holds the draw, then the token.
+//   rest_kernel   (drafts drawn, one refused) the same of max(p - q, 0), whose p needs all of
+//                 the row's masses.
+//   pick_kernel   the part that holds the draw, then the token. (In the walk's last workgroup of
+//                 each request instead, the releases and acquires of all others took 20 us
+//                 more with 32 requests.)
+
+#include <algorithm>
 
 #include "logit_rows.h"
 
@@ -34,6 +39,12 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kShare = kThreads * kVec * kAhead;  // logits of a workgroup
 constexpr int kRequests = 64;                     // requests of one launch
 constexpr int kMaxNodes = 256;
+// The last row of a path goes to more workgroups, a load of logits a thread: its masses in 64 bits
+// take as long as one thread's chain of operations.
+constexpr int kPart = kThreads * kVec;
+// Workgroups of one walk launch, about: 16 trees of 26 nodes 12.0 us at 1024, 10.2 at 2048 and more
+// (a part each), 32 chains of 5 24.5, 15.0 and 16.5 at 256, 1024 and more.
+constexpr int kWalkers = 2048;
 
 struct Request {
   float temp;
@@ -75,7 +86,7 @@ struct Share {
   float max, sum;
   uint64_t best;
 };
-// Masses of a share of a request's last row: all of it, and what the draw is from.
+// Masses of a part of a request's last row: all of it, and what the draw is from.
 struct Mass {
   double all, left;
 };
@@ -94,12 +105,13 @@ struct Tree {
   int64_t drafts_ld;
 };
 
-// This thread's logits of a share: kAhead loads of kVec, load a from index first + a * step on.
+// This thread's logits of a share: loads of kVec, load a from index first + a * step on.
 // Past the row's end the last logit is repeated.
+template <int kLoads>
 __device__ __forceinline__ void load_share(const uint16_t *x, int vocab, int first, int step,
-                                           u32x4 (&w)[kAhead]) {
+                                           u32x4 (&w)[kLoads]) {
 #pragma unroll
-  for (int a = 0; a < kAhead; ++a) {
+  for (int a = 0; a < kLoads; ++a) {
     const int i = first + a * step;
     if (i + kVec <= vocab) {
       __builtin_memcpy(&w[a], x + i, sizeof(w[a]));
@@ -111,25 +123,132 @@ __device__ __forceinline__ void load_share(const uint16_t *x, int vocab, int fir
     }
   }
 }
-__device__ __forceinline__ uint32_t key_in(const u32x4 &w, int j) {
-  return merge_zero((keys_of(w[j >> 1]) >> (16 * (j & 1))) & 0xffffu);
+// The j-th logit of a load.
+template <bool kBf16>
+__device__ __forceinline__ float value_in(const u32x4 &w, int j) {
+  const uint32_t word = w[j >> 1];
+  if (kBf16) return j & 1 ? bf16_hi(word) : bf16_lo(word);
+  return static_cast<float>(
+      __builtin_bit_cast(_Float16, static_cast<uint16_t>(j & 1 ? word >> 16 : word)));
 }
-__device__ __forceinline__ bool kept(const RowCut &cut, uint32_t key, int index) {
-  return static_cast<int>(key) >= cut.low && !(static_cast<int>(key) == cut.cut && index > cut.last);
+// Where a row is cut, by value: logits of at least `low`, except those that are `at` and come
+// after `last`.
+struct Cut {
+  float low, at;
+  int last;
+  bool ok;
+  __device__ __forceinline__ bool keeps(float x, int index) const {
+    return x >= low && !(x == at && index > last);
+  }
+};
+__device__ __forceinline__ Cut no_cut() { return {-INFINITY, NAN, 0, true}; }
+template <bool kBf16>
+__device__ __forceinline__ Cut cut_of(const RowCut &c) {
+  return {c.low > 0 ? value_of<kBf16>(c.low) : -INFINITY, c.cut > 0 ? value_of<kBf16>(c.cut) : NAN,
+          c.last, c.ok == 1};
 }
-__device__ __forceinline__ RowCut no_cut(int vocab) { return {0, 0, vocab, 1, 0.f}; }
 
-// Sums over the workgroup in a fixed order, in every thread.
-__device__ __forceinline__ double block_sum(double v, double *box) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Rotations within a row of 16 lanes, and the sums and maxima made of them: register moves, where
+// a shuffle of 64 bits takes two trips through LDS.
+template <int N>
+__device__ __forceinline__ uint32_t ror(uint32_t x) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x120 + N, 0xf, 0xf, false));
+}
+template <int N>
+__device__ __forceinline__ double ror(double x) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
+  const uint64_t hi = ror<N>(static_cast<uint32_t>(u >> 32)), lo = ror<N>(static_cast<uint32_t>(u));
+  return __longlong_as_double(static_cast<long long>(hi << 32 | lo));
+}
+__device__ __forceinline__ double row_sum(double v) {
+  v += ror<8>(v);
+  v += ror<4>(v);
+  v += ror<2>(v);
+  return v + ror<1>(v);
+}
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __uint_as_float(ror<8>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(ror<4>(__float_as_uint(v))));
+  v = fmaxf(v, __uint_as_float(ror<2>(__float_as_uint(v))));
+  return fmaxf(v, __uint_as_float(ror<1>(__float_as_uint(v))));
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), lane));
+  return __longlong_as_double(static_cast<long long>(hi << 32 | lo));
+}
+// Over all 64 lanes, which take part.
+__device__ __forceinline__ double wave_sum(double v) {
+  v = row_sum(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+// Over the workgroup, in a fixed order and in every thread: of two values at once.
+struct Pair {
+  double a, b;
+};
+__device__ __forceinline__ Pair block_sums(double a, double b, Pair *box) {
+  const Pair mine = {wave_sum(a), wave_sum(b)};
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = mine;
   __syncthreads();
-  v = box[0];
+  Pair all = box[0];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) v += box[i];
-  return v;
+  for (int i = 1; i < kWaves; ++i) {
+    all.a += box[i].a;
+    all.b += box[i].b;
+  }
+  return all;
+}
+
+// The first largest logit of a workgroup's share as rank_of() has it; a NaN is the largest of all.
+// Keys in pairs: of three operations a logit nothing but the maximum comes, and the threads
+// that hold it look for its place.
+template <bool kBf16>
+__device__ __forceinline__ uint64_t best_of_share(const u32x4 (&w)[kAhead], int first, int step,
+                                                  int vocab, uint32_t *top_box, int *first_box) {
+  constexpr uint32_t kInf = kInfBits<kBf16>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u16x2 top2 = {0, 0}, mag2 = {0, 0};
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j) {
+      const uint32_t word = keys_of(w[a][j]);
+      const uint32_t mag = w[a][j] & 0x7fff7fffu;
+      top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2, word));
+      mag2 = __builtin_elementwise_max(mag2, __builtin_bit_cast(u16x2, mag));
+    }
+  // (what a tail repeats past the row's end changes neither)
+  uint32_t top = max(top2[0], top2[1]);
+  const bool nan = max(mag2[0], mag2[1]) > kInf;
+  if (top == 0x7fffu) top = 0x8000u;  // zeros are one value
+  if (nan) top = 0x10000u;
+  uint32_t t = top;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t = max(t, static_cast<uint32_t>(__shfl_xor(static_cast<int>(t), o)));
+  if (lane == 0) top_box[wave] = t;
+  if (threadIdx.x == 0) *first_box = vocab;
+  __syncthreads();
+  t = top_box[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) t = max(t, top_box[i]);
+  if (top == t) {
+    int at = vocab;
+#pragma unroll
+    for (int a = kAhead - 1; a >= 0; --a)
+#pragma unroll
+      for (int j = kVec - 1; j >= 0; --j) {
+        const uint32_t bits = w[a][j >> 1] >> (16 * (j & 1)) & 0xffffu;
+        const bool is = t == 0x10000u ? (bits & 0x7fffu) > kInf : merge_zero(keys_of(bits) & 0xffffu) == t;
+        const int i = first + a * step + j;
+        if (is && i < vocab) at = i;
+      }
+    atomicMin(first_box, at);
+  }
+  __syncthreads();
+  return rank_of(t, *first_box);
 }
 
 // Grid (shares, rows).
@@ -138,113 +257,284 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
     const RowCut *__restrict__ cuts, Share *__restrict__ shares, uint8_t *__restrict__ valid,
     bool first_rows) {
-  __shared__ uint64_t best[kWaves];
   __shared__ float maxes[kWaves];
-  __shared__ double box[kWaves];
+  __shared__ uint32_t tops[kWaves];
+  __shared__ int place;
+  __shared__ Pair box[kWaves];
   if (first_rows && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *valid = 1;
   const int row = blockIdx.y;
-  const int b = requests.of_row(row);
-  const Request req = requests.r[b];
-  const int i0 = blockIdx.x * kShare + kVec * threadIdx.x;
   constexpr int kRound = kThreads * kVec;
+  const int i0 = blockIdx.x * kShare + kVec * threadIdx.x;
   u32x4 w[kAhead];
   load_share(logits + row * ld, vocab, i0, kRound, w);
+  const int b = requests.of_row(row);
+  const float temp = requests.r[b].temp;
   Share *out = shares + static_cast<int64_t>(row) * gridDim.x + blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr uint32_t kInf = kInfBits<kBf16>;
-  if (req.temp == 0.f) {  // a NaN counts as the largest
-    uint64_t top = 0;
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        uint32_t key = key_in(w[a], j);
-        if (key > (0x8000u | kInf) || key < 0x7fffu - kInf) key = 0xffffu;
-        const int i = i0 + a * kRound + j;
-        const uint64_t r = i < vocab ? rank_of(key, i) : 0;
-        top = r > top ? r : top;
-      }
-    top = wave_best(top);
-    if (lane == 0) best[wave] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-      for (int i = 1; i < kWaves; ++i) top = best[i] > top ? best[i] : top;
-      out->best = top;
-    }
+  if (temp == 0.f) {
+    const uint64_t best = best_of_share<kBf16>(w, i0, kRound, vocab, tops, &place);
+    if (threadIdx.x == 0) out->best = best;
     return;
   }
-  const RowCut cut = requests.cut(b, vocab) ? cuts[row] : no_cut(vocab);
-  bool nan = cut.ok != 1;
+  bool ok = true;
   float x[kAhead][kVec], m = -INFINITY;
 #pragma unroll
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const uint32_t key = key_in(w[a], j);
-      const int i = i0 + a * kRound + j;
-      nan = nan || key > (0x8000u | kInf) || key < 0x7fffu - kInf;
-      x[a][j] = i < vocab && kept(cut, key, i) ? value_of<kBf16>(key) : -INFINITY;
-      m = fmaxf(m, x[a][j]);
-    }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if (lane == 0) maxes[wave] = m;
-  nan = __syncthreads_or(nan);
-  m = maxes[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, maxes[i]);
-  const float slope = 1.0f / req.temp * kLog2eS;
-  float s = 0.f;
-  if (m != -INFINITY) {
+    for (int j = 0; j < kVec; ++j) x[a][j] = value_in<kBf16>(w[a], j);
+  if (requests.cut(b, vocab)) {
+    const Cut cut = cut_of<kBf16>(cuts[row]);
+    ok = cut.ok;
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) s += __builtin_amdgcn_exp2f((x[a][j] - m) * slope);
+      for (int j = 0; j < kVec; ++j)
+        if (!cut.keeps(x[a][j], i0 + a * kRound + j)) x[a][j] = -INFINITY;
   }
-  const double sum = block_sum(s, box);
+  if ((static_cast<int>(blockIdx.x) + 1) * static_cast<int64_t>(kShare) > vocab) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (i0 + a * kRound + j >= vocab) x[a][j] = -INFINITY;
+  }
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) m = fmaxf(m, x[a][j]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((threadIdx.x & 63) == 0) maxes[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = maxes[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, maxes[i]);
+  const float slope = 1.0f / temp * kLog2eS;
+  // The differences are scaled, not the terms: at small temperatures those are far apart. NaN,
+  // and infinities less each other, make the sum NaN; a share without a finite logit is
+  // measured from 0.
+  const float from = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) s += __builtin_amdgcn_exp2f((x[a][j] - from) * slope);
+  const double sum = block_sums(s, 0.0, box).a;
   if (threadIdx.x == 0) {
-    out->max = nan ? NAN : m;
+    out->max = ok && sum == sum ? m : NAN;
     out->sum = static_cast<float>(sum);
   }
 }
 
-// exp((x - max) / temp) of this thread's kept logits of a share, 0 elsewhere: f(mass, index).
-template <bool kBf16, class F>
-__device__ __forceinline__ void each_mass(const u32x4 (&w)[kAhead], int first, int step, int vocab,
-                                          const RowCut &cut, float max, float temp, F f) {
+// exp(x), x <= 0, to about 1e-10: 2^n times the Taylor series of the rest, |r| <= ln(2) / 2 and a
+// little, its terms from the fourth on (r^4 / 24 < 7e-4) in 32 bits. Operations of 64 bits bound
+// the kernels that call it.
+__device__ __forceinline__ double exp_of(double x) {
+  constexpr long double kLn2 = 0.693147180559945309417232L;
+  constexpr double kHead = 45426.0 / 65536;  // n times it is exact
+  constexpr double kTail = static_cast<double>(kLn2 - 45426.0L / 65536);
+  const float n = rintf(static_cast<float>(x) * static_cast<float>(1 / kLn2));
+  double r = fma(static_cast<double>(n), -kHead, x);
+  r = fma(static_cast<double>(n), -kTail, r);
+  const float s = static_cast<float>(r);
+  float q = 1.0f / 362880;
 #pragma unroll
-  for (int a = 0; a < kAhead; ++a) {
+  for (const float c : {1.0f / 40320, 1.0f / 5040, 1.0f / 720, 1.0f / 120, 1.0f / 24})
+    q = __builtin_fmaf(q, s, c);
+  double p = fma(static_cast<double>(q), r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return x < -740.0 ? 0.0 : ldexp(p, static_cast<int>(n));
+}
+
+// exp((x - max) / temp) of kVec logits from index `first` on, 0 for those cut off. Without a
+// branch, so that the eight chains of dependent operations run side by side.
+template <bool kBf16>
+__device__ __forceinline__ void masses_of(const u32x4 &w, int first, int vocab, const Cut &cut,
+                                          double max, double inv_temp, double (&e)[kVec]) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const uint32_t key = key_in(w[a], j);
-      const int i = first + a * step + j;
-      if (i < vocab && kept(cut, key, i))
-        f(exp((static_cast<double>(value_of<kBf16>(key)) - max) / static_cast<double>(temp)), i);
+  for (int j = 0; j < kVec; ++j) {
+    const float x = value_in<kBf16>(w, j);
+    const double mass = exp_of((static_cast<double>(x) - max) * inv_temp);
+    e[j] = first + j < vocab && cut.keeps(x, first + j) ? mass : 0.0;
+  }
+}
+
+// kVec draft probabilities from index i on; past the row's end the last one.
+__device__ __forceinline__ void load_drafts(const float *q, int i, int vocab, float (&v)[kVec]) {
+  if (i + kVec <= vocab) {
+    __builtin_memcpy(v, q + i, sizeof(v));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = q[min(i + j, vocab - 1)];
+  }
+}
+
+// Marks the tokens of a part that the draw leaves out, those of the last node's children: every
+// thread has a node (or -1 as its parent) and its token.
+__device__ __forceinline__ void mark_refused(uint32_t *bits, int parent, int64_t token, int last,
+                                             int first) {
+  static_assert(kThreads >= kMaxNodes, "a node a thread");
+  static_assert(kPart / 32 <= kThreads, "a word a thread");
+  __syncthreads();  // earlier readers are done
+  if (threadIdx.x < kPart / 32) bits[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t at = token - first;
+  if (parent == last && at >= 0 && at < kPart) atomicOr(&bits[at >> 5], 1u << (at & 31));
+  __syncthreads();
+}
+
+// What a wave has found of a place: the first one behind the target and the last with any mass,
+// -1 where there is none, and what of the target is left at their start.
+struct Found {
+  int past, last;
+  double past_rest, last_rest;
+};
+struct PickRoom {
+  double all[kWaves], left[kWaves];
+  Found parts[kWaves], tokens[kWaves];
+};
+// Neighbouring lanes hold neighbouring places. (Ballots: an LDS atomic of 64 lanes on one word
+// is taken lane by lane, 2 us.)
+__device__ __forceinline__ void tell_found(Found *of_wave, bool past, bool any, int place, double rest) {
+  const uint64_t p = __ballot(past), a = __ballot(any);
+  const int first = p ? __ffsll(static_cast<long long>(p)) - 1 : 0;
+  const int last = a ? 63 - __clzll(static_cast<long long>(a)) : 0;
+  const Found f = {p ? __shfl(place, first) : -1, a ? __shfl(place, last) : -1, __shfl(rest, first),
+                   __shfl(rest, last)};
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = f;
+}
+// The first place behind the target, else the last with any mass (0 if there is none).
+__device__ __forceinline__ int take_found(const Found *of_waves, double &rest) {
+  int place = -1, last = 0;
+  double last_rest = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (place < 0 && of_waves[i].past >= 0) {
+      place = of_waves[i].past;
+      rest = of_waves[i].past_rest;
+    }
+    if (of_waves[i].last >= 0) {
+      last = of_waves[i].last;
+      last_rest = of_waves[i].last_rest;
     }
   }
+  if (place >= 0) return place;
+  rest = last_rest;
+  return last;
 }
 
-// Marks the tokens of a share that the draw leaves out: those of the last node's children.
-__device__ __forceinline__ void mark_refused(uint32_t *bits, const int32_t *parents,
-                                             const int64_t *tokens, int nodes, int last, int first) {
-  for (int i = threadIdx.x; i < kShare / 32; i += kThreads) bits[i] = 0;
-  __syncthreads();
-  for (int j = threadIdx.x; j < nodes; j += kThreads) {
-    const int64_t at = tokens[j] - first;
-    if (j > 0 && parents[j] == last && at >= 0 && at < kShare)
-      atomicOr(&bits[at >> 5], 1u << (at & 31));
+// The draw of one request, by a whole workgroup: the smallest token whose running mass exceeds
+// `number` times the total (where rounding leaves none, the last token with any). The masses are
+// max(p - q, 0) with rests (the parts') and q (the row of draft probabilities), else those of p
+// without the children of `last`, of which every thread has one's parent and token.
+template <bool kBf16>
+__device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const Cut &cut, float max,
+                                          double inv_temp, double number, const Mass *masses,
+                                          const double *rests, const float *q, int n_parts,
+                                          int parent, int64_t token, int last, uint32_t *bits,
+                                          PickRoom &room) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto scan = [&](double v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  // A thread has neighbouring parts.
+  const int per = (n_parts + kThreads - 1) / kThreads;
+  const int from = min(tid * per, n_parts), to = min(from + per, n_parts);
+  double all = 0, left = 0;
+  for (int i = from; i < to; ++i) {
+    all += masses[i].all;
+    left += rests ? rests[i] : masses[i].left;
+  }
+  const double all_with = scan(all), left_with = scan(left);
+  if (lane == 63) {
+    room.all[wave] = all_with;
+    room.left[wave] = left_with;
   }
   __syncthreads();
+  double z = 0, some = 0, all_before = all_with - all, left_before = left_with - left;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < wave) {
+      all_before += room.all[i];
+      left_before += room.left[i];
+    }
+    z += room.all[i];
+    some += room.left[i];
+  }
+  const bool whole = !(some > 0);  // where nothing is left, all of p
+  const double target = number * (whole ? z : some);
+  const double own = whole ? all : left, before = whole ? all_before : left_before;
+  int part = 0;  // of this thread's: where the sum passes the target, or the last with any mass
+  double rest = 0;
+  if (own > 0) {
+    double at = before;
+    for (int i = from; i < to; ++i) {
+      const double v = whole ? masses[i].all : rests ? rests[i] : masses[i].left;
+      if (v > 0) {
+        part = i;
+        rest = target - at;
+        if (at + v > target) break;
+      }
+      at += v;
+    }
+  }
+  tell_found(room.parts, own > 0 && before + own > target, own > 0, part, rest);
+  __syncthreads();
+  const int chosen = take_found(room.parts, rest);
+  const int first = chosen * kPart, at = kVec * tid, mine = first + at;
+  u32x4 w[1];
+  load_share(row, vocab, mine, 0, w);
+  mark_refused(bits, whole || rests ? -2 : parent, token, last, first);
+  double e[kVec];
+  masses_of<kBf16>(w[0], mine, vocab, cut, max, inv_temp, e);
+  if (!whole && rests) {
+    const double inv_z = 1.0 / z;
+    float qv[kVec];
+    load_drafts(q, mine, vocab, qv);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      e[j] = mine + j < vocab ? fmax(fma(e[j], inv_z, -static_cast<double>(qv[j])), 0.0) : 0.0;
+  }
+  const uint32_t out = bits[at >> 5] >> (at & 31);
+  double sum = 0;
+  int tail = -1;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    e[j] = out >> j & 1 ? 0.0 : e[j];
+    sum += e[j];
+    if (e[j] > 0) tail = mine + j;
+  }
+  const double with = scan(sum);
+  if (lane == 63) room.all[wave] = with;
+  __syncthreads();
+  double running = with - sum;
+  for (int i = 0; i < wave; ++i) running += room.all[i];
+  int found = -1;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    running += e[j];
+    if (found < 0 && e[j] > 0 && running > rest) found = mine + j;
+  }
+  tell_found(room.tokens, found >= 0, tail >= 0, found >= 0 ? found : tail, 0.0);
+  __syncthreads();
+  return take_found(room.tokens, rest);
 }
 
-// Grid (shares, requests).
+// Grid (parts or fewer, requests).
 template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void walk_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
-    const RowCut *__restrict__ cuts, const Share *__restrict__ shares, Tree tree,
-    State *__restrict__ states, Mass *__restrict__ masses, int32_t *__restrict__ paths, int levels,
-    int32_t *__restrict__ lengths, int64_t *__restrict__ next, uint8_t *__restrict__ valid) {
+    const RowCut *__restrict__ cuts, const Share *__restrict__ shares, int n_shares,
+    int n_parts, Tree tree,
+    State *__restrict__ states, Mass *__restrict__ masses,
+    int32_t *__restrict__ paths, int levels, int32_t *__restrict__ lengths,
+    int64_t *__restrict__ next, uint8_t *__restrict__ valid) {
   __shared__ float max_of[kMaxNodes];
   __shared__ double sum_of[kMaxNodes];
   __shared__ double p_of[kMaxNodes];  // p(x) of a node's token under its parent; greedy: 1 or 0
@@ -252,87 +542,74 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
   __shared__ float u_of[kMaxNodes];
   __shared__ int best_of[kMaxNodes], token_of[kMaxNodes], refused[kMaxNodes];
   __shared__ State sh;
-  __shared__ uint32_t bits[kShare / 32];
-  __shared__ double box[kWaves];
+  __shared__ uint32_t bits[kPart / 32];
+  __shared__ Pair box[kWaves];
   const int b = blockIdx.y;
   const Request req = requests.r[b];
   const int nodes = requests.nodes(b), row0 = req.first;
   const bool greedy = req.temp == 0.f, cut_rows = requests.cut(b, vocab);
+  const double inv_temp = greedy ? 0.0 : 1.0 / req.temp;
   const int32_t *parents = tree.parents + row0;
   const int64_t *tokens = tree.tokens + row0;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int n_shares = gridDim.x;
 
-  int32_t up = 0;
-  if (tid < nodes) {
-    const int64_t x = tokens[tid];
-    token_of[tid] = x >= 0 && x < vocab ? static_cast<int32_t>(x) : -1;
-    u_of[tid] = tree.uniforms[row0 + tid];
-    if (tid > 0) up = min(max(parents[tid], 0), tid - 1);
-  }
+  // (all loads that depend on nothing go out before the first is waited for)
+  const int mine = min(tid, nodes - 1);
+  const int64_t my_token = tokens[mine];
+  const int32_t up = min(max(parents[mine], 0), max(mine - 1, 0));
+  const float my_u = tree.uniforms[row0 + mine];
   int par[kMaxNodes / 64];  // of nodes 64 i + lane
 #pragma unroll
-  for (int i = 0; i < kMaxNodes / 64; ++i)
-    par[i] = 64 * i + lane < nodes && 64 * i + lane > 0 ? parents[64 * i + lane] : -1;
-  // Every row's maximum and sum (or largest logit), from its shares: 32 lanes a row.
-  const int l32 = tid & 31;
+  for (int i = 0; i < kMaxNodes / 64; ++i) {
+    par[i] = parents[min(64 * i + lane, nodes - 1)];
+    if (64 * i + lane >= nodes || 64 * i + lane == 0) par[i] = -1;
+  }
+  // Every row's maximum and sum (or largest logit), from its shares: 16 lanes a row.
+  const int l16 = tid & 15;
   const float slope = greedy ? 0.f : 1.0f / req.temp * kLog2eS;
-#pragma unroll 2
-  for (int r = tid >> 5; r < nodes; r += kThreads / 32) {
-    const Share *s = shares + static_cast<int64_t>(row0 + r) * n_shares;
+  for (int r0 = 0; r0 < nodes; r0 += kThreads / 16) {
+    const int r = r0 + (tid >> 4);
+    const Share *s = shares + static_cast<int64_t>(row0 + min(r, nodes - 1)) * n_shares;
     if (greedy) {
       uint64_t top = 0;
-      for (int i = l32; i < n_shares; i += 32) top = s[i].best > top ? s[i].best : top;
+      for (int i = l16; i < n_shares; i += 16) top = s[i].best > top ? s[i].best : top;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
+      for (int o = 8; o > 0; o >>= 1) {
         const uint64_t t = __shfl_xor(static_cast<unsigned long long>(top), o);
         top = t > top ? t : top;
       }
-      if (l32 == 0) best_of[r] = index_of(top);
+      if (l16 == 0 && r < nodes) best_of[r] = index_of(top);
       continue;
     }
     float m = -INFINITY;
-    double z = 0;
-    bool nan = false;
-    for (int i = l32; i < n_shares; i += 32) {
-      const float sm = s[i].max, ss = s[i].sum;
-      nan = nan || sm != sm;
-      if (sm > m) {
-        z *= __builtin_amdgcn_exp2f((m - sm) * slope);
-        m = sm;
-      }
-      if (ss > 0.f) z += static_cast<double>(ss) * __builtin_amdgcn_exp2f((sm - m) * slope);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float om = __shfl_xor(m, o);
-      const double oz = __shfl_xor(z, o);
-      const float top = fmaxf(m, om);
-      z = (z > 0 ? z * __builtin_amdgcn_exp2f((m - top) * slope) : 0) +
-          (oz > 0 ? oz * __builtin_amdgcn_exp2f((om - top) * slope) : 0);
-      m = top;
-      nan = nan || __shfl_xor(static_cast<int>(nan), o);
-    }
-    if (l32 == 0) {
-      max_of[r] = nan || isinf(m / req.temp) ? NAN : m;
+    for (int i = l16; i < n_shares; i += 16) m = fmaxf(m, s[i].max);
+    m = row_max(m);
+    const float from = m == -INFINITY ? 0.f : m;
+    double z = 0;  // (a share's NaN makes it NaN)
+    for (int i = l16; i < n_shares; i += 16)
+      z += static_cast<double>(s[i].sum * __builtin_amdgcn_exp2f((s[i].max - from) * slope));
+    z = row_sum(z);
+    if (l16 == 0 && r < nodes) {
+      max_of[r] = z != z || isinf(m / req.temp) ? NAN : m;
       sum_of[r] = z;
     }
   }
+  const int x = my_token >= 0 && my_token < vocab ? static_cast<int>(my_token) : -1;
+  if (tid < nodes) {
+    token_of[tid] = x;
+    u_of[tid] = my_u;
+  }
   __syncthreads();
   if (tid > 0 && tid < nodes) {
-    const int x = token_of[tid];
     double p = 0, q = 0;
     if (greedy) {
       p = x == best_of[up];
     } else if (x >= 0) {
-      const uint32_t word = logits[(row0 + up) * ld + x];
-      const uint32_t key = merge_zero(keys_of(word) & 0xffffu);
-      const RowCut cut = cut_rows ? cuts[row0 + up] : no_cut(vocab);
+      const u32x4 word = {logits[(row0 + up) * ld + x], 0u, 0u, 0u};
+      const Cut cut = cut_rows ? cut_of<kBf16>(cuts[row0 + up]) : no_cut();
       if (tree.drafts) q = tree.drafts[(row0 + tid) * tree.drafts_ld + x];
-      if (kept(cut, key, x))
-        p = exp((static_cast<double>(value_of<kBf16>(key)) - max_of[up]) /
-                static_cast<double>(req.temp)) /
-            sum_of[up];
+      const float v = value_in<kBf16>(word, 0);
+      if (cut.keeps(v, x)) p = exp_of((static_cast<double>(v) - max_of[up]) * inv_temp) / sum_of[up];
     }
     p_of[tid] = p;
     q_of[tid] = q;
@@ -409,47 +686,62 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
   }
   __syncthreads();
   if (greedy || sh.bad) return;
-  const int row = row0 + sh.last, first = blockIdx.x * kShare;
-  if (!tree.drafts) mark_refused(bits, parents, tokens, nodes, sh.last, first);
-  u32x4 w[kAhead];
-  load_share(logits + row * ld, vocab, first + kVec * tid, kThreads * kVec, w);
-  double all = 0, left = 0;
-  each_mass<kBf16>(w, first + kVec * tid, kThreads * kVec, vocab,
-                   cut_rows ? cuts[row] : no_cut(vocab), sh.max, req.temp, [&](double e, int i) {
-                     all += e;
-                     const int at = i - first;
-                     if (tree.drafts || !(bits[at >> 5] >> (at & 31) & 1)) left += e;
-                   });
-  all = block_sum(all, box);
-  left = block_sum(left, box);
-  if (tid == 0) masses[static_cast<int64_t>(b) * n_shares + blockIdx.x] = {all, left};
+  const int row = row0 + sh.last, at = kVec * tid;
+  const uint16_t *x_row = logits + row * ld;
+  const Cut cut = cut_rows ? cut_of<kBf16>(cuts[row]) : no_cut();
+  const int my_parent = tree.drafts || tid == 0 || tid >= nodes ? -2 : up;
+  u32x4 w[1];
+  load_share(x_row, vocab, blockIdx.x * kPart + at, 0, w);
+  for (int part = blockIdx.x; part < n_parts; part += gridDim.x) {
+    const int first = part * kPart;
+    mark_refused(bits, my_parent, my_token, sh.last, first);
+    const uint32_t out = bits[at >> 5] >> (at & 31);
+    double e[kVec], all = 0, left = 0;
+    masses_of<kBf16>(w[0], first + at, vocab, cut, sh.max, inv_temp, e);
+    if (part + static_cast<int>(gridDim.x) < n_parts)
+      load_share(x_row, vocab, first + static_cast<int>(gridDim.x) * kPart + at, 0, w);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      all += e[j];
+      left += out >> j & 1 ? 0.0 : e[j];
+    }
+    const Pair sums = block_sums(all, left, box);
+    if (tid == 0) masses[static_cast<int64_t>(b) * n_parts + part] = {sums.a, sums.b};
+  }
 }
 
-// Grid (shares, requests): of requests whose drawn draft was refused, the masses of max(p - q, 0).
+// Grid (parts, requests): of requests whose drawn draft was refused, the masses of max(p - q, 0).
 template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void rest_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
     const RowCut *__restrict__ cuts, Tree tree, const State *__restrict__ states,
     const Mass *__restrict__ masses, double *__restrict__ rests) {
-  __shared__ double box[kWaves];
-  const int b = blockIdx.y;
+  __shared__ Pair box[kWaves];
+  const int b = blockIdx.y, tid = threadIdx.x, n_parts = gridDim.x;
   const Request req = requests.r[b];
+  if (req.temp == 0.f) return;
   const State st = states[b];
-  if (req.temp == 0.f || st.bad || st.child < 0) return;
-  const Mass *m = masses + static_cast<int64_t>(b) * gridDim.x;
-  double z = 0;
-  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kThreads) z += m[i].all;
-  z = block_sum(z, box);
-  const int row = req.first + st.last, first = blockIdx.x * kShare + kVec * threadIdx.x;
-  u32x4 w[kAhead];
-  load_share(logits + row * ld, vocab, first, kThreads * kVec, w);
+  if (st.bad || st.child < 0) return;
+  const Mass *mass = masses + static_cast<int64_t>(b) * n_parts;
+  const int row = req.first + st.last, first = blockIdx.x * kPart + kVec * tid;
+  const uint16_t *x_row = logits + row * ld;
   const float *q = tree.drafts + (req.first + st.child) * tree.drafts_ld;
-  double left = 0;
-  each_mass<kBf16>(w, first, kThreads * kVec, vocab,
-                   requests.cut(b, vocab) ? cuts[row] : no_cut(vocab), st.max, req.temp,
-                   [&](double e, int i) { left += fmax(e / z - q[i], 0.0); });
-  left = block_sum(left, box);
-  if (threadIdx.x == 0) rests[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = left;
+  const double inv_temp = 1.0 / req.temp;
+  u32x4 w[1];
+  load_share(x_row, vocab, first, 0, w);
+  float qv[kVec];
+  load_drafts(q, first, vocab, qv);
+  const Cut cut = requests.cut(b, vocab) ? cut_of<kBf16>(cuts[row]) : no_cut();
+  double z = 0;
+  for (int i = tid; i < n_parts; i += kThreads) z += mass[i].all;
+  const double inv_z = 1.0 / block_sums(z, 0.0, box).a;
+  double e[kVec], left = 0;
+  masses_of<kBf16>(w[0], first, vocab, cut, st.max, inv_temp, e);
+#pragma unroll
+  for (int j = 0; j < kVec; ++j)
+    if (first + j < vocab) left += fmax(fma(e[j], inv_z, -static_cast<double>(qv[j])), 0.0);
+  left = block_sums(left, 0.0, box).a;
+  if (tid == 0) rests[static_cast<int64_t>(b) * n_parts + blockIdx.x] = left;
 }
 
 // Grid (requests).
@@ -457,110 +749,41 @@ template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void pick_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
     const RowCut *__restrict__ cuts, Tree tree, const State *__restrict__ states,
-    const Mass *__restrict__ masses, const double *__restrict__ rests, int n_shares,
+    const Mass *__restrict__ masses, const double *__restrict__ rests, int n_parts,
     int64_t *__restrict__ next) {
-  __shared__ uint32_t bits[kShare / 32];
-  __shared__ double box[kWaves];
-  __shared__ struct {
-    int share, found, tail;
-    double before;
-  } sh;
-  const int b = blockIdx.x;
+  __shared__ uint32_t bits[kPart / 32];
+  __shared__ PickRoom room;
+  const int b = blockIdx.x, tid = threadIdx.x;
   const Request req = requests.r[b];
+  if (req.temp == 0.f) return;
+  // (loads that depend on nothing go out first)
+  const int nodes = requests.nodes(b), mine = req.first + min(tid, nodes - 1);
+  const int parent = tree.drafts || tid == 0 || tid >= nodes ? -2 : tree.parents[mine];
+  const int64_t token = tree.tokens[mine];
+  const double number = tree.draws[b];
   const State st = states[b];
-  if (req.temp == 0.f || st.bad) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (st.bad) return;
+  const int row = req.first + st.last;
+  const Cut cut = requests.cut(b, vocab) ? cut_of<kBf16>(cuts[row]) : no_cut();
   const bool drawn = tree.drafts && st.child >= 0;  // the draw is from max(p - q, 0)
-  const Mass *m = masses + static_cast<int64_t>(b) * n_shares;
-  const double *rest = rests + static_cast<int64_t>(b) * n_shares;
-  double z = 0, some = 0;
-  for (int i = tid; i < n_shares; i += kThreads) {
-    z += m[i].all;
-    some += drawn ? rest[i] : m[i].left;
-  }
-  z = block_sum(z, box);
-  some = block_sum(some, box);
-  // where nothing is left, all of p
-  const bool whole = !(some > 0);
-  auto mass_at = [&](int i) { return whole ? m[i].all : drawn ? rest[i] : m[i].left; };
-  // the share in which the running sum passes the target (a few hundred at most: one thread)
-  if (tid == 0) {
-    double total = 0;
-    for (int i = 0; i < n_shares; ++i) total += mass_at(i);
-    const double target = static_cast<double>(tree.draws[b]) * total;
-    double sum = 0;
-    sh.share = 0;
-    sh.before = target;
-    for (int i = 0; i < n_shares; ++i) {
-      const double v = mass_at(i);
-      if (v > 0) {
-        sh.share = i;
-        sh.before = target - sum;
-        if (sum + v > target) break;
-      }
-      sum += v;
-    }
-    sh.found = vocab;
-    sh.tail = -1;
-  }
-  __syncthreads();
-  const int row = req.first + st.last, first = sh.share * kShare;
-  const double target = sh.before;  // within the share
-  if (!drawn)
-    mark_refused(bits, tree.parents + req.first, tree.tokens + req.first, requests.nodes(b), st.last,
-                 first);
-  const float *q = drawn ? tree.drafts + (req.first + st.child) * tree.drafts_ld : nullptr;
-  // a thread's logits lie in a row here
-  const int own = first + kVec * kAhead * tid;
-  u32x4 w[kAhead];
-  load_share(logits + row * ld, vocab, own, kVec, w);
-  const RowCut cut = requests.cut(b, vocab) ? cuts[row] : no_cut(vocab);
-  auto mass = [&](double e, int i) {
-    if (whole) return e;
-    if (drawn) return fmax(e / z - q[i], 0.0);
-    return bits[(i - first) >> 5] >> ((i - first) & 31) & 1 ? 0.0 : e;
-  };
-  double sum = 0;
-  int tail = -1;
-  each_mass<kBf16>(w, own, kVec, vocab, cut, st.max, req.temp, [&](double e, int i) {
-    const double v = mass(e, i);
-    sum += v;
-    if (v > 0) tail = i;
-  });
-  double with = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double u = __shfl_up(with, o);
-    if (lane >= o) with += u;
-  }
-  if (lane == 63) box[wave] = with;
-  __syncthreads();
-  double before = with - sum;
-  for (int i = 0; i < wave; ++i) before += box[i];
-  if (tail >= 0) atomicMax(&sh.tail, tail);
-  if (sum > 0 && before + sum > target) {
-    double at = before;
-    int found = vocab;
-    each_mass<kBf16>(w, own, kVec, vocab, cut, st.max, req.temp, [&](double e, int i) {
-      const double v = mass(e, i);
-      at += v;
-      if (v > 0 && at > target && i < found) found = i;
-    });
-    atomicMin(&sh.found, found);
-  }
-  __syncthreads();
-  // (a target that the share's own sum just misses by rounding takes its last token)
-  if (tid == 0) next[b] = sh.found < vocab ? sh.found : max(sh.tail, 0);
+  const int got = pick_token<kBf16>(
+      logits + row * ld, vocab, cut, st.max, 1.0 / req.temp, number,
+      masses + static_cast<int64_t>(b) * n_parts,
+      drawn ? rests + static_cast<int64_t>(b) * n_parts : nullptr,
+      drawn ? tree.drafts + (req.first + st.child) * tree.drafts_ld : nullptr, n_parts, parent, token,
+      st.last, bits, room);
+  if (tid == 0) next[b] = got;
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t share_count(int64_t vocab) { return (vocab + kShare - 1) / kShare; }
+int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
 
 struct Room {
   int64_t cuts, shares, states, masses, rests, all;
 };
 Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
-  const int64_t n = share_count(vocab);
+  const int64_t n = share_count(vocab), parts = part_count(vocab);
   requests = requests < kRequests ? requests : kRequests;
   Room r{};
   int64_t at = 0;
@@ -572,8 +795,8 @@ Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
   r.cuts = take(rows * static_cast<int64_t>(sizeof(RowCut)));
   r.shares = take(rows * n * static_cast<int64_t>(sizeof(Share)));
   r.states = take(requests * static_cast<int64_t>(sizeof(State)));
-  r.masses = take(requests * n * static_cast<int64_t>(sizeof(Mass)));
-  r.rests = take(requests * n * static_cast<int64_t>(sizeof(double)));
+  r.masses = take(requests * parts * static_cast<int64_t>(sizeof(Mass)));
+  r.rests = take(requests * parts * static_cast<int64_t>(sizeof(double)));
   r.all = at;
   return r;
 }
@@ -582,7 +805,7 @@ template <bool kBf16>
 void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, const Requests &req, bool cuts,
             const Tree &tree, char *ws, const Room &room, int32_t *paths, int levels,
             int32_t *lengths, int64_t *next, uint8_t *valid, bool first_rows) {
-  const int n = static_cast<int>(share_count(vocab));
+  const int n = static_cast<int>(share_count(vocab)), parts = static_cast<int>(part_count(vocab));
   auto *cut = reinterpret_cast<RowCut *>(ws + room.cuts);
   auto *shares = reinterpret_cast<Share *>(ws + room.shares);
   auto *states = reinterpret_cast<State *>(ws + room.states);
@@ -593,16 +816,19 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, const Requ
                        ld, vocab, req, static_cast<int64_t *>(nullptr), cut);
   hipLaunchKernelGGL(mass_kernel<kBf16>, dim3(n, req.rows), dim3(kThreads), 0, st, x, ld, vocab, req,
                      cut, shares, valid, first_rows);
-  hipLaunchKernelGGL(walk_kernel<kBf16>, dim3(n, req.count), dim3(kThreads), 0, st, x, ld, vocab,
-                     req, cut, shares, tree, states, masses, paths, levels, lengths, next, valid);
   bool sampled = false;
   for (int b = 0; b < req.count; ++b) sampled = sampled || req.r[b].temp != 0.f;
+  // Every workgroup of a request repeats its walk: no more of them than fill the GPU.
+  const int walkers = sampled ? std::min(parts, std::max(1, kWalkers / req.count)) : 1;
+  hipLaunchKernelGGL(walk_kernel<kBf16>, dim3(walkers, req.count), dim3(kThreads), 0, st, x, ld,
+                     vocab, req, cut, shares, n, parts, tree, states, masses, paths, levels, lengths,
+                     next, valid);
   if (!sampled) return;
   if (tree.drafts)
-    hipLaunchKernelGGL(rest_kernel<kBf16>, dim3(n, req.count), dim3(kThreads), 0, st, x, ld, vocab,
-                       req, cut, tree, states, masses, rests);
+    hipLaunchKernelGGL(rest_kernel<kBf16>, dim3(parts, req.count), dim3(kThreads), 0, st, x, ld,
+                       vocab, req, cut, tree, states, masses, rests);
   hipLaunchKernelGGL(pick_kernel<kBf16>, dim3(req.count), dim3(kThreads), 0, st, x, ld, vocab, req,
-                     cut, tree, states, masses, rests, n, next);
+                     cut, tree, states, masses, rests, parts, next);
 }
 
 }  // namespace

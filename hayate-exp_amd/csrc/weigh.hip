@@ -15,6 +15,7 @@
 // 8 (i / 4) + 4 h + i % 4 of a 32-key block), so a lane adds up its row's weights key by key over
 // the whole range and the 32 rows of a block are only joined at the end.
 
+#include "attend.h"
 #include "hy_common.h"
 #include "weigh_shape.h"
 
@@ -23,6 +24,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStageElems = kWeighRows * kHeadDim;
+constexpr int kStages = 3;
 
 __device__ __forceinline__ void load_to_lds(const uint16_t *g, const uint16_t *lds) {
   const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -34,11 +36,23 @@ __device__ __forceinline__ void load_to_lds(const uint16_t *g, const uint16_t *l
                    : "memory");
 }
 
-// Every load of this wave done: vmcnt(0) lgkmcnt(0).
-__device__ __forceinline__ void wait_all() {
-  __builtin_amdgcn_s_waitcnt(0x0070);
+// At most N vector-memory loads of this wave outstanding (they return in order), and no LDS or
+// scalar access.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 16, "the counter's low bits");
+  __builtin_amdgcn_s_waitcnt(N | 7 << 4);
   __asm__ volatile("" ::: "memory");
 }
+
+template <int N>
+__device__ __forceinline__ float ror16(float x) {
+  return __int_as_float(
+      __builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + N, 0xf, 0xf, false));
+}
+
+constexpr int kSchedMfma = 0x008;
+constexpr int kSchedValu = 0x002 | 0x400;  // VALU, transcendentals too
 
 // Item = {seq, key0, token0, token1, part, q_row, cache_len, offset}: keys from key0 (a multiple
 // of 256), the sequence's tokens [token0, token1) of this tick. Sums go to
@@ -50,12 +64,14 @@ void weigh_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, in
                   const int32_t *__restrict__ page_table, int64_t pt_stride,
                   const int32_t *__restrict__ items, const float2 *__restrict__ row_ml,
                   float *__restrict__ partials, int64_t stride, int num_kv_heads, int page_shift,
-                  float scale_log2, bool q_aligned) {
-  __shared__ __attribute__((aligned(1024))) uint16_t smem[2 * kStageElems];
+                  float scale_log2) {
+  __shared__ __attribute__((aligned(1024))) uint16_t smem[kStages * kStageElems];
   const int32_t *it = items + 8 * blockIdx.y;
   const int kvh = blockIdx.x;
-  const int seq = it[0], key0 = it[1], tok0 = it[2], tok1 = it[3];
+  const int seq = it[0], key0 = it[1], tok1 = it[3];
   const int part = it[4], q_row = it[5], cache = it[6], off = it[7];
+  // tokens before the block's first key see none of it
+  const int tok0 = max(it[2], key0 - cache);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int c = lane & 31, h = lane >> 5;
@@ -68,22 +84,26 @@ void weigh_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, in
   // lanes reading one chunk of 16 rows touch every bank once. Rows past the end repeat the
   // last one.
   const int chunk8 = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
-  const uint16_t *qb = q + seq * q_ss + static_cast<int64_t>(q_row) * q_st + kvh * G * q_sh;
-  auto issue = [&](int s) {
-    uint16_t *dst = smem + (s & 1) * kStageElems;
+  const uint16_t *qb =
+      q + seq * q_ss + static_cast<int64_t>(q_row + tok0) * q_st + kvh * G * q_sh + chunk8;
+  auto issue = [&](int s) __attribute__((always_inline)) {
+    uint16_t *dst = smem + (s % kStages) * kStageElems + 2048 * wave;
+    const int row = min(kWeighRows * s + 16 * wave + (lane >> 2), n_rows - 1);
+    const uint16_t *src = qb + static_cast<int64_t>(row / G) * q_st + (row % G) * q_sh;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * wave + j;
-      const int row = min(kWeighRows * s + 16 * (i >> 2) + (lane >> 2), n_rows - 1);
-      const uint16_t *src =
-          qb + static_cast<int64_t>(tok0 + row / G) * q_st + (row % G) * q_sh + 32 * (i & 3) + chunk8;
-      if (q_aligned)
-        load_to_lds(src, dst + i * 512);
-      else
-        *reinterpret_cast<u32x4 *>(dst + i * 512 + 8 * lane) = load16(src);
-    }
+    for (int j = 0; j < 4; ++j) load_to_lds(src + 32 * j, dst + 512 * j);
   };
-  issue(0);
+  // This lane's row of row block r: its exponent base and the inverse of its sum. Rows past the
+  // end weigh nothing.
+  const float2 *ml_rows = row_ml + static_cast<int64_t>(q_row + tok0) * num_kv_heads * G + kvh * G;
+  auto load_ml = [&](int r) __attribute__((always_inline)) {
+    const uint32_t row = min(32 * r + c, n_rows - 1);
+    return ml_rows[row / G * (num_kv_heads * G) + row % G];
+  };
+  auto usable = [&](float2 ml, int r) __attribute__((always_inline)) {
+    const bool live = 32 * r + c < n_rows;
+    return make_float2(live ? ml.x : INFINITY, live ? __builtin_amdgcn_rcpf(ml.y) : 0.f);
+  };
 
   // K of the wave's two blocks (A operand: row c, dims 16 kk + 8 h ..).
   bf16x8 kop[2][8];
@@ -98,75 +118,121 @@ void weigh_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, in
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) kop[b][kk] = __builtin_bit_cast(bf16x8, load16(src + 16 * kk));
   }
+  float2 ml_next[2] = {load_ml(0), load_ml(1)};
   float sum[2][16];
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[b][i] = 0.f;
 
-  // This lane's row of row block r: its exponent base and the inverse of its sum.
-  auto row_of = [&](int r) {
-    const int row = 32 * r + c;
-    if (row >= n_rows) return make_float2(INFINITY, 0.f);
-    const int64_t tok = q_row + tok0 + row / G;
-    const float2 ml = row_ml[tok * num_kv_heads * G + kvh * G + row % G];
-    return make_float2(ml.x, 1.0f / ml.y);
-  };
   int base[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     base[i] = (c >> 4) * 2048 + (c & 15) * 32 + 8 * ((2 * i + h) ^ ((c >> 2) & 3));
-
-  wait_all();
-  __syncthreads();
-  for (int s = 0; s < n_stages; ++s) {
-    if (s + 1 < n_stages) issue(s + 1);
-    const uint16_t *stage = smem + (s & 1) * kStageElems;
+  auto read_q = [&](bf16x8 (&op)[8], int s, int rb) __attribute__((always_inline)) {
+    const uint16_t *at = smem + (s % kStages) * kStageElems + 4096 * rb;
 #pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
-      const int r = 2 * s + rb;
-      if (32 * r >= n_rows) break;
-      // a block whose last row sees none of the wave's keys adds nothing
-      const int end = min(tok1 - 1, tok0 + (32 * r + 31) / G) + cache;
-      if (end < first) continue;
-      const float2 ml = row_of(r);
-      const int place = cache + tok0 + (32 * r + c) / G;
-      const bool cut = cache + tok0 + 32 * r / G < first + 63;  // some row does not see all keys
-      bf16x8 qop[8];
+    for (int kk = 0; kk < 8; ++kk)
+      op[kk] = *reinterpret_cast<const bf16x8 *>(at + base[kk & 1] + 512 * (kk >> 1));
+  };
+  auto scores = [&](const bf16x8 (&k)[8], const bf16x8 (&op)[8]) __attribute__((always_inline)) {
+    f32x16 sc;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        qop[kk] = *reinterpret_cast<const bf16x8 *>(stage + 4096 * rb + base[kk & 1] + 512 * (kk >> 1));
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x16 sc;
+    for (int kk = 0; kk < 8; ++kk)
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[kk], op[kk], sc, 0, 0, 0);
+    return sc;
+  };
+  // Keys that a row of row block r does not see.
+  auto mask = [&](f32x16 &sc, int b, int r) __attribute__((always_inline)) {
+    const int last = cache + tok0 + (32 * r + c) / G - (first + 32 * b + 4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+    for (int i = 0; i < 16; ++i) sc[i] = 8 * (i >> 2) + (i & 3) > last ? -INFINITY : sc[i];
+  };
+  auto add = [&](const f32x16 &sc, int b, const float2 &ml) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[b][kk], qop[kk], sc, 0, 0, 0);
-        if (cut) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (first + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) > place) sc[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -ml.x));
-          sum[b][i] = __builtin_fmaf(p, ml.y, sum[b][i]);
-        }
-      }
+    for (int i = 0; i < 16; ++i) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -ml.x));
+      sum[b][i] = __builtin_fmaf(p, ml.y, sum[b][i]);
     }
-    wait_all();
+  };
+  // One product's matrix instructions among another's exponentials. The sums count as used here,
+  // so that the compiler keeps what makes them in this straight piece of code.
+  auto mix = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedValu, 6, 0);
+    }
+    const float(&x)[16] = sum[b];
+    __asm__ volatile("" ::"v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]),
+                     "v"(x[6]), "v"(x[7]), "v"(x[8]), "v"(x[9]), "v"(x[10]), "v"(x[11]),
+                     "v"(x[12]), "v"(x[13]), "v"(x[14]), "v"(x[15]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  issue(0);
+  if (n_stages > 1) issue(1);
+  wait_loads<0>();  // K too, which no wait of the loop is to be for
+  __syncthreads();
+  bf16x8 qa[8], qc[8];
+  read_q(qa, 0, 0);
+  f32x16 sa = scores(kop[0], qa), sb;
+  for (int s = 0; s < n_stages; ++s) {
+    // (these were loaded a stage ago: waited for behind new loads, they would wait for those too)
+    const float2 ml0 = usable(ml_next[0], 2 * s), ml1 = usable(ml_next[1], 2 * s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 2 < n_stages) issue(s + 2);
+    ml_next[0] = load_ml(2 * s + 2);
+    ml_next[1] = load_ml(2 * s + 3);
+    // whether some row of the row block does not see all keys of the wave
+    const bool cut0 = cache + tok0 + 64 * s / G < first + 63;
+    const bool cut1 = cache + tok0 + (64 * s + 32) / G < first + 63;
+    // The scores of each (row block, key block) are made while the ones before are used: straight
+    // code, which the scheduler can mix (a mask comes before it).
+    if (cut0) mask(sa, 0, 2 * s);
+    read_q(qc, s, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    sb = scores(kop[1], qa);
+    add(sa, 0, ml0);
+    mix(0);
+    if (cut0) mask(sb, 1, 2 * s);
+    __builtin_amdgcn_sched_barrier(0);
+    sa = scores(kop[0], qc);
+    add(sb, 1, ml0);
+    mix(1);
+    if (cut1) mask(sa, 0, 2 * s + 1);
+    // stage s + 1 has arrived in every wave (what is read of it past the last stage is unused)
+    if (s + 2 < n_stages)
+      wait_loads<4>();
+    else
+      wait_loads<0>();
     __syncthreads();
+    read_q(qa, s + 1 < n_stages ? s + 1 : s, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    sb = scores(kop[1], qc);
+    add(sa, 0, ml1);
+    mix(0);
+    if (cut1) mask(sb, 1, 2 * s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    sa = scores(kop[0], qa);
+    add(sb, 1, ml1);
+    mix(1);
   }
   // Join the 32 rows; lane (0, h) has four keys in a row.
   float *dst = partials + (static_cast<int64_t>(part) * num_kv_heads + kvh) * stride + off + first;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) sum[b][i] += __shfl_xor(sum[b][i], o);
+    for (int i = 0; i < 16; ++i) {
+      float x = sum[b][i];
+      x += ror16<8>(x);
+      x += ror16<4>(x);
+      x += ror16<2>(x);
+      x += ror16<1>(x);
+      sum[b][i] = x + __shfl_xor(x, 16);
+    }
   if (c == 0) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -228,67 +294,52 @@ __global__ __launch_bounds__(256) void add_kernel(
 }  // namespace
 }  // namespace hy
 
-using hy::kHeadDim;
-
-extern "C" int hy_token_weights(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok, int64_t q_stride_head,
-    const void *k_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *items, int32_t n_items, const int32_t *adds,
-    int32_t n_adds, const float *scores, int64_t score_stride, float *partials,
-    int64_t partial_stride, const float *row_ml, float *weights, int64_t weights_stride,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale,
-    void *stream) {
-  hy::clear_error();
-  HY_REQUIRE(scale > 0.f, "softmax scale must be positive");
-  HY_REQUIRE(num_kv_heads >= 1 && num_q_heads >= num_kv_heads &&
-                 num_q_heads % num_kv_heads == 0,
-             "num_q_heads (%d) must be a positive multiple of num_kv_heads (%d)",
-             num_q_heads, num_kv_heads);
-  HY_REQUIRE_SUPPORTED(head_dim == kHeadDim, "head_dim %d unsupported (need %d)", head_dim,
-                       kHeadDim);
-  HY_REQUIRE_SUPPORTED(page_size >= 32 && (page_size & (page_size - 1)) == 0,
-                       "page_size %d unsupported (power of two >= 32 required)", page_size);
+int hy::token_weights(const char *name, const Rows &q, const Pools &pools, const Shape &shape,
+                      const int32_t *items, int32_t n_items, const int32_t *adds, int32_t n_adds,
+                      const Scores &scores, float *partials, int64_t partial_stride,
+                      const float *row_ml, float *weights, int64_t weights_stride, void *stream) {
+  // (shape, scale and page size are those that the attention before it was checked for)
   HY_REQUIRE(n_items >= 0 && n_items <= 65535 && n_adds >= 0,
-             "hy_token_weights: %d items (0 to 65535), %d additions", n_items, n_adds);
+             "%s: %d items (0 to 65535), %d additions", name, n_items, n_adds);
   if (n_adds == 0) return HY_OK;
-  HY_REQUIRE(q && k_pool && page_table && adds && row_ml && weights && (n_items == 0 || items),
-             "hy_token_weights: null pointer argument");
-  HY_REQUIRE(scores || partials, "hy_token_weights: null pointer argument");
-  HY_REQUIRE(n_items == 0 || partials, "hy_token_weights: null pointer argument");
-  HY_REQUIRE(((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(partials)) & 15) ==
+  HY_REQUIRE(q.at && pools.k && pools.page_table && adds && row_ml && weights && (n_items == 0 || items),
+             "%s: null pointer argument", name);
+  HY_REQUIRE(scores.at || partials, "%s: null pointer argument", name);
+  HY_REQUIRE(n_items == 0 || partials, "%s: null pointer argument", name);
+  HY_REQUIRE(((reinterpret_cast<uintptr_t>(scores.at) | reinterpret_cast<uintptr_t>(partials)) & 15) ==
                      0 &&
-                 score_stride % 4 == 0 && partial_stride % 4 == 0,
-             "hy_token_weights: scores and partial sums lie on 16 bytes");
+                 scores.stride % 4 == 0 && partial_stride % 4 == 0,
+             "%s: scores and partial sums lie on 16 bytes", name);
+  const int num_q_heads = shape.num_q_heads, num_kv_heads = shape.num_kv_heads;
   const int G = num_q_heads / num_kv_heads;
-  const float scale_log2 = scale * hy::kLog2e;
-  const int page_shift = __builtin_ctz(static_cast<unsigned>(page_size));
+  const float scale_log2 = shape.scale * kLog2e;
+  const int page_shift = __builtin_ctz(static_cast<unsigned>(shape.page_size));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const uint16_t *qq = static_cast<const uint16_t *>(q);
-  const uint16_t *kp = static_cast<const uint16_t *>(k_pool);
+  const uint16_t *qq = static_cast<const uint16_t *>(q.at);
+  const uint16_t *kp = static_cast<const uint16_t *>(pools.k);
   const float2 *ml = reinterpret_cast<const float2 *>(row_ml);
-  const bool q_aligned = (reinterpret_cast<uintptr_t>(q) & 15) == 0 &&
-                         ((q_stride_seq | q_stride_tok | q_stride_head) & 7) == 0;
+  HY_REQUIRE((reinterpret_cast<uintptr_t>(q.at) & 15) == 0 && ((q.seq | q.tok | q.head) & 7) == 0,
+             "%s: q rows lie on 16 bytes", name);
   if (n_items > 0) {
     void (*kernel)(const uint16_t *, int64_t, int64_t, int64_t, const uint16_t *, int64_t,
                    const int32_t *, int64_t, const int32_t *, const float2 *, float *, int64_t, int,
-                   int, float, bool) = nullptr;
+                   int, float) = nullptr;
     switch (G) {
-      case 1: kernel = hy::weigh_kernel<1>; break;
-      case 2: kernel = hy::weigh_kernel<2>; break;
-      case 4: kernel = hy::weigh_kernel<4>; break;
-      case 8: kernel = hy::weigh_kernel<8>; break;
-      case 16: kernel = hy::weigh_kernel<16>; break;
+      case 1: kernel = weigh_kernel<1>; break;
+      case 2: kernel = weigh_kernel<2>; break;
+      case 4: kernel = weigh_kernel<4>; break;
+      case 8: kernel = weigh_kernel<8>; break;
+      case 16: kernel = weigh_kernel<16>; break;
       default:
         hy::set_error("GQA group size %d unsupported (1, 2, 4, 8, 16)", G);
         return HY_EUNSUPPORTED;
     }
-    hipLaunchKernelGGL(kernel, dim3(num_kv_heads, n_items), dim3(256), 0, st, qq, q_stride_seq,
-                       q_stride_tok, q_stride_head, kp, pool_head_stride, page_table,
-                       page_table_stride, items, ml, partials, partial_stride, num_kv_heads,
-                       page_shift, scale_log2, q_aligned);
+    hipLaunchKernelGGL(kernel, dim3(num_kv_heads, n_items), dim3(256), 0, st, qq, q.seq, q.tok, q.head,
+                       kp, pools.head_stride, pools.page_table, pools.page_table_stride, items, ml, partials, partial_stride, num_kv_heads,
+                       page_shift, scale_log2);
   }
-  hipLaunchKernelGGL(hy::add_kernel, dim3(n_adds), dim3(256), 0, st, adds, scores, score_stride,
+  hipLaunchKernelGGL(add_kernel, dim3(n_adds), dim3(256), 0, st, adds, scores.at, scores.stride,
                      partials, partial_stride, ml, num_q_heads, scale_log2, weights,
                      weights_stride);
-  return hy::launch_status("hy_token_weights");
+  return hy::launch_status(name);
 }

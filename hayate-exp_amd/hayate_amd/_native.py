@@ -145,47 +145,27 @@ _SIGNATURES = {
          _I32, _P],
         ctypes.c_int,
     ),
-    "hy_paged_decode_window": (
-        [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _I32,
-         _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+    "hy_paged_window": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P,
+         _P, _I32, _P, _I32, _I32, _P, _I64, _P, _I32, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32,
+         _I32, _I32, _I32, _I32, _F32, _P],
         ctypes.c_int,
     ),
-    "hy_paged_decode_append_window": (
+    "hy_paged_window_append": (
         [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64,
-         _I64, _P, _P, _F32, _F32, _P, _P, _I32, _P, _P, _P, _I64, _P, _I64, _P, _P, _P, _I32,
-         _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
-        ctypes.c_int,
-    ),
-    "hy_paged_prefill_window": (
-        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
-         _P, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+         _I64, _P, _P, _F32, _F32, _P, _P, _I32, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P,
+         _P, _P, _I32, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32,
+         _P],
         ctypes.c_int,
     ),
     "hy_plan_weigh": (
         [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P],
         ctypes.c_int,
     ),
-    "hy_paged_decode_weigh": (
-        [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _I32,
-         _I32, _I32, _I32, _I32, _F32, _P, _P, _I64, _P],
-        ctypes.c_int,
-    ),
-    "hy_paged_decode_merge_weigh": (
-        [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _P, _P],
-        ctypes.c_int,
-    ),
-    "hy_paged_prefill_weigh": (
-        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
-         _P, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _P, _P],
-        ctypes.c_int,
-    ),
-    "hy_paged_prefill_merge_weigh": (
-        [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P, _P],
-        ctypes.c_int,
-    ),
-    "hy_token_weights": (
-        [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _P, _I64, _P, _I64, _P, _P,
-         _I64, _I32, _I32, _I32, _I32, _F32, _P],
+    "hy_paged_weigh": (
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _P,
+         _P, _I32, _P, _I32, _I32, _P, _I64, _P, _I32, _P, _I32, _I32, _P, _I64, _I32, _I32, _I32,
+         _I32, _I32, _P, _I32, _P, _I32, _P, _P, _I64, _P, _I64, _P, _P, _I64, _F32, _P],
         ctypes.c_int,
     ),
     "hy_keep_positions": (
@@ -408,9 +388,9 @@ def plan_weigh(q_lens: np.ndarray, kv_lens: np.ndarray, rows: np.ndarray, num_q_
     q_lens, kv_lens, rows = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, kv_lens, rows))
     n = len(q_lens)
     blocks = -(-kv_lens.astype(np.int64) // 256)
-    # a range holds 256 rows at least, of at most 16 heads a token
-    ranges = -(-q_lens.astype(np.int64) // 16)
-    items = np.zeros((int((blocks * ranges)[q_lens > 1].sum()) + 1, 8), dtype=np.int32)
+    # (at most 32 ranges of the longest chunk's tokens)
+    chunks = q_lens > 1
+    items = np.zeros((32 * int(blocks[chunks].sum()) + 1, 8), dtype=np.int32)
     adds = np.zeros((int(blocks.sum()) + 1, 8), dtype=np.int32)
     starts, counts = np.zeros(n, dtype=np.int32), np.zeros(5, dtype=np.int64)
     rc = lib().hy_plan_weigh(

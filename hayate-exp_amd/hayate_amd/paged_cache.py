@@ -255,6 +255,8 @@ class PagedKVBatch:
     sinks: int = 0
     # where attention adds up the weight of every cached token: row handle.slot, entry slot
     weights: Optional[torch.Tensor] = None
+    # of batches with one of them: the calls that attend, by query-head count
+    _forms: Optional[dict[int, tuple]] = None
 
     def __init__(
         self,
@@ -274,9 +276,10 @@ class PagedKVBatch:
     ):
         if window is not None:
             self.window, self.sinks = window, sinks
+            self._forms = {}
         if weights is not None:
             self.weights, self._weight_rows = weights, list(weight_rows)
-            self._weigh_plans: dict[int, _DeviceWeighPlan] = {}
+            self._forms, self._weigh_plans = {}, {}
         self.k_cache = manager.k_cache
         self.v_cache = manager.v_cache
         self.page_size = manager.page_size
@@ -636,14 +639,23 @@ class PagedKVBatch:
                 float(scale), stream,
             )
             return a.q_out, result
-        name, windowed = ("hy_paged_decode_append", ()) if self.window is None else (
-            "hy_paged_decode_append_window", (self.window, self.sinks))
-        self._launch(name, getattr(lib, name),
+        if self.window is not None:
+            with _current_device(self.device):
+                self._launch("hy_paged_window_append", lib.hy_paged_window_append,
+                    *a.head, *eps_pair, *a.tables, result.data_ptr(), *os_, k_ptr, v_ptr, hs,
+                    self._pt_ptr, self._pt_stride, self._q_start_ptr, self._cache_lens_ptr,
+                    plan.decode_ptr, plan.n_decode, plan.merge_ptr, plan.n_merge, plan.n_slots,
+                    plan.workspace_ptr, plan.workspace_bytes, self.num_seqs, num_q_heads,
+                    self.num_kv_heads, self.head_dim, self.page_size, float(scale), self.window,
+                    self.sinks, stream,
+                )
+            return a.q_out, result
+        self._launch("hy_paged_decode_append", lib.hy_paged_decode_append,
             *a.head, *eps_pair, *a.tables, result.data_ptr(), k_ptr, v_ptr, hs,
             self._pt_ptr, self._pt_stride, self._q_start_ptr, self._cache_lens_ptr,
             plan.decode_ptr, plan.n_decode, plan.n_slots, plan.workspace_ptr,
             plan.workspace_bytes, self.num_seqs, num_q_heads, self.num_kv_heads,
-            self.head_dim, self.page_size, float(scale), *windowed, stream,
+            self.head_dim, self.page_size, float(scale), stream,
         )
         self._launch("hy_paged_decode_merge", lib.hy_paged_decode_merge,
             result.data_ptr(), *os_, self._q_start_ptr,
@@ -692,8 +704,7 @@ class PagedKVBatch:
         _require_hip(q, "attend_layer")
         if q.dtype != self.k_cache.dtype:
             raise TypeError("q dtype must match the pool dtype")
-        if ((self.window is not None or self.weights is not None)
-                and torch.cuda.current_device() != self.device.index):
+        if self._forms is not None and torch.cuda.current_device() != self.device.index:
             with torch.cuda.device(self.device):  # the launches go to its current stream
                 return self.attend_layer(q, layer_idx, scale)
         q, qs = self._rows(q, "bhtd")
@@ -711,63 +722,70 @@ class PagedKVBatch:
             raise ValueError("query heads must be a multiple of kv heads")
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
+        if self._forms is not None:
+            name, args = self._tick_form(num_q_heads)
+            if self.weights is not None:
+                args = (*args, self.weights.data_ptr(), self.weights.stride(0))
+            self._launch(name, getattr(_native.lib(), name), q.data_ptr(), *qs, result.data_ptr(),
+                         *os_, *self._layer_pools(layer_idx), *args, float(scale), self._stream())
+            return result
         plan = self.plan(num_q_heads)
         k_ptr, v_ptr, hs = self._layer_pools(layer_idx)
         stream = self._stream()
         lib = _native.lib()
-        # the calls' variants and what they take besides
-        kind, merge_kind, window, scores, row_ml = "", "", (), (), ()
-        weigh = None
-        if self.window is not None:
-            kind, window = "_window", (self.window, self.sinks)
-        elif self.weights is not None:
-            weigh = self._weigh_plan(num_q_heads)
-            kind = merge_kind = "_weigh"
-            scores, row_ml = weigh.scores_args, (weigh.row_ml_ptr,)
         if plan.n_decode:
-            name = "hy_paged_decode" + kind
-            self._launch(name, getattr(lib, name),
-                q.data_ptr(), *qs, result.data_ptr(), *(() if kind else os_),
+            self._launch("hy_paged_decode", lib.hy_paged_decode,
+                q.data_ptr(), *qs, result.data_ptr(), *os_,
                 k_ptr, v_ptr, hs,
                 self._pt_ptr, self._pt_stride, self._q_start_ptr, plan.decode_ptr,
                 plan.n_decode, plan.n_slots, plan.workspace_ptr, plan.workspace_bytes, self.num_seqs, num_q_heads,
-                self.num_kv_heads, self.head_dim, self.page_size, float(scale), *window, *scores,
+                self.num_kv_heads, self.head_dim, self.page_size, float(scale),
                 stream,
             )
         if plan.n_merge:
-            name = "hy_paged_decode_merge" + merge_kind
-            self._launch(name, getattr(lib, name),
+            self._launch("hy_paged_decode_merge", lib.hy_paged_decode_merge,
                 result.data_ptr(), *os_, self._q_start_ptr,
                 plan.merge_ptr, plan.n_merge, plan.n_slots,
                 plan.workspace_ptr, plan.workspace_bytes, num_q_heads,
-                self.head_dim, *row_ml, stream,
+                self.head_dim, stream,
             )
         if plan.n_prefill:
-            name = "hy_paged_prefill" + kind
-            self._launch(name, getattr(lib, name),
+            self._launch("hy_paged_prefill", lib.hy_paged_prefill,
                 q.data_ptr(), *qs, result.data_ptr(), *os_,
                 k_ptr, v_ptr, hs,
                 self._pt_ptr, self._pt_stride, self._q_start_ptr, self._kv_lens_ptr,
                 plan.prefill_ptr, plan.n_prefill, plan.n_prefill_slots,
                 plan.prefill_workspace_ptr, plan.prefill_workspace_bytes, self.num_seqs, num_q_heads,
-                self.num_kv_heads, self.head_dim, self.page_size, float(scale), *window, *row_ml,
+                self.num_kv_heads, self.head_dim, self.page_size, float(scale),
                 stream,
             )
         if plan.n_prefill_merge:
-            name = "hy_paged_prefill_merge" + merge_kind
-            self._launch(name, getattr(lib, name),
+            self._launch("hy_paged_prefill_merge", lib.hy_paged_prefill_merge,
                 result.data_ptr(), *os_, self._q_start_ptr,
                 plan.prefill_merge_ptr, plan.n_prefill_merge, plan.n_prefill_slots,
                 plan.prefill_workspace_ptr, plan.prefill_workspace_bytes,
-                num_q_heads, self.num_kv_heads, self.head_dim, *row_ml, stream,
-            )
-        if weigh is not None:
-            self._launch("hy_token_weights", lib.hy_token_weights,
-                q.data_ptr(), *qs, k_ptr, hs, self._pt_ptr, self._pt_stride, *weigh.args,
-                self.weights.data_ptr(), self.weights.stride(0), num_q_heads, self.num_kv_heads,
-                self.head_dim, self.page_size, float(scale), stream,
+                num_q_heads, self.num_kv_heads, self.head_dim, stream,
             )
         return result
+
+    def _tick_form(self, num_q_heads: int) -> tuple:
+        """How a batch with a window or weights attends, in one call: its name, and the arguments
+        between the pools and the scale (the table of weights, or the scale)."""
+        cached = self._forms.get(num_q_heads)
+        if cached is None:
+            plan = self.plan(num_q_heads)
+            args = (self._pt_ptr, self._pt_stride, self._q_start_ptr, self._kv_lens_ptr,
+                    plan.decode_ptr, plan.n_decode, plan.merge_ptr, plan.n_merge, plan.n_slots,
+                    plan.workspace_ptr, plan.workspace_bytes, plan.prefill_ptr, plan.n_prefill,
+                    plan.prefill_merge_ptr, plan.n_prefill_merge, plan.n_prefill_slots,
+                    plan.prefill_workspace_ptr, plan.prefill_workspace_bytes, self.num_seqs,
+                    num_q_heads, self.num_kv_heads, self.head_dim, self.page_size)
+            if self.window is not None:
+                cached = "hy_paged_window", args + (self.window, self.sinks)
+            else:
+                cached = "hy_paged_weigh", args + self._weigh_plan(num_q_heads).args
+            self._forms[num_q_heads] = cached
+        return cached
 
 
 class _DeviceWeighPlan:
@@ -790,14 +808,12 @@ class _DeviceWeighPlan:
         self.memory = (lists, room)
         at = lists.data_ptr()
         items = at + 4 * starts.size
-        self.row_ml_ptr = room.data_ptr()
-        scores_ptr = self.row_ml_ptr + 4 * row_ml if scores else None
-        partials_ptr = self.row_ml_ptr + 4 * (row_ml + scores) if host.parts else None
-        self.scores_args = (scores_ptr, at, host.scores)
-        # hy_token_weights' arguments between the page table and the table of weights
+        base = room.data_ptr()
+        # hy_paged_weigh's arguments between the shape and the table of weights
         self.args = (items if len(host.items) else None, len(host.items),
-                     items + 4 * host.items.size, len(host.adds), scores_ptr, host.scores,
-                     partials_ptr, host.partials, self.row_ml_ptr)
+                     items + 4 * host.items.size, len(host.adds), at,
+                     base + 4 * row_ml if scores else None, host.scores,
+                     base + 4 * (row_ml + scores) if host.parts else None, host.partials, base)
 
 
 class PagedTreeBatch(PagedKVBatch):
@@ -825,6 +841,14 @@ class PagedTreeBatch(PagedKVBatch):
     handles: Sequence[PagedCacheHandle] = ()
     # whether commit_tree took its nodes over already
     committed = False
+    _tree_kind: Optional[tuple[bool, bool]] = None
+
+    def tree_kind(self) -> tuple[bool, bool]:
+        """Whether every tree has one root, and whether no node has two children."""
+        if self._tree_kind is None:
+            self._tree_kind = (all((p[1:] >= 0).all() for p in self.parents),
+                               all(len(np.unique(p)) == len(p) for p in self.parents))
+        return self._tree_kind
 
     def __init__(self, manager: "PagedKVCacheManager", parents: Sequence[np.ndarray],
                  cache_lens_host: list[int], page_lists: list[list[int]],

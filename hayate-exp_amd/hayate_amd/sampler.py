@@ -181,14 +181,17 @@ def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tenso
     if not len(temperature) == len(top_k) == len(top_p) == requests:
         raise ValueError("one temperature, top_k and top_p per request is required")
     for t, k, p in zip(temperature, top_k, top_p):
-        validate_parameters(t, k, p)
-        if t and not 1e-30 <= t <= 1e30:
-            raise ValueError("verification takes temperatures of 0 or 1e-30 to 1e30")
-    for parents in batch.parents:
-        if (parents[1:] < 0).any():
-            raise ValueError("a tree to verify has one root, node 0")
-        if draft_probs is not None and len(np.unique(parents)) != len(parents):
-            raise NotImplementedError("with draft_probs a node has at most one child")
+        # (the usual types in the usual ranges need no closer look)
+        if not ((k is None or type(k) is int and k >= 1) and (p is None or type(p) is float and 0 < p <= 1)
+                and type(t) is float and (t == 0 or 1e-30 <= t <= 1e30)):
+            validate_parameters(t, k, p)
+            if t and not 1e-30 <= t <= 1e30:
+                raise ValueError("verification takes temperatures of 0 or 1e-30 to 1e30")
+    one_root, chains = batch.tree_kind()
+    if not one_root:
+        raise ValueError("a tree to verify has one root, node 0")
+    if draft_probs is not None and not chains:
+        raise NotImplementedError("with draft_probs a node has at most one child")
     if logits.dim() == 3 and logits.shape[1] == 1:
         logits = logits[:, 0]
     if logits.dtype not in _DTYPES:
@@ -207,23 +210,26 @@ def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tenso
         if draft_probs.shape != (n, vocab):
             raise ValueError(f"draft_probs must be ({n}, {vocab})")
         given.append(draft_probs)
-    if any(t.device != batch.device for t in given):
-        raise ValueError(f"logits, tokens and uniforms must be on the pool's device, {batch.device}")
-    if batch.device.type != "cuda":
+    dev = batch.device
+    for t in given:
+        if t.device != dev:
+            raise ValueError(f"logits, tokens and uniforms must be on the pool's device, {dev}")
+    if dev.type != "cuda":
         raise RuntimeError("verify_tree runs only on a HIP device; there is no CPU implementation")
-    if torch.cuda.current_device() != batch.device.index:
-        with torch.cuda.device(batch.device):
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
             return verify_tree(batch, logits, tokens, temperature, top_k, top_p, uniforms,
                                draft_probs)
-    logits, tokens, uniforms = (t if t.stride(-1) == 1 else t.contiguous()
-                                for t in (logits, tokens, uniforms))
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    tokens, uniforms = tokens.contiguous(), uniforms.contiguous()
     if draft_probs is not None and draft_probs.stride(1) != 1:
         draft_probs = draft_probs.contiguous()
-    dev, lib = batch.device, _native.lib()
-    temp = np.asarray(list(map(float, temperature)), dtype=np.float32)
-    k = np.asarray([vocab if v is None else min(v, vocab) for v in top_k], dtype=np.int32)
-    p = np.asarray([1.0 if v is None else max(float(v), _TINY) for v in top_p], dtype=np.float32)
-    q_lens = np.asarray(batch.q_lens, dtype=np.int32)
+    lib = _native.lib()
+    temp = np.array(temperature, dtype=np.float32)
+    k = np.array([vocab if v is None or v > vocab else v for v in top_k], dtype=np.int32)
+    p = np.array([1.0 if v is None else max(v, _TINY) for v in top_p], dtype=np.float32)
+    q_lens = np.array(batch.q_lens, dtype=np.int32)
     paths = torch.empty((requests, batch.levels), dtype=torch.int32, device=dev)
     lengths = torch.empty(requests, dtype=torch.int32, device=dev)
     drawn = torch.empty((requests, 1), dtype=torch.int64, device=dev)

@@ -555,20 +555,22 @@ int hy_page_copy(void *k_pool, void *v_pool, int64_t pool_layer_stride,
                  void *stream);
 
 /*
- * Attention with a sliding window and sinks: the query of sequence b at
- * position i sees the keys j <= i with i - j < window or j < sinks, positions
- * being slots of the cache. window >= 1, 0 <= sinks <= 2^30.
+ * Attention with a sliding window and sinks, of a whole tick in one call: the
+ * query of sequence b at position i sees the keys j <= i with i - j < window or
+ * j < sinks, positions being slots of the cache. window >= 1, 0 <= sinks <=
+ * 2^30. What K and V of a key hold that a row does not see (infinities, NaN)
+ * never reaches the row. The arguments are those of hy_paged_decode,
+ * hy_paged_decode_merge, hy_paged_prefill and hy_paged_prefill_merge, whose
+ * launches the call makes.
  *
  * hy_plan_tick_window is hy_plan_tick for it. The key ranges of its lists
- * count the keys in sight only: with u = 32 for decode pieces and 64 for
- * prefill items, and p the position of the sequence's token or of the item's
- * first one, keys are left out from ns = ceil(sinks / u) u up to
- * floor((p - window + 1) / u) u, and number x from ns on is key x + gap, gap
- * being how many they are. The other calls take these lists and the same
- * window and sinks as their counterparts without "_window", and write what
- * those write; hy_paged_decode_merge and hy_paged_prefill_merge follow. What
- * K and V of a key hold that a row does not see (infinities, NaN) never
- * reaches the row.
+ * count the keys in sight only: with p the position of the sequence's token or
+ * of the item's first one, keys are left out from ns = ceil(sinks / 32) 32 up
+ * to floor((p - window + 1) / 32) 32, and number x from ns on is key x + gap,
+ * gap being how many they are.
+ *
+ * hy_paged_window_append is hy_paged_decode_append and its merge with a
+ * window, from the same lists (sequences with one token each).
  * No reference counterpart: the reference attends to the whole cache.
  */
 int hy_plan_tick_window(const int32_t *q_lens, const int32_t *kv_lens,
@@ -582,18 +584,22 @@ int hy_plan_tick_window(const int32_t *q_lens, const int32_t *kv_lens,
                         int32_t *prefill_merge_items,
                         int32_t prefill_merge_capacity, int32_t *counts_out);
 
-int hy_paged_decode_window(
+int hy_paged_window(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
-    int64_t q_stride_head, void *out, const void *k_pool, const void *v_pool,
-    int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *decode_items, int32_t n_decode, int32_t n_slots,
-    void *workspace, int64_t workspace_bytes, int32_t num_seqs,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t page_size, float scale, int32_t window, int32_t sinks,
-    void *stream);
+    int64_t q_stride_head, void *out, int64_t o_stride_seq,
+    int64_t o_stride_tok, int64_t o_stride_head, const void *k_pool,
+    const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
+    int64_t page_table_stride, const int32_t *q_start, const int32_t *kv_lens,
+    const int32_t *decode_items, int32_t n_decode, const int32_t *merge_items,
+    int32_t n_merge, int32_t n_slots, void *workspace,
+    int64_t workspace_bytes, const int32_t *prefill_items, int32_t n_prefill,
+    const int32_t *prefill_merge_items, int32_t n_prefill_merge,
+    int32_t n_prefill_slots, void *prefill_workspace,
+    int64_t prefill_workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t window,
+    int32_t sinks, float scale, void *stream);
 
-int hy_paged_decode_append_window(
+int hy_paged_window_append(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
     int64_t q_stride_head, void *q_out, int64_t qo_stride_seq,
     int64_t qo_stride_tok, int64_t qo_stride_head, const void *k,
@@ -602,48 +608,38 @@ int hy_paged_decode_append_window(
     int64_t v_stride_head, const void *q_norm_weight,
     const void *k_norm_weight, float q_eps, float k_eps,
     const float *cos_table, const float *sin_table, int32_t max_positions,
-    void *out, void *k_pool, void *v_pool, int64_t pool_head_stride,
-    const int32_t *page_table, int64_t page_table_stride,
-    const int32_t *q_start, const int32_t *cache_lens,
-    const int32_t *decode_items, int32_t n_decode, int32_t n_slots,
+    void *out, int64_t o_stride_seq, int64_t o_stride_tok,
+    int64_t o_stride_head, void *k_pool, void *v_pool,
+    int64_t pool_head_stride, const int32_t *page_table,
+    int64_t page_table_stride, const int32_t *q_start,
+    const int32_t *cache_lens, const int32_t *decode_items, int32_t n_decode,
+    const int32_t *merge_items, int32_t n_merge, int32_t n_slots,
     void *workspace, int64_t workspace_bytes, int32_t num_seqs,
     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
     int32_t page_size, float scale, int32_t window, int32_t sinks,
     void *stream);
 
-int hy_paged_prefill_window(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
-    int64_t q_stride_head, void *out, int64_t o_stride_seq,
-    int64_t o_stride_tok, int64_t o_stride_head, const void *k_pool,
-    const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill,
-    int32_t n_slots, void *workspace, int64_t workspace_bytes,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, int32_t page_size, float scale, int32_t window,
-    int32_t sinks, void *stream);
-
 /*
- * What weight every cached token got: weights[rows[b] * weights_stride + j] +=
- * the sum, over the tokens of sequence b's tick and all query heads, of the
- * softmax probability of key j (fp32; j < kv_lens[b], other entries are left
- * alone). Attention itself runs as above, through the calls with "_weigh",
- * which besides leave what the sums need:
- *   row_ml   per packed row and query head the exponent base (exp2 domain) and
- *            the sum of its softmax: 2 fp32 each, total tokens * num_q_heads;
- *   scores   of sequences with one token the raw scores q . k: fp32, one row of
- *            score_stride (>= the planned count, a multiple of 4, 16-byte
- *            aligned) per query head, sequence b's from score_start[b] on.
- * hy_token_weights, enqueued after them on the same stream, adds the weights:
- * those of single tokens from the scores, those of chunks from their products,
- * computed again, through partials (partial_stride * planned parts *
- * num_kv_heads fp32, 16-byte aligned).
+ * Attention of a whole tick (lists of hy_plan_tick) that also adds up what
+ * weight every cached token got: weights[rows[b] * weights_stride + j] += the
+ * sum, over the tokens of sequence b's tick and all query heads, of the softmax
+ * probability of key j (fp32; j < kv_lens[b], other entries are left alone).
+ * Rows of q lie on 16 bytes.
+ * Besides the lists of hy_plan_weigh the call takes room for what its launches
+ * leave each other:
+ *   row_ml    2 fp32 a packed row and query head, on 8 bytes: the exponent base
+ *             (exp2 domain) and the sum of its softmax;
+ *   scores    the raw scores of sequences with one token: num_q_heads rows of
+ *             score_stride fp32 (at least the planned count, a multiple of 4,
+ *             on 16 bytes);
+ *   partials  the sums of chunks, whose products are computed again: planned
+ *             parts * num_kv_heads rows of partial_stride fp32, likewise.
  * Results do not depend on the order in which workgroups run.
  *
  * hy_plan_weigh (host) makes the lists. score_start has num_seqs entries, items
  * and adds 8 int32 a record, counts_out five: items, additions, scores a row,
  * partials a row, parts. ceil(kv_len / 256) additions a sequence, and for
- * chunks at most ceil(kv_len / 256) * ceil(q_len / 16) items.
+ * chunks at most 32 times as many items.
  * No reference counterpart: the reference keeps no attention weights.
  */
 int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens,
@@ -652,53 +648,23 @@ int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens,
                   int32_t *items, int32_t item_capacity, int32_t *adds,
                   int32_t add_capacity, int64_t *counts_out);
 
-int hy_paged_decode_weigh(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
-    int64_t q_stride_head, void *out, const void *k_pool, const void *v_pool,
-    int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *decode_items, int32_t n_decode, int32_t n_slots,
-    void *workspace, int64_t workspace_bytes, int32_t num_seqs,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t page_size, float scale, float *scores,
-    const int32_t *score_start, int64_t score_stride, void *stream);
-
-int hy_paged_decode_merge_weigh(
-    void *out, int64_t o_stride_seq, int64_t o_stride_tok,
-    int64_t o_stride_head, const int32_t *q_start, const int32_t *merge_items,
-    int32_t n_merge, int32_t n_slots, const void *workspace,
-    int64_t workspace_bytes, int32_t num_q_heads, int32_t head_dim,
-    float *row_ml, void *stream);
-
-int hy_paged_prefill_weigh(
+int hy_paged_weigh(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
     int64_t q_stride_head, void *out, int64_t o_stride_seq,
     int64_t o_stride_tok, int64_t o_stride_head, const void *k_pool,
     const void *v_pool, int64_t pool_head_stride, const int32_t *page_table,
-    int64_t page_table_stride, const int32_t *q_start,
-    const int32_t *kv_lens, const int32_t *prefill_items, int32_t n_prefill,
-    int32_t n_slots, void *workspace, int64_t workspace_bytes,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, int32_t page_size, float scale, float *row_ml,
-    void *stream);
-
-int hy_paged_prefill_merge_weigh(
-    void *out, int64_t o_stride_seq, int64_t o_stride_tok,
-    int64_t o_stride_head, const int32_t *q_start, const int32_t *merge_items,
-    int32_t n_merge, int32_t n_slots, const void *workspace,
-    int64_t workspace_bytes, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, float *row_ml, void *stream);
-
-int hy_token_weights(
-    const void *q, int64_t q_stride_seq, int64_t q_stride_tok,
-    int64_t q_stride_head, const void *k_pool, int64_t pool_head_stride,
-    const int32_t *page_table, int64_t page_table_stride,
-    const int32_t *items, int32_t n_items, const int32_t *adds,
-    int32_t n_adds, const float *scores, int64_t score_stride,
-    float *partials, int64_t partial_stride, const float *row_ml,
-    float *weights, int64_t weights_stride, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float scale,
-    void *stream);
+    int64_t page_table_stride, const int32_t *q_start, const int32_t *kv_lens,
+    const int32_t *decode_items, int32_t n_decode, const int32_t *merge_items,
+    int32_t n_merge, int32_t n_slots, void *workspace,
+    int64_t workspace_bytes, const int32_t *prefill_items, int32_t n_prefill,
+    const int32_t *prefill_merge_items, int32_t n_prefill_merge,
+    int32_t n_prefill_slots, void *prefill_workspace,
+    int64_t prefill_workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, const int32_t *weigh_items,
+    int32_t n_weigh, const int32_t *add_items, int32_t n_add,
+    const int32_t *score_start, float *scores, int64_t score_stride,
+    float *partials, int64_t partial_stride, float *row_ml, float *weights,
+    int64_t weights_stride, float scale, void *stream);
 
 /*
  * Which tokens stay when caches are cut to `budget`: of sequence b with
