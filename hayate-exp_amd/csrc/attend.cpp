@@ -21,9 +21,7 @@ struct Tick {
   hy::Shape shape;
 };
 
-int attend(const char *name, const Tick &t, const hy::Window &window, const hy::Scores &scores,
-           float *row_ml, void *stream) {
-  // (every list is looked at before the first launch)
+int check(const char *name, const Tick &t) {
   if (t.decode.count < 0 || t.decode_merge.count < 0 || t.prefill.count < 0 ||
       t.prefill_merge.count < 0) {
     hy::set_error("%s: item counts must be non-negative", name);
@@ -34,12 +32,11 @@ int attend(const char *name, const Tick &t, const hy::Window &window, const hy::
     hy::set_error("%s: a merge list without the work before it, or the reverse", name);
     return HY_EINVAL;
   }
-  if (int rc = hy::decode(name, t.q, t.out, t.pools, t.q_start, t.decode, t.decode_ws, t.shape,
-                          window, scores, nullptr, stream))
-    return rc;
-  if (int rc = hy::decode_merge(name, t.out, t.q_start, t.decode_merge, t.decode_ws, t.shape, row_ml,
-                                stream))
-    return rc;
+  return HY_OK;
+}
+
+int attend_chunks(const char *name, const Tick &t, const hy::Window &window, float *row_ml,
+                  void *stream) {
   if (int rc = hy::prefill(name, t.q, t.out, t.pools, t.q_start, t.kv_lens, t.prefill, t.prefill_ws,
                            t.shape, window, row_ml, stream))
     return rc;
@@ -78,7 +75,14 @@ extern "C" int hy_paged_window(
   hy::clear_error();
   const hy::Window w{window, sinks};
   if (int rc = hy::check_window(name, w)) return rc;
-  return attend(name, HY_TICK, w, {}, nullptr, stream);
+  const Tick t = HY_TICK;
+  if (int rc = check(name, t)) return rc;
+  if (int rc = hy::decode(name, t.q, t.out, t.pools, t.q_start, t.decode, t.decode_ws, t.shape, w, {},
+                          nullptr, stream))
+    return rc;
+  if (int rc = hy::decode_merge(name, t.out, t.q_start, t.decode_merge, t.decode_ws, t.shape, stream))
+    return rc;
+  return attend_chunks(name, t, w, nullptr, stream);
 }
 
 extern "C" int hy_paged_weigh(
@@ -97,16 +101,20 @@ extern "C" int hy_paged_weigh(
     int64_t weights_stride, float scale, void *stream) {
   const char *name = "hy_paged_weigh";
   hy::clear_error();
-  if ((n_decode > 0 && !(scores && score_start)) || (n_prefill > 0 && !partials) ||
-      ((n_decode > 0 || n_prefill > 0) && !(row_ml && weights && add_items)) || n_weigh < 0 ||
-      n_weigh > 65535 || n_add < 0 || (n_weigh > 0 && !(weigh_items && partials))) {
-    hy::set_error("%s: null pointer argument, or %d items (0 to 65535)", name, n_weigh);
+  const Tick t = HY_TICK;
+  if (int rc = check(name, t)) return rc;
+  if ((n_decode > 0 && !(scores && score_start)) || (n_prefill > 0 && !(partials && row_ml))) {
+    hy::set_error("%s: null pointer argument", name);
     return HY_EINVAL;
   }
-  const Tick tick = HY_TICK;
-  const hy::Scores of{n_decode > 0 ? scores : nullptr, score_start, score_stride};
-  if (int rc = attend(name, tick, {}, of, row_ml, stream)) return rc;
-  return hy::token_weights(name, tick.q, tick.pools, tick.shape, weigh_items, n_weigh, add_items,
-                           n_add, of, partials, partial_stride, row_ml, weights, weights_stride,
-                           stream);
+  const hy::Weigh w{weigh_items, n_weigh,        add_items, n_add,
+                    {n_decode > 0 ? scores : nullptr, score_start, score_stride},
+                    partials,    partial_stride, row_ml,    weights, weights_stride};
+  if (int rc = hy::check_weigh(name, t.q, t.shape, w)) return rc;
+  if (int rc = hy::decode(name, t.q, t.out, t.pools, t.q_start, t.decode, t.decode_ws, t.shape, {},
+                          w.scores, nullptr, stream))
+    return rc;
+  if (int rc = attend_chunks(name, t, {}, row_ml, stream)) return rc;
+  if (int rc = hy::weigh_chunks(name, t.q, t.pools, t.shape, w, stream)) return rc;
+  return hy::finish_weights(name, t.out, t.decode_merge, t.decode_ws, t.shape, w, stream);
 }

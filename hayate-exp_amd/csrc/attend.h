@@ -45,17 +45,33 @@ int decode(const char *name, const Rows &q, const Rows &out, const Pools &pools,
            const int32_t *q_start, const Items &items, const Workspace &ws, const Shape &shape,
            const Window &window, const Scores &scores, const AppendArgs *append, void *stream);
 int decode_merge(const char *name, const Rows &out, const int32_t *q_start, const Items &items,
-                 const Workspace &ws, const Shape &shape, float *row_ml, void *stream);
+                 const Workspace &ws, const Shape &shape, void *stream);
 int prefill(const char *name, const Rows &q, const Rows &out, const Pools &pools,
             const int32_t *q_start, const int32_t *kv_lens, const Items &items,
             const Workspace &ws, const Shape &shape, const Window &window, float *row_ml,
             void *stream);
 int prefill_merge(const char *name, const Rows &out, const int32_t *q_start, const Items &items,
                   const Workspace &ws, const Shape &shape, float *row_ml, void *stream);
-int token_weights(const char *name, const Rows &q, const Pools &pools, const Shape &shape,
-                  const int32_t *items, int32_t n_items, const int32_t *adds, int32_t n_adds,
-                  const Scores &scores, float *partials, int64_t partial_stride,
-                  const float *row_ml, float *weights, int64_t weights_stride, void *stream);
+// The weights of a tick's tokens: what its chunks' products (computed again) and its decode tokens'
+// scores say. finish_weights() joins the decode tokens' partials, as decode_merge() does, and adds
+// to the table.
+struct Weigh {
+  const int32_t *items;
+  int32_t n_items;
+  const int32_t *adds;
+  int32_t n_adds;
+  Scores scores;
+  float *partials;
+  int64_t partial_stride;
+  float *row_ml;
+  float *weights;
+  int64_t weights_stride;
+};
+int check_weigh(const char *name, const Rows &q, const Shape &shape, const Weigh &weigh);
+int weigh_chunks(const char *name, const Rows &q, const Pools &pools, const Shape &shape,
+                 const Weigh &weigh, void *stream);
+int finish_weights(const char *name, const Rows &out, const Items &merge, const Workspace &ws,
+                   const Shape &shape, const Weigh &weigh, void *stream);
 
 int check_window(const char *name, const Window &window);
 

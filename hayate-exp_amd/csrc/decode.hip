@@ -565,13 +565,11 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // partial (the split index is clamped to the last one) and the ones past
 // num_partials are then replaced by the empty partial, so no load sits
 // behind a branch. A lane whose head is past num_q_heads computes on a
-// clamped head and does not store. row_ml (if given) gets each row's maximum, in the exp2
-// domain, and sum, by packed row and query head.
+// clamped head and does not store.
 __global__ __launch_bounds__(128) void decode_merge_kernel(
     uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
     const int32_t *__restrict__ q_start, const int32_t *__restrict__ items,
-    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_q_heads,
-    float2 *__restrict__ row_ml) {
+    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml, int num_q_heads) {
   const int4 it = *reinterpret_cast<const int4 *>(items + 4 * blockIdx.x);
   const int seq = it.x;
   const int first = it.y;
@@ -615,7 +613,6 @@ __global__ __launch_bounds__(128) void decode_merge_kernel(
     mx = cmx;
   }
   if (hq_lane >= num_q_heads) return;
-  if (row_ml != nullptr && d == 0) row_ml[qs * num_q_heads + hq] = make_float2(mx, lsum);
   uint16_t *dst = out + seq * o_ss + qs * o_st + hq * o_sh + d;
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2_rne(a[0] / lsum, a[1] / lsum),
                                                pack_bf16x2_rne(a[2] / lsum, a[3] / lsum));
@@ -798,7 +795,7 @@ int decode_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t
                       int64_t o_stride_head, const int32_t *q_start, const int32_t *merge_items,
                       int32_t n_merge, int32_t n_slots, const void *workspace,
                       int64_t workspace_bytes, int32_t num_q_heads, int32_t head_dim,
-                      void *stream, float *row_ml = nullptr) {
+                      void *stream) {
   HY_REQUIRE(n_merge >= 0 && n_slots >= 0, "item counts must be non-negative");
   if (n_merge == 0) return HY_OK;
   HY_REQUIRE_SUPPORTED(head_dim == kHeadDim, "head_dim %d unsupported (need %d)", head_dim,
@@ -819,7 +816,7 @@ int decode_merge_impl(const char *name, void *out, int64_t o_stride_seq, int64_t
   hipLaunchKernelGGL(hy::decode_merge_kernel, dim3(n_merge, (num_q_heads + 3) / 4), dim3(128), 0,
                      static_cast<hipStream_t>(stream), static_cast<uint16_t *>(out),
                      o_stride_seq, o_stride_tok, o_stride_head, q_start, merge_items, ws_acc,
-                     ws_ml, num_q_heads, reinterpret_cast<float2 *>(row_ml));
+                     ws_ml, num_q_heads);
   return hy::launch_status(name);
 }
 
@@ -890,9 +887,9 @@ int hy::decode(const char *name, const Rows &q, const Rows &out, const Pools &po
 }
 
 int hy::decode_merge(const char *name, const Rows &out, const int32_t *q_start, const Items &items,
-                     const Workspace &ws, const Shape &s, float *row_ml, void *stream) {
+                     const Workspace &ws, const Shape &s, void *stream) {
   return decode_merge_impl(name, out.at, out.seq, out.tok, out.head, q_start, items.at, items.count,
-                           items.slots, ws.at, ws.bytes, s.num_q_heads, s.head_dim, stream, row_ml);
+                           items.slots, ws.at, ws.bytes, s.num_q_heads, s.head_dim, stream);
 }
 
 extern "C" int hy_paged_window_append(
@@ -927,8 +924,7 @@ extern "C" int hy_paged_window_append(
                                            page_table_stride},
                           q_start, {decode_items, n_decode, n_slots}, ws, shape, w, {}, &ap, stream))
     return rc;
-  return hy::decode_merge(name, to, q_start, {merge_items, n_merge, n_slots}, ws, shape, nullptr,
-                          stream);
+  return hy::decode_merge(name, to, q_start, {merge_items, n_merge, n_slots}, ws, shape, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -919,7 +919,7 @@ int64_t weigh_range(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_s
 
 int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
                int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
-               int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds,
+               const int32_t *merge_items, int32_t n_merge, int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds,
                int32_t add_capacity, int64_t *counts_out) {
   constexpr int64_t keys = hy::kWeighKeys;
   const int64_t G = num_q_heads / num_kv_heads;
@@ -928,7 +928,14 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
       std::max<int64_t>(1, (num_cus > 0 ? num_cus : 256) * kWeighPerCu / num_kv_heads);
   const int64_t range = weigh_range(q_lens, kv_lens, num_seqs, G, slots);
   int64_t scores = 0, partials = 0, q_row = 0, n_items = 0, n_adds = 0, parts_max = 0;
+  // the partial slots of every decode token
+  std::vector<const int32_t *> slots_of(static_cast<size_t>(num_seqs), nullptr);
+  for (int i = 0; i < n_merge; ++i) slots_of[merge_items[4 * i]] = merge_items + 4 * i;
   for (int b = 0; b < num_seqs; ++b) {
+    if (q_lens[b] == 1 && slots_of[b] == nullptr) {
+      hy::set_error("hy_plan_weigh: sequence %d has no merge item", b);
+      return HY_EINVAL;
+    }
     const int64_t kv = kv_lens[b], ql = q_lens[b], cache = kv - ql;
     const bool chunk = ql > 1;
     const WeighParts parts(ql, range);
@@ -945,9 +952,9 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
       a[0] = rows[b];
       a[1] = static_cast<int32_t>(t0);
       a[2] = static_cast<int32_t>(std::min(kv, t0 + keys));
-      a[3] = static_cast<int32_t>(chunk ? (n_parts - first) * num_kv_heads : num_q_heads);
-      a[4] = static_cast<int32_t>(chunk ? first * num_kv_heads : 0);
-      a[5] = static_cast<int32_t>(chunk ? -1 : q_row);
+      a[3] = chunk ? static_cast<int32_t>((n_parts - first) * num_kv_heads) : slots_of[b][2];
+      a[4] = chunk ? static_cast<int32_t>(first * num_kv_heads) : slots_of[b][1];
+      a[5] = !chunk;
       a[6] = static_cast<int32_t>(chunk ? partials : scores);
       a[7] = 0;
       for (int64_t p = first; chunk && p < n_parts; ++p) {
@@ -998,15 +1005,22 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
 
 extern "C" int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
                              int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
-                             int32_t num_cus, int32_t *score_start, int32_t *items,
-                             int32_t item_capacity, int32_t *adds, int32_t add_capacity,
+                             int32_t num_cus, const int32_t *merge_items, int32_t n_merge,
+                             int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds, int32_t add_capacity,
                              int64_t *counts_out) {
   hy::clear_error();
   if (num_seqs < 0 || counts_out == nullptr ||
       (num_seqs > 0 && (!q_lens || !kv_lens || !rows || !score_start)) ||
-      (item_capacity > 0 && items == nullptr) || (add_capacity > 0 && adds == nullptr)) {
+      (item_capacity > 0 && items == nullptr) || (add_capacity > 0 && adds == nullptr) ||
+      n_merge < 0 || (n_merge > 0 && merge_items == nullptr)) {
     hy::set_error("hy_plan_weigh: invalid arrays");
     return HY_EINVAL;
+  }
+  for (int i = 0; i < n_merge; ++i) {
+    if (merge_items[4 * i] < 0 || merge_items[4 * i] >= num_seqs) {
+      hy::set_error("hy_plan_weigh: merge item %d is of sequence %d", i, merge_items[4 * i]);
+      return HY_EINVAL;
+    }
   }
   if (num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads % num_kv_heads) {
     hy::set_error("hy_plan_weigh: num_q_heads (%d) must be a multiple of num_kv_heads (%d)",
@@ -1027,7 +1041,8 @@ extern "C" int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, cons
   }
   try {
     return plan_weigh(q_lens, kv_lens, rows, num_seqs, num_q_heads, num_kv_heads, num_cus,
-                      score_start, items, item_capacity, adds, add_capacity, counts_out);
+                      merge_items, n_merge, score_start, items, item_capacity, adds, add_capacity,
+                      counts_out);
   } catch (const std::bad_alloc &) {
     hy::set_error("hy_plan_weigh: out of host memory");
     return HY_ENOSPACE;

@@ -1,13 +1,15 @@
 // What weight every cached token got from a tick's queries, added to a table (gfx950):
 //   w[t] += sum over the sequence's rows i and query heads h of
 //           exp(scale q_ih . k_t - max_ih) / sum_ih,   t <= position of i,
-// with the row maxima and sums that the attention kernels leave (row_ml, exp2 domain).
+// with the rows' maxima and sums that the attention kernels leave (exp2 domain).
 //
 // Single tokens: the decode kernel has stored its raw scores, 4 bytes a head and key where K and
-// V take 512 bytes a kv head and key; add_kernel turns them into weights and sums the heads.
+// V take 512 bytes a kv head and key; finish_kernel turns them into weights and sums the heads,
+// beside the workgroups that join the decode partials (instead of a launch of its own behind the
+// merge: 18.1 -> 15.1 us for one token on 2,000, 91 -> 89 for 32 on 4,096).
 // Chunks: storing scores would cost more than the products (512 rows x 32 heads x 4 bytes a key),
 // so weigh_kernel computes them again from K and Q, an item 256 keys by a range of rows, and
-// leaves a sum per kv head, range and key; add_kernel adds those. Every sum has a fixed order.
+// leaves a sum per kv head, range and key; finish_kernel adds those. Every sum has a fixed order.
 //
 // weigh_kernel: one workgroup of four waves per (kv head, item), each wave 64 keys whose K it
 // keeps in registers; the rows go through LDS, 64 a stage, and meet them in
@@ -25,6 +27,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStageElems = kWeighRows * kHeadDim;
 constexpr int kStages = 3;
+constexpr int kMaxHeads = 1024;  // query heads
 
 __device__ __forceinline__ void load_to_lds(const uint16_t *g, const uint16_t *lds) {
   const uint32_t m0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -243,42 +246,151 @@ void weigh_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, in
   }
 }
 
-// Item = {row of the table, t0, t1, sources, first source, q_row or -1, offset, 0}: at most 256
-// tokens [t0, t1). With q_row >= 0 the sources are the scores of the query heads, turned into
-// weights by the row's maxima and sums; else partial sums. Source x of token t is at
-// src[x * stride + offset + t]. Four waves take the sources in turn.
-__global__ __launch_bounds__(256) void add_kernel(
+// Partials of a decode token that one lane joins in a round.
+constexpr int kRound = 8;
+
+// One decode token's output from its partials: the sums of decode_merge_kernel in its order, by 32
+// lanes a head, with the next round's loads out before a round is used. it = {seq, first slot,
+// slots, q_row}.
+__device__ __forceinline__ void join_partials(const int32_t *it, int heads0, uint16_t *out,
+                                              int64_t o_ss, int64_t o_st, int64_t o_sh,
+                                              const float *ws_acc, const float *ws_ml,
+                                              int num_q_heads) {
+  const int seq = it[0], first = it[1], n = it[2];
+  const int64_t q_row = it[3];
+  const int mine = heads0 + static_cast<int>(threadIdx.x >> 5);
+  const int hq = min(mine, num_q_heads - 1);
+  const int d = (threadIdx.x & 31) * 4;
+  struct Round {
+    float2 ml[kRound];
+    f32x4 x[kRound];
+  };
+  auto load = [&](Round &r, int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kRound; ++j) {
+      const int64_t at = static_cast<int64_t>(first + min(s0 + j, n - 1)) * num_q_heads + hq;
+      r.ml[j] = *reinterpret_cast<const float2 *>(ws_ml + at * 2);
+      r.x[j] = *reinterpret_cast<const f32x4 *>(ws_acc + at * kHeadDim + d);
+    }
+  };
+  float mx = -INFINITY, lsum = 0.f;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  auto join = [&](const Round &r, int s0) __attribute__((always_inline)) {
+    float m[kRound], top = mx;
+#pragma unroll
+    for (int j = 0; j < kRound; ++j) {
+      m[j] = s0 + j < n ? r.ml[j].x : -INFINITY;
+      top = fmaxf(top, m[j]);
+    }
+    const float old = mx == -INFINITY ? 0.f : exp2f(mx - top);
+    lsum *= old;
+    a *= old;
+#pragma unroll
+    for (int j = 0; j < kRound; ++j) {
+      const bool live = s0 + j < n;
+      const float f = m[j] == -INFINITY ? 0.f : exp2f(m[j] - top);
+      lsum += f * (live ? r.ml[j].y : 0.f);
+      a += f * (live ? r.x[j] : f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    mx = top;
+  };
+  Round even, odd;
+  load(even, 0);
+  for (int s0 = 0; s0 < n; s0 += 2 * kRound) {
+    if (s0 + kRound < n) load(odd, s0 + kRound);
+    join(even, s0);
+    if (s0 + kRound >= n) break;
+    if (s0 + 2 * kRound < n) load(even, s0 + 2 * kRound);
+    join(odd, s0 + kRound);
+  }
+  if (mine >= num_q_heads) return;
+  uint16_t *dst = out + seq * o_ss + q_row * o_st + hq * o_sh + d;
+  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2_rne(a[0] / lsum, a[1] / lsum),
+                                               pack_bf16x2_rne(a[2] / lsum, a[3] / lsum));
+}
+
+// The first n_join * groups workgroups join the partials of eight heads of a decode token each; the
+// others add to the table. Item = {row of the table, t0, t1, sources, first source, decode,
+// offset, 0}: at most 256 tokens [t0, t1). Of a chunk the sources are rows of partial sums; of a
+// decode token they are its partial slots, whose maxima and sums turn the scores of all query
+// heads into weights. Source or head x of token t is at src[x * stride + offset + t]; four waves
+// take them in turn.
+__global__ __launch_bounds__(256) void finish_kernel(
+    uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
+    const int32_t *__restrict__ join_items, int n_join, int groups,
+    const float *__restrict__ ws_acc, const float *__restrict__ ws_ml,
     const int32_t *__restrict__ items, const float *__restrict__ scores, int64_t score_stride,
-    const float *__restrict__ partials, int64_t partial_stride,
-    const float2 *__restrict__ row_ml, int num_q_heads, float scale_log2,
+    const float *__restrict__ partials, int64_t partial_stride, int num_q_heads, float scale_log2,
     float *__restrict__ weights, int64_t weights_stride) {
   __shared__ f32x4 box[3][64];
-  const int32_t *it = items + 8 * blockIdx.x;
-  const int row = it[0], t0 = it[1], t1 = it[2], n = it[3], from = it[4], q_row = it[5];
+  __shared__ float2 head_ml[kMaxHeads], part_ml[4][64];
+  const int bid = blockIdx.x;
+  if (bid < n_join * groups) {
+    join_partials(join_items + 4 * (bid / groups), 8 * (bid % groups), out, o_ss, o_st, o_sh,
+                  ws_acc, ws_ml, num_q_heads);
+    return;
+  }
+  const int32_t *it = items + 8 * (bid - n_join * groups);
+  const int row = it[0], t0 = it[1], t1 = it[2], n = it[3], from = it[4];
+  const bool decode = it[5] != 0;
   const int64_t off = it[6];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int t = t0 + 4 * lane;
   const bool live = t < t1;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    if (q_row >= 0) {
-      const float2 *ml = row_ml + static_cast<int64_t>(q_row) * num_q_heads;
-#pragma unroll 4
-      for (int x = wave; x < n; x += 4) {
+  if (decode) {
+    // every head's maximum and inverse sum: lanes are heads, waves take the slots in turn
+    for (int h0 = 0; h0 < num_q_heads; h0 += 64) {
+      const int h = min(h0 + lane, num_q_heads - 1);
+      float m = -INFINITY, l = 0.f;
+      for (int s0 = wave; s0 < n; s0 += 4 * kRound) {
+        float2 ml[kRound];
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < kRound; ++j) {
+          const int64_t slot = from + min(s0 + 4 * j, n - 1);
+          ml[j] = *reinterpret_cast<const float2 *>(ws_ml + (slot * num_q_heads + h) * 2);
+          if (s0 + 4 * j >= n) ml[j] = make_float2(-INFINITY, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < kRound; ++j) top = fmaxf(top, ml[j].x);
+        l = m == -INFINITY ? 0.f : l * exp2f(m - top);
+#pragma unroll
+        for (int j = 0; j < kRound; ++j)
+          if (ml[j].x != -INFINITY) l += ml[j].y * exp2f(ml[j].x - top);
+        m = top;
+      }
+      part_ml[wave][lane] = make_float2(m, l);
+      __syncthreads();
+      if (wave == 0 && h0 + lane < num_q_heads) {
+        float top = -INFINITY, all = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, part_ml[w][lane].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 p = part_ml[w][lane];
+          if (p.x != -INFINITY) all += p.y * exp2f(p.x - top);
+        }
+        head_ml[h0 + lane] = make_float2(top, 1.0f / all);
+      }
+      __syncthreads();
+    }
+    if (live) {
+#pragma unroll 8
+      for (int x = wave; x < num_q_heads; x += 4) {
         const f32x4 s = *reinterpret_cast<const f32x4 *>(scores + x * score_stride + off + t);
-        const float2 r = ml[x];
-        const float inv = 1.0f / r.y;
+        const float2 r = head_ml[x];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           sum[e] = __builtin_fmaf(
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -r.x)), inv, sum[e]);
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -r.x)), r.y, sum[e]);
       }
-    } else {
-#pragma unroll 4
-      for (int x = wave; x < n; x += 4)
-        sum += *reinterpret_cast<const f32x4 *>(partials + (from + x) * partial_stride + off + t);
     }
+  } else if (live) {
+#pragma unroll 4
+    for (int x = wave; x < n; x += 4)
+      sum += *reinterpret_cast<const f32x4 *>(partials + (from + x) * partial_stride + off + t);
   }
   if (wave > 0) box[wave - 1][lane] = sum;
   __syncthreads();
@@ -291,55 +403,69 @@ __global__ __launch_bounds__(256) void add_kernel(
     if (t + e < t1) dst[e] += sum[e];
 }
 
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
 }  // namespace
 }  // namespace hy
 
-int hy::token_weights(const char *name, const Rows &q, const Pools &pools, const Shape &shape,
-                      const int32_t *items, int32_t n_items, const int32_t *adds, int32_t n_adds,
-                      const Scores &scores, float *partials, int64_t partial_stride,
-                      const float *row_ml, float *weights, int64_t weights_stride, void *stream) {
-  // (shape, scale and page size are those that the attention before it was checked for)
-  HY_REQUIRE(n_items >= 0 && n_items <= 65535 && n_adds >= 0,
-             "%s: %d items (0 to 65535), %d additions", name, n_items, n_adds);
-  if (n_adds == 0) return HY_OK;
-  HY_REQUIRE(q.at && pools.k && pools.page_table && adds && row_ml && weights && (n_items == 0 || items),
+int hy::check_weigh(const char *name, const Rows &q, const Shape &s, const Weigh &w) {
+  HY_REQUIRE(w.n_items >= 0 && w.n_items <= 65535 && w.n_adds >= 0,
+             "%s: %d items (0 to 65535), %d additions", name, w.n_items, w.n_adds);
+  HY_REQUIRE_SUPPORTED(s.num_q_heads <= kMaxHeads, "%s: %d query heads (at most %d)", name,
+                       s.num_q_heads, kMaxHeads);
+  HY_REQUIRE(w.n_adds == 0 || (w.adds && w.weights && (w.scores.at || w.partials)),
              "%s: null pointer argument", name);
-  HY_REQUIRE(scores.at || partials, "%s: null pointer argument", name);
-  HY_REQUIRE(n_items == 0 || partials, "%s: null pointer argument", name);
-  HY_REQUIRE(((reinterpret_cast<uintptr_t>(scores.at) | reinterpret_cast<uintptr_t>(partials)) & 15) ==
-                     0 &&
-                 scores.stride % 4 == 0 && partial_stride % 4 == 0,
+  HY_REQUIRE(w.n_items == 0 || (w.items && w.partials && w.row_ml), "%s: null pointer argument", name);
+  HY_REQUIRE(((reinterpret_cast<uintptr_t>(w.scores.at) | reinterpret_cast<uintptr_t>(w.partials)) &
+              15) == 0 &&
+                 w.scores.stride % 4 == 0 && w.partial_stride % 4 == 0,
              "%s: scores and partial sums lie on 16 bytes", name);
-  const int num_q_heads = shape.num_q_heads, num_kv_heads = shape.num_kv_heads;
-  const int G = num_q_heads / num_kv_heads;
-  const float scale_log2 = shape.scale * kLog2e;
-  const int page_shift = __builtin_ctz(static_cast<unsigned>(shape.page_size));
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const uint16_t *qq = static_cast<const uint16_t *>(q.at);
-  const uint16_t *kp = static_cast<const uint16_t *>(pools.k);
-  const float2 *ml = reinterpret_cast<const float2 *>(row_ml);
   HY_REQUIRE((reinterpret_cast<uintptr_t>(q.at) & 15) == 0 && ((q.seq | q.tok | q.head) & 7) == 0,
              "%s: q rows lie on 16 bytes", name);
-  if (n_items > 0) {
-    void (*kernel)(const uint16_t *, int64_t, int64_t, int64_t, const uint16_t *, int64_t,
-                   const int32_t *, int64_t, const int32_t *, const float2 *, float *, int64_t, int,
-                   int, float) = nullptr;
-    switch (G) {
-      case 1: kernel = weigh_kernel<1>; break;
-      case 2: kernel = weigh_kernel<2>; break;
-      case 4: kernel = weigh_kernel<4>; break;
-      case 8: kernel = weigh_kernel<8>; break;
-      case 16: kernel = weigh_kernel<16>; break;
-      default:
-        hy::set_error("GQA group size %d unsupported (1, 2, 4, 8, 16)", G);
-        return HY_EUNSUPPORTED;
-    }
-    hipLaunchKernelGGL(kernel, dim3(num_kv_heads, n_items), dim3(256), 0, st, qq, q.seq, q.tok, q.head,
-                       kp, pools.head_stride, pools.page_table, pools.page_table_stride, items, ml, partials, partial_stride, num_kv_heads,
-                       page_shift, scale_log2);
+  return HY_OK;
+}
+
+int hy::weigh_chunks(const char *name, const Rows &q, const Pools &pools, const Shape &s,
+                     const Weigh &w, void *stream) {
+  if (w.n_items == 0) return HY_OK;
+  const int G = s.num_q_heads / s.num_kv_heads;
+  decltype(&weigh_kernel<1>) kernel = nullptr;
+  switch (G) {
+    case 1: kernel = weigh_kernel<1>; break;
+    case 2: kernel = weigh_kernel<2>; break;
+    case 4: kernel = weigh_kernel<4>; break;
+    case 8: kernel = weigh_kernel<8>; break;
+    case 16: kernel = weigh_kernel<16>; break;
+    default:
+      hy::set_error("GQA group size %d unsupported (1, 2, 4, 8, 16)", G);
+      return HY_EUNSUPPORTED;
   }
-  hipLaunchKernelGGL(add_kernel, dim3(n_adds), dim3(256), 0, st, adds, scores.at, scores.stride,
-                     partials, partial_stride, ml, num_q_heads, scale_log2, weights,
-                     weights_stride);
+  hipLaunchKernelGGL(kernel, dim3(s.num_kv_heads, w.n_items), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), static_cast<const uint16_t *>(q.at), q.seq,
+                     q.tok, q.head, static_cast<const uint16_t *>(pools.k), pools.head_stride,
+                     pools.page_table, pools.page_table_stride, w.items,
+                     reinterpret_cast<const float2 *>(w.row_ml), w.partials, w.partial_stride,
+                     s.num_kv_heads, __builtin_ctz(static_cast<unsigned>(s.page_size)),
+                     s.scale * kLog2e);
+  return hy::launch_status(name);
+}
+
+int hy::finish_weights(const char *name, const Rows &out, const Items &merge, const Workspace &ws,
+                       const Shape &s, const Weigh &w, void *stream) {
+  const int groups = (s.num_q_heads + 7) / 8;
+  const int64_t blocks = static_cast<int64_t>(merge.count) * groups + w.n_adds;
+  HY_REQUIRE(blocks <= INT32_MAX, "%s: too many records", name);
+  if (blocks == 0) return HY_OK;
+  HY_REQUIRE(merge.count == 0 || (out.at && merge.at && ws.at), "%s: null pointer argument", name);
+  // (the decode call before has checked that the partials fit)
+  const float *acc = static_cast<const float *>(ws.at);
+  const float *ml = reinterpret_cast<const float *>(
+      static_cast<const char *>(ws.at) +
+      align256(static_cast<int64_t>(merge.slots) * s.num_q_heads * kHeadDim * 4));
+  hipLaunchKernelGGL(finish_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), static_cast<uint16_t *>(out.at), out.seq,
+                     out.tok, out.head, merge.at, merge.count, groups, acc, ml, w.adds, w.scores.at,
+                     w.scores.stride, w.partials, w.partial_stride, s.num_q_heads, s.scale * kLog2e,
+                     w.weights, w.weights_stride);
   return hy::launch_status(name);
 }

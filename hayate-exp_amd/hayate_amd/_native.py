@@ -159,7 +159,7 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "hy_plan_weigh": (
-        [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P],
+        [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _I32, _P, _P, _I32, _P, _I32, _P],
         ctypes.c_int,
     ),
     "hy_paged_weigh": (
@@ -376,15 +376,16 @@ class WeighPlan:
     def __init__(self, score_start, items, adds, scores, partials, parts):
         self.score_start = score_start  # int32 (sequences): its scores' first place in a row
         self.items = items  # int32 (n, 8) {seq, key0, token0, token1, part, q_row, cache, offset}
-        self.adds = adds  # int32 (n, 8) {row, t0, t1, sources, first, q_row or -1, offset, 0}
+        self.adds = adds  # int32 (n, 8) {row, t0, t1, sources, first, decode, offset, 0}
         self.scores = scores  # places a row of scores has
         self.partials = partials  # and a row of partial sums
         self.parts = parts
 
 
 def plan_weigh(q_lens: np.ndarray, kv_lens: np.ndarray, rows: np.ndarray, num_q_heads: int,
-               num_kv_heads: int, num_cus: int) -> WeighPlan:
-    """Run the native planner of attention weights."""
+               num_kv_heads: int, num_cus: int, merge: np.ndarray) -> WeighPlan:
+    """Run the native planner of attention weights; `merge`: the tick plan's decode merge items."""
+    merge = np.ascontiguousarray(merge, dtype=np.int32)
     q_lens, kv_lens, rows = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, kv_lens, rows))
     n = len(q_lens)
     blocks = -(-kv_lens.astype(np.int64) // 256)
@@ -395,8 +396,8 @@ def plan_weigh(q_lens: np.ndarray, kv_lens: np.ndarray, rows: np.ndarray, num_q_
     starts, counts = np.zeros(n, dtype=np.int32), np.zeros(5, dtype=np.int64)
     rc = lib().hy_plan_weigh(
         q_lens.ctypes.data, kv_lens.ctypes.data, rows.ctypes.data, n, num_q_heads, num_kv_heads,
-        num_cus, starts.ctypes.data, items.ctypes.data, len(items), adds.ctypes.data, len(adds),
-        counts.ctypes.data,
+        num_cus, merge.ctypes.data, len(merge), starts.ctypes.data, items.ctypes.data, len(items),
+        adds.ctypes.data, len(adds), counts.ctypes.data,
     )
     check(rc, "hy_plan_weigh")
     n_items, n_adds, scores, partials, parts = counts.tolist()

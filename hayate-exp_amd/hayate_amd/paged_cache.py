@@ -404,7 +404,8 @@ class PagedKVBatch:
         if cached is None:
             host = _native.plan_weigh(
                 np.asarray(self.q_lens), np.asarray(self.kv_lens_host),
-                np.asarray(self._weight_rows), num_q_heads, self.num_kv_heads, self._num_cus)
+                np.asarray(self._weight_rows), num_q_heads, self.num_kv_heads, self._num_cus,
+                self._plans[num_q_heads].host.merge)
             cached = _DeviceWeighPlan(host, self, num_q_heads)
             self._own(*cached.memory)
             self._weigh_plans[num_q_heads] = cached

@@ -627,8 +627,8 @@ int hy_paged_window_append(
  * Rows of q lie on 16 bytes.
  * Besides the lists of hy_plan_weigh the call takes room for what its launches
  * leave each other:
- *   row_ml    2 fp32 a packed row and query head, on 8 bytes: the exponent base
- *             (exp2 domain) and the sum of its softmax;
+ *   row_ml    of chunks, 2 fp32 a packed row and query head, on 8 bytes: the
+ *             exponent base (exp2 domain) and the sum of its softmax;
  *   scores    the raw scores of sequences with one token: num_q_heads rows of
  *             score_stride fp32 (at least the planned count, a multiple of 4,
  *             on 16 bytes);
@@ -636,7 +636,8 @@ int hy_paged_window_append(
  *             parts * num_kv_heads rows of partial_stride fp32, likewise.
  * Results do not depend on the order in which workgroups run.
  *
- * hy_plan_weigh (host) makes the lists. score_start has num_seqs entries, items
+ * hy_plan_weigh (host) makes the lists, for the tick's decode merge items (at
+ * most 1,024 query heads). score_start has num_seqs entries, items
  * and adds 8 int32 a record, counts_out five: items, additions, scores a row,
  * partials a row, parts. ceil(kv_len / 256) additions a sequence, and for
  * chunks at most 32 times as many items.
@@ -644,9 +645,10 @@ int hy_paged_window_append(
  */
 int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens,
                   const int32_t *rows, int32_t num_seqs, int32_t num_q_heads,
-                  int32_t num_kv_heads, int32_t num_cus, int32_t *score_start,
-                  int32_t *items, int32_t item_capacity, int32_t *adds,
-                  int32_t add_capacity, int64_t *counts_out);
+                  int32_t num_kv_heads, int32_t num_cus,
+                  const int32_t *merge_items, int32_t n_merge,
+                  int32_t *score_start, int32_t *items, int32_t item_capacity,
+                  int32_t *adds, int32_t add_capacity, int64_t *counts_out);
 
 int hy_paged_weigh(
     const void *q, int64_t q_stride_seq, int64_t q_stride_tok,

@@ -81,7 +81,8 @@ def test_weigh_lists_cover_every_pair_once(hq, hkv, cus):
     q = np.array([1, 2, 300, 1, 512, 17, 1], dtype=np.int32)
     kv = q + rng.integers(0, 900, len(q)).astype(np.int32)
     rows = np.array([4, 0, 2, 9, 1, 3, 7], dtype=np.int32)
-    p = _native.plan_weigh(q, kv, rows, hq, hkv, cus)
+    merge = _native.plan_tick(q, kv, hq, hkv, 128, cus).merge
+    p = _native.plan_weigh(q, kv, rows, hq, hkv, cus, merge)
     start = np.cumsum(q) - q
     taken = np.zeros(p.scores, dtype=bool)
     for b in range(len(q)):
@@ -89,8 +90,9 @@ def test_weigh_lists_cover_every_pair_once(hq, hkv, cus):
         assert [t for a in adds for t in range(a[1], a[2])] == list(range(kv[b]))
         assert (adds[:, 2] - adds[:, 1] <= 256).all() and (adds[:, 1] % 256 == 0).all()
         if q[b] == 1:
-            assert (adds[:, 3] == hq).all() and (adds[:, 4] == 0).all()
-            assert (adds[:, 5] == start[b]).all() and (adds[:, 6] == p.score_start[b]).all()
+            slots = merge[merge[:, 0] == b][0]
+            assert (adds[:, 3] == slots[2]).all() and (adds[:, 4] == slots[1]).all()
+            assert (adds[:, 5] == 1).all() and (adds[:, 6] == p.score_start[b]).all()
             assert p.score_start[b] % 4 == 0
             # whole slices of 32 scores, none of another sequence's
             room = slice(p.score_start[b], p.score_start[b] + -(-kv[b] // 32) * 32)
@@ -105,7 +107,7 @@ def test_weigh_lists_cover_every_pair_once(hq, hkv, cus):
             of = items[items[:, 1] == a[1]]
             of = of[np.argsort(of[:, 4])]
             # the parts that the addition reads, and each of them written
-            assert a[4] == of[0, 4] * hkv and a[3] == len(of) * hkv and a[5] == -1
+            assert a[4] == of[0, 4] * hkv and a[3] == len(of) * hkv and a[5] == 0
             assert [x for x in of[:, 4]] == list(range(of[0, 4], of[0, 4] + len(of)))
             assert of[-1, 4] < p.parts and of[0, 7] + a[1] + 256 <= p.partials
             tokens = [t for x in of for t in range(x[2], x[3])]
