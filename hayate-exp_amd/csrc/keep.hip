@@ -17,7 +17,36 @@ constexpr int kKeepThreads = 1024;
 constexpr int kKeepWaves = kKeepThreads / 64;
 constexpr int kKeepHeld = 32;   // keys of a lane in registers
 constexpr int kKeepRows = 64;   // requests of one launch
+constexpr int kKeepGroup = 4;   // rounds taken together
 constexpr int kBins = 2048;
+// Copies of the first pass's counts: weights share few exponents, and lanes that add to one
+// word follow each other, so lane l adds to copy l % 8.
+constexpr int kCopies = 8;
+
+struct KeepShared {
+  uint32_t first[kBins * kCopies];  // [bin][copy]
+  uint32_t later[2][kBins];
+  uint32_t sums[kKeepWaves], same[kKeepWaves];
+  uint32_t found[2];
+};
+
+// Sum of x over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
+// Sum of the waves' values before `wave`.
+__device__ __forceinline__ uint32_t waves_before(const uint32_t *of, int wave) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t upto = lanes_up_to(of[lane & (kKeepWaves - 1)]);
+  return wave == 0 ? 0 : __builtin_amdgcn_readlane(upto, wave - 1);
+}
 
 struct KeepRow {
   int32_t row, len;
@@ -37,7 +66,7 @@ __device__ __forceinline__ uint32_t key_of(float w) {
 template <bool kHeld>
 __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int want,
                                          int32_t *__restrict__ out, int first_pos,
-                                         uint32_t *hist, uint32_t *wave_cnt) {
+                                         KeepShared &sh) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -53,12 +82,20 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
 #pragma unroll
     for (int i = 0; i < kKeepHeld; ++i) held[i] = load(i);
   }
+  {
+    uint4 *all = reinterpret_cast<uint4 *>(&sh);
+    for (int i = tid; i < kBins * (kCopies + 2) / 4; i += kKeepThreads) all[i] = uint4{0, 0, 0, 0};
+  }
+  __syncthreads();
   // f(key, round) for the lane's keys (0: none), in order
   auto each = [&](auto f) __attribute__((always_inline)) {
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < kKeepHeld; ++i)
-        if (i < rounds) f(held[i], i);
+      for (int i = 0; i < kKeepHeld; i += kKeepGroup) {
+        if (i >= rounds) break;
+#pragma unroll
+        for (int j = 0; j < kKeepGroup; ++j) f(held[i + j], i + j);
+      }
     } else {
 #pragma unroll 4
       for (int i = 0; i < rounds; ++i) f(load(i), i);
@@ -72,37 +109,54 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
     const int bits = pass < 2 ? 11 : 10;
     const int high = shift;  // key >> high equals the prefix
     shift -= bits;
-    for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
-    __syncthreads();
     const uint32_t mask = (1u << bits) - 1;
     each([&](uint32_t key, int) __attribute__((always_inline)) {
-      if (key != 0 && (pass == 0 || key >> high == prefix)) atomicAdd(&hist[key >> shift & mask], 1u);
+      const uint32_t bin = key >> shift & mask;
+      if (pass == 0) {
+        if (key != 0) atomicAdd(&sh.first[bin * kCopies + (lane & (kCopies - 1))], 1u);
+      } else if (key != 0 && key >> high == prefix) {
+        atomicAdd(&sh.later[pass - 1][bin], 1u);
+      }
     });
     __syncthreads();
     // thread t holds the bins 2047 - 2t and 2046 - 2t: a scan from the largest digit down
     const int top = kBins - 1 - 2 * tid;
-    const uint32_t a = hist[top], b = hist[top - 1];
-    uint32_t with = a + b;
+    uint32_t a, b;
+    if (pass == 0) {
+      static_assert(kCopies == 8, "four reads a thread");
+      const uint4 *at = reinterpret_cast<const uint4 *>(sh.first + (top - 1) * kCopies);
+      uint32_t sum[4];
+      // (each quarter of 16 lanes starts at another bank)
+      const int turn = lane >> 2;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = __shfl_up(with, o);
-      if (lane >= o) with += u;
+      for (int j = 0; j < 4; ++j) {
+        const uint4 v = at[(turn + j) & 3];
+        sum[j] = v.x + v.y + v.z + v.w;
+      }
+      b = a = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool low = ((turn + j) & 3) < 2;
+        b += low ? sum[j] : 0;
+        a += low ? 0 : sum[j];
+      }
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2 *>(sh.later[pass - 1] + top - 1);
+      b = v.x;
+      a = v.y;
     }
-    if (lane == 63) wave_cnt[wave] = with;
+    const uint32_t with = lanes_up_to(a + b);
+    if (lane == 63) sh.sums[wave] = with;
     __syncthreads();
-    uint32_t before = with - a - b;
-    for (int x = 0; x < wave; ++x) before += wave_cnt[x];
-    if (before < left && left <= before + a) {
-      wave_cnt[kKeepWaves] = top;
-      wave_cnt[kKeepWaves + 1] = before;
-    } else if (before + a < left && left <= before + a + b) {
-      wave_cnt[kKeepWaves] = top - 1;
-      wave_cnt[kKeepWaves + 1] = before + a;
+    const uint32_t before = waves_before(sh.sums, wave) + with - a - b;
+    if (before < left && left <= before + a + b) {
+      const bool second = left > before + a;
+      sh.found[0] = top - second;
+      sh.found[1] = before + (second ? a : 0);
     }
     __syncthreads();
-    prefix = prefix << bits | wave_cnt[kKeepWaves];
-    left -= wave_cnt[kKeepWaves + 1];
-    __syncthreads();
+    prefix = prefix << bits | __builtin_amdgcn_readfirstlane(sh.found[0]);
+    left -= __builtin_amdgcn_readfirstlane(sh.found[1]);
   }
   // `prefix` is the last key that stays, `left` how many of its equals do, the first ones.
   uint32_t more = 0, same = 0;
@@ -110,16 +164,14 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
     more += __popcll(__ballot(key > prefix));
     same += __popcll(__ballot(key == prefix));
   });
+  // (sums was read before the last barrier)
   if (lane == 0) {
-    wave_cnt[wave] = more;
-    wave_cnt[kKeepWaves + wave] = same;
+    sh.sums[wave] = more;
+    sh.same[wave] = same;
   }
   __syncthreads();
-  uint32_t more_before = 0, same_before = 0;
-  for (int x = 0; x < wave; ++x) {
-    more_before += wave_cnt[x];
-    same_before += wave_cnt[kKeepWaves + x];
-  }
+  uint32_t more_before = waves_before(sh.sums, wave);
+  uint32_t same_before = waves_before(sh.same, wave);
   const uint64_t below = (1ull << lane) - 1;
   each([&](uint32_t key, int i) __attribute__((always_inline)) {
     const uint64_t gt = __ballot(key > prefix), eq = __ballot(key == prefix);
@@ -135,8 +187,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(const float *__restr
                                                             int64_t stride, KeepRows rows,
                                                             int budget, int sinks, int recent,
                                                             int32_t *__restrict__ out) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t wave_cnt[2 * kKeepWaves];
+  __shared__ __attribute__((aligned(16))) KeepShared sh;
   const KeepRow row = rows.r[blockIdx.x];
   int32_t *o = out + static_cast<int64_t>(blockIdx.x) * budget;
   const int n = row.len;
@@ -151,9 +202,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(const float *__restr
   const float *w = weights + row.row * stride + sinks;
   const int between = n - sinks - recent;
   if (between <= kKeepHeld * kKeepThreads)
-    keep_row<true>(w, between, want, o + sinks, sinks, hist, wave_cnt);
+    keep_row<true>(w, between, want, o + sinks, sinks, sh);
   else
-    keep_row<false>(w, between, want, o + sinks, sinks, hist, wave_cnt);
+    keep_row<false>(w, between, want, o + sinks, sinks, sh);
 }
 
 }  // namespace
