@@ -72,7 +72,9 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t v) {
   return v;
 }
 
-// rows.row(i): row i's settings; Rows::kCutsOnly: only rows with a top-k or top-p are read.
+// rows.row(i): row i's settings. With Rows::kCutsOnly only rows with a top-k or top-p are read, and
+// rows.mass(i, largest logit or NaN, sum) gets the kept logits' sum of exp((x - largest) / temp),
+// which the counts tell without another read of the row.
 template <bool kBf16, class Rows>
 __global__ __launch_bounds__(kCutThreads) void cut_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Rows rows,
@@ -215,10 +217,11 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
   const float mx = score_of(value_of<kBf16>(top_key), temp, rcp);
   // softmax of such a row has no probabilities
   if (nan || isinf(mx)) {
-    if (tid == 0) {
-      if (!Rows::kCutsOnly) out[blockIdx.x] = 0;
-      cuts[blockIdx.x].ok = 0;
-    }
+    if constexpr (Rows::kCutsOnly)
+      rows.mass(blockIdx.x, NAN, NAN);
+    else if (tid == 0)
+      out[blockIdx.x] = 0;
+    if (tid == 0) cuts[blockIdx.x].ok = 0;
     return;
   }
   auto finish = [&]() __attribute__((always_inline)) {
@@ -427,6 +430,46 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
       if (tid == 0) sh.cut = 0;
       __syncthreads();
     }
+  }
+  if constexpr (Rows::kCutsOnly) {
+    const int low = max(sh.kth, sh.cut);
+    double sum = 0;
+    // the held words from the largest key's down to `low`'s
+    auto add = [&]() __attribute__((always_inline)) {
+      const int base = wide ? held << 15 : 0, shift = wide ? 0 : 1;
+      const int from = max(low - base, 0) >> shift;
+      const int to = min(static_cast<int>(top_key) - base, (kWords << shift) - 1) >> shift;
+      float s = 0.f;
+      auto of = [&](int key, uint32_t n) __attribute__((always_inline)) {
+        // (without a top-p `cut` is 0, which is no number's key)
+        if (n && key >= low) s += (key == sh.cut ? sh.cut_keep : n) * mass_of(key);
+      };
+#pragma unroll 4
+      for (int w = to - tid; w >= from; w -= kCutThreads) {
+        const uint32_t c = hist[w];
+        if (wide) {
+          of(base + w, c);
+        } else {
+          of(2 * w + 1, c >> 16);
+          of(2 * w, c & 0xffffu);
+        }
+      }
+      sum += s;
+    };
+    __syncthreads();
+    add();
+    if (wide) {
+      build(!held);
+      add();
+    }
+    __shared__ double wave_sum[kCutWaves];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < kCutWaves; ++w) sum += wave_sum[w];
+    rows.mass(blockIdx.x, top_value, static_cast<float>(sum));
   }
   // A value that the cut splits keeps its first logits by index: count it by
   // rounds, then find the last kept one in its round.

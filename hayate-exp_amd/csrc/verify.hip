@@ -14,9 +14,11 @@
 // The draw takes the smallest token whose cumulative mass exceeds u times the total; where
 // nothing is left (all mass refused) it is from p.
 //
-//   cut_kernel    rows of requests with top-k or top-p only: where they are cut.
-//   mass_kernel   many workgroups a row: the maximum and the sum of exponentials of each one's
-//                 share of the logits (greedy: its largest logit).
+//   cut_kernel    rows of requests with top-k or top-p only: where they are cut, and the sum of
+//                 exponentials of what is kept, from the counts that find the cut (16 trees of up
+//                 to 26 nodes, half of them cut: 63.6 -> 60.1 us against a second read).
+//   mass_kernel   the other rows, many workgroups a row: the maximum and the sum of exponentials
+//                 of each one's share of the logits (greedy: its largest logit).
 //   walk_kernel   the walk, in every workgroup of the request: its tests need the shares of its
 //                 rows and a logit a node, a few reads that all nodes make at once. Then the
 //                 masses of its part of the last node's row, in 64 bits: a border between
@@ -46,6 +48,12 @@ constexpr int kPart = kThreads * kVec;
 // (a part each), 32 chains of 5 24.5, 15.0 and 16.5 at 256, 1024 and more.
 constexpr int kWalkers = 2048;
 
+// A workgroup's share of a row: the largest kept logit and the sum of exp((x - max) / temp); of a
+// greedy row rank_of() of the largest.
+struct Share {
+  float max, sum;
+  uint64_t best;
+};
 struct Request {
   float temp;
   int32_t k;
@@ -56,6 +64,8 @@ struct Requests {
   static constexpr bool kCutsOnly = true;
   Request r[kRequests];
   int32_t count, rows;
+  Share *shares;
+  int32_t n_shares;  // of a row
 
   __device__ __forceinline__ int of_row(int row) const {
     int lo = 0, hi = count;
@@ -75,17 +85,19 @@ struct Requests {
     const Request &q = r[of_row(i)];
     return {q.temp, q.k, q.p, 0};
   }
+  // Row i's shares, by the whole workgroup: the first has all of it.
+  __device__ __forceinline__ void mass(int i, float max, float sum) const {
+    for (int x = threadIdx.x; x < n_shares; x += blockDim.x) {
+      Share *s = shares + static_cast<int64_t>(i) * n_shares + x;
+      s->max = x == 0 ? max : -INFINITY;
+      s->sum = x == 0 ? sum : 0.f;
+    }
+  }
   __device__ __forceinline__ bool cut(int b, int vocab) const {
     return r[b].temp != 0.f && (r[b].k < vocab || r[b].p < 1.f);
   }
 };
 
-// A workgroup's share of a row: the largest kept logit and the sum of exp((x - max) / temp); of a
-// greedy row rank_of() of the largest.
-struct Share {
-  float max, sum;
-  uint64_t best;
-};
 // Masses of a part of a request's last row: all of it, and what the draw is from.
 struct Mass {
   double all, left;
@@ -251,23 +263,23 @@ __device__ __forceinline__ uint64_t best_of_share(const u32x4 (&w)[kAhead], int 
   return rank_of(t, *first_box);
 }
 
-// Grid (shares, rows).
+// Grid (shares, rows): of the rows that are not cut.
 template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void mass_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
-    const RowCut *__restrict__ cuts, Share *__restrict__ shares, uint8_t *__restrict__ valid,
-    bool first_rows) {
+    Share *__restrict__ shares, uint8_t *__restrict__ valid, bool first_rows) {
   __shared__ float maxes[kWaves];
   __shared__ uint32_t tops[kWaves];
   __shared__ int place;
   __shared__ Pair box[kWaves];
   if (first_rows && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *valid = 1;
   const int row = blockIdx.y;
+  const int b = requests.of_row(row);
+  if (requests.cut(b, vocab)) return;
   constexpr int kRound = kThreads * kVec;
   const int i0 = blockIdx.x * kShare + kVec * threadIdx.x;
   u32x4 w[kAhead];
   load_share(logits + row * ld, vocab, i0, kRound, w);
-  const int b = requests.of_row(row);
   const float temp = requests.r[b].temp;
   Share *out = shares + static_cast<int64_t>(row) * gridDim.x + blockIdx.x;
   if (temp == 0.f) {
@@ -275,21 +287,11 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
     if (threadIdx.x == 0) out->best = best;
     return;
   }
-  bool ok = true;
   float x[kAhead][kVec], m = -INFINITY;
 #pragma unroll
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) x[a][j] = value_in<kBf16>(w[a], j);
-  if (requests.cut(b, vocab)) {
-    const Cut cut = cut_of<kBf16>(cuts[row]);
-    ok = cut.ok;
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (!cut.keeps(x[a][j], i0 + a * kRound + j)) x[a][j] = -INFINITY;
-  }
   if ((static_cast<int>(blockIdx.x) + 1) * static_cast<int64_t>(kShare) > vocab) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
     for (int j = 0; j < kVec; ++j) s += __builtin_amdgcn_exp2f((x[a][j] - from) * slope);
   const double sum = block_sums(s, 0.0, box).a;
   if (threadIdx.x == 0) {
-    out->max = ok && sum == sum ? m : NAN;
+    out->max = sum == sum ? m : NAN;
     out->sum = static_cast<float>(sum);
   }
 }
@@ -802,7 +804,7 @@ Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
 }
 
 template <bool kBf16>
-void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, const Requests &req, bool cuts,
+void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &req, bool cuts,
             const Tree &tree, char *ws, const Room &room, int32_t *paths, int levels,
             int32_t *lengths, int64_t *next, uint8_t *valid, bool first_rows) {
   const int n = static_cast<int>(share_count(vocab)), parts = static_cast<int>(part_count(vocab));
@@ -811,11 +813,13 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, const Requ
   auto *states = reinterpret_cast<State *>(ws + room.states);
   auto *masses = reinterpret_cast<Mass *>(ws + room.masses);
   auto *rests = reinterpret_cast<double *>(ws + room.rests);
+  req.shares = shares;
+  req.n_shares = n;
   if (cuts)
     hipLaunchKernelGGL((cut_kernel<kBf16, Requests>), dim3(req.rows), dim3(kCutThreads), 0, st, x,
                        ld, vocab, req, static_cast<int64_t *>(nullptr), cut);
   hipLaunchKernelGGL(mass_kernel<kBf16>, dim3(n, req.rows), dim3(kThreads), 0, st, x, ld, vocab, req,
-                     cut, shares, valid, first_rows);
+                     shares, valid, first_rows);
   bool sampled = false;
   for (int b = 0; b < req.count; ++b) sampled = sampled || req.r[b].temp != 0.f;
   // Every workgroup of a request repeats its walk: no more of them than fill the GPU.

@@ -197,6 +197,36 @@ def test_equal_tokens_and_certain_ones():
         assert walk(chain, logits[:2], tokens[:2], [1.0], [None], [None], numbers, q) == [([0], want)]
 
 
+@pytest.mark.parametrize("value", [-1.0, 2.5, 0.0])
+def test_more_equal_logits_than_16_bits_count(value):
+    """70,000 to 100,000 of a row are equal (of the zeros, half are negative): cut within,
+    above and below them."""
+    vocab, tree = 140_000, [-1, 0, 0, 2, 2, 2]
+    settings = [(1.0, None, 0.97), (0.8, 100, None), (1.0, 120_000, 0.6), (1.5, 80_000, None),
+                (0.7, None, 0.2)]
+    trees = [tree] * len(settings)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    logits = torch.randn((30, vocab), generator=g, device=DEV)
+    for i in range(30):
+        same = torch.randperm(vocab, generator=g, device=DEV)[: 70_000 + 1000 * i]
+        logits[i, same] = value
+        logits[i, same[::2]] *= -1 if value == 0 else 1
+    peaks = torch.randint(0, vocab, (30, 3), generator=g, device=DEV)
+    for j in range(3):
+        logits[torch.arange(30), peaks[:, j]] = 11.0 + j / 4
+    logits = logits.to(torch.bfloat16)
+    parent = torch.tensor([6 * b + max(p, 0) for b in range(5) for p in tree], device=DEV)
+    tokens = peaks[parent, torch.randint(0, 3, (30,), generator=g, device=DEV)]
+    for _ in range(3):
+        uniforms = torch.rand(35, generator=g, device=DEV)
+        t, k, p = map(list, zip(*settings))
+        paths, lengths, drawn = verify_tree(batch_of(trees), logits, tokens, t, k, p, uniforms)
+        want = walk(trees, logits, tokens, t, k, p, uniforms, None)
+        for b, (path, token) in enumerate(want):
+            assert paths[b, : len(path)].tolist() == path and int(lengths[b]) == len(path)
+            assert int(drawn[b]) == token
+
+
 def test_tokens_outside_the_vocabulary_are_refused():
     logits = torch.randn(6, 30, device=DEV).to(torch.bfloat16)
     tokens = torch.tensor([0, -1, 30, 2**40, -(2**40), 31], device=DEV)
