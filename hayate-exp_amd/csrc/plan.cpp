@@ -919,13 +919,12 @@ int64_t weigh_range(const int32_t *q_lens, const int32_t *kv_lens, int32_t num_s
 
 int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
                int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t num_cus,
-               const int32_t *merge_items, int32_t n_merge, int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds,
-               int32_t add_capacity, int64_t *counts_out) {
+               const int32_t *merge_items, int32_t n_merge, int32_t *score_start, int32_t *items,
+               int32_t item_capacity, int32_t *adds, int32_t add_capacity, int64_t *counts_out) {
   constexpr int64_t keys = hy::kWeighKeys;
   const int64_t G = num_q_heads / num_kv_heads;
   const int64_t cus = num_cus > 0 ? num_cus : 256;
-  const int64_t slots =
-      std::max<int64_t>(1, (num_cus > 0 ? num_cus : 256) * kWeighPerCu / num_kv_heads);
+  const int64_t slots = std::max<int64_t>(1, cus * kWeighPerCu / num_kv_heads);
   const int64_t range = weigh_range(q_lens, kv_lens, num_seqs, G, slots);
   int64_t scores = 0, partials = 0, q_row = 0, n_items = 0, n_adds = 0, parts_max = 0;
   // the partial slots of every decode token
@@ -1006,8 +1005,8 @@ int plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *row
 extern "C" int hy_plan_weigh(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *rows,
                              int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
                              int32_t num_cus, const int32_t *merge_items, int32_t n_merge,
-                             int32_t *score_start, int32_t *items, int32_t item_capacity, int32_t *adds, int32_t add_capacity,
-                             int64_t *counts_out) {
+                             int32_t *score_start, int32_t *items, int32_t item_capacity,
+                             int32_t *adds, int32_t add_capacity, int64_t *counts_out) {
   hy::clear_error();
   if (num_seqs < 0 || counts_out == nullptr ||
       (num_seqs > 0 && (!q_lens || !kv_lens || !rows || !score_start)) ||

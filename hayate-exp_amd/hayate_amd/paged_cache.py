@@ -26,6 +26,7 @@ Data operations need the pool on a HIP device; on any other device they raise
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import itertools
 import math
 import operator
@@ -1463,14 +1464,14 @@ class PagedKVCacheManager:
         _require_hip(self.k_cache, "keep_positions")
         if not handles:
             return torch.empty((0, budget), dtype=torch.int32, device=self.device)
-        self._check_weights(weights, [h.slot for h in handles], [h.length for h in handles])
-        rows = np.array([[h.slot for h in handles], [h.length for h in handles]], dtype=np.int32)
+        rows, lengths = [h.slot for h in handles], [int(h.length) for h in handles]
+        self._check_weights(weights, rows, lengths)
+        array = ctypes.c_int32 * len(handles)
         out = torch.empty((len(handles), budget), dtype=torch.int32, device=self.device)
         with _current_device(self.device):
             rc = _native.lib().hy_keep_positions(
-                weights.data_ptr(), weights.stride(0), rows.ctypes.data,
-                rows.ctypes.data + rows.strides[0], len(handles), budget, sinks, recent,
-                out.data_ptr(), _stream_handle(self.device),
+                weights.data_ptr(), weights.stride(0), array(*rows), array(*lengths), len(handles),
+                budget, sinks, recent, out.data_ptr(), _stream_handle(self.device),
             )
         _native.check(rc, "hy_keep_positions")
         return out
@@ -1644,6 +1645,8 @@ class PagedKVCacheManager:
                 raise ValueError("window must be positive")
             if sinks < 0:
                 raise ValueError("sinks must be non-negative")
+            if self.k_cache.dtype != torch.bfloat16:
+                raise TypeError("a window needs a bfloat16 pool")
             if weights is not None:
                 raise NotImplementedError("weights are of attention to the whole cache, "
                                           "without a window")

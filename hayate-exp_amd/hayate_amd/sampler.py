@@ -19,6 +19,7 @@ from the same generator.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Sequence
 
@@ -184,6 +185,7 @@ def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tenso
         # (the usual types in the usual ranges need no closer look)
         if not ((k is None or type(k) is int and k >= 1) and (p is None or type(p) is float and 0 < p <= 1)
                 and type(t) is float and (t == 0 or 1e-30 <= t <= 1e30)):
+            t, k, p = (v.item() if isinstance(v, np.generic) else v for v in (t, k, p))
             validate_parameters(t, k, p)
             if t and not 1e-30 <= t <= 1e30:
                 raise ValueError("verification takes temperatures of 0 or 1e-30 to 1e30")
@@ -226,10 +228,10 @@ def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tenso
     if draft_probs is not None and draft_probs.stride(1) != 1:
         draft_probs = draft_probs.contiguous()
     lib = _native.lib()
-    temp = np.array(temperature, dtype=np.float32)
-    k = np.array([vocab if v is None or v > vocab else v for v in top_k], dtype=np.int32)
-    p = np.array([1.0 if v is None else max(v, _TINY) for v in top_p], dtype=np.float32)
-    q_lens = np.array(batch.q_lens, dtype=np.int32)
+    # (an array's address as numpy gives it takes a microsecond)
+    floats, ints = ctypes.c_float * requests, ctypes.c_int32 * requests
+    k = [vocab if v is None or v > vocab else int(v) for v in top_k]
+    p = [1.0 if v is None else max(v, _TINY) for v in top_p]
     paths = torch.empty((requests, batch.levels), dtype=torch.int32, device=dev)
     lengths = torch.empty(requests, dtype=torch.int32, device=dev)
     drawn = torch.empty((requests, 1), dtype=torch.int64, device=dev)
@@ -238,14 +240,14 @@ def verify_tree(batch: PagedTreeBatch, logits: torch.Tensor, tokens: torch.Tenso
                        device=dev)
     rc = lib.hy_verify_tree(
         logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], vocab,
-        batch.packed_parents.data_ptr(), tokens.data_ptr(), q_lens.ctypes.data, requests,
-        temp.ctypes.data, k.ctypes.data, p.ctypes.data, uniforms.data_ptr(),
+        batch.packed_parents.data_ptr(), tokens.data_ptr(), ints(*batch.q_lens), requests,
+        floats(*temperature), ints(*k), floats(*p), uniforms.data_ptr(),
         None if draft_probs is None else draft_probs.data_ptr(),
         0 if draft_probs is None else draft_probs.stride(0), paths.data_ptr(), batch.levels,
         lengths.data_ptr(), drawn.data_ptr(), valid.data_ptr(), work.data_ptr(), work.numel(),
         batch._stream())
     _native.check(rc, "hy_verify_tree")
-    if temp.any():
+    if any(temperature):
         torch._assert_async(valid, "logits hold NaN or have no finite maximum")
     return paths, lengths, drawn
 

@@ -79,6 +79,14 @@ def test_values_that_differ_in_their_last_bit():
     choose([9000], bits.view(torch.float32), 4000, 10, 10)
 
 
+def test_a_length_of_another_whole_type():
+    m = PagedKVCacheManager(1, 1, D, 256, 128, 1, torch.bfloat16, DEV)
+    h = m.allocate()
+    m.commit_tick([h], np.array([m.reserve_tick([h], np.array([9]))[0]]))
+    weights = torch.arange(9.0, device=DEV)[None]
+    assert m.keep_positions([h], weights, 3, sinks=1, recent=0).tolist() == [[0, 7, 8]]
+
+
 def test_captured_and_on_another_stream():
     r = Requests([900, 50], [0, 0], seed=1)
     weights = torch.rand(r.m.max_requests, 900, generator=r.g, device=DEV)

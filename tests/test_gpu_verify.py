@@ -326,6 +326,16 @@ def test_strided_inputs():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_parameter_types():
+    trees = [[-1, 0, 0, 1], [-1, 0], [-1]]
+    logits, tokens, uniforms, _ = inputs(trees, 500, 9)
+    want = verify_tree(batch_of(trees), logits, tokens, [1.0, 0.5, 0.0], [7, None, 3],
+                       [1.0, 0.75, None], uniforms)
+    got = verify_tree(batch_of(trees), logits, tokens, [1, np.float32(0.5), np.int64(0)],
+                      [np.int64(7), None, np.int32(3)], [1, np.float64(0.75), None], uniforms)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_the_samplers_form():
     class Request:
         def __init__(self, temperature, top_k=None, top_p=None):

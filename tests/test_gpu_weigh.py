@@ -62,6 +62,12 @@ def test_head_groups(hq, hkv):
                    seed=hq), what=f"{hq}/{hkv}")
 
 
+@pytest.mark.parametrize("hq,hkv", [(128, 8), (2, 1), (80, 5)])
+def test_more_and_fewer_heads_than_a_waves_lanes(hq, hkv):
+    """(partials of 64 heads are read at a time, outputs of eight joined)"""
+    check(Requests([2500, 0, 40], [1, 1, 33], hq=hq, hkv=hkv, seed=hq), what=f"{hq}/{hkv}")
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_mixed_ticks(seed):
     g = torch.Generator().manual_seed(seed)

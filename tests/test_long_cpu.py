@@ -147,6 +147,9 @@ def test_refusals_of_a_tick():
     m16 = PagedKVCacheManager(1, 8, 128, 256, 128, 1, torch.float16, "cpu", num_q_heads=32)
     with pytest.raises(TypeError):
         m16.begin_tick([m16.allocate()], [1], weights=good)
+    m16 = PagedKVCacheManager(1, 8, 128, 256, 128, 1, torch.float16, "cpu", num_q_heads=32)
+    with pytest.raises(TypeError, match="window"):
+        m16.begin_tick([m16.allocate()], [1], window=9)
 
 
 def test_a_tick_with_a_form_of_its_own():
