@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kKeepThreads = 1024;
 constexpr int kKeepWaves = kKeepThreads / 64;
-constexpr int kKeepHeld = 32;   // keys of a lane in registers
+constexpr int kKeepFew = 8;     // keys of a lane in registers, all loads in flight at once
+constexpr int kKeepMost = 32;
 constexpr int kKeepRows = 64;   // requests of one launch
 constexpr int kKeepGroup = 4;   // rounds taken together
 constexpr int kBins = 2048;
@@ -63,7 +64,8 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <bool kHeld>
+// kHeld: rounds whose keys are held, or 0.
+template <int kHeld>
 __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int want,
                                          int32_t *__restrict__ out, int first_pos,
                                          KeepShared &sh) {
@@ -73,14 +75,18 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
   // wave's stretch: rounds of 64 positions
   const int rounds = ((n + 64 * kKeepWaves - 1) / (64 * kKeepWaves));
   const int from = wave * 64 * rounds;
-  uint32_t held[kHeld ? kKeepHeld : 1];
-  auto load = [&](int i) -> uint32_t {
-    const int at = from + 64 * i + lane;
-    return i < rounds && at < n ? key_of(w[at]) : 0u;
+  uint32_t held[kHeld ? kHeld : 1];
+  // (a load behind a branch would wait for the one before)
+  auto value_at = [&](int i) { return w[min(from + 64 * i + lane, n - 1)]; };
+  auto key_at = [&](int i, float v) {
+    return i < rounds && from + 64 * i + lane < n ? key_of(v) : 0u;
   };
   if constexpr (kHeld) {
+    float v[kHeld];
 #pragma unroll
-    for (int i = 0; i < kKeepHeld; ++i) held[i] = load(i);
+    for (int i = 0; i < kHeld; ++i) v[i] = value_at(i);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = key_at(i, v[i]);
   }
   {
     uint4 *all = reinterpret_cast<uint4 *>(&sh);
@@ -91,14 +97,19 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
   auto each = [&](auto f) __attribute__((always_inline)) {
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < kKeepHeld; i += kKeepGroup) {
+      for (int i = 0; i < kHeld; i += kKeepGroup) {
         if (i >= rounds) break;
 #pragma unroll
         for (int j = 0; j < kKeepGroup; ++j) f(held[i + j], i + j);
       }
     } else {
-#pragma unroll 4
-      for (int i = 0; i < rounds; ++i) f(load(i), i);
+      for (int i = 0; i < rounds; i += kKeepFew) {
+        float v[kKeepFew];
+#pragma unroll
+        for (int j = 0; j < kKeepFew; ++j) v[j] = value_at(i + j);
+#pragma unroll
+        for (int j = 0; j < kKeepFew; ++j) f(key_at(i + j, v[j]), i + j);
+      }
     }
   };
   // Radix select of the want-th largest key, want of [1, n].
@@ -170,16 +181,22 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
     sh.same[wave] = same;
   }
   __syncthreads();
-  uint32_t more_before = waves_before(sh.sums, wave);
-  uint32_t same_before = waves_before(sh.same, wave);
-  const uint64_t below = (1ull << lane) - 1;
+  const uint32_t same_before = waves_before(sh.same, wave);
+  uint32_t at = waves_before(sh.sums, wave) + min(same_before, left);
+  left -= min(same_before, left);  // equals that stay from this wave on
   each([&](uint32_t key, int i) __attribute__((always_inline)) {
-    const uint64_t gt = __ballot(key > prefix), eq = __ballot(key == prefix);
-    const uint32_t eq_rank = same_before + __popcll(eq & below);
-    const uint32_t at = more_before + __popcll(gt & below) + min(eq_rank, left);
-    if (key > prefix || (key == prefix && eq_rank < left)) out[at] = first_pos + from + 64 * i + lane;
-    more_before += __popcll(gt);
-    same_before += __popcll(eq);
+    uint64_t stay = __ballot(key > prefix);
+    if (left > 0) {
+      const uint64_t eq = __ballot(key == prefix);
+      const uint32_t rank = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(eq >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(eq), 0));
+      stay |= __ballot(key == prefix && rank < left);
+      left -= min(static_cast<uint32_t>(__popcll(eq)), left);
+    }
+    const uint32_t mine = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(stay >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(stay), at));
+    if (stay >> lane & 1) out[mine] = first_pos + from + 64 * i + lane;
+    at += __popcll(stay);
   });
 }
 
@@ -201,10 +218,12 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(const float *__restr
   if (want == 0) return;
   const float *w = weights + row.row * stride + sinks;
   const int between = n - sinks - recent;
-  if (between <= kKeepHeld * kKeepThreads)
-    keep_row<true>(w, between, want, o + sinks, sinks, sh);
+  if (between <= kKeepFew * kKeepThreads)
+    keep_row<kKeepFew>(w, between, want, o + sinks, sinks, sh);
+  else if (between <= kKeepMost * kKeepThreads)
+    keep_row<kKeepMost>(w, between, want, o + sinks, sinks, sh);
   else
-    keep_row<false>(w, between, want, o + sinks, sinks, sh);
+    keep_row<0>(w, between, want, o + sinks, sinks, sh);
 }
 
 }  // namespace
