@@ -21,8 +21,8 @@ constexpr int kKeepRows = 64;   // requests of one launch
 constexpr int kKeepGroup = 4;   // rounds taken together
 constexpr int kBins = 2048;
 // Copies of the first pass's counts: weights share few exponents, and lanes that add to one
-// word follow each other, so lane l adds to copy l % 8.
-constexpr int kCopies = 8;
+// word follow each other, so lane l adds to copy l % 4.
+constexpr int kCopies = 4;
 
 struct KeepShared {
   uint32_t first[kBins * kCopies];  // [bin][copy]
@@ -56,12 +56,12 @@ struct KeepRows {
   KeepRow r[kKeepRows];
 };
 
-// Ordered keys: larger key, larger weight; -0 is 0 and NaN the largest. No key is 0.
+// Ordered keys: larger key, larger weight; -0 is 0 and NaN the largest. A number's key is at least
+// that of -inf; 0 stands for none.
 __device__ __forceinline__ uint32_t key_of(float w) {
-  const uint32_t u = __float_as_uint(w);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  if ((u & 0x7fffffffu) == 0) return 0x80000000u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  const uint32_t key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return w != w ? 0xffffffffu : key;
 }
 
 // kHeld: rounds whose keys are held, or 0.
@@ -122,34 +122,29 @@ __device__ __forceinline__ void keep_row(const float *__restrict__ w, int n, int
     shift -= bits;
     const uint32_t mask = (1u << bits) - 1;
     each([&](uint32_t key, int) __attribute__((always_inline)) {
-      const uint32_t bin = key >> shift & mask;
-      if (pass == 0) {
-        if (key != 0) atomicAdd(&sh.first[bin * kCopies + (lane & (kCopies - 1))], 1u);
-      } else if (key != 0 && key >> high == prefix) {
-        atomicAdd(&sh.later[pass - 1][bin], 1u);
-      }
+      // (no number's key has the first digit 0, and no number is searched for behind them all)
+      if (pass == 0)
+        atomicAdd(&sh.first[(key >> shift) * kCopies + (lane & (kCopies - 1))], 1u);
+      else if (key >> high == prefix)
+        atomicAdd(&sh.later[pass - 1][key >> shift & mask], 1u);
     });
     __syncthreads();
     // thread t holds the bins 2047 - 2t and 2046 - 2t: a scan from the largest digit down
     const int top = kBins - 1 - 2 * tid;
     uint32_t a, b;
     if (pass == 0) {
-      static_assert(kCopies == 8, "four reads a thread");
       const uint4 *at = reinterpret_cast<const uint4 *>(sh.first + (top - 1) * kCopies);
-      uint32_t sum[4];
-      // (each quarter of 16 lanes starts at another bank)
-      const int turn = lane >> 2;
+      // (lanes whose counts lie 256 bytes apart start at different ones)
+      constexpr int kReads = kCopies / 2;
+      const int turn = lane / (32 / kCopies);
+      a = b = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 v = at[(turn + j) & 3];
-        sum[j] = v.x + v.y + v.z + v.w;
-      }
-      b = a = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool low = ((turn + j) & 3) < 2;
-        b += low ? sum[j] : 0;
-        a += low ? 0 : sum[j];
+      for (int j = 0; j < kReads; ++j) {
+        const int i = (turn + j) & (kReads - 1);
+        const uint4 v = at[i];
+        const uint32_t sum = v.x + v.y + v.z + v.w;
+        b += i < kReads / 2 ? sum : 0;
+        a += i < kReads / 2 ? 0 : sum;
       }
     } else {
       const uint2 v = *reinterpret_cast<const uint2 *>(sh.later[pass - 1] + top - 1);
