@@ -22,9 +22,9 @@
 //   walk_kernel   the walk, in every workgroup of the request: its tests need the shares of its
 //                 rows and a logit a node, a few reads that all nodes make at once. Then the
 //                 masses of its part of the last node's row, in 64 bits: a border between
-//                 two of 151,936 tokens is met by one draw in thousands of 32-bit sums.
-//   rest_kernel   (drafts drawn, one refused) the same of max(p - q, 0), whose p needs all of
-//                 the row's masses.
+//                 two of 151,936 tokens is met by one draw in thousands of 32-bit sums. (Of
+//                 max(p - q, 0) in the same pass, see Mass: in one of its own, once the row's sum
+//                 was known, 32 chains of 5 took 46 us instead of 39.)
 //   pick_kernel   the part that holds the draw, then the token. (In the walk's last workgroup of
 //                 each request instead, the releases and acquires of all others took 20 us
 //                 more with 32 requests.)
@@ -98,9 +98,12 @@ struct Requests {
   }
 };
 
-// Masses of a part of a request's last row: all of it, and what the draw is from.
+// Masses of a part of a request's last row: all of it, and what the draw is from. Where that is
+// max(p - q, 0), `left` and `drafts` are the sums of exp and of q over the tokens with p > q:
+// left / sum - drafts, once all parts have told the row's sum. (Which tokens these are goes by the
+// shares' sum; one on the wrong side differs from 0 by the error of that sum times q.)
 struct Mass {
-  double all, left;
+  double all, left, drafts;
 };
 struct State {
   int32_t last, child;  // the path's last node, and its refused child where drafts are drawn, or -1
@@ -327,9 +330,10 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
   }
 }
 
-// exp(x), x <= 0, to about 1e-10: 2^n times the Taylor series of the rest, |r| <= ln(2) / 2 and a
-// little, its terms from the fourth on (r^4 / 24 < 7e-4) in 32 bits. Operations of 64 bits bound
-// the kernels that call it.
+// exp(x), x <= 0, to about 1e-12: 2^n times the Taylor series of the rest, |r| <= ln(2) / 2 and a
+// little, its terms from the sixth on (r^6 / 720 < 3e-6) in 32 bits. Operations of 64 bits bound
+// the kernels that call it: with the fourth and fifth term in 32 bits as well (1e-10, which one
+// draw in ten thousand notices where little of p is left) 32 drawn chains take 0.8 us less.
 __device__ __forceinline__ double exp_of(double x) {
   constexpr long double kLn2 = 0.693147180559945309417232L;
   constexpr double kHead = 45426.0 / 65536;  // n times it is exact
@@ -338,14 +342,13 @@ __device__ __forceinline__ double exp_of(double x) {
   double r = fma(static_cast<double>(n), -kHead, x);
   r = fma(static_cast<double>(n), -kTail, r);
   const float s = static_cast<float>(r);
-  float q = 1.0f / 362880;
+  float q = 1.0f / 39916800;
 #pragma unroll
-  for (const float c : {1.0f / 40320, 1.0f / 5040, 1.0f / 720, 1.0f / 120, 1.0f / 24})
+  for (const float c : {1.0f / 3628800, 1.0f / 362880, 1.0f / 40320, 1.0f / 5040, 1.0f / 720})
     q = __builtin_fmaf(q, s, c);
-  double p = fma(static_cast<double>(q), r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
+  double p = static_cast<double>(q);
+#pragma unroll
+  for (const double c : {1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0}) p = fma(p, r, c);
   return x < -740.0 ? 0.0 : ldexp(p, static_cast<int>(n));
 }
 
@@ -428,14 +431,13 @@ __device__ __forceinline__ int take_found(const Found *of_waves, double &rest) {
 
 // The draw of one request, by a whole workgroup: the smallest token whose running mass exceeds
 // `number` times the total (where rounding leaves none, the last token with any). The masses are
-// max(p - q, 0) with rests (the parts') and q (the row of draft probabilities), else those of p
-// without the children of `last`, of which every thread has one's parent and token.
+// max(p - q, 0) with q (the row of draft probabilities), else those of p without the children of
+// `last`, of which every thread has one's parent and token.
 template <bool kBf16>
 __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const Cut &cut, float max,
                                           double inv_temp, double number, const Mass *masses,
-                                          const double *rests, const float *q, int n_parts,
-                                          int parent, int64_t token, int last, uint32_t *bits,
-                                          PickRoom &room) {
+                                          const float *q, int n_parts, int parent, int64_t token,
+                                          int last, uint32_t *bits, PickRoom &room) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto scan = [&](double v) __attribute__((always_inline)) {
 #pragma unroll
@@ -448,27 +450,28 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   // A thread has neighbouring parts.
   const int per = (n_parts + kThreads - 1) / kThreads;
   const int from = min(tid * per, n_parts), to = min(from + per, n_parts);
-  double all = 0, left = 0;
-  for (int i = from; i < to; ++i) {
-    all += masses[i].all;
-    left += rests ? rests[i] : masses[i].left;
-  }
-  const double all_with = scan(all), left_with = scan(left);
-  if (lane == 63) {
-    room.all[wave] = all_with;
-    room.left[wave] = left_with;
-  }
-  __syncthreads();
-  double z = 0, some = 0, all_before = all_with - all, left_before = left_with - left;
+  // The sum before this thread's own, and of all.
+  auto sums = [&](double own, double *box, double &before) __attribute__((always_inline)) {
+    const double with = scan(own);
+    if (lane == 63) box[wave] = with;
+    __syncthreads();
+    double total = 0;
+    before = with - own;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < wave) {
-      all_before += room.all[i];
-      left_before += room.left[i];
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) before += box[i];
+      total += box[i];
     }
-    z += room.all[i];
-    some += room.left[i];
-  }
+    return total;
+  };
+  double all = 0, left = 0, all_before, left_before;
+  for (int i = from; i < to; ++i) all += masses[i].all;
+  const double z = sums(all, room.all, all_before), inv_z = 1.0 / z;
+  auto left_of = [&](const Mass &m) {
+    return q ? fmax(fma(m.left, inv_z, -m.drafts), 0.0) : m.left;
+  };
+  for (int i = from; i < to; ++i) left += left_of(masses[i]);
+  const double some = sums(left, room.left, left_before);
   const bool whole = !(some > 0);  // where nothing is left, all of p
   const double target = number * (whole ? z : some);
   const double own = whole ? all : left, before = whole ? all_before : left_before;
@@ -477,7 +480,7 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   if (own > 0) {
     double at = before;
     for (int i = from; i < to; ++i) {
-      const double v = whole ? masses[i].all : rests ? rests[i] : masses[i].left;
+      const double v = whole ? masses[i].all : left_of(masses[i]);
       if (v > 0) {
         part = i;
         rest = target - at;
@@ -492,11 +495,10 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   const int first = chosen * kPart, at = kVec * tid, mine = first + at;
   u32x4 w[1];
   load_share(row, vocab, mine, 0, w);
-  mark_refused(bits, whole || rests ? -2 : parent, token, last, first);
+  mark_refused(bits, whole || q ? -2 : parent, token, last, first);
   double e[kVec];
   masses_of<kBf16>(w[0], mine, vocab, cut, max, inv_temp, e);
-  if (!whole && rests) {
-    const double inv_z = 1.0 / z;
+  if (!whole && q) {
     float qv[kVec];
     load_drafts(q, mine, vocab, qv);
 #pragma unroll
@@ -692,58 +694,33 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
   const uint16_t *x_row = logits + row * ld;
   const Cut cut = cut_rows ? cut_of<kBf16>(cuts[row]) : no_cut();
   const int my_parent = tree.drafts || tid == 0 || tid >= nodes ? -2 : up;
+  const bool drawn = tree.drafts && sh.child >= 0;  // the draw is from max(p - q, 0)
+  const float *q = drawn ? tree.drafts + (row0 + sh.child) * tree.drafts_ld : nullptr;
+  const double inv_sum = 1.0 / sum_of[sh.last];
   u32x4 w[1];
   load_share(x_row, vocab, blockIdx.x * kPart + at, 0, w);
   for (int part = blockIdx.x; part < n_parts; part += gridDim.x) {
     const int first = part * kPart;
     mark_refused(bits, my_parent, my_token, sh.last, first);
     const uint32_t out = bits[at >> 5] >> (at & 31);
-    double e[kVec], all = 0, left = 0;
+    double e[kVec], all = 0, left = 0, drafts = 0;
+    float qv[kVec];
+    if (drawn) load_drafts(q, first + at, vocab, qv);
     masses_of<kBf16>(w[0], first + at, vocab, cut, sh.max, inv_temp, e);
     if (part + static_cast<int>(gridDim.x) < n_parts)
       load_share(x_row, vocab, first + static_cast<int>(gridDim.x) * kPart + at, 0, w);
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
+      // (e is 0 past the row's end)
+      const bool in = drawn ? e[j] * inv_sum > qv[j] : !(out >> j & 1);
       all += e[j];
-      left += out >> j & 1 ? 0.0 : e[j];
+      left += in ? e[j] : 0.0;
+      if (drawn) drafts += in ? qv[j] : 0.0;
     }
     const Pair sums = block_sums(all, left, box);
-    if (tid == 0) masses[static_cast<int64_t>(b) * n_parts + part] = {sums.a, sums.b};
+    if (drawn) drafts = block_sums(drafts, 0.0, box).a;
+    if (tid == 0) masses[static_cast<int64_t>(b) * n_parts + part] = {sums.a, sums.b, drafts};
   }
-}
-
-// Grid (parts, requests): of requests whose drawn draft was refused, the masses of max(p - q, 0).
-template <bool kBf16>
-__global__ __launch_bounds__(kThreads) void rest_kernel(
-    const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
-    const RowCut *__restrict__ cuts, Tree tree, const State *__restrict__ states,
-    const Mass *__restrict__ masses, double *__restrict__ rests) {
-  __shared__ Pair box[kWaves];
-  const int b = blockIdx.y, tid = threadIdx.x, n_parts = gridDim.x;
-  const Request req = requests.r[b];
-  if (req.temp == 0.f) return;
-  const State st = states[b];
-  if (st.bad || st.child < 0) return;
-  const Mass *mass = masses + static_cast<int64_t>(b) * n_parts;
-  const int row = req.first + st.last, first = blockIdx.x * kPart + kVec * tid;
-  const uint16_t *x_row = logits + row * ld;
-  const float *q = tree.drafts + (req.first + st.child) * tree.drafts_ld;
-  const double inv_temp = 1.0 / req.temp;
-  u32x4 w[1];
-  load_share(x_row, vocab, first, 0, w);
-  float qv[kVec];
-  load_drafts(q, first, vocab, qv);
-  const Cut cut = requests.cut(b, vocab) ? cut_of<kBf16>(cuts[row]) : no_cut();
-  double z = 0;
-  for (int i = tid; i < n_parts; i += kThreads) z += mass[i].all;
-  const double inv_z = 1.0 / block_sums(z, 0.0, box).a;
-  double e[kVec], left = 0;
-  masses_of<kBf16>(w[0], first, vocab, cut, st.max, inv_temp, e);
-#pragma unroll
-  for (int j = 0; j < kVec; ++j)
-    if (first + j < vocab) left += fmax(fma(e[j], inv_z, -static_cast<double>(qv[j])), 0.0);
-  left = block_sums(left, 0.0, box).a;
-  if (tid == 0) rests[static_cast<int64_t>(b) * n_parts + blockIdx.x] = left;
 }
 
 // Grid (requests).
@@ -751,8 +728,7 @@ template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void pick_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
     const RowCut *__restrict__ cuts, Tree tree, const State *__restrict__ states,
-    const Mass *__restrict__ masses, const double *__restrict__ rests, int n_parts,
-    int64_t *__restrict__ next) {
+    const Mass *__restrict__ masses, int n_parts, int64_t *__restrict__ next) {
   __shared__ uint32_t bits[kPart / 32];
   __shared__ PickRoom room;
   const int b = blockIdx.x, tid = threadIdx.x;
@@ -771,7 +747,6 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(
   const int got = pick_token<kBf16>(
       logits + row * ld, vocab, cut, st.max, 1.0 / req.temp, number,
       masses + static_cast<int64_t>(b) * n_parts,
-      drawn ? rests + static_cast<int64_t>(b) * n_parts : nullptr,
       drawn ? tree.drafts + (req.first + st.child) * tree.drafts_ld : nullptr, n_parts, parent, token,
       st.last, bits, room);
   if (tid == 0) next[b] = got;
@@ -782,7 +757,7 @@ int64_t share_count(int64_t vocab) { return (vocab + kShare - 1) / kShare; }
 int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
 
 struct Room {
-  int64_t cuts, shares, states, masses, rests, all;
+  int64_t cuts, shares, states, masses, all;
 };
 Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
   const int64_t n = share_count(vocab), parts = part_count(vocab);
@@ -798,7 +773,6 @@ Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
   r.shares = take(rows * n * static_cast<int64_t>(sizeof(Share)));
   r.states = take(requests * static_cast<int64_t>(sizeof(State)));
   r.masses = take(requests * parts * static_cast<int64_t>(sizeof(Mass)));
-  r.rests = take(requests * parts * static_cast<int64_t>(sizeof(double)));
   r.all = at;
   return r;
 }
@@ -812,7 +786,6 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &
   auto *shares = reinterpret_cast<Share *>(ws + room.shares);
   auto *states = reinterpret_cast<State *>(ws + room.states);
   auto *masses = reinterpret_cast<Mass *>(ws + room.masses);
-  auto *rests = reinterpret_cast<double *>(ws + room.rests);
   req.shares = shares;
   req.n_shares = n;
   if (cuts)
@@ -828,11 +801,8 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &
                      vocab, req, cut, shares, n, parts, tree, states, masses, paths, levels, lengths,
                      next, valid);
   if (!sampled) return;
-  if (tree.drafts)
-    hipLaunchKernelGGL(rest_kernel<kBf16>, dim3(parts, req.count), dim3(kThreads), 0, st, x, ld,
-                       vocab, req, cut, tree, states, masses, rests);
   hipLaunchKernelGGL(pick_kernel<kBf16>, dim3(req.count), dim3(kThreads), 0, st, x, ld, vocab, req,
-                     cut, tree, states, masses, rests, parts, next);
+                     cut, tree, states, masses, parts, next);
 }
 
 }  // namespace
