@@ -44,9 +44,10 @@ constexpr int kMaxNodes = 256;
 // The last row of a path goes to more workgroups, a load of logits a thread: its masses in 64 bits
 // take as long as one thread's chain of operations.
 constexpr int kPart = kThreads * kVec;
-// Workgroups of one walk launch, about: 16 trees of 26 nodes 12.0 us at 1024, 10.2 at 2048 and more
-// (a part each), 32 chains of 5 24.5, 15.0 and 16.5 at 256, 1024 and more.
-constexpr int kWalkers = 2048;
+// Workgroups of one walk launch, about: as many as run at once, so that none begins its walk when
+// others end theirs. 32 drawn chains of 5 took 19.0, 19.2, 17.3 and 20.9 us at 768, 1024, 1536 and
+// 2048, 16 trees of 26 nodes 11.9, 13.6, 10.8 and 10.8.
+constexpr int kWalkers = 1536;
 
 // A workgroup's share of a row: the largest kept logit and the sum of exp((x - max) / temp); of a
 // greedy row rank_of() of the largest.
