@@ -48,7 +48,13 @@
 //
 // With a window (kWindow) the stream holds only the keys in sight, numbered as window.h says:
 // the planner cuts those numbers, a slice's K and V rows lie at its number or `gap` keys
-// further, and a slice at the edge of the sinks or the window is masked as the last one is.
+// further, and a slice at the edge of the sinks or the window is masked as the last one is. Bound
+// by HBM as the whole-cache form: 20 requests that see 4,096 + 64 of 8,000 to 32,000 tokens take
+// 53 us for 341 MB (6.4 TB/s), 32 that see 1,000 + 4 22 us (5.1 TB/s); one takes 6 us, a launch
+// and the chain items, page table, K and V.
+//
+// With kScores a lane also stores its raw scores, 4 bytes a head and key beside 512 bytes of K and V
+// a kv head and key: 32 requests of 256 to 8,000 tokens 83 us for 428 MB (5.2 TB/s).
 
 #include <mutex>
 

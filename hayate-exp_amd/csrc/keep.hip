@@ -7,6 +7,10 @@
 // the 16 waves holds a stretch of positions, 64 a round, so that the output's order is that of
 // wave, round and lane and needs one exchange of counts. Up to 32,768 tokens the keys stay in
 // registers between the passes; longer rows are read again.
+//
+// Bound by one CU's instructions: five sweeps of about ten a key. 1,024 of 4,001 tokens take 5.1 us,
+// 2,047 of 32,700 15.4 us (20 requests side by side the same). Several workgroups a row would
+// meet three times in between, a launch of 2.5 us and more each.
 
 #include "hy_common.h"
 

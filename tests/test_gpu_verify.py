@@ -31,7 +31,9 @@ def target(row, t, k, p):
     score = row.double() / float(np.float32(t))
     if k is not None:
         score[score < torch.topk(score, min(k, len(score))).values[-1]] = -math.inf
-    prob = torch.softmax(score, 0)
+    # (torch's softmax of float64 is off by up to 2e-6 of a probability on the GPU)
+    prob = torch.exp(score - score.max())
+    prob /= prob.sum()
     if p is not None and p < 1:
         value, index = torch.sort(prob, descending=True, stable=True)
         over = (torch.cumsum(value, 0) > float(np.float32(p))).nonzero()
