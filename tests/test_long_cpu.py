@@ -165,3 +165,92 @@ def test_a_tick_with_a_form_of_its_own():
     assert batch.window is None and batch.weights is None
     with pytest.raises(NotImplementedError):
         m.begin_tick([h], [1], window=3).decode_layer(0, *[None] * 8, no_alloc=True)
+
+
+# Pointers that no entry may follow: every call below is refused before anything is enqueued.
+AT = 1 << 20
+
+
+def _tick_args(**kw):
+    a = dict(q=AT, q_seq=0, q_tok=4096, q_head=128, out=AT, o_seq=0, o_tok=4096, o_head=128, k=AT, v=AT,
+             pool_head=128 * 256, table=AT, table_stride=2, q_start=AT, kv_lens=AT, decode=AT,
+             n_decode=1, merge=AT, n_merge=1, n_slots=2, ws=AT, ws_bytes=1 << 30, prefill=AT,
+             n_prefill=1, prefill_merge=AT, n_prefill_merge=0, n_prefill_slots=0, prefill_ws=AT,
+             prefill_ws_bytes=1 << 30, num_seqs=2, hq=32, hkv=8, head_dim=128, page=128)
+    assert not set(kw) - set(a)
+    return list({**a, **kw}.values())
+
+
+EINVAL, EUNSUPPORTED, ENOSPACE = -1, -3, -4
+
+
+@pytest.mark.parametrize("kw,tail,code", [
+    ({}, (0, 0, 0.1), EINVAL), ({}, (5, -1, 0.1), EINVAL), ({}, (5, 2**30 + 1, 0.1), EINVAL),
+    ({}, (5, 0, 0.0), EINVAL), ({"n_merge": 0}, (5, 0, 0.1), EINVAL),
+    ({"n_decode": 0}, (5, 0, 0.1), EINVAL), ({"n_decode": -1}, (5, 0, 0.1), EINVAL),
+    ({"n_decode": 0, "n_merge": 0, "n_prefill": 0, "n_prefill_merge": 1}, (5, 0, 0.1), EINVAL),
+    ({"q": None}, (5, 0, 0.1), EINVAL), ({"hq": 30}, (5, 0, 0.1), EINVAL),
+    ({"head_dim": 64}, (5, 0, 0.1), EUNSUPPORTED), ({"hq": 24}, (5, 0, 0.1), EUNSUPPORTED),
+    ({"ws_bytes": 100}, (5, 0, 0.1), ENOSPACE),
+])
+def test_the_windowed_entry_refuses(kw, tail, code):
+    assert _native.lib().hy_paged_window(*_tick_args(**kw), *tail, None) == code
+    assert _native.lib().hy_last_error()
+
+
+@pytest.mark.parametrize("kw,weigh,code", [
+    ({}, {"n_weigh": -1}, EINVAL), ({}, {"n_weigh": 65536}, EINVAL), ({}, {"n_add": -1}, EINVAL),
+    ({}, {"scores": None}, EINVAL), ({}, {"score_start": None}, EINVAL),
+    ({}, {"scores": AT + 4}, EINVAL), ({}, {"score_stride": 30}, EINVAL),
+    ({}, {"partials": None}, EINVAL), ({}, {"partials": AT + 8}, EINVAL),
+    ({}, {"partial_stride": 30}, EINVAL), ({}, {"row_ml": None}, EINVAL),
+    ({}, {"weights": None}, EINVAL), ({}, {"adds": None}, EINVAL), ({}, {"items": None}, EINVAL),
+    ({"q": AT + 2}, {}, EINVAL), ({"q_tok": 4095}, {}, EINVAL), ({"n_merge": 0}, {}, EINVAL),
+    ({"hq": 2048, "hkv": 128}, {}, EUNSUPPORTED), ({"head_dim": 64}, {}, EUNSUPPORTED),
+])
+def test_the_weighing_entry_refuses(kw, weigh, code):
+    tail = dict(items=AT, n_weigh=1, adds=AT, n_add=1, score_start=AT, scores=AT, score_stride=64,
+                partials=AT, partial_stride=256, row_ml=AT, weights=AT, weights_stride=100, scale=0.1)
+    assert not set(weigh) - set(tail)
+    tail = {**tail, **weigh}.values()
+    assert _native.lib().hy_paged_weigh(*_tick_args(**kw), *tail, None) == code
+    assert _native.lib().hy_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    {"n": -1}, {"budget": 0}, {"sinks": -1}, {"recent": -1}, {"sinks": 8}, {"sinks": 4, "recent": 4},
+    {"weights": None}, {"out": None}, {"rows": None}, {"lens": None}, {"row": -1}, {"len": -1},
+    {"len": 2**30 + 1},
+])
+def test_the_keeping_entry_refuses(kw):
+    a = dict(weights=AT, n=2, budget=7, sinks=1, recent=2, out=AT, row=0, len=9, rows=0, lens=0)
+    a = {**a, **kw}
+    rows, lens = np.array([0, a["row"]], dtype=np.int32), np.array([3, a["len"]], dtype=np.int32)
+    rc = _native.lib().hy_keep_positions(
+        a["weights"], 100, None if a["rows"] is None else rows.ctypes.data,
+        None if a["lens"] is None else lens.ctypes.data, a["n"], a["budget"], a["sinks"], a["recent"],
+        a["out"], None)
+    assert rc == EINVAL and _native.lib().hy_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"dtype": 2}, EINVAL), ({"vocab": 0}, EINVAL), ({"levels": 0}, EINVAL), ({"n": -1}, EINVAL),
+    ({"vocab": 2**23}, EUNSUPPORTED), ({"logits": None}, EINVAL), ({"valid": None}, EINVAL),
+    ({"q_len": 0}, EINVAL), ({"q_len": 257}, EINVAL), ({"temperature": -1.0}, EUNSUPPORTED),
+    ({"temperature": float("nan")}, EUNSUPPORTED), ({"temperature": 1e31}, EUNSUPPORTED),
+    ({"top_k": 0}, EINVAL), ({"top_p": 0.0}, EINVAL), ({"ws_bytes": -1}, ENOSPACE),
+])
+def test_the_verifying_entry_refuses(kw, code):
+    lib = _native.lib()
+    a = dict(logits=AT, dtype=0, vocab=1000, levels=3, n=2, valid=AT, q_len=4, temperature=1.0,
+             top_k=5, top_p=0.5, ws_bytes=0)
+    a = {**a, **kw}
+    need = lib.hy_verify_workspace_bytes(3 + a["q_len"], 2, a["vocab"])
+    ints = lambda x: np.array([3, x], dtype=np.int32)  # noqa: E731
+    q_lens, top_k = ints(a["q_len"]), ints(a["top_k"])
+    temperature, top_p = (np.array([1, a[x]], dtype=np.float32) for x in ("temperature", "top_p"))
+    rc = lib.hy_verify_tree(
+        a["logits"], 1000, a["dtype"], a["vocab"], AT, AT, q_lens.ctypes.data, a["n"],
+        temperature.ctypes.data, top_k.ctypes.data, top_p.ctypes.data, AT, None, 0, AT, a["levels"], AT,
+        AT, a["valid"], AT, need + a["ws_bytes"], None)
+    assert rc == code and lib.hy_last_error()
