@@ -74,9 +74,8 @@
 // token: the half of a tile whose numbers are from ns on lies `gap` keys further.
 // Blocks that hold a key between the sinks and some row's window are masked like those on the
 // diagonal. A masked key's V may be infinite or NaN, which 0 times is NaN: masked blocks are
-// looked through for such values on the way to the second product (see clean_v: 1.5 instructions
-// a value of the masked blocks only; zeroing V by key in LDS instead would put a pass and a barrier
-// before every tile). Bound by MFMA and softmax as without a window: 4 chunks of 512 behind 0 to
+// looked through for such values on the way to the second product (see clean_v: one instruction
+// a value, of the masked blocks only). Bound by MFMA and softmax as without a window: 4 chunks of 512 behind 0 to
 // 5,000 tokens, window 1,024, 44 us a call for 31.3 GFLOP of visible pairs (711 TFLOP/s; a
 // 64-token tile's 32-key blocks hold a tenth more).
 
