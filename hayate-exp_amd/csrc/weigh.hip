@@ -5,8 +5,9 @@
 //
 // Single tokens: the decode kernel has stored its raw scores, 4 bytes a head and key where K and
 // V take 512 bytes a kv head and key; finish_kernel turns them into weights and sums the heads,
-// beside the workgroups that join the decode partials (instead of a launch of its own behind the
-// merge: 18.1 -> 15.1 us for one token on 2,000, 91 -> 89 for 32 on 4,096).
+// beside the workgroups that join the decode partials (18.1 -> 15.1 us a call for one token on 2,000
+// against a launch behind the merge, 91 -> 89 for 32 on up to 8,000; 13.5 with the loads of up to 64
+// partials, and of the first scores, in flight together: 6.0 us of its own instead of 9.1).
 // Chunks: storing scores would cost more than the products (512 rows x 32 heads x 4 bytes a key),
 // so weigh_kernel computes them again from K and Q, an item 256 keys by a range of rows, and
 // leaves a sum per kv head, range and key; finish_kernel adds those. Every sum has a fixed order.
@@ -251,91 +252,102 @@ void weigh_kernel(const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, in
   }
 }
 
-// Partials of a decode token that one lane joins in a round.
-constexpr int kRound = 8;
-
-// One decode token's output from its partials: the sums of decode_merge_kernel in its order, by 32
-// lanes a head, with the next round's loads out before a round is used. it = {seq, first slot,
-// slots, q_row}.
-__device__ __forceinline__ void join_partials(const int32_t *it, int heads0, uint16_t *out,
+// One decode token's output from its partials, a dim a lane and a head two waves: the sums of
+// decode_merge_kernel in its order (rounds of eight, each with the maximum so far as its base).
+// 64 partials are in flight at a time; their factors are made a lane each. it = {seq, first
+// slot, slots, q_row}.
+__device__ __forceinline__ void join_partials(const int32_t *it, int head0, uint16_t *out,
                                               int64_t o_ss, int64_t o_st, int64_t o_sh,
                                               const float *ws_acc, const float *ws_ml,
                                               int num_q_heads) {
   const int seq = it[0], first = it[1], n = it[2];
   const int64_t q_row = it[3];
-  const int mine = heads0 + static_cast<int>(threadIdx.x >> 5);
-  const int hq = min(mine, num_q_heads - 1);
-  const int d = (threadIdx.x & 31) * 4;
-  struct Round {
-    float2 ml[kRound];
-    f32x4 x[kRound];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int hq = head0 + (wave >> 1);
+  if (hq >= num_q_heads) return;
+  const int d = 64 * (wave & 1) + lane;
+  float mx = -INFINITY, lsum = 0.f, acc = 0.f;
+  auto lane_of = [](float v, int i) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
   };
-  auto load = [&](Round &r, int s0) __attribute__((always_inline)) {
+  for (int s0 = 0; s0 < n; s0 += 64) {
+    const int count = min(n - s0, 64);
+    const int64_t slot0 = first + s0;
+    float2 ml = *reinterpret_cast<const float2 *>(
+        ws_ml + ((slot0 + min(lane, count - 1)) * num_q_heads + hq) * 2);
+    float x[64];
 #pragma unroll
-    for (int j = 0; j < kRound; ++j) {
-      const int64_t at = static_cast<int64_t>(first + min(s0 + j, n - 1)) * num_q_heads + hq;
-      r.ml[j] = *reinterpret_cast<const float2 *>(ws_ml + at * 2);
-      r.x[j] = *reinterpret_cast<const f32x4 *>(ws_acc + at * kHeadDim + d);
-    }
-  };
-  float mx = -INFINITY, lsum = 0.f;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  auto join = [&](const Round &r, int s0) __attribute__((always_inline)) {
-    float m[kRound], top = mx;
+    for (int r = 0; r < 8; ++r) {
+      if (8 * r >= count) break;
 #pragma unroll
-    for (int j = 0; j < kRound; ++j) {
-      m[j] = s0 + j < n ? r.ml[j].x : -INFINITY;
-      top = fmaxf(top, m[j]);
+      for (int j = 0; j < 8; ++j)
+        x[8 * r + j] = ws_acc[((slot0 + min(8 * r + j, count - 1)) * num_q_heads + hq) * kHeadDim + d];
     }
-    const float old = mx == -INFINITY ? 0.f : exp2f(mx - top);
-    lsum *= old;
-    a *= old;
+    if (lane >= count) ml = make_float2(-INFINITY, 0.f);
+    // the maximum of the lane's eight, and of all before them
+    float top = ml.x;
 #pragma unroll
-    for (int j = 0; j < kRound; ++j) {
-      const bool live = s0 + j < n;
-      const float f = m[j] == -INFINITY ? 0.f : exp2f(m[j] - top);
-      lsum += f * (live ? r.ml[j].y : 0.f);
-      a += f * (live ? r.x[j] : f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    float base = mx, before = mx, after = mx;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float next = fmaxf(after, lane_of(top, 8 * r));
+      if (lane >> 3 == r) {
+        before = after;
+        base = next;
+      }
+      after = next;
     }
-    mx = top;
-  };
-  Round even, odd;
-  load(even, 0);
-  for (int s0 = 0; s0 < n; s0 += 2 * kRound) {
-    if (s0 + kRound < n) load(odd, s0 + kRound);
-    join(even, s0);
-    if (s0 + kRound >= n) break;
-    if (s0 + 2 * kRound < n) load(even, s0 + 2 * kRound);
-    join(odd, s0 + kRound);
+    mx = after;
+    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - base);
+    const float fl = f * ml.y;
+    const float rebase = before == -INFINITY ? 0.f : exp2f(before - base);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (8 * r >= count) break;
+      const float old = lane_of(rebase, 8 * r);
+      lsum *= old;
+      acc *= old;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (8 * r + j >= count) break;
+        lsum += lane_of(fl, 8 * r + j);
+        acc += lane_of(f, 8 * r + j) * x[8 * r + j];
+      }
+    }
   }
-  if (mine >= num_q_heads) return;
-  uint16_t *dst = out + seq * o_ss + q_row * o_st + hq * o_sh + d;
-  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2_rne(a[0] / lsum, a[1] / lsum),
-                                               pack_bf16x2_rne(a[2] / lsum, a[3] / lsum));
+  const float o = acc / lsum;
+  out[seq * o_ss + q_row * o_st + hq * o_sh + d] = static_cast<uint16_t>(pack_bf16x2_rne(o, o));
 }
 
-// The first n_join * groups workgroups join the partials of eight heads of a decode token each; the
-// others add to the table. Item = {row of the table, t0, t1, sources, first source, decode,
+// Slots of a decode token that one wave of the additions loads at a time, and scores.
+constexpr int kSlotsAhead = 16;
+constexpr int kScoresAhead = 8;
+
+// The first n_adds workgroups add to the table, the others join the partials of two heads of a
+// decode token each. Item = {row of the table, t0, t1, sources, first source, decode,
 // offset, 0}: at most 256 tokens [t0, t1). Of a chunk the sources are rows of partial sums; of a
 // decode token they are its partial slots, whose maxima and sums turn the scores of all query
 // heads into weights. Source or head x of token t is at src[x * stride + offset + t]; four waves
 // take them in turn.
 __global__ __launch_bounds__(256) void finish_kernel(
     uint16_t *__restrict__ out, int64_t o_ss, int64_t o_st, int64_t o_sh,
-    const int32_t *__restrict__ join_items, int n_join, int groups,
+    const int32_t *__restrict__ join_items, int groups,
     const float *__restrict__ ws_acc, const float *__restrict__ ws_ml,
-    const int32_t *__restrict__ items, const float *__restrict__ scores, int64_t score_stride,
+    const int32_t *__restrict__ items, int n_adds, const float *__restrict__ scores,
+    int64_t score_stride,
     const float *__restrict__ partials, int64_t partial_stride, int num_q_heads, float scale_log2,
     float *__restrict__ weights, int64_t weights_stride) {
   __shared__ f32x4 box[3][64];
   __shared__ float2 head_ml[kMaxHeads], part_ml[4][64];
   const int bid = blockIdx.x;
-  if (bid < n_join * groups) {
-    join_partials(join_items + 4 * (bid / groups), 8 * (bid % groups), out, o_ss, o_st, o_sh,
-                  ws_acc, ws_ml, num_q_heads);
+  if (bid >= n_adds) {
+    join_partials(join_items + 4 * ((bid - n_adds) / groups), 2 * ((bid - n_adds) % groups), out,
+                  o_ss, o_st, o_sh, ws_acc, ws_ml, num_q_heads);
     return;
   }
-  const int32_t *it = items + 8 * (bid - n_join * groups);
+  const int32_t *it = items + 8 * bid;
   const int row = it[0], t0 = it[1], t1 = it[2], n = it[3], from = it[4];
   const bool decode = it[5] != 0;
   const int64_t off = it[6];
@@ -344,25 +356,39 @@ __global__ __launch_bounds__(256) void finish_kernel(
   const int t = t0 + 4 * lane;
   const bool live = t < t1;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  // (loads that depend on nothing go out first: what is in the table, and the first scores)
+  float *dst = weights + row * weights_stride + t;
+  float was[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) was[e] = wave == 0 && t + e < t1 ? dst[e] : 0.f;
   if (decode) {
+    const int t_in = live ? t : t0;
+    auto load_score = [&](int i) __attribute__((always_inline)) {
+      return *reinterpret_cast<const f32x4 *>(scores + min(wave + 4 * i, num_q_heads - 1) * score_stride +
+                                              off + t_in);
+    };
+    f32x4 sc[kScoresAhead];
+#pragma unroll
+    for (int i = 0; i < kScoresAhead; ++i) sc[i] = load_score(i);
     // every head's maximum and inverse sum: lanes are heads, waves take the slots in turn
     for (int h0 = 0; h0 < num_q_heads; h0 += 64) {
       const int h = min(h0 + lane, num_q_heads - 1);
       float m = -INFINITY, l = 0.f;
-      for (int s0 = wave; s0 < n; s0 += 4 * kRound) {
-        float2 ml[kRound];
+      for (int s0 = wave; s0 < n; s0 += 4 * kSlotsAhead) {
+        float2 ml[kSlotsAhead];
         float top = m;
 #pragma unroll
-        for (int j = 0; j < kRound; ++j) {
-          const int64_t slot = from + min(s0 + 4 * j, n - 1);
-          ml[j] = *reinterpret_cast<const float2 *>(ws_ml + (slot * num_q_heads + h) * 2);
-          if (s0 + 4 * j >= n) ml[j] = make_float2(-INFINITY, 0.f);
+        for (int j = 0; j < kSlotsAhead; ++j) {
+          ml[j] = make_float2(-INFINITY, 0.f);
+          if (s0 + 4 * j >= n) continue;
+          ml[j] = *reinterpret_cast<const float2 *>(
+              ws_ml + (static_cast<int64_t>(from + s0 + 4 * j) * num_q_heads + h) * 2);
         }
 #pragma unroll
-        for (int j = 0; j < kRound; ++j) top = fmaxf(top, ml[j].x);
+        for (int j = 0; j < kSlotsAhead; ++j) top = fmaxf(top, ml[j].x);
         l = m == -INFINITY ? 0.f : l * exp2f(m - top);
 #pragma unroll
-        for (int j = 0; j < kRound; ++j)
+        for (int j = 0; j < kSlotsAhead; ++j)
           if (ml[j].x != -INFINITY) l += ml[j].y * exp2f(ml[j].x - top);
         m = top;
       }
@@ -381,16 +407,20 @@ __global__ __launch_bounds__(256) void finish_kernel(
       }
       __syncthreads();
     }
-    if (live) {
-#pragma unroll 8
-      for (int x = wave; x < num_q_heads; x += 4) {
-        const f32x4 s = *reinterpret_cast<const f32x4 *>(scores + x * score_stride + off + t);
+    for (int i0 = 0; wave + 4 * i0 < num_q_heads; i0 += kScoresAhead) {
+#pragma unroll
+      for (int i = 0; i < kScoresAhead; ++i) {
+        const int x = wave + 4 * (i0 + i);
+        if (x >= num_q_heads) break;
         const float2 r = head_ml[x];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           sum[e] = __builtin_fmaf(
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -r.x)), r.y, sum[e]);
+              __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][e], scale_log2, -r.x)), r.y, sum[e]);
       }
+      if (wave + 4 * (i0 + kScoresAhead) >= num_q_heads) break;
+#pragma unroll
+      for (int i = 0; i < kScoresAhead; ++i) sc[i] = load_score(i0 + kScoresAhead + i);
     }
   } else if (live) {
 #pragma unroll 4
@@ -402,10 +432,9 @@ __global__ __launch_bounds__(256) void finish_kernel(
   if (wave != 0 || !live) return;
 #pragma unroll
   for (int w = 0; w < 3; ++w) sum += box[w][lane];
-  float *dst = weights + row * weights_stride + t;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (t + e < t1) dst[e] += sum[e];
+    if (t + e < t1) dst[e] = was[e] + sum[e];
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -457,7 +486,7 @@ int hy::weigh_chunks(const char *name, const Rows &q, const Pools &pools, const 
 
 int hy::finish_weights(const char *name, const Rows &out, const Items &merge, const Workspace &ws,
                        const Shape &s, const Weigh &w, void *stream) {
-  const int groups = (s.num_q_heads + 7) / 8;
+  const int groups = (s.num_q_heads + 1) / 2;
   const int64_t blocks = static_cast<int64_t>(merge.count) * groups + w.n_adds;
   HY_REQUIRE(blocks <= INT32_MAX, "%s: too many records", name);
   if (blocks == 0) return HY_OK;
@@ -469,7 +498,7 @@ int hy::finish_weights(const char *name, const Rows &out, const Items &merge, co
       align256(static_cast<int64_t>(merge.slots) * s.num_q_heads * kHeadDim * 4));
   hipLaunchKernelGGL(finish_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), static_cast<uint16_t *>(out.at), out.seq,
-                     out.tok, out.head, merge.at, merge.count, groups, acc, ml, w.adds, w.scores.at,
+                     out.tok, out.head, merge.at, groups, acc, ml, w.adds, w.n_adds, w.scores.at,
                      w.scores.stride, w.partials, w.partial_stride, s.num_q_heads, s.scale * kLog2e,
                      w.weights, w.weights_stride);
   return hy::launch_status(name);

@@ -783,10 +783,12 @@ class PagedKVBatch:
                     plan.prefill_workspace_ptr, plan.prefill_workspace_bytes, self.num_seqs,
                     num_q_heads, self.num_kv_heads, self.head_dim, self.page_size)
             if self.window is not None:
-                cached = "hy_paged_window", args + (self.window, self.sinks)
+                name, args = "hy_paged_window", args + (self.window, self.sinks)
             else:
-                cached = "hy_paged_weigh", args + self._weigh_plan(num_q_heads).args
-            self._forms[num_q_heads] = cached
+                name, args = "hy_paged_weigh", args + self._weigh_plan(num_q_heads).args
+            # (as the library's types once, not with every call)
+            types = getattr(_native.lib(), name).argtypes[11:]
+            cached = self._forms[num_q_heads] = name, tuple(t(x) for t, x in zip(types, args))
         return cached
 
 
