@@ -454,6 +454,7 @@ int hy::check_weigh(const char *name, const Rows &q, const Shape &s, const Weigh
               15) == 0 &&
                  w.scores.stride % 4 == 0 && w.partial_stride % 4 == 0,
              "%s: scores and partial sums lie on 16 bytes", name);
+  HY_REQUIRE((reinterpret_cast<uintptr_t>(w.row_ml) & 7) == 0, "%s: row_ml lies on 8 bytes", name);
   HY_REQUIRE((reinterpret_cast<uintptr_t>(q.at) & 15) == 0 && ((q.seq | q.tok | q.head) & 7) == 0,
              "%s: q rows lie on 16 bytes", name);
   return HY_OK;

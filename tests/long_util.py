@@ -19,18 +19,20 @@ def normal(g, *shape, std=1.0):
 
 class Requests:
     """A pool of N(0, 1) whose requests hold `cached` tokens on pages in shuffled order, with
-    room for `fresh` more."""
+    room for `fresh` more. The pool's first `skip` pages are neither used nor written."""
 
-    def __init__(self, cached, fresh, hq=32, hkv=8, page=128, seed=0, layers=1, spare=3):
+    def __init__(self, cached, fresh, hq=32, hkv=8, page=128, seed=0, layers=1, spare=3, skip=0):
         self.g = torch.Generator(device=DEV).manual_seed(seed)
         self.cached, self.fresh, self.hq, self.hkv = list(cached), list(fresh), hq, hkv
         need = [-(-(c + n) // page) for c, n in zip(cached, fresh)]
-        pages = sum(need) + spare
+        pages = skip + sum(need) + spare
         self.m = PagedKVCacheManager(layers, hkv, D, pages * page, page, len(need) + 2,
                                      torch.bfloat16, DEV, num_q_heads=hq)
         for pool in (self.m.k_cache, self.m.v_cache):
-            pool.copy_(normal(self.g, *pool.shape))
-        order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed + 1)).tolist()
+            used = pool[..., skip * page :, :]
+            used.copy_(normal(self.g, *used.shape))
+        order = (skip + torch.randperm(pages - skip, generator=torch.Generator().manual_seed(
+            seed + 1))).tolist()
         self.handles = []
         for c, n in zip(self.cached, need):
             h = self.m.allocate()

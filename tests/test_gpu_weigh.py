@@ -62,6 +62,17 @@ def test_head_groups(hq, hkv):
                    seed=hq), what=f"{hq}/{hkv}")
 
 
+@pytest.mark.parametrize("split", [32, 96, 1000])
+def test_partials_by_the_hundred(split):
+    """(64 of a decode token's are joined at a time)"""
+    r = Requests([9000, 2048, 700, 63], [1, 1, 1, 1], seed=split)
+    r.m.tokens_per_split = split
+    check(r, what=f"split {split}")
+    one = Requests([9000], [1], hq=64, hkv=8, seed=split)
+    one.m.tokens_per_split = split
+    check(one, what=f"split {split}, one")
+
+
 @pytest.mark.parametrize("hq,hkv", [(128, 8), (2, 1), (80, 5)])
 def test_more_and_fewer_heads_than_a_waves_lanes(hq, hkv):
     """(partials of 64 heads are read at a time, outputs of eight joined)"""
@@ -76,6 +87,16 @@ def test_random_mixed_ticks(seed):
     fresh = [1 if pick(0, 2) else pick(2, 200) for _ in range(n)]
     r = Requests([pick(0, 2500) for _ in range(n)], fresh, seed=seed)
     check(r, scale=0.05 if seed == 3 else None, what=f"seed {seed}")
+
+
+def test_keys_behind_32_bit_offsets():
+    """Pools whose last pages lie 2^31 elements and more into each head: 9 GB."""
+    r = Requests([700, 90, 0], [1, 150, 70], hq=8, hkv=1, seed=2, skip=(2**31 // 128) // 128 + 1)
+    assert min(min(h.pages) for h in r.handles) * 128 * 128 >= 2**31
+    check(r, what="far")
+    out = r.m.begin_tick(r.handles, r.fresh, window=100, sinks=3).attend_layer(r.q, 0)
+    expected, bound, _ = r.expected(100, 3)
+    assert_close(out, expected, bound, "far, window")
 
 
 def test_rows_of_the_table():

@@ -203,7 +203,7 @@ def test_the_windowed_entry_refuses(kw, tail, code):
     ({}, {"scores": None}, EINVAL), ({}, {"score_start": None}, EINVAL),
     ({}, {"scores": AT + 4}, EINVAL), ({}, {"score_stride": 30}, EINVAL),
     ({}, {"partials": None}, EINVAL), ({}, {"partials": AT + 8}, EINVAL),
-    ({}, {"partial_stride": 30}, EINVAL), ({}, {"row_ml": None}, EINVAL),
+    ({}, {"partial_stride": 30}, EINVAL), ({}, {"row_ml": None}, EINVAL), ({}, {"row_ml": AT + 4}, EINVAL),
     ({}, {"weights": None}, EINVAL), ({}, {"adds": None}, EINVAL), ({}, {"items": None}, EINVAL),
     ({"q": AT + 2}, {}, EINVAL), ({"q_tok": 4095}, {}, EINVAL), ({"n_merge": 0}, {}, EINVAL),
     ({"hq": 2048, "hkv": 128}, {}, EUNSUPPORTED), ({"head_dim": 64}, {}, EUNSUPPORTED),
