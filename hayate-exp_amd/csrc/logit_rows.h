@@ -497,10 +497,20 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
     while (before + tie_cnt[round] < sh.cut_keep) before += tie_cnt[round++];
     const uint32_t want = sh.cut_keep - before;  // the want-th of this round, from 1
     const int i0 = round * kStep + kVec * tid;
-    auto is_cut = [&](int i) { return i < vocab && merge_zero(keys_of(x[i]) & 0xffffu) == cut; };
+    u32x4 mine = {0u, 0u, 0u, 0u};
+    if (i0 + kVec <= vocab) {
+      __builtin_memcpy(&mine, x + i0, sizeof(mine));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        mine[j >> 1] |= static_cast<uint32_t>(x[min(i0 + j, vocab - 1)]) << (16 * (j & 1));
+    }
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j) mine[j] = keys_of(mine[j]);
+    auto is_cut = [&](int j) { return i0 + j < vocab && merge_zero(key_at(mine, j)) == cut; };
     uint32_t c = 0;
-#pragma unroll 1
-    for (int j = 0; j < kVec; ++j) c += is_cut(i0 + j);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) c += is_cut(j);
     uint32_t ci = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -512,9 +522,9 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
     for (int w = 0; w < wave; ++w) ci += wave_cnt[w];
     if (ci - c < want && want <= ci) {
       uint32_t at = ci - c;
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < kVec; ++j)
-        if (is_cut(i0 + j) && ++at == want) sh.last = i0 + j;
+        if (is_cut(j) && ++at == want) sh.last = i0 + j;
     }
     __syncthreads();
   }
