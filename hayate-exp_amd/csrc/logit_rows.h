@@ -75,10 +75,11 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t v) {
 // rows.row(i): row i's settings. With Rows::kCutsOnly only rows with a top-k or top-p are read, and
 // rows.mass(i, largest logit or NaN, sum) gets the kept logits' sum of exp((x - largest) / temp),
 // which the counts tell without another read of the row.
+// A whole workgroup of kCutThreads takes row i.
 template <bool kBf16, class Rows>
-__global__ __launch_bounds__(kCutThreads) void cut_kernel(
-    const uint16_t *__restrict__ logits, int64_t ld, int vocab, Rows rows,
-    int64_t *__restrict__ out, RowCut *__restrict__ cuts) {
+__device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int64_t ld, int vocab,
+                                        const Rows &rows, int i_row, int64_t *__restrict__ out,
+                                        RowCut *__restrict__ cuts) {
   __shared__ uint32_t hist[kWords];
   __shared__ uint64_t best[kCutWaves];
   __shared__ uint32_t wave_cnt[kCutWaves];
@@ -94,8 +95,8 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
-  const SampleRow row = rows.row(blockIdx.x);
-  const uint16_t *x = logits + blockIdx.x * ld;
+  const SampleRow row = rows.row(i_row);
+  const uint16_t *x = logits + i_row * ld;
   const bool greedy = row.temp == 0.f;
   const bool use_k = !greedy && row.k < vocab;
   const bool use_p = !greedy && row.p < 1.f;
@@ -209,8 +210,8 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
     }
     const uint64_t b = block_best(rank_of(1, first));
     if (tid == 0) {
-      out[blockIdx.x] = index_of(b);
-      cuts[blockIdx.x].ok = -1;
+      out[i_row] = index_of(b);
+      cuts[i_row].ok = -1;
     }
     return;
   }
@@ -218,15 +219,15 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
   // softmax of such a row has no probabilities
   if (nan || isinf(mx)) {
     if constexpr (Rows::kCutsOnly)
-      rows.mass(blockIdx.x, NAN, NAN);
+      rows.mass(i_row, NAN, NAN);
     else if (tid == 0)
-      out[blockIdx.x] = 0;
-    if (tid == 0) cuts[blockIdx.x].ok = 0;
+      out[i_row] = 0;
+    if (tid == 0) cuts[i_row].ok = 0;
     return;
   }
   auto finish = [&]() __attribute__((always_inline)) {
     if (tid == 0)
-      cuts[blockIdx.x] = {max(sh.kth, sh.cut), sh.cut, sh.last, 1, mx};
+      cuts[i_row] = {max(sh.kth, sh.cut), sh.cut, sh.last, 1, mx};
   };
   if (!filter) {
     finish();
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(kCutThreads) void cut_kernel(
     __syncthreads();
     sum = 0;
     for (int w = 0; w < kCutWaves; ++w) sum += wave_sum[w];
-    rows.mass(blockIdx.x, top_value, static_cast<float>(sum));
+    rows.mass(i_row, top_value, static_cast<float>(sum));
   }
   // A value that the cut splits keeps its first logits by index: count it by
   // rounds, then find the last kept one in its round.

@@ -43,6 +43,14 @@ struct SampleRows {
   __device__ __forceinline__ SampleRow row(int i) const { return r[i]; }
 };
 
+// Grid (rows).
+template <bool kBf16>
+__global__ __launch_bounds__(kCutThreads) void cut_kernel(
+    const uint16_t *__restrict__ logits, int64_t ld, int vocab, SampleRows rows,
+    int64_t *__restrict__ out, RowCut *__restrict__ cuts) {
+  cut_row<kBf16>(logits, ld, vocab, rows, blockIdx.x, out, cuts);
+}
+
 // Grid (shares of a row, rows): the best p / q of kDrawShare logits.
 template <bool kBf16>
 __global__ __launch_bounds__(kDrawThreads) void draw_kernel(
@@ -195,8 +203,7 @@ extern "C" int hy_sample(const void *logits, int64_t row_stride, int32_t dtype, 
     const uint16_t *x = static_cast<const uint16_t *>(logits) + r0 * row_stride;
     auto *cuts = static_cast<hy::RowCut *>(workspace);
     auto *bests = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + hy::cut_bytes(n));
-    auto cut = dtype == 0 ? hy::cut_kernel<true, hy::SampleRows>
-                          : hy::cut_kernel<false, hy::SampleRows>;
+    auto cut = dtype == 0 ? hy::cut_kernel<true> : hy::cut_kernel<false>;
     auto draw = dtype == 0 ? hy::draw_kernel<true> : hy::draw_kernel<false>;
     hipLaunchKernelGGL(cut, dim3(n), dim3(hy::kCutThreads), 0, st, x, row_stride, vocab, rows,
                        out + r0, cuts);

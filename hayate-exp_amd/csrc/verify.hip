@@ -14,11 +14,13 @@
 // The draw takes the smallest token whose cumulative mass exceeds u times the total; where
 // nothing is left (all mass refused) it is from p.
 //
-//   cut_kernel    rows of requests with top-k or top-p only: where they are cut, and the sum of
-//                 exponentials of what is kept, from the counts that find the cut (16 trees of up
-//                 to 26 nodes, half of them cut: 63.6 -> 60.1 us against a second read).
-//   mass_kernel   the other rows, many workgroups a row: the maximum and the sum of exponentials
-//                 of each one's share of the logits (greedy: its largest logit).
+//   mass_kernel   many workgroups a row: the maximum and the sum of exponentials of each one's
+//                 share of the logits (greedy: its largest logit).
+//   cut_mass_kernel  instead, where a request has top-k or top-p: its rows are cut first (a
+//                 workgroup each), and what the cut's counts sum up to is their mass, without a
+//                 second read; the other rows' shares go to the CUs beside them. 16 trees of up
+//                 to 26 nodes, half of them cut: 63.6 us with two launches and a second read,
+//                 60.0 without it, 49.6 in one launch.
 //   walk_kernel   the walk, in every workgroup of the request: its tests need the shares of its
 //                 rows and a logit a node, a few reads that all nodes make at once. Then the
 //                 masses of its part of the last node's row, in 64 bits: a border between
@@ -32,8 +34,8 @@
 //
 // A call is bound by its chain of dependent launches: 8 nodes of 151,936 tokens take 4.3 us (mass),
 // 6.5 (walk) and 6.1 (pick), less than the host's 27. With many rows the cuts lead (16 trees of up
-// to 26 nodes: 31, 12, 11 and 7 us; a CU's reads and LDS counts), then the masses' exponentials
-// (32 drawn chains of 5: 11, 17 and 8).
+// to 26 nodes: 32.7 with the masses, 10.8 and 7.0 us; a CU's reads and LDS counts), then the
+// masses' exponentials (32 drawn chains of 5: 11, 17 and 8).
 
 #include <algorithm>
 
@@ -65,7 +67,8 @@ struct Request {
   float temp;
   int32_t k;
   float p;
-  int32_t first;  // its first row
+  int32_t first;       // its first row
+  int32_t cut_before;  // rows before it that are cut
 };
 struct Requests {
   static constexpr bool kCutsOnly = true;
@@ -84,6 +87,19 @@ struct Requests {
         hi = mid;
     }
     return lo;
+  }
+  // The i-th row that is cut, or that is not.
+  __device__ __forceinline__ int nth_row(bool is_cut, int i) const {
+    auto before = [&](int b) { return is_cut ? r[b].cut_before : r[b].first - r[b].cut_before; };
+    int lo = 0, hi = count;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before(mid) <= i)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return r[lo].first + i - before(lo);
   }
   __device__ __forceinline__ int nodes(int b) const {
     return (b + 1 < count ? r[b + 1].first : rows) - r[b].first;
@@ -206,14 +222,14 @@ __device__ __forceinline__ double wave_sum(double v) {
   v = row_sum(v);
   return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
-// Over the workgroup, in a fixed order and in every thread: of two values at once.
+// Over each kThreads of the workgroup, in a fixed order and in every thread: of two values at once.
 struct Pair {
   double a, b;
 };
 __device__ __forceinline__ Pair block_sums(double a, double b, Pair *box) {
   const Pair mine = {wave_sum(a), wave_sum(b)};
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = mine;
+  if ((threadIdx.x & 63) == 0) box[(threadIdx.x >> 6) % kWaves] = mine;
   __syncthreads();
   Pair all = box[0];
 #pragma unroll
@@ -224,14 +240,14 @@ __device__ __forceinline__ Pair block_sums(double a, double b, Pair *box) {
   return all;
 }
 
-// The first largest logit of a workgroup's share as rank_of() has it; a NaN is the largest of all.
+// The first largest logit of a share as rank_of() has it; a NaN is the largest of all.
 // Keys in pairs: of three operations a logit nothing but the maximum comes, and the threads
 // that hold it look for its place.
 template <bool kBf16>
 __device__ __forceinline__ uint64_t best_of_share(const u32x4 (&w)[kAhead], int first, int step,
                                                   int vocab, uint32_t *top_box, int *first_box) {
   constexpr uint32_t kInf = kInfBits<kBf16>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % kWaves;
   u16x2 top2 = {0, 0}, mag2 = {0, 0};
 #pragma unroll
   for (int a = 0; a < kAhead; ++a)
@@ -251,7 +267,7 @@ __device__ __forceinline__ uint64_t best_of_share(const u32x4 (&w)[kAhead], int 
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t = max(t, static_cast<uint32_t>(__shfl_xor(static_cast<int>(t), o)));
   if (lane == 0) top_box[wave] = t;
-  if (threadIdx.x == 0) *first_box = vocab;
+  if (threadIdx.x % kThreads == 0) *first_box = vocab;
   __syncthreads();
   t = top_box[0];
 #pragma unroll
@@ -273,28 +289,27 @@ __device__ __forceinline__ uint64_t best_of_share(const u32x4 (&w)[kAhead], int 
   return rank_of(t, *first_box);
 }
 
-// Grid (shares, rows): of the rows that are not cut.
+struct MassRoom {
+  float maxes[kWaves];
+  uint32_t tops[kWaves];
+  int place;
+  Pair box[kWaves];
+};
+// One share of a row that is not cut, by kThreads threads; the others of the workgroup have
+// shares of the same row.
 template <bool kBf16>
-__global__ __launch_bounds__(kThreads) void mass_kernel(
-    const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
-    Share *__restrict__ shares, uint8_t *__restrict__ valid, bool first_rows) {
-  __shared__ float maxes[kWaves];
-  __shared__ uint32_t tops[kWaves];
-  __shared__ int place;
-  __shared__ Pair box[kWaves];
-  if (first_rows && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *valid = 1;
-  const int row = blockIdx.y;
-  const int b = requests.of_row(row);
-  if (requests.cut(b, vocab)) return;
+__device__ __forceinline__ void mass_of_share(const uint16_t *row, int vocab, float temp, int share,
+                                              int n_shares, Share *shares, MassRoom &room) {
+  const int tid = threadIdx.x % kThreads;
   constexpr int kRound = kThreads * kVec;
-  const int i0 = blockIdx.x * kShare + kVec * threadIdx.x;
+  const int i0 = min(share, n_shares - 1) * kShare + kVec * tid;
   u32x4 w[kAhead];
-  load_share(logits + row * ld, vocab, i0, kRound, w);
-  const float temp = requests.r[b].temp;
-  Share *out = shares + static_cast<int64_t>(row) * gridDim.x + blockIdx.x;
+  load_share(row, vocab, i0, kRound, w);
+  const bool tells = tid == 0 && share < n_shares;
+  Share *out = shares + share;
   if (temp == 0.f) {
-    const uint64_t best = best_of_share<kBf16>(w, i0, kRound, vocab, tops, &place);
-    if (threadIdx.x == 0) out->best = best;
+    const uint64_t best = best_of_share<kBf16>(w, i0, kRound, vocab, room.tops, &room.place);
+    if (tells) out->best = best;
     return;
   }
   float x[kAhead][kVec], m = -INFINITY;
@@ -302,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) x[a][j] = value_in<kBf16>(w[a], j);
-  if ((static_cast<int>(blockIdx.x) + 1) * static_cast<int64_t>(kShare) > vocab) {
+  if ((share + 1) * static_cast<int64_t>(kShare) > vocab) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
@@ -315,11 +330,11 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
     for (int j = 0; j < kVec; ++j) m = fmaxf(m, x[a][j]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if ((threadIdx.x & 63) == 0) maxes[threadIdx.x >> 6] = m;
+  if ((threadIdx.x & 63) == 0) room.maxes[tid >> 6] = m;
   __syncthreads();
-  m = maxes[0];
+  m = room.maxes[0];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, maxes[i]);
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, room.maxes[i]);
   const float slope = 1.0f / temp * kLog2eS;
   // The differences are scaled, not the terms: at small temperatures those are far apart. NaN,
   // and infinities less each other, make the sum NaN; a share without a finite logit is
@@ -330,11 +345,44 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) s += __builtin_amdgcn_exp2f((x[a][j] - from) * slope);
-  const double sum = block_sums(s, 0.0, box).a;
-  if (threadIdx.x == 0) {
+  const double sum = block_sums(s, 0.0, room.box).a;
+  if (tells) {
     out->max = sum == sum ? m : NAN;
     out->sum = static_cast<float>(sum);
   }
+}
+
+// Grid (shares, rows): no row is cut.
+template <bool kBf16>
+__global__ __launch_bounds__(kThreads) void mass_kernel(const uint16_t *__restrict__ logits, int64_t ld,
+                                                        int vocab, Requests requests,
+                                                        uint8_t *__restrict__ valid, bool first_rows) {
+  __shared__ MassRoom room;
+  if (first_rows && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *valid = 1;
+  const int row = blockIdx.y;
+  mass_of_share<kBf16>(logits + row * ld, vocab, requests.r[requests.of_row(row)].temp, blockIdx.x,
+                       gridDim.x, requests.shares + static_cast<int64_t>(row) * gridDim.x, room);
+}
+
+// The first n_cut workgroups find the cuts, a row each; the others, four shares each, fill the
+// CUs beside them.
+template <bool kBf16>
+__global__ __launch_bounds__(kCutThreads) void cut_mass_kernel(
+    const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests, int n_cut,
+    RowCut *__restrict__ cuts, uint8_t *__restrict__ valid, bool first_rows) {
+  constexpr int kShares = kCutThreads / kThreads;
+  __shared__ MassRoom rooms[kShares];
+  if (first_rows && blockIdx.x == 0 && threadIdx.x == 0) *valid = 1;
+  const int block = blockIdx.x;
+  if (block < n_cut) {
+    cut_row<kBf16>(logits, ld, vocab, requests, requests.nth_row(true, block), nullptr, cuts);
+    return;
+  }
+  const int per_row = (requests.n_shares + kShares - 1) / kShares, group = threadIdx.x / kThreads;
+  const int row = requests.nth_row(false, (block - n_cut) / per_row);
+  mass_of_share<kBf16>(logits + row * ld, vocab, requests.r[requests.of_row(row)].temp,
+                       (block - n_cut) % per_row * kShares + group, requests.n_shares,
+                       requests.shares + static_cast<int64_t>(row) * requests.n_shares, rooms[group]);
 }
 
 // exp(x), x <= 0, to about 1e-12: 2^n times the Taylor series of the rest, |r| <= ln(2) / 2 and a
@@ -785,7 +833,7 @@ Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
 }
 
 template <bool kBf16>
-void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &req, bool cuts,
+void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &req, int n_cut,
             const Tree &tree, char *ws, const Room &room, int32_t *paths, int levels,
             int32_t *lengths, int64_t *next, uint8_t *valid, bool first_rows) {
   const int n = static_cast<int>(share_count(vocab)), parts = static_cast<int>(part_count(vocab));
@@ -795,11 +843,15 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &
   auto *masses = reinterpret_cast<Mass *>(ws + room.masses);
   req.shares = shares;
   req.n_shares = n;
-  if (cuts)
-    hipLaunchKernelGGL((cut_kernel<kBf16, Requests>), dim3(req.rows), dim3(kCutThreads), 0, st, x,
-                       ld, vocab, req, static_cast<int64_t *>(nullptr), cut);
-  hipLaunchKernelGGL(mass_kernel<kBf16>, dim3(n, req.rows), dim3(kThreads), 0, st, x, ld, vocab, req,
-                     shares, valid, first_rows);
+  if (n_cut > 0) {
+    constexpr int kShares = kCutThreads / kThreads;
+    const int64_t blocks = n_cut + static_cast<int64_t>(req.rows - n_cut) * ((n + kShares - 1) / kShares);
+    hipLaunchKernelGGL(cut_mass_kernel<kBf16>, dim3(static_cast<uint32_t>(blocks)), dim3(kCutThreads),
+                       0, st, x, ld, vocab, req, n_cut, cut, valid, first_rows);
+  } else {
+    hipLaunchKernelGGL(mass_kernel<kBf16>, dim3(n, req.rows), dim3(kThreads), 0, st, x, ld, vocab, req,
+                       valid, first_rows);
+  }
   bool sampled = false;
   for (int b = 0; b < req.count; ++b) sampled = sampled || req.r[b].temp != 0.f;
   // Every workgroup of a request repeats its walk: no more of them than fill the GPU.
@@ -859,19 +911,19 @@ extern "C" int hy_verify_tree(const void *logits, int64_t row_stride, int32_t dt
   for (int32_t b0 = 0; b0 < num_seqs; b0 += hy::kRequests) {
     hy::Requests req{};
     req.count = num_seqs - b0 < hy::kRequests ? num_seqs - b0 : hy::kRequests;
-    bool cuts = false;
+    int n_cut = 0;
     for (int i = 0; i < req.count; ++i) {
       const int b = b0 + i;
       const int32_t k = top_k[b] < vocab ? top_k[b] : vocab;
-      req.r[i] = {temperature[b], k, top_p[b], req.rows};
+      req.r[i] = {temperature[b], k, top_p[b], req.rows, n_cut};
       req.rows += q_lens[b];
-      cuts = cuts || (temperature[b] != 0.f && (k < vocab || top_p[b] < 1.f));
+      if (temperature[b] != 0.f && (k < vocab || top_p[b] < 1.f)) n_cut += q_lens[b];
     }
     const hy::Tree tree{parents + row0, tokens + row0, uniforms + row0, uniforms + rows + b0,
                         draft_probs ? draft_probs + row0 * draft_stride : nullptr, draft_stride};
     (dtype == 0 ? hy::launch<true> : hy::launch<false>)(
         static_cast<hipStream_t>(stream), static_cast<const uint16_t *>(logits) + row0 * row_stride,
-        row_stride, vocab, req, cuts, tree, static_cast<char *>(workspace), room,
+        row_stride, vocab, req, n_cut, tree, static_cast<char *>(workspace), room,
         paths + static_cast<int64_t>(b0) * levels, levels, lengths + b0, next_tokens + b0, valid,
         b0 == 0);
     row0 += req.rows;
