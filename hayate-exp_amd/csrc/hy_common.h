@@ -93,6 +93,17 @@ __device__ __forceinline__ float row_bcast(float x) {
       0, __float_as_int(x), 0x150 + src, 0xf, 0xf, false));
 }
 
+// Sum of x over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
 // Sum / max over the 16 lanes of a row (xor butterfly).
 __device__ __forceinline__ float row16_sum(float x) {
   x += __shfl_xor(x, 8, 16);

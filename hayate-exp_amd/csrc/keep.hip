@@ -35,17 +35,6 @@ struct KeepShared {
   uint32_t found[2];
 };
 
-// Sum of x over the lanes up to this one.
-__device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
-  return x;
-}
-
 // Sum of the waves' values before `wave`.
 __device__ __forceinline__ uint32_t waves_before(const uint32_t *of, int wave) {
   const int lane = threadIdx.x & 63;

@@ -260,7 +260,7 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
     __syncthreads();
   };
   // This thread's words, in an order that spreads a wave over the banks.
-  constexpr int kSpan = kWords / kCutThreads;
+  constexpr int kSpan = kWords / kCutThreads, kBatch = 8;
   const int top_word = kWords - 1 - kSpan * tid;
   auto my_word = [&](int i) { return top_word - ((i + tid) & (kSpan - 1)); };
   // Keys and counts of a word: two in 16 bits, or one.
@@ -277,12 +277,12 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
   uint32_t cnt, above;
   auto scan_counts = [&](uint32_t cnt0) __attribute__((always_inline)) {
     cnt = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < kSpan; ++i) {
       const uint32_t c = hist[my_word(i)];
       cnt += wide ? c : (c >> 16) + (c & 0xffffu);
     }
-    const uint32_t ci = wave_scan(cnt);
+    const uint32_t ci = lanes_up_to(cnt);
     __syncthreads();
     if (lane == 63) wave_cnt[wave] = ci;
     __syncthreads();
@@ -322,15 +322,22 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
     const int kth = sh.kth;
     if ((key_of_word(top_word) | 1) >= kth) {
 #pragma unroll 1
-      for (int i = 0; i < kSpan; ++i) {
-        const int w = my_word(i);
-        const uint32_t c = hist[w];
-        const int key = key_of_word(w);
-        if (wide) {
-          if (c && key >= kth) s += c * mass_of(key);
-        } else {
-          if (c >> 16 && key + 1 >= kth) s += (c >> 16) * mass_of(key + 1);
-          if ((c & 0xffffu) && key >= kth) s += (c & 0xffffu) * mass_of(key);
+      for (int i0 = 0; i0 < kSpan; i0 += kBatch) {
+        uint32_t c[kBatch], some = 0;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          c[j] = hist[my_word(i0 + j)];
+          some |= c[j];
+        }
+        // (few of the keys occur; those that do, side by side and without a branch)
+        if (!__any(some)) continue;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int key = key_of_word(my_word(i0 + j));
+          const uint32_t high = wide ? 0 : c[j] >> 16, low = wide ? c[j] : c[j] & 0xffffu;
+          const float of_high = high * mass_of(key + 1), of_low = low * mass_of(key);
+          s += high && key + 1 >= kth ? of_high : 0.f;
+          s += low && key >= kth ? of_low : 0.f;
         }
       }
     }
