@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "hy_common.h"
 
 namespace hy {
@@ -72,6 +74,19 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t v) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+  auto turned = [](uint32_t x, auto by) __attribute__((always_inline)) {  // within 16 lanes
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x120 + decltype(by)::value, 0xf, 0xf, false));
+  };
+  v = max(v, turned(v, std::integral_constant<int, 8>{}));
+  v = max(v, turned(v, std::integral_constant<int, 4>{}));
+  v = max(v, turned(v, std::integral_constant<int, 2>{}));
+  v = max(v, turned(v, std::integral_constant<int, 1>{}));
+  auto lane_of = [&](int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), i)); };
+  return max(max(lane_of(0), lane_of(16)), max(lane_of(32), lane_of(48)));
+}
+
 // rows.row(i): row i's settings. With Rows::kCutsOnly only rows with a top-k or top-p are read, and
 // rows.mass(i, largest logit or NaN, sum) gets the kept logits' sum of exp((x - largest) / temp),
 // which the counts tell without another read of the row.
@@ -80,7 +95,7 @@ template <bool kBf16, class Rows>
 __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int64_t ld, int vocab,
                                         const Rows &rows, int i_row, int64_t *__restrict__ out,
                                         RowCut *__restrict__ cuts) {
-  __shared__ uint32_t hist[kWords];
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kWords];
   __shared__ uint64_t best[kCutWaves];
   __shared__ uint32_t wave_cnt[kCutWaves];
   __shared__ float wave_mass[kCutWaves];
@@ -146,8 +161,12 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
 
   const bool filter = use_k || use_p;
   if (Rows::kCutsOnly && !filter) return;
-  if (filter)
-    for (int i = tid; i < kWords; i += kCutThreads) hist[i] = 0;
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; i += kCutThreads)
+      reinterpret_cast<u32x4 *>(hist)[i + tid] = u32x4{0u, 0u, 0u, 0u};
+  };
+  if (filter) clear();
   if (tid == 0) {
     sh.kth = use_k ? -1 : 0;
     sh.cut = use_p ? -1 : 0;
@@ -188,9 +207,23 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
     }
   });
   const uint32_t mag = max(mag2[0], mag2[1]) & 0x7fffu;
-  const uint64_t top = block_best(rank_of(my_key, my_load));
-  const uint32_t top_key = merge_zero(static_cast<uint32_t>(top >> 32));
-  const bool nan = __syncthreads_or(mag > kInfBits<kBf16>);
+  const bool my_nan = mag > kInfBits<kBf16>;
+  uint64_t top = 0;
+  uint32_t top_key;
+  bool nan;
+  if (greedy) {
+    top = block_best(rank_of(my_key, my_load));
+    top_key = merge_zero(static_cast<uint32_t>(top >> 32));
+    nan = __syncthreads_or(my_nan);
+  } else {
+    top_key = wave_largest(my_nan ? 0x10000u : my_key);
+    if (lane == 0) wave_cnt[wave] = top_key;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kCutWaves; ++w) top_key = max(top_key, wave_cnt[w]);
+    nan = top_key == 0x10000u;
+    top_key = merge_zero(top_key);
+  }
 
   if (greedy) {
     // the first logit of the largest value; a NaN counts as the largest
@@ -248,7 +281,7 @@ __device__ __forceinline__ void cut_row(const uint16_t *__restrict__ logits, int
   auto build = [&](int half) __attribute__((always_inline)) {
     held = half;
     __syncthreads();
-    for (int i = tid; i < kWords; i += kCutThreads) hist[i] = 0;
+    clear();
     __syncthreads();
     each([&](const u32x4 &w, int, int n) __attribute__((always_inline)) {
 #pragma unroll

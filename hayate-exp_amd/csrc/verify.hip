@@ -19,8 +19,9 @@
 //   cut_mass_kernel  instead, where a request has top-k or top-p: its rows are cut first (a
 //                 workgroup each), and what the cut's counts sum up to is their mass, without a
 //                 second read; the other rows' shares go to the CUs beside them. 16 trees of up
-//                 to 26 nodes, half of them cut: 63.6 us with two launches and a second read,
-//                 60.0 without it, 49.6 in one launch.
+//                 to 26 nodes, half of them cut: 63.6 us a call with two launches and a second
+//                 read, 60.0 without it, 47.3 in one launch (with two shares' loads in flight a
+//                 workgroup 52.6: fewer, longer ones end later).
 //   walk_kernel   the walk, in every workgroup of the request: its tests need the shares of its
 //                 rows and a logit a node, a few reads that all nodes make at once. Then the
 //                 masses of its part of the last node's row, in 64 bits: a border between
@@ -30,11 +31,10 @@
 //   pick_kernel   the part that holds the draw, then the token. (In the walk's last workgroup of
 //                 each request instead, the releases and acquires of all others took 20 us
 //                 more with 32 requests.)
-
 //
 // A call is bound by its chain of dependent launches: 8 nodes of 151,936 tokens take 4.3 us (mass),
 // 6.5 (walk) and 6.1 (pick), less than the host's 27. With many rows the cuts lead (16 trees of up
-// to 26 nodes: 32.7 with the masses, 10.8 and 7.0 us; a CU's reads and LDS counts), then the
+// to 26 nodes: 30.4 with the masses, 10.9 and 6.8 us; a CU's reads and LDS counts), then the
 // masses' exponentials (32 drawn chains of 5: 11, 17 and 8).
 
 #include <algorithm>
@@ -211,6 +211,9 @@ __device__ __forceinline__ float row_max(float v) {
   v = fmaxf(v, __uint_as_float(ror<2>(__float_as_uint(v))));
   return fmaxf(v, __uint_as_float(ror<1>(__float_as_uint(v))));
 }
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
 __device__ __forceinline__ double lane_of(double v, int lane) {
   const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
   const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
@@ -293,7 +296,7 @@ struct MassRoom {
   float maxes[kWaves];
   uint32_t tops[kWaves];
   int place;
-  Pair box[kWaves];
+  double sums[kWaves];
 };
 // One share of a row that is not cut, by kThreads threads; the others of the workgroup have
 // shares of the same row.
@@ -328,8 +331,8 @@ __device__ __forceinline__ void mass_of_share(const uint16_t *row, int vocab, fl
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) m = fmaxf(m, x[a][j]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  m = row_max(m);
+  m = fmaxf(fmaxf(lane_of(m, 0), lane_of(m, 16)), fmaxf(lane_of(m, 32), lane_of(m, 48)));
   if ((threadIdx.x & 63) == 0) room.maxes[tid >> 6] = m;
   __syncthreads();
   m = room.maxes[0];
@@ -345,7 +348,12 @@ __device__ __forceinline__ void mass_of_share(const uint16_t *row, int vocab, fl
   for (int a = 0; a < kAhead; ++a)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) s += __builtin_amdgcn_exp2f((x[a][j] - from) * slope);
-  const double sum = block_sums(s, 0.0, room.box).a;
+  const double mine = wave_sum(static_cast<double>(s));
+  if ((threadIdx.x & 63) == 0) room.sums[tid >> 6] = mine;
+  __syncthreads();
+  double sum = room.sums[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) sum += room.sums[i];
   if (tells) {
     out->max = sum == sum ? m : NAN;
     out->sum = static_cast<float>(sum);
