@@ -166,6 +166,17 @@ def test_more_requests_than_one_launch_takes():
     check(chains, 2000, 7, *map(list, zip(*settings)), drafts=True)
 
 
+@pytest.mark.parametrize("cut", [{70}, {0}, {63, 64}, set(range(80)) - {5, 66}])
+def test_cut_requests_among_others(cut):
+    """Which rows are cut differs by launch of 64 requests: in none, one, or nearly all of them."""
+    g = torch.Generator().manual_seed(len(cut))
+    trees = [random_tree(g, int(torch.randint(1, 6, (1,), generator=g))) for _ in range(80)]
+    temps = [0.0 if b % 5 == 1 and b not in cut else 0.9 for b in range(80)]
+    ks = [11 if b in cut and b % 2 else None for b in range(80)]
+    ps = [0.7 if b in cut and not b % 2 else None for b in range(80)]
+    check(trees, 9000, 17, temps, ks, ps)
+
+
 def test_equal_tokens_and_certain_ones():
     """Siblings with one token: refused once, refused for good. A token that has all the mass
     stands whatever the number; where everything is refused the draw is from p."""
