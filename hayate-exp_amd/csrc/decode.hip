@@ -53,8 +53,9 @@
 // 53 us for 341 MB (6.4 TB/s), 32 that see 1,000 + 4 22 us (5.1 TB/s); one takes 6 us, a launch
 // and the chain items, page table, K and V.
 //
-// With kScores a lane also stores its raw scores, 4 bytes a head and key beside 512 bytes of K and V
-// a kv head and key: 32 requests of 256 to 8,000 tokens 83 us for 428 MB (5.2 TB/s).
+// With kScores the raw scores go to memory too, 4 bytes a head and key beside 512 bytes of K and V a
+// kv head and key, from LDS in as few bursts as fit there (see kHeldScores): 32 requests of 256 to
+// 8,000 tokens 72.6 us for 428 MB and 15 MB of scores and partials (6.1 TB/s).
 
 #include <mutex>
 
@@ -72,6 +73,11 @@ constexpr int kWaves = kDecodeWaves;
 constexpr int kSlice = 32;                       // tokens per slice
 constexpr int kVRow = kHeadDim + 16;             // LDS V row stride (u16): 288 bytes
 constexpr int kSliceElems = kSlice * kVRow;      // u16 per V transpose buffer
+// Slices times heads whose scores a wave holds. HBM slows down where writes come between reads: 32
+// requests of 256 to 8,000 tokens (51 slices a wave, 4 heads) take 88 us a call with a store after
+// every slice, by the wave itself or by another one, 84 with 128 held (one store on the way), 78 with
+// 256 and more; without any store 71. 32 of 8,000 to 16,000 306 and, with 416, 255.
+constexpr int kHeldScores = 416;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -134,7 +140,7 @@ __device__ __forceinline__ s16x4 read_vt(const uint16_t *lane_base, int key0, in
 // `vbuf`. vt_base is this lane's transposed-read base in that buffer.
 // With a window, tokens of [sinks, low) are masked as those from tok_end on are; every slice
 // that is issued holds one that is not.
-// kScores: the raw scores of head n < G go to score_row (this lane's four tokens of every 16).
+// kScores: the raw scores of head n < G go to score_row in LDS (this lane's four tokens of every 16).
 template <int G, bool kWindow, bool kScores>
 __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t *vt_base,
                                               const bf16x8 (&qop)[4], int t0, int tok_end,
@@ -235,6 +241,7 @@ __device__ __forceinline__ void consume_slice(const SliceRegs &r, const uint16_t
 struct Piece {
   int seq, t0, t1, slot, sb, qt, nsl, ends;
   int ns, gap, low;  // with a window: its keys, and the first number in sight behind the sinks
+  int score;         // with kScores: its sequence's first place in a row of scores
 };
 
 static_assert(kWindowUnit == kSlice, "a slice lies on one side of the keys left out");
@@ -313,7 +320,7 @@ namespace {
 // that slice (only the one workgroup that owns the row reads it). The
 // values are those of qknorm_rope_append_kernel, bit for bit.
 template <int G, bool kFused, bool kWindow, bool kScores>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void decode_kernel(
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(kScores ? 1 : 2, 2))) void decode_kernel(
     const uint16_t *__restrict__ q, int64_t q_ss, int64_t q_st, int64_t q_sh,
     uint16_t *__restrict__ k_pool, uint16_t *__restrict__ v_pool,
     int64_t pool_hs, const int32_t *__restrict__ page_table, int64_t pt_stride,
@@ -325,6 +332,11 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   constexpr int kMaxPieces = decode_max_pieces(G);
   __shared__ __attribute__((aligned(16))) uint16_t sV[kWaves][kSliceElems];
   __shared__ __attribute__((aligned(16))) uint16_t sQ[kMaxPieces * G * kHeadDim];
+  // With kScores, the scores of a wave's last slices and where they go (the workgroup is alone on
+  // its CU, so LDS is free): stored when as many have come, or at the chunk's end.
+  constexpr int kHeld = kScores ? kHeldScores / G : 1;
+  __shared__ __attribute__((aligned(16))) float sScore[kScores ? kWaves : 1][kHeld * G * kSlice];
+  __shared__ int sPlace[kScores ? kWaves : 1][kHeld];
 
   // Grid (kv head, chunk): heads vary fastest, so with 8 kv heads every
   // XCD streams one head.
@@ -363,17 +375,21 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   ipc.nsl = (ipc.t1 - ipc.t0 + kSlice - 1) / kSlice;
   ipc.ends = pieces[8 * pb + 7];
   if constexpr (kWindow) set_window(ipc, pieces[8 * pb + 6], ex.window, ex.sinks);
+  if constexpr (kScores) ipc.score = ex.score_start[ipc.seq];
   // Loads slice k of the chunk (k-th 32-token slice in piece order) into r.
   // locate() moves the cursor to slice k and describes it; issue() also
   // loads it.
   auto locate = [&](SliceMeta &m, int k) {
-    while (k >= ipc.sb + ipc.nsl) ipc = load_piece<kWindow>(pieces, ++ip, ex.window, ex.sinks);
+    while (k >= ipc.sb + ipc.nsl) {
+      ipc = load_piece<kWindow>(pieces, ++ip, ex.window, ex.sinks);
+      if constexpr (kScores) ipc.score = ex.score_start[ipc.seq];
+    }
     m.piece = ip;
     m.t0 = ipc.t0 + (k - ipc.sb) * kSlice;
     m.tend = ipc.t1;
     m.newrow = ipc.ends && m.t0 + kSlice >= ipc.t1 ? ipc.t1 - 1 - m.t0 : -1;
     if constexpr (kWindow) m.low = ipc.low;
-    if constexpr (kScores) m.score = ex.score_start[ipc.seq] + m.t0;
+    if constexpr (kScores) m.score = ipc.score + m.t0;
   };
   // The first token of the located slice in its cache.
   auto first_token = [&](const SliceMeta &m) {
@@ -383,11 +399,28 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
     locate(m, k);
     issue_slice(r, kh, vh, page_table + ipc.seq * pt_stride, first_token(m), page_shift, lane);
   };
+  // Stores the scores of the slices held (the wave's own).
+  int held = 0;
+  auto store_scores = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+    for (int e = lane; e < held * (8 * G); e += 64) {  // 16 bytes each
+      const int head = (e >> 3) & (G - 1);
+      const int at = sPlace[wave][e / (8 * G)] + 4 * (e & 7);
+      *reinterpret_cast<f32x4 *>(ex.scores + (h0 + head) * ex.score_stride + at) =
+          *reinterpret_cast<const f32x4 *>(sScore[wave] + 4 * e);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    held = 0;
+  };
   auto consume = [&](const SliceRegs &r, const SliceMeta &m, const bf16x8 (&qop)[4], float &m_run,
                      float &l_run, f32x4 (&acc)[8]) __attribute__((always_inline)) {
     float *row = nullptr;
-    if constexpr (kScores)
-      row = ex.scores + (h0 + n) * ex.score_stride + m.score + 4 * g;
+    if constexpr (kScores) {
+      row = sScore[wave] + (held * G + (n & (G - 1))) * kSlice + 4 * g;
+      if (lane == 0) sPlace[wave][held] = m.score;
+      ++held;
+    }
     consume_slice<G, kWindow, kScores>(r, vt_base, qop, m.t0, m.tend, ex.sinks, kWindow ? m.low : 0,
                                        row, lane, scale_log2, m_run, l_run, acc);
   };
@@ -535,6 +568,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   // the tail is peeled.
   if (k < n_sl) {
     while (k + 2 * kWaves < n_sl) {
+      if constexpr (kScores) {
+        if (held + 4 > kHeld) store_scores();  // (two here, two behind the loop)
+      }
       stage_v(ra, vbuf, lane);
       issue(rb, mb, k + kWaves);
       if (ma.piece != cp) move_to(ma.piece);
@@ -557,6 +593,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       if (ma.piece != cp) move_to(ma.piece);
       consume(ra, ma, qop, m_run, l_run, acc);
     }
+    if constexpr (kScores) store_scores();
   }
   // Close the last piece and any later ones this wave had no slice of.
   flush(c_slot + wave);
