@@ -28,12 +28,12 @@
 //                 two of 151,936 tokens is met by one draw in thousands of 32-bit sums. (Of
 //                 max(p - q, 0) in the same pass, see Mass: in one of its own, once the row's sum
 //                 was known, 32 chains of 5 took 46 us instead of 39.)
-//   pick_kernel   the part that holds the draw, then the token. (In the walk's last workgroup of
-//                 each request instead, the releases and acquires of all others took 20 us
-//                 more with 32 requests.)
+//   pick_kernel   the part that holds the draw, then the token; with few requests in the walk's
+//                 last workgroup of each instead (see kPickers; with releases and acquires in
+//                 place of single values past the caches, 32 requests took 20 us more).
 //
-// A call is bound by its chain of dependent launches: 8 nodes of 151,936 tokens take 4.3 us (mass),
-// 6.5 (walk) and 6.1 (pick), less than the host's 27. With many rows the cuts lead (16 trees of up
+// A call is bound by its chain of dependent launches: 8 nodes of 151,936 tokens take 3.9 us (mass)
+// and 12.6 (walk and pick), less than the host's 23. With many rows the cuts lead (16 trees of up
 // to 26 nodes: 30.4 with the masses, 10.9 and 6.8 us; a CU's reads and LDS counts), then the
 // masses' exponentials (32 drawn chains of 5: 11, 17 and 8).
 
@@ -63,6 +63,14 @@ struct Share {
   float max, sum;
   uint64_t best;
 };
+// Workgroups of a walk up to which its last ones pick. In a row, without and with a launch for the
+// picks (us, 151,936 tokens): 1 request 23.2 and 28.4, 4 23.6 and 28.6, 8 24.5 and 29.8 (600
+// workgroups), 16 trees of 26 (1,200) 50.6 and 47.3, 32 drawn chains 38.6 and 35.5; 32 chains of
+// 32,000 tokens (512) 31.0 and 35.8. In a graph 16.9 and 17.3, 19.9 and 18.8, 25.0 and 22.3; 20.6
+// and 20.0: the writes past the caches and the count, two dependent trips, outlast a launch where
+// workgroups wait for a place.
+constexpr int kPickers = 512;
+
 struct Request {
   float temp;
   int32_t k;
@@ -128,6 +136,21 @@ struct Requests {
 struct Mass {
   double all, left, drafts;
 };
+// The workgroups of a request tell their parts' masses, the one that is done last reads them: each
+// value by itself is written through and read past the caches (an agent's atomics), and is in
+// place before the count says so. A release and an acquire instead would write back and drop whole
+// caches.
+__device__ __forceinline__ void write_through(double *at, double v) {
+  __hip_atomic_store(reinterpret_cast<long long *>(at), __double_as_longlong(v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool kPast>
+__device__ __forceinline__ double read_mass(const double *at) {
+  if (!kPast) return *at;
+  return __longlong_as_double(
+      __hip_atomic_load(const_cast<long long *>(reinterpret_cast<const long long *>(at)),
+                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 struct State {
   int32_t last, child;  // the path's last node, and its refused child where drafts are drawn, or -1
   float max;            // largest kept logit of the last node's row
@@ -360,13 +383,21 @@ __device__ __forceinline__ void mass_of_share(const uint16_t *row, int vocab, fl
   }
 }
 
+// What the walk starts from: no part is done, nothing is bad.
+__device__ __forceinline__ void begin(const Requests &requests, int32_t *done, uint8_t *valid,
+                                      bool first_rows) {
+  if (static_cast<int>(threadIdx.x) < requests.count) done[threadIdx.x] = 0;
+  if (first_rows && threadIdx.x == 0) *valid = 1;
+}
+
 // Grid (shares, rows): no row is cut.
 template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void mass_kernel(const uint16_t *__restrict__ logits, int64_t ld,
                                                         int vocab, Requests requests,
+                                                        int32_t *__restrict__ done,
                                                         uint8_t *__restrict__ valid, bool first_rows) {
   __shared__ MassRoom room;
-  if (first_rows && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *valid = 1;
+  if (blockIdx.x == 0 && blockIdx.y == 0) begin(requests, done, valid, first_rows);
   const int row = blockIdx.y;
   mass_of_share<kBf16>(logits + row * ld, vocab, requests.r[requests.of_row(row)].temp, blockIdx.x,
                        gridDim.x, requests.shares + static_cast<int64_t>(row) * gridDim.x, room);
@@ -377,10 +408,11 @@ __global__ __launch_bounds__(kThreads) void mass_kernel(const uint16_t *__restri
 template <bool kBf16>
 __global__ __launch_bounds__(kCutThreads) void cut_mass_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests, int n_cut,
-    RowCut *__restrict__ cuts, uint8_t *__restrict__ valid, bool first_rows) {
+    RowCut *__restrict__ cuts, int32_t *__restrict__ done, uint8_t *__restrict__ valid,
+    bool first_rows) {
   constexpr int kShares = kCutThreads / kThreads;
   __shared__ MassRoom rooms[kShares];
-  if (first_rows && blockIdx.x == 0 && threadIdx.x == 0) *valid = 1;
+  if (blockIdx.x == 0) begin(requests, done, valid, first_rows);
   const int block = blockIdx.x;
   if (block < n_cut) {
     cut_row<kBf16>(logits, ld, vocab, requests, requests.nth_row(true, block), nullptr, cuts);
@@ -496,7 +528,7 @@ __device__ __forceinline__ int take_found(const Found *of_waves, double &rest) {
 // `number` times the total (where rounding leaves none, the last token with any). The masses are
 // max(p - q, 0) with q (the row of draft probabilities), else those of p without the children of
 // `last`, of which every thread has one's parent and token.
-template <bool kBf16>
+template <bool kBf16, bool kPast>
 __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const Cut &cut, float max,
                                           double inv_temp, double number, const Mass *masses,
                                           const float *q, int n_parts, int parent, int64_t token,
@@ -528,10 +560,11 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
     return total;
   };
   double all = 0, left = 0, all_before, left_before;
-  for (int i = from; i < to; ++i) all += masses[i].all;
+  for (int i = from; i < to; ++i) all += read_mass<kPast>(&masses[i].all);
   const double z = sums(all, room.all, all_before), inv_z = 1.0 / z;
   auto left_of = [&](const Mass &m) {
-    return q ? fmax(fma(m.left, inv_z, -m.drafts), 0.0) : m.left;
+    const double some = read_mass<kPast>(&m.left);
+    return q ? fmax(fma(some, inv_z, -read_mass<kPast>(&m.drafts)), 0.0) : some;
   };
   for (int i = from; i < to; ++i) left += left_of(masses[i]);
   const double some = sums(left, room.left, left_before);
@@ -543,7 +576,7 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   if (own > 0) {
     double at = before;
     for (int i = from; i < to; ++i) {
-      const double v = whole ? masses[i].all : left_of(masses[i]);
+      const double v = whole ? read_mass<kPast>(&masses[i].all) : left_of(masses[i]);
       if (v > 0) {
         part = i;
         rest = target - at;
@@ -593,13 +626,13 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   return take_found(room.tokens, rest);
 }
 
-// Grid (parts or fewer, requests).
-template <bool kBf16>
+// Grid (parts or fewer, requests). kPicks: the workgroup of a request that is done last picks.
+template <bool kBf16, bool kPicks>
 __global__ __launch_bounds__(kThreads) void walk_kernel(
     const uint16_t *__restrict__ logits, int64_t ld, int vocab, Requests requests,
     const RowCut *__restrict__ cuts, const Share *__restrict__ shares, int n_shares,
     int n_parts, Tree tree,
-    State *__restrict__ states, Mass *__restrict__ masses,
+    State *__restrict__ states, Mass *__restrict__ masses, int32_t *__restrict__ done,
     int32_t *__restrict__ paths, int levels, int32_t *__restrict__ lengths,
     int64_t *__restrict__ next, uint8_t *__restrict__ valid) {
   __shared__ float max_of[kMaxNodes];
@@ -611,6 +644,8 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
   __shared__ State sh;
   __shared__ uint32_t bits[kPart / 32];
   __shared__ Pair box[kWaves];
+  __shared__ PickRoom room;
+  __shared__ bool picks;
   const int b = blockIdx.y;
   const Request req = requests.r[b];
   const int nodes = requests.nodes(b), row0 = req.first;
@@ -740,7 +775,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
       sh = {last, child, greedy ? 0.f : max_of[last], bad};
       if (tell) {
         lengths[b] = length;
-        states[b] = sh;
+        if (!kPicks) states[b] = sh;
         if (greedy) next[b] = best_of[last];
         if (bad) {
           next[b] = 0;
@@ -782,8 +817,28 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
     }
     const Pair sums = block_sums(all, left, box);
     if (drawn) drafts = block_sums(drafts, 0.0, box).a;
-    if (tid == 0) masses[static_cast<int64_t>(b) * n_parts + part] = {sums.a, sums.b, drafts};
+    Mass *m = masses + static_cast<int64_t>(b) * n_parts + part;
+    if (kPicks && tid == 0) {
+      write_through(&m->all, sums.a);
+      write_through(&m->left, sums.b);
+      write_through(&m->drafts, drafts);
+    } else if (tid == 0) {
+      *m = {sums.a, sums.b, drafts};
+    }
   }
+  if constexpr (!kPicks) return;
+  if (tid == 0) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int mine = (n_parts - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1;
+    picks = __hip_atomic_fetch_add(done + b, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + mine ==
+            n_parts;
+  }
+  __syncthreads();
+  if (!picks) return;
+  const int got = pick_token<kBf16, true>(x_row, vocab, cut, sh.max, inv_temp, tree.draws[b],
+                                    masses + static_cast<int64_t>(b) * n_parts, q, n_parts, my_parent,
+                                    my_token, sh.last, bits, room);
+  if (tid == 0) next[b] = got;
 }
 
 // Grid (requests).
@@ -807,7 +862,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(
   const int row = req.first + st.last;
   const Cut cut = requests.cut(b, vocab) ? cut_of<kBf16>(cuts[row]) : no_cut();
   const bool drawn = tree.drafts && st.child >= 0;  // the draw is from max(p - q, 0)
-  const int got = pick_token<kBf16>(
+  const int got = pick_token<kBf16, false>(
       logits + row * ld, vocab, cut, st.max, 1.0 / req.temp, number,
       masses + static_cast<int64_t>(b) * n_parts,
       drawn ? tree.drafts + (req.first + st.child) * tree.drafts_ld : nullptr, n_parts, parent, token,
@@ -820,7 +875,7 @@ int64_t share_count(int64_t vocab) { return (vocab + kShare - 1) / kShare; }
 int64_t part_count(int64_t vocab) { return (vocab + kPart - 1) / kPart; }
 
 struct Room {
-  int64_t cuts, shares, states, masses, all;
+  int64_t cuts, shares, states, done, masses, all;
 };
 Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
   const int64_t n = share_count(vocab), parts = part_count(vocab);
@@ -835,6 +890,7 @@ Room room_of(int64_t rows, int64_t requests, int64_t vocab) {
   r.cuts = take(rows * static_cast<int64_t>(sizeof(RowCut)));
   r.shares = take(rows * n * static_cast<int64_t>(sizeof(Share)));
   r.states = take(requests * static_cast<int64_t>(sizeof(State)));
+  r.done = take(requests * static_cast<int64_t>(sizeof(int32_t)));
   r.masses = take(requests * parts * static_cast<int64_t>(sizeof(Mass)));
   r.all = at;
   return r;
@@ -848,6 +904,7 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &
   auto *cut = reinterpret_cast<RowCut *>(ws + room.cuts);
   auto *shares = reinterpret_cast<Share *>(ws + room.shares);
   auto *states = reinterpret_cast<State *>(ws + room.states);
+  auto *done = reinterpret_cast<int32_t *>(ws + room.done);
   auto *masses = reinterpret_cast<Mass *>(ws + room.masses);
   req.shares = shares;
   req.n_shares = n;
@@ -855,19 +912,20 @@ void launch(hipStream_t st, const uint16_t *x, int64_t ld, int vocab, Requests &
     constexpr int kShares = kCutThreads / kThreads;
     const int64_t blocks = n_cut + static_cast<int64_t>(req.rows - n_cut) * ((n + kShares - 1) / kShares);
     hipLaunchKernelGGL(cut_mass_kernel<kBf16>, dim3(static_cast<uint32_t>(blocks)), dim3(kCutThreads),
-                       0, st, x, ld, vocab, req, n_cut, cut, valid, first_rows);
+                       0, st, x, ld, vocab, req, n_cut, cut, done, valid, first_rows);
   } else {
     hipLaunchKernelGGL(mass_kernel<kBf16>, dim3(n, req.rows), dim3(kThreads), 0, st, x, ld, vocab, req,
-                       valid, first_rows);
+                       done, valid, first_rows);
   }
   bool sampled = false;
   for (int b = 0; b < req.count; ++b) sampled = sampled || req.r[b].temp != 0.f;
   // Every workgroup of a request repeats its walk: no more of them than fill the GPU.
   const int walkers = sampled ? std::min(parts, std::max(1, kWalkers / req.count)) : 1;
-  hipLaunchKernelGGL(walk_kernel<kBf16>, dim3(walkers, req.count), dim3(kThreads), 0, st, x, ld,
-                     vocab, req, cut, shares, n, parts, tree, states, masses, paths, levels, lengths,
-                     next, valid);
-  if (!sampled) return;
+  const bool picks = walkers * req.count <= kPickers;
+  auto walk = picks ? walk_kernel<kBf16, true> : walk_kernel<kBf16, false>;
+  hipLaunchKernelGGL(walk, dim3(walkers, req.count), dim3(kThreads), 0, st, x, ld, vocab, req, cut,
+                     shares, n, parts, tree, states, masses, done, paths, levels, lengths, next, valid);
+  if (!sampled || picks) return;
   hipLaunchKernelGGL(pick_kernel<kBf16>, dim3(req.count), dim3(kThreads), 0, st, x, ld, vocab, req,
                      cut, tree, states, masses, parts, next);
 }

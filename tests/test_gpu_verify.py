@@ -177,6 +177,37 @@ def test_cut_requests_among_others(cut):
     check(trees, 9000, 17, temps, ks, ps)
 
 
+def test_more_parts_than_workgroups_that_pick():
+    g = torch.Generator().manual_seed(12)
+    trees = [random_tree(g, 1 + i % 5) for i in range(30)]
+    settings = [SETTINGS[i % len(SETTINGS)] for i in range(30)]
+    check(trees, 40_000, 8, *map(list, zip(*settings)))
+    chains = [list(range(-1, i % 4)) for i in range(30)]
+    check(chains, 40_000, 9, *map(list, zip(*settings)), drafts=True)
+
+
+@pytest.mark.parametrize("requests,vocab", [(1, 151_936), (3, 151_936), (6, 151_936), (40, 20_000)])
+def test_draws_from_new_rows_time_after_time(requests, vocab):
+    """The masses of a row's parts, told from workgroup to workgroup, are those of this call and of
+    none before: rows of one peak each, at a place of its own, many draws in a row."""
+    g = torch.Generator(device=DEV).manual_seed(requests)
+    batch = batch_of([[-1]] * requests)
+    settings = [0.9] * requests, [None] * requests, [None] * requests
+    tokens = torch.zeros(requests, dtype=torch.int64, device=DEV)
+    base = torch.randn((requests, vocab), generator=g, device=DEV).to(torch.bfloat16)
+    got, want = [], []
+    for _ in range(150):
+        at = torch.randint(0, vocab, (requests, 1), generator=g, device=DEV)
+        logits = base.scatter(1, at, 9.0)  # half of the mass, about
+        uniforms = torch.rand(2 * requests, generator=g, device=DEV)
+        got.append(verify_tree(batch, logits, tokens, *settings, uniforms)[2][:, 0])
+        score = logits.double() / float(np.float32(0.9))
+        mass = torch.cumsum(torch.exp(score - score.amax(1, keepdim=True)), 1)
+        over = mass > uniforms[requests:, None].double() * mass[:, -1:]
+        want.append(over.byte().argmax(1))
+    assert torch.equal(torch.stack(got), torch.stack(want))
+
+
 def test_equal_tokens_and_certain_ones():
     """Siblings with one token: refused once, refused for good. A token that has all the mass
     stands whatever the number; where everything is refused the draw is from p."""
