@@ -29,8 +29,7 @@
 //                 max(p - q, 0) in the same pass, see Mass: in one of its own, once the row's sum
 //                 was known, 32 chains of 5 took 46 us instead of 39.)
 //   pick_kernel   the part that holds the draw, then the token; with few requests in the walk's
-//                 last workgroup of each instead (see kPickers; with releases and acquires in
-//                 place of single values past the caches, 32 requests took 20 us more).
+//                 last workgroup of each instead (see kPickers; with 32 requests, 20 us more).
 //
 // A call is bound by its chain of dependent launches: 8 nodes of 151,936 tokens take 3.9 us (mass)
 // and 12.6 (walk and pick), less than the host's 23. With many rows the cuts lead (16 trees of up
@@ -64,12 +63,11 @@ struct Share {
   uint64_t best;
 };
 // Workgroups of a walk up to which its last ones pick. In a row, without and with a launch for the
-// picks (us, 151,936 tokens): 1 request 23.2 and 28.4, 4 23.6 and 28.6, 8 24.5 and 29.8 (600
-// workgroups), 16 trees of 26 (1,200) 50.6 and 47.3, 32 drawn chains 38.6 and 35.5; 32 chains of
-// 32,000 tokens (512) 31.0 and 35.8. In a graph 16.9 and 17.3, 19.9 and 18.8, 25.0 and 22.3; 20.6
-// and 20.0: the writes past the caches and the count, two dependent trips, outlast a launch where
-// workgroups wait for a place.
-constexpr int kPickers = 512;
+// picks (us, 151,936 tokens): 1 request 23.5 and 28.4, 4 (300 workgroups) 23.6 and 28.6, 16 chains
+// of 32,000 tokens (256) 26.8 and 31.5; 16 trees of 26 (1,200) 50.6 and 47.3. In a graph, where the
+// host does not count, 17.3 and 17.3, 20.4 and 18.8, 19.5 and 18.3: each workgroup's release, the
+// count and the last one's acquire are dependent trips, which many workgroups wait for.
+constexpr int kPickers = 320;
 
 struct Request {
   float temp;
@@ -136,21 +134,6 @@ struct Requests {
 struct Mass {
   double all, left, drafts;
 };
-// The workgroups of a request tell their parts' masses, the one that is done last reads them: each
-// value by itself is written through and read past the caches (an agent's atomics), and is in
-// place before the count says so. A release and an acquire instead would write back and drop whole
-// caches.
-__device__ __forceinline__ void write_through(double *at, double v) {
-  __hip_atomic_store(reinterpret_cast<long long *>(at), __double_as_longlong(v), __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
-}
-template <bool kPast>
-__device__ __forceinline__ double read_mass(const double *at) {
-  if (!kPast) return *at;
-  return __longlong_as_double(
-      __hip_atomic_load(const_cast<long long *>(reinterpret_cast<const long long *>(at)),
-                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
 struct State {
   int32_t last, child;  // the path's last node, and its refused child where drafts are drawn, or -1
   float max;            // largest kept logit of the last node's row
@@ -528,7 +511,7 @@ __device__ __forceinline__ int take_found(const Found *of_waves, double &rest) {
 // `number` times the total (where rounding leaves none, the last token with any). The masses are
 // max(p - q, 0) with q (the row of draft probabilities), else those of p without the children of
 // `last`, of which every thread has one's parent and token.
-template <bool kBf16, bool kPast>
+template <bool kBf16>
 __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const Cut &cut, float max,
                                           double inv_temp, double number, const Mass *masses,
                                           const float *q, int n_parts, int parent, int64_t token,
@@ -560,11 +543,10 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
     return total;
   };
   double all = 0, left = 0, all_before, left_before;
-  for (int i = from; i < to; ++i) all += read_mass<kPast>(&masses[i].all);
+  for (int i = from; i < to; ++i) all += masses[i].all;
   const double z = sums(all, room.all, all_before), inv_z = 1.0 / z;
   auto left_of = [&](const Mass &m) {
-    const double some = read_mass<kPast>(&m.left);
-    return q ? fmax(fma(some, inv_z, -read_mass<kPast>(&m.drafts)), 0.0) : some;
+    return q ? fmax(fma(m.left, inv_z, -m.drafts), 0.0) : m.left;
   };
   for (int i = from; i < to; ++i) left += left_of(masses[i]);
   const double some = sums(left, room.left, left_before);
@@ -576,7 +558,7 @@ __device__ __forceinline__ int pick_token(const uint16_t *row, int vocab, const 
   if (own > 0) {
     double at = before;
     for (int i = from; i < to; ++i) {
-      const double v = whole ? read_mass<kPast>(&masses[i].all) : left_of(masses[i]);
+      const double v = whole ? masses[i].all : left_of(masses[i]);
       if (v > 0) {
         part = i;
         rest = target - at;
@@ -817,25 +799,18 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(
     }
     const Pair sums = block_sums(all, left, box);
     if (drawn) drafts = block_sums(drafts, 0.0, box).a;
-    Mass *m = masses + static_cast<int64_t>(b) * n_parts + part;
-    if (kPicks && tid == 0) {
-      write_through(&m->all, sums.a);
-      write_through(&m->left, sums.b);
-      write_through(&m->drafts, drafts);
-    } else if (tid == 0) {
-      *m = {sums.a, sums.b, drafts};
-    }
+    if (tid == 0) masses[static_cast<int64_t>(b) * n_parts + part] = {sums.a, sums.b, drafts};
   }
   if constexpr (!kPicks) return;
   if (tid == 0) {
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int mine = (n_parts - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1;
-    picks = __hip_atomic_fetch_add(done + b, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + mine ==
+    picks = __hip_atomic_fetch_add(done + b, mine, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) + mine ==
             n_parts;
   }
   __syncthreads();
   if (!picks) return;
-  const int got = pick_token<kBf16, true>(x_row, vocab, cut, sh.max, inv_temp, tree.draws[b],
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const int got = pick_token<kBf16>(x_row, vocab, cut, sh.max, inv_temp, tree.draws[b],
                                     masses + static_cast<int64_t>(b) * n_parts, q, n_parts, my_parent,
                                     my_token, sh.last, bits, room);
   if (tid == 0) next[b] = got;
@@ -862,7 +837,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(
   const int row = req.first + st.last;
   const Cut cut = requests.cut(b, vocab) ? cut_of<kBf16>(cuts[row]) : no_cut();
   const bool drawn = tree.drafts && st.child >= 0;  // the draw is from max(p - q, 0)
-  const int got = pick_token<kBf16, false>(
+  const int got = pick_token<kBf16>(
       logits + row * ld, vocab, cut, st.max, 1.0 / req.temp, number,
       masses + static_cast<int64_t>(b) * n_parts,
       drawn ? tree.drafts + (req.first + st.child) * tree.drafts_ld : nullptr, n_parts, parent, token,
