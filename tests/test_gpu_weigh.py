@@ -62,15 +62,19 @@ def test_head_groups(hq, hkv):
                    seed=hq), what=f"{hq}/{hkv}")
 
 
-@pytest.mark.parametrize("split", [32, 96, 1000])
-def test_partials_by_the_hundred(split):
-    """(64 of a decode token's are joined at a time)"""
+@pytest.mark.parametrize("split", [32, 96, 1000, 100_000])
+def test_many_partials_and_long_chunks(split):
+    """Hundreds of partials, of which 64 are joined at a time, and chunks of more slices than
+    a wave holds the scores of (104 with four heads to a kv head, 52 with eight)."""
     r = Requests([9000, 2048, 700, 63], [1, 1, 1, 1], seed=split)
     r.m.tokens_per_split = split
     check(r, what=f"split {split}")
     one = Requests([9000], [1], hq=64, hkv=8, seed=split)
     one.m.tokens_per_split = split
     check(one, what=f"split {split}, one")
+    if split == 100_000:
+        chunks = one.m.begin_tick(one.handles, one.fresh).plan(64).host.decode[:, 2]
+        assert int(chunks[0]) > 4 * 52
 
 
 @pytest.mark.parametrize("hq,hkv", [(128, 8), (2, 1), (80, 5)])
